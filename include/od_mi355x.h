@@ -568,6 +568,53 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
                const float* head, const float* none_logit, float inv_temperature, int64_t B, int64_t n_opt, int64_t t,
                int64_t t0, int64_t H, int64_t chunks, double* part, float* out, od_stream_t stream);
 
+/*
+ * A paged K/V cache (no reference counterpart: the reference keeps one rectangular cache per batch,
+ * src/opendecider/backbone.py:435-468). A layer's K and V are two pools of n_pages pages of `page` token rows (a power of
+ * two >= 16) for every KV head:
+ *   k_pages, v_pages  int8 [n_pages, Hkv, page, D] with k_scale, v_scale fp32 [n_pages, Hkv, page], or bf16 with both
+ *                     scales NULL; contiguous, 16-byte aligned; D in {64, 128, 256}
+ *   table             int32 [B, cols], row stride ld_table: position j of sequence b is row j % page of page
+ *                     table[b, j / page]. An entry outside [0, n_pages) is no page: no key is there, nothing is written
+ *   start             int32 [B + 1]: sequence b's new tokens are the packed rows start[b] .. start[b + 1] - 1 (ascending;
+ *                     rows of no sequence, e.g. behind start[B], are neither read as tokens nor written)
+ *   ctx_len           int32 [B]: sequence b's cached tokens (negative: 0; past the table: the table's end)
+ * All on the device; the host needs none of them.
+ *
+ * od_page_append: k, v bf16 [N, Hkv, D] (element strides per token and head, multiples of 8) of the new tokens into the
+ *   pages of their sequences at the positions ctx_len[b], ctx_len[b] + 1, ...; int8 pages take the bytes and scales of
+ *   od_kv_quant_append, bf16 pages the values. Two rows at one place (a page in two sequences, a page twice in one) race.
+ * od_page_read: the first `length[b]` (<= T) tokens of every sequence into contiguous [B, Hkv, T, D], zeros behind them and
+ *   where there is no page: form OD_READ_BF16 or OD_READ_FP32 the values q * s (an fp32 product, rounded once to bf16), or
+ *   OD_READ_INT8 the rows with their scales [B, Hkv, T] (int8 pages only; ks_out and vs_out NULL otherwise).
+ * od_paged_attn: every new token of a sequence attends that sequence's ctx_len[b] cached tokens and its new tokens from
+ *   row_begin[n] (int32 [N], counted from start[b]; NULL: 0) up to itself, as they come in bf16 (k and v NULL: the cached
+ *   ones only). q, out bf16 [N, Hq, D], lse fp32 [N, Hq] or NULL (natural log, of the scaled scores); a token that sees
+ *   nothing gets 0 and -inf. The pages are read, not written: append before or after. scale > 0 and finite. max_new and
+ *   max_ctx are the caller's bounds on a sequence's new and cached tokens; they size the grid, the key splits and the
+ *   workspace (od_paged_attn_ws floats, 16-byte aligned, NULL where that is 0), not the result.
+ */
+#define OD_READ_BF16 0
+#define OD_READ_FP32 1
+#define OD_READ_INT8 2
+int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh, void* k_pages,
+                   float* k_scale, void* v_pages, float* v_scale, int64_t n_pages, int64_t page, const int32_t* table,
+                   int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx_len, int64_t B, int64_t N,
+                   int64_t Hkv, int64_t D, od_stream_t stream);
+int od_page_read(const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale, int64_t n_pages,
+                 int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* length, int64_t B,
+                 int64_t T, int64_t Hkv, int64_t D, int form, void* k_out, float* ks_out, void* v_out, float* vs_out,
+                 od_stream_t stream);
+int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx,
+                     int64_t* ws_floats);
+int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
+                  const uint16_t* v, int64_t svt, int64_t svh, const void* k_pages, const float* k_scale,
+                  const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page, const int32_t* table,
+                  int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx_len, const int32_t* row_begin,
+                  uint16_t* out, int64_t sot, int64_t soh, float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+                  int64_t D, int64_t max_new, int64_t max_ctx, float scale, float* ws, int64_t ws_floats,
+                  od_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

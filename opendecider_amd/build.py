@@ -23,7 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libod_mi355x.so")
 SOURCES = ["od_quant.hip", "od_gemm.hip", "od_attn.hip", "od_wide.hip", "od_layer.hip", "od_lmhead.hip", "od_gdn.hip",
-           "od_gdn_chunk.hip"]
+           "od_gdn_chunk.hip", "od_paged.hip"]
 # the matrix-core ceiling probe bench.py reports beside the rooflines, in a library of its own
 PROBE_SOURCE = "od_probe.hip"
 PROBE_LIB = os.path.join(PKG, "libod_probe.so")
@@ -35,7 +35,8 @@ PROBE_LIB = os.path.join(PKG, "libod_probe.so")
 # fits 220 VGPRs and two workgroups per CU with it); at head_dims 64 / 128 no accumulator register is used either way
 SOURCE_FLAGS = {"od_gdn_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 "od_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                "od_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                "od_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "od_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Xclang", "-target-feature",
          "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-inline-asm"]

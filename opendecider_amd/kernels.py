@@ -1018,3 +1018,145 @@ def gdn_norm_quant(o: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
                                   ptr(inv_s), eps, M, n_v, dv, ptr(xq), xq.stride(0), ptr(sx), stream_of(o)),
           "od_gdn_norm_quant")
     return xq, sx
+
+
+# ------------------------------------------------------------------------------------------------ paged K/V cache
+def _paged(cache, table, start, ctx_len, name):
+    """The arguments of a paged batch that every entry point takes, checked: (pages, table) and the sequence count."""
+    k = cache.k
+    B = ctx_len.numel()
+    if table.dtype != torch.int32 or ctx_len.dtype != torch.int32 or (start is not None and start.dtype != torch.int32):
+        raise TypeError(f"{name}: table, start and the lengths must be int32")
+    if table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name}: table must be (sequences, pages per sequence) with contiguous rows, one row per length")
+    if not ctx_len.is_contiguous() or (start is not None and (start.numel() != B + 1 or not start.is_contiguous())):
+        raise ValueError(f"{name}: start must be (sequences + 1,) and the lengths (sequences,), contiguous")
+    dev = k.device
+    for t in (cache.v, table, ctx_len, start):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on one device")
+    cols = table.shape[1]
+    return B, (k.data_ptr(), ptr(cache.k_scale), cache.v.data_ptr(), ptr(cache.v_scale), k.shape[0], k.shape[2],
+               table.data_ptr(), max(table.stride(0), cols) if B > 1 else cols, cols)
+
+
+def _new_rows(x, N, H, D, cache, name):
+    """bf16 rows (N, H, D) whose strides the 16-byte loads take (else a contiguous copy)."""
+    _lib.bf16_bits(x)
+    if x.shape != (N, H, D):
+        raise ValueError(f"{name}: expected {(N, H, D)}, got {tuple(x.shape)}")
+    if x.device != cache.k.device:
+        raise ValueError(f"{name}: all tensors must be on one device")
+    x = _rows_aligned(x)
+    return x.clone() if x.data_ptr() % 16 else x  # contiguous rows at an odd address stay where they are above
+
+
+def _on_device(t: torch.Tensor):
+    """The tensor's device as the current one, for a library call (a launch goes to the current device)."""
+    return torch.cuda.device(t.device)
+
+
+def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, start: torch.Tensor,
+                ctx_len: torch.Tensor) -> None:
+    """od_page_append: the new tokens' k and v (N, Hkv, D) bf16 into the pages of a PagedKVCache, quantized per (token,
+    head) where the pages are int8 (the bytes of kv_quant_append). table int32 (B, pages per sequence); start int32
+    (B + 1,): sequence b's tokens are the rows start[b] .. start[b + 1] - 1; ctx_len int32 (B,): the tokens it holds
+    before, which is where they go. Tokens without a page are not written. The lengths stay: advance them once every layer
+    has its tokens."""
+    require_gpu(k, v, cache.k, table, start, ctx_len, name="page_append")
+    B, pages = _paged(cache, table, start, ctx_len, "page_append")
+    _, H, _, D = cache.k.shape
+    N = k.shape[0]
+    k, v = _new_rows(k, N, H, D, cache, "page_append: k"), _new_rows(v, N, H, D, cache, "page_append: v")
+    with _on_device(k):
+        check(lib().od_page_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *pages,
+                                   start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
+
+
+def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: torch.dtype = torch.bfloat16):
+    """od_page_read: the first length[b] (at most T) tokens of every sequence as dense (B, Hkv, T, D) K and V, zeros behind
+    them. dtype bfloat16 or float32: the values q * s, one fp32 product (Int8Tensor.dequantize rounds the scale to bf16
+    first). int8 (int8 pages only): two Int8Tensors, the stored bytes and scales (scales (B, Hkv, T, 1))."""
+    require_gpu(cache.k, table, length, name="page_read")
+    B, pages = _paged(cache, table, None, length, "page_read")
+    if T < 0:
+        raise ValueError(f"page_read: T must not be negative, got {T}")
+    forms = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
+    if dtype not in forms or (dtype == torch.int8 and cache.k_scale is None):
+        raise TypeError(f"page_read: cannot read {cache.k.dtype} pages as {dtype}")
+    _, H, _, D = cache.k.shape
+    dev = cache.k.device
+    k, v = (torch.empty(B, H, T, D, dtype=dtype, device=dev) for _ in range(2))
+    ks = vs = None
+    if dtype == torch.int8:
+        ks, vs = (torch.empty(B, H, T, dtype=torch.float32, device=dev) for _ in range(2))
+    with _on_device(k):
+        check(lib().od_page_read(*pages, length.data_ptr(), B, T, H, D, forms[dtype], k.data_ptr(), ptr(ks), v.data_ptr(),
+                                 ptr(vs), stream_of(k)), "od_page_read")
+    if ks is None:
+        return k, v
+    from .quant import Int8Tensor
+    return Int8Tensor(k, ks[..., None], torch.bfloat16), Int8Tensor(v, vs[..., None], torch.bfloat16)
+
+
+_PAGED_WS: dict = {}
+
+
+def paged_attn_workspace_floats(B: int, N: int, Hq: int, Hkv: int, D: int, max_new: int, max_ctx: int, device) -> int:
+    """Floats of od_paged_attn's workspace for these sizes on the device (0: the keys are not split)."""
+    key = (device.index, B, N, Hq, Hkv, D, max_new, max_ctx)
+    n = _PAGED_WS.get(key)
+    if n is None:
+        if len(_PAGED_WS) >= 65536:  # the sizes are cheap to ask for again
+            _PAGED_WS.clear()
+        w = ctypes.c_int64(0)
+        with torch.cuda.device(device):
+            check(lib().od_paged_attn_ws(B, N, Hq, Hkv, D, max_new, max_ctx, ctypes.byref(w)), "od_paged_attn_ws")
+        n = _PAGED_WS[key] = w.value
+    return n
+
+
+def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.Tensor, ctx_len: torch.Tensor, scale: float,
+               row_begin=None, max_new: int | None = None, max_ctx: int | None = None, out=None, return_lse: bool = False):
+    """od_paged_attn: the new tokens' queries q (N, Hq, D) bf16 attend the ctx_len[b] cached tokens of their sequence and
+    its new tokens k, v (N, Hkv, D) bf16 causally (both None: the cached ones only). table, start and ctx_len as
+    page_append. row_begin int32 (N,): the first new token that a token sees, counted from its sequence's first (option
+    rows and packed documents see their own tokens only); None: 0. max_new, max_ctx: bounds on a sequence's new and cached
+    tokens that the caller knows on the host (the work is split by them; the result is right for any). The pages are only
+    read; int8 rows count as the exact q * s. Returns out (N, Hq, D) bf16 [, lse (N, Hq) fp32]; a token that sees nothing
+    gets 0 and -inf, rows of no sequence are left as they were."""
+    require_gpu(q, k, v, cache.k, table, start, ctx_len, row_begin, out, name="paged_attn")
+    B, pages = _paged(cache, table, start, ctx_len, "paged_attn")
+    n_pages, H, page, D = cache.k.shape
+    N, Hq = q.shape[0], q.shape[1]
+    q = _new_rows(q, N, Hq, D, cache, "paged_attn: q")
+    if (k is None) != (v is None):
+        raise ValueError("paged_attn: k and v come together")
+    if Hq % H:
+        raise ValueError(f"paged_attn: {Hq} query heads over {H} K/V heads")
+    if not 0.0 < float(scale) < float("inf"):
+        raise ValueError(f"paged_attn: the scale must be positive and finite, got {scale}")
+    kst = vst = (None, 0, 0)
+    if k is not None:
+        k, v = _new_rows(k, N, H, D, cache, "paged_attn: k"), _new_rows(v, N, H, D, cache, "paged_attn: v")
+        kst, vst = (k.data_ptr(), k.stride(0), k.stride(1)), (v.data_ptr(), v.stride(0), v.stride(1))
+    if row_begin is not None and (row_begin.dtype != torch.int32 or row_begin.numel() != N or
+                                  not row_begin.is_contiguous() or row_begin.device != q.device):
+        raise ValueError("paged_attn: row_begin must be int32 (N,), contiguous, on the queries' device")
+    most = table.shape[1] * page
+    max_new = N if max_new is None else min(max(int(max_new), 0), N)
+    max_ctx = most if max_ctx is None else min(max(int(max_ctx), 0), most)
+    given, out = out, _check_out(out, (N, Hq, D), q.device, "paged_attn")
+    dst = out if given is None or (not out.data_ptr() % 16 and not any(s % 8 for s in out.stride()[:2])) else \
+        torch.empty(N, Hq, D, dtype=out.dtype, device=out.device).copy_(out)
+    lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device) if return_lse else None
+    n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    with _on_device(q):
+        check(lib().od_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), *kst, *vst, *pages, start.data_ptr(),
+                                  ctx_len.data_ptr(), ptr(row_begin), dst.data_ptr(), dst.stride(0), dst.stride(1),
+                                  ptr(lse), B, N, Hq, H, D, max_new, max_ctx, float(scale), ptr(ws), n, stream_of(q)),
+              "od_paged_attn")
+    if dst is not out:
+        out.copy_(dst)
+    return (out, lse) if return_lse else out
