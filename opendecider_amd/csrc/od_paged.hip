@@ -42,6 +42,17 @@ __device__ __forceinline__ int64_t row_of(const Paged& p, int b, int h, int64_t 
   return (((int64_t)pg * p.Hkv + h) << p.shift) + (pos & ((1 << p.shift) - 1));
 }
 
+// A load at a wave-uniform address through the scalar path, whose wait does not include the vector loads in flight.
+__device__ __forceinline__ int uniform_load(const int32_t* p) {
+  return *(__attribute__((address_space(4))) const int32_t*)(uintptr_t)p;
+}
+// row_of for wave-uniform arguments
+__device__ __forceinline__ int64_t uniform_row_of(const Paged& p, int b, int h, int pos) {
+  const int pg = uniform_load(p.table + b * p.ld_table + (pos >> p.shift));
+  if (pg < 0 || pg >= p.n_pages) return -1;
+  return (((int64_t)pg * p.Hkv + h) << p.shift) + (pos & ((1 << p.shift) - 1));
+}
+
 // The last sequence that starts at or before packed row t, by all 64 lanes together (a 64-way search: one load per lane
 // and level, one level up to 64 sequences, two up to 4096); 0 if there is none. t is wave-uniform. In bounds for any
 // contents of start.
@@ -207,6 +218,10 @@ __global__ __launch_bounds__(kThreads) void page_read_kernel(ReadArgs a) {
 // New token i of sequence b (packed row n = start[b] + i) sees the cached positions 0 .. ctx[b] - 1 and the new tokens
 // row_begin[n] .. i of its own sequence (row_begin null: from 0), bf16 as they come: o = sum_j p_j v_j / sum_j p_j with
 // p_j = exp(scale q.k_j - max), lse = max + log sum p; a token that sees nothing has o = 0 and lse = -inf.
+//
+// A "slot" is a (new token, head of the KV group) pair: slot z of a sequence is token z / rep, head g rep + z % rep. Both
+// kernels go over the keys once with a running maximum m and sum l in fp32 (log2 units). m moves only when a block's maximum
+// lies more than 2^kSlack above it, so most blocks do not rescale the output: p <= 2^kSlack.
 struct AttnArgs {
   Paged p;
   const uint16_t* q;
@@ -215,72 +230,1031 @@ struct AttnArgs {
   const int32_t* row_begin;
   uint16_t* out;
   float* lse;
+  float* part;  // splits: normalized outputs [nsplit, N, Hq, D], then their LSEs [nsplit, N, Hq] (log2 units)
   int64_t sqt, sqh, skt, skh, svt, svh, sot, soh;
   int Hq, rep;
   float scale_log2;
+  int nsplit, chunk;  // split sp takes the key tiles sp chunk .. of a sequence, the last split all that are left
+  int tiles;          // slot tiles of a sequence that the grid covers (the workgroups go on from there)
 };
 
-// One wave per (packed row, query head), 64 keys at a time: a lane takes a key's whole score, then D / 64 columns of the
-// output over the 64 probabilities.
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kSlack = 8.0f;
+
+// One sequence as a workgroup sees it (all wave-uniform).
+struct Seq {
+  int s0, n;  // its new tokens are the packed rows s0 .. s0 + n - 1
+  int ctx;    // its cached tokens, within the table
+};
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int b) {
+  Seq s;
+  s.s0 = a.p.start[b];
+  s.n = a.p.start[b + 1] - s.s0;
+  if (s.s0 < 0 || s.n < 0 || s.s0 > a.p.N - s.n) s.n = 0;  // not a range of packed rows
+  s.ctx = min(max(a.p.ctx[b], 0), a.p.cols << a.p.shift);
+  return s;
+}
+// The splits of a sequence with `tiles` key tiles that hold any (split 0 holds the new tokens too).
+__device__ __forceinline__ int splits_of(const AttnArgs& a, int tiles) {
+  return max(1, min((tiles + a.chunk - 1) / a.chunk, a.nsplit));
+}
+
+__device__ __forceinline__ uint32_t fin_bf16x2(uint32_t w) {  // infinities and NaN -> 0
+  uint32_t r = w;
+  if ((w & 0x7f80u) == 0x7f80u) r &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) r &= 0xffffu;
+  return r;
+}
+// 1 where a bf16 of the pair is NaN or the infinity of this sign (0: positive), else 0
+__device__ __forceinline__ uint32_t inf_bf16x2(uint32_t w, uint32_t sign) {
+  uint32_t r = 0;
+  const uint32_t lo = w & 0xffffu, hi = w >> 16;
+  if ((lo & 0x7fffu) > 0x7f80u || lo == (0x7f80u | sign)) r |= 0x3f80u;
+  if ((hi & 0x7fffu) > 0x7f80u || hi == (0x7f80u | sign)) r |= 0x3f800000u;
+  return r;
+}
+__device__ __forceinline__ v4u fin_bf16x8(v4u w) {
+  return v4u{fin_bf16x2(w[0]), fin_bf16x2(w[1]), fin_bf16x2(w[2]), fin_bf16x2(w[3])};
+}
+__device__ __forceinline__ v4u inf_bf16x8(v4u w, uint32_t s) {
+  return v4u{inf_bf16x2(w[0], s), inf_bf16x2(w[1], s), inf_bf16x2(w[2], s), inf_bf16x2(w[3], s)};
+}
+__device__ __forceinline__ bool any_inf_bf16x8(v4u w) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = od_absmax_bf16x2(m, w[i]);
+  return (m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u;
+}
+
+// 4 int8 -> 4 exact bf16: |q| <= 128 has at most 8 significant bits, so the top half of the fp32 value is it
+__device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t f0 = __float_as_uint((float)(int8_t)(w & 0xffu)), f1 = __float_as_uint((float)(int8_t)((w >> 8) & 0xffu));
+  const uint32_t f2 = __float_as_uint((float)(int8_t)((w >> 16) & 0xffu)), f3 = __float_as_uint((float)(int8_t)(w >> 24));
+  lo = __builtin_amdgcn_perm(f1, f0, 0x07060302u);
+  hi = __builtin_amdgcn_perm(f3, f2, 0x07060302u);
+}
+
+// ------------------------------------------------------------------------------------------ few slots: streaming
+// Up to 16 slots of a (sequence, KV head): decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of int8 K and V: bound by
+// reading the pages. A wave holds all 16 slots as the columns of V_MFMA_F32_16X16X32_BF16 and takes 32-key tiles straight
+// from memory into registers; the waves of a workgroup take every NW-th tile of the split's range and merge in LDS.
+// Lane (j, g) = (lane % 16, lane / 16):
+//  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: k-step ks takes the dims g D / 4 + 8 ks .. + 7 on both sides (a
+//    permutation of the reduction index), so a lane reads D / 4 contiguous values of its keys; int8 values enter as exact
+//    bf16 integers and the score takes the fp32 factor ks_j. The result gives lane (j, g) slot j and keys 16 kr + 4 g + i;
+//  * O^T[dt] += V^T[dt] P^T with output row r of d tile dt being d = (D / 16) r + dt and the keys in the order 4 g + i (i < 4),
+//    12 + 4 g + i: the B operand is the lane's own 8 probabilities, the A operand value dt of the D / 16 contiguous values it
+//    reads of each of those keys. P (times vs_j) enters as bf16 hi + lo parts, 16 significant bits: the columns of the
+//    matrix instructions are mostly empty here, and no scale of the values can leave the range.
+// Half tiles are reached through buffer descriptors of their own (a half tile never crosses a page), whose length ends at
+// the last cached token: what lies behind reads as zeros. K of the next tile is asked for when this tile's scores are
+// done, V when its products are, into the same registers: with 4 waves a SIMD some 100 KB a CU are in flight.
 template <int D, bool Q8>
-__global__ __launch_bounds__(64) void paged_attn_rows_kernel(AttnArgs a) {
-  constexpr int C = D / 64;
-  __shared__ float sq[D];
-  const Paged& p = a.p;
-  const int n = blockIdx.x, head = blockIdx.y, g = head / a.rep, lane = threadIdx.x;
-  int b = seq_search(p.start, p.B, n);
-  if (p.start[b] > n || p.start[b + 1] <= n) return;
-  const int i = n - p.start[b], s0 = p.start[b];
-  const int64_t ctx = min((int64_t)max(p.ctx[b], 0), (int64_t)p.cols << p.shift);
-  const int begin = a.row_begin ? max(a.row_begin[n], 0) : 0;
-  for (int d = lane; d < D; d += 64) sq[d] = od_bf16_to_f32(a.q[n * a.sqt + head * a.sqh + d]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, o[C];
+struct STile {
+  static constexpr int KW = D / 4 * (Q8 ? 1 : 2) / 16;  // 16-byte loads of a key's D / 4 values
+  static constexpr int VB = D / 16 * (Q8 ? 1 : 2);      // bytes of a key's D / 16 values: 4, 8, 16 or 32
+  v4u k[2][KW];
+  uint32_t v[8][VB / 4];
+  float ks, vs;  // lane l: the scales of key l % 32
+};
+__device__ __forceinline__ int s_key(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
+
+constexpr int kOnce = 2;  // non-temporal: each byte is read once
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+}
+
+// The two half tiles of the tile at position kb: first rows and lengths (0: none).
+struct STileAt {
+  int64_t row[2];
+  int len[2];
+};
+__device__ __forceinline__ STileAt s_at(const AttnArgs& a, const Seq& s, int b, int g, int kb) {
+  STileAt t;
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = 0.0f;
-  const int64_t total = ctx + (a.k ? i + 1 : 0);
-  for (int64_t j0 = 0; j0 < total; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const int64_t row = j < ctx ? row_of(p, b, g, j) : -1;
-    const bool cached = row >= 0, own = j >= ctx && j < total && j - ctx >= begin;
-    float y = -INFINITY;
-    if (cached || own) {
-      float s = 0.0f;
-      if (cached && Q8) {
-        const int8_t* kr = static_cast<const int8_t*>(p.k) + row * D;
-        for (int d = 0; d < D; ++d) s = fmaf(sq[d], (float)kr[d], s);
-        s *= p.ks[row];
+  for (int r = 0; r < 2; ++r) {
+    const int pos = kb + 16 * r;
+    const int64_t row = pos < s.ctx ? uniform_row_of(a.p, b, g, pos) : -1;
+    t.row[r] = row < 0 ? 0 : row;
+    t.len[r] = row < 0 ? 0 : min(16, s.ctx - pos);
+  }
+  return t;
+}
+template <int D, bool Q8>
+__device__ __forceinline__ void s_load_k(const AttnArgs& a, const STileAt& t, STile<D, Q8>& x) {
+  constexpr int E = Q8 ? 1 : 2;
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const auto d = rsrc(static_cast<const char*>(a.p.k) + t.row[r] * (D * E), t.len[r] * (D * E));
+#pragma unroll
+    for (int w = 0; w < STile<D, Q8>::KW; ++w)
+      x.k[r][w] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, (j * D + g * (D / 4)) * E + 16 * w, 0, kOnce));
+  }
+}
+template <int D, bool Q8>
+__device__ __forceinline__ void s_load_v(const AttnArgs& a, const STileAt& t, STile<D, Q8>& x) {
+  constexpr int E = Q8 ? 1 : 2, VB = STile<D, Q8>::VB;
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const auto d = rsrc(static_cast<const char*>(a.p.v) + t.row[r] * (D * E), t.len[r] * (D * E));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = (4 * g + i) * D * E + j * VB;
+      if constexpr (VB == 4) {
+        x.v[4 * r + i][0] = __builtin_amdgcn_raw_buffer_load_b32(d, at, 0, kOnce);
+      } else if constexpr (VB == 8) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b64(d, at, 0, kOnce);
+        x.v[4 * r + i][0] = u[0];
+        x.v[4 * r + i][1] = u[1];
       } else {
-        const uint16_t* kr = cached ? static_cast<const uint16_t*>(p.k) + row * D : a.k + (s0 + j - ctx) * a.skt + g * a.skh;
-        for (int d = 0; d < D; ++d) s = fmaf(sq[d], od_bf16_to_f32(kr[d]), s);
-      }
-      y = s * a.scale_log2;
-    }
-    const float mx = od_wave_max(y), m2 = fmaxf(m, mx), ms = m2 == -INFINITY ? 0.0f : m2;
-    const float alpha = __builtin_amdgcn_exp2f(m - ms), pr = __builtin_amdgcn_exp2f(y - ms);
-    l = l * alpha + od_wave_sum_dpp(pr);
-    m = m2;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] *= alpha;
-    for (int t = 0; t < 64; ++t) {
-      const int64_t r = __shfl((long long)row, t, 64), jt = j0 + t;
-      const float pt = __shfl(pr, t, 64);
-      const int ok = __shfl((int)(cached || own), t, 64);
-      if (!ok) continue;
+        for (int w = 0; w < VB / 16; ++w) {
+          const v4u u = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, at + 16 * w, 0, kOnce));
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int d = c * 64 + lane;
-        float vv;
-        if (r >= 0 && Q8) vv = (float)static_cast<const int8_t*>(p.v)[r * D + d] * p.vs[r];
-        else vv = od_bf16_to_f32(r >= 0 ? static_cast<const uint16_t*>(p.v)[r * D + d] : a.v[(s0 + jt - ctx) * a.svt + g * a.svh + d]);
-        o[c] = fmaf(pt, vv, o[c]);
+          for (int c = 0; c < 4; ++c) x.v[4 * r + i][4 * w + c] = u[c];
+        }
       }
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+}
+// lane l: the scales of key l % 32 (each half of 16 lanes its half tile's)
+__device__ __forceinline__ void s_load_scales(const AttnArgs& a, const STileAt& t, float& ks, float& vs) {
+  const int c = threadIdx.x & 31, r = c >> 4;
+  const bool in = (c & 15) < (r ? t.len[1] : t.len[0]);
+  const int64_t at = (r ? t.row[1] : t.row[0]) + (c & 15);
+  ks = in ? a.p.ks[at] : 0.0f;
+  vs = in ? a.p.vs[at] : 0.0f;
+}
+
+__device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The slot state of a lane: column j's running max and its share of the sum, output rows 4 g + i of every d tile.
+template <int D>
+struct SAcc {
+  float m, l;
+  v4f o[D / 16];
+};
+
+// One tile's online softmax into bf16 hi and lo parts: y the lane's 8 scores (log2 units, -inf masked), f a factor on p for
+// the P.V product only (the V scales).
+template <int D, bool F>
+__device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
+  float mx = y[0];
 #pragma unroll
-  for (int c = 0; c < C; ++c) a.out[n * a.sot + head * a.soh + c * 64 + lane] = od_f32_to_bf16(l == 0.0f ? 0.0f : o[c] * inv);
-  if (a.lse && lane == 0) a.lse[(int64_t)n * a.Hq + head] = (m + __log2f(l)) * kLn2;
+  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, y[i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = od_xor32_max(mx);
+  const bool move = mx > x.m + kSlack;
+  if (__builtin_amdgcn_ballot_w64(move) != 0) {
+    const float c = move ? __builtin_amdgcn_exp2f(x.m - mx) : 1.0f;  // m = -inf: 0
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.o[dt][i] *= c;
+    x.l *= c;
+    if (move) x.m = mx;
+  }
+  const float ms = x.m == -INFINITY ? 0.0f : x.m;
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(y[i] - ms);
+    x.l += p[i];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float u = F ? p[2 * e] * f[2 * e] : p[2 * e], w = F ? p[2 * e + 1] * f[2 * e + 1] : p[2 * e + 1];
+    hi[e] = od_pack_bf16x2(u, w);
+    lo[e] = od_pack_bf16x2(u - __uint_as_float(hi[e] << 16), w - __uint_as_float(hi[e] & 0xffff0000u));
+  }
+}
+
+// value dt of each of the lane's 8 keys, as the bf16 A operand
+template <int D, bool Q8>
+__device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[8][STile<D, Q8>::VB / 4], int dt) {
+  v4u r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (Q8) {
+      const uint32_t a = v[2 * e][dt / 4], b = v[2 * e + 1][dt / 4];
+      const int sh = 8 * (dt % 4);
+      r[e] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(b >> sh)), __float_as_uint((float)(int8_t)(a >> sh)), 0x07060302u);
+    } else {
+      r[e] = __builtin_amdgcn_perm(v[2 * e + 1][dt / 2], v[2 * e][dt / 2], dt % 2 ? 0x07060302u : 0x05040100u);
+    }
+  }
+  return r;
+}
+
+constexpr int s_waves(int D) { return D == 256 ? 4 : 8; }  // the merge holds every wave's 16 x D outputs in LDS
+
+template <int D, bool Q8>
+__global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void paged_stream_kernel(AttnArgs a) {
+  constexpr int NW = s_waves(D), KS = D / 32, QR = D + 8;  // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
+  __shared__ __attribute__((aligned(16))) union {
+    uint16_t q[16 * QR];
+    float o[NW][16][D + 4];
+  } sm;
+  __shared__ float sml[NW][2][16];
+  __shared__ float4 skf[NW][2][8];  // a tile's per-key factors, from lane order to score order (one wave writes and reads)
+  const int sp = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const Seq s = seq_of(a, b);
+  const int tiles = (s.ctx + 31) >> 5, nv = splits_of(a, tiles);
+  if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
+  const int t_lo = sp * a.chunk, t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = lane & 15, qd = lane >> 4, c = lane & 31;
+  for (int z0 = 0; z0 < s.n * a.rep; z0 += 16) {  // one round unless max_new was too small
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 8); i += NW * 64) {
+      const int z = z0 + i / (D / 8), d0 = (i % (D / 8)) * 8;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (z < s.n * a.rep)
+        w = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt + (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
+      *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + d0) = w;
+    }
+    __syncthreads();
+    auto qfrag = [&](int ks) {
+      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + j * QR + qd * (D / 4) + 8 * ks));
+    };
+    SAcc<D> x;
+    x.m = -INFINITY;
+    x.l = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
+
+    int tt = t_lo + wave;
+    if (tt < t_hi) {
+      STile<D, Q8> tl;
+      STileAt at = s_at(a, s, b, g, tt * 32);
+      s_load_k<D, Q8>(a, at, tl);
+      if constexpr (Q8) s_load_scales(a, at, tl.ks, tl.vs);
+      s_load_v<D, Q8>(a, at, tl);
+      for (; tt < t_hi; tt += NW) {
+        const int nx = tt + NW < t_hi ? tt + NW : tt;
+        const STileAt next = s_at(a, s, b, g, nx * 32);
+        if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
+          reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
+          reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
+        }
+        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            v4u k8;
+            if constexpr (Q8) {
+              uint32_t w[4];
+              i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1)], w[0], w[1]);
+              i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1) + 1], w[2], w[3]);
+              k8 = v4u{w[0], w[1], w[2], w[3]};
+            } else {
+              k8 = tl.k[r][ks];
+            }
+            sc[r] = mfma16(k8, qfrag(ks), sc[r]);
+          }
+        s_load_k<D, Q8>(a, next, tl);
+        float y[8], f[8];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float4 kf = Q8 ? skf[wave][0][4 * r + qd] : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
+          const float4 vf = Q8 ? skf[wave][1][4 * r + qd] : make_float4(1, 1, 1, 1);
+          const float kk[4] = {kf.x, kf.y, kf.z, kf.w}, vv[4] = {vf.x, vf.y, vf.z, vf.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[4 * r + i] = sc[r][i] * kk[i];
+            f[4 * r + i] = vv[i];
+          }
+        }
+        if (at.len[0] + at.len[1] != 32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (4 * qd + (i & 3) >= at.len[i >> 2]) y[i] = -INFINITY;
+        }
+        if constexpr (Q8) s_load_scales(a, next, tl.ks, tl.vs);
+        v4u hi, lo;
+        s_softmax<D, Q8>(y, f, x, hi, lo);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          const v4u v8 = s_vfrag<D, Q8>(tl.v, dt);
+          x.o[dt] = mfma16(v8, hi, x.o[dt]);
+          x.o[dt] = mfma16(v8, lo, x.o[dt]);
+        }
+        s_load_v<D, Q8>(a, next, tl);
+        at = next;
+      }
+    }
+
+    // the new tokens: tiles of 32 bf16 keys, in split 0
+    if (sp == 0 && a.k) {
+      const int z = z0 + j, tok = min(z / a.rep, s.n - 1);
+      const int begin = a.row_begin ? max(a.row_begin[s.s0 + tok], 0) : 0;
+      const int t_end = min((z0 + 15) / a.rep, s.n - 1);  // last token of these slots
+      for (int k0 = 32 * wave; k0 <= t_end; k0 += 32 * NW) {
+        const int left = min(32, s.n - k0);
+        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int key = min(16 * r + j, left - 1);
+          const uint16_t* kp = a.k + (int64_t)(s.s0 + k0 + key) * a.skt + (int64_t)g * a.skh + qd * (D / 4);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            sc[r] = mfma16(__builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + 8 * ks)), qfrag(ks), sc[r]);
+        }
+        float y[8], f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = k0 + s_key(qd, i);
+          y[i] = z < s.n * a.rep && key >= begin && key <= tok ? sc[i >> 2][i & 3] * a.scale_log2 : -INFINITY;
+          f[i] = 1.0f;
+        }
+        uint32_t v[8][D / 32];
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = min(s_key(qd, i), left - 1);
+          const uint16_t* vp = a.v + (int64_t)(s.s0 + k0 + key) * a.svt + (int64_t)g * a.svh + j * (D / 16);
+          if constexpr (D == 64) {
+            const uint2 u = *reinterpret_cast<const uint2*>(vp);
+            v[i][0] = u.x;
+            v[i][1] = u.y;
+          } else {
+#pragma unroll
+            for (int w = 0; w < D / 128; ++w) {
+              const uint4 u = *reinterpret_cast<const uint4*>(vp + 8 * w);
+              v[i][4 * w] = u.x;
+              v[i][4 * w + 1] = u.y;
+              v[i][4 * w + 2] = u.z;
+              v[i][4 * w + 3] = u.w;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) odd |= fin_bf16x2(v[i][w]) != v[i][w];
+        }
+        v4u hi, lo;
+        s_softmax<D, false>(y, f, x, hi, lo);
+        if (__builtin_amdgcn_ballot_w64(odd) == 0) {
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) {
+            const v4u v8 = s_vfrag<D, false>(v, dt);
+            x.o[dt] = mfma16(v8, hi, x.o[dt]);
+            x.o[dt] = mfma16(v8, lo, x.o[dt]);
+          }
+        } else {  // infinities or NaN among the values: 0 times one must not reach a slot that does not see it
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) {
+            const v4u v8 = s_vfrag<D, false>(v, dt), fin = fin_bf16x8(v8);
+            x.o[dt] = mfma16(fin, hi, x.o[dt]);
+            x.o[dt] = mfma16(fin, lo, x.o[dt]);
+            const v4f pos = mfma16(inf_bf16x8(v8, 0), hi, v4f{0, 0, 0, 0}), neg = mfma16(inf_bf16x8(v8, 0x8000u), hi, v4f{0, 0, 0, 0});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.o[dt][i] += (pos[i] > 0.0f ? INFINITY : 0.0f) + (neg[i] > 0.0f ? -INFINITY : 0.0f);
+          }
+        }
+      }
+    }
+
+    // merge the waves, then the output or this split's normalized partial
+    float l = x.l + __shfl_xor(x.l, 16, 64);
+    l = od_xor32_sum(l);
+    __syncthreads();  // every wave is done with the queries
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d4 = 0; d4 < D / 64; ++d4)
+        *reinterpret_cast<float4*>(&sm.o[wave][j][(4 * qd + i) * (D / 16) + 4 * d4]) =
+            make_float4(x.o[4 * d4][i], x.o[4 * d4 + 1][i], x.o[4 * d4 + 2][i], x.o[4 * d4 + 3][i]);
+    if (qd == 0) {
+      sml[wave][0][j] = x.m;
+      sml[wave][1][j] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+      const int zz = i / (D / 4), d0 = (i % (D / 4)) * 4, z = z0 + zz;
+      if (z >= s.n * a.rep) continue;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][0][zz]);
+      float L = 0.0f;
+      float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = sml[w][0][zz];
+        const float e = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+        const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][zz][d0]);
+        L += e * sml[w][1][zz];
+        acc.x += e * v.x;
+        acc.y += e * v.y;
+        acc.z += e * v.z;
+        acc.w += e * v.w;
+      }
+      // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L);
+      const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (nv == 1) {
+        *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(acc.x, acc.y), od_pack_bf16x2(acc.z, acc.w));
+        if (a.lse && d0 == 0) a.lse[n * a.Hq + head] = ls * kLn2;
+      } else {
+        const int64_t slot = ((int64_t)sp * a.p.N + n) * a.Hq + head;
+        *reinterpret_cast<float4*>(a.part + slot * D + d0) = acc;
+        if (d0 == 0) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + slot] = ls;
+      }
+    }
+  }
+}
+
+// The splits of a sequence's slots merged by log-sum-exp: a wave per packed row and 64 / (D / 8) heads. `width`: keys per tile.
+template <int D>
+__global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int width) {
+  constexpr int G = D / 8, HW = 64 / G;
+  const int n = blockIdx.x, lane = threadIdx.x & 63;
+  const int head = (blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6)) * HW + lane / G, d0 = (lane % G) * 8;
+  const int b = seq_search(a.p.start, a.p.B, n);
+  const Seq s = seq_of(a, b);
+  const int nv = splits_of(a, (s.ctx + width - 1) / width);
+  if (n < s.s0 || n >= s.s0 + s.n || nv == 1 || head >= a.Hq) return;
+  const int64_t slot = (int64_t)n * a.Hq + head, step = (int64_t)a.p.N * a.Hq;
+  const float* ls = a.part + (int64_t)a.nsplit * step * D;
+  float M = -INFINITY, L = 0.0f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  // one pass with a running max, unrolled: several splits' loads are in flight together
+#pragma unroll 4
+  for (int sp = 0; sp < nv; ++sp) {
+    const float l = ls[sp * step + slot];
+    const float4* po = reinterpret_cast<const float4*>(a.part + (sp * step + slot) * D + d0);
+    const float4 u = po[0], w = po[1];
+    if (l == -INFINITY) continue;  // a split that sees nothing
+    if (l > M) {
+      const float r = __builtin_amdgcn_exp2f(M - l);
+      L *= r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= r;
+      M = l;
+    }
+    const float f = __builtin_amdgcn_exp2f(l - M);
+    L += f;
+    acc[0] += f * u.x; acc[1] += f * u.y; acc[2] += f * u.z; acc[3] += f * u.w;
+    acc[4] += f * w.x; acc[5] += f * w.y; acc[6] += f * w.z; acc[7] += f * w.w;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<uint4*>(a.out + n * a.sot + head * a.soh + d0) =
+      make_uint4(od_pack_bf16x2(acc[0] * inv, acc[1] * inv), od_pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                 od_pack_bf16x2(acc[4] * inv, acc[5] * inv), od_pack_bf16x2(acc[6] * inv, acc[7] * inv));
+  if (a.lse && d0 == 0) a.lse[slot] = (M + __log2f(L)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------------------ many slots: tiles
+// Chunks and option rows: bound by the matrix cores and the softmax's vector work. A workgroup of NW waves owns 32 slots per
+// wave of one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'. Scores are taken
+// transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so that a slot's softmax is
+// lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them; V^T comes from row-major LDS
+// by transposing reads. At D = 256 a wave accumulates 128 of the value columns and two waves share 32 slots (each takes the
+// scores again): 256 columns of accumulators beside 256-wide queries do not fit its registers.
+//
+// int8 blocks are converted once per workgroup on the way into LDS, to fp16 in power-of-two frames: K' = fp16(q ks_j 2^(7 - E))
+// with 2^E above the block's largest scale, V' = fp16(q vs_j 2^(7 - F)) with 2^F above the largest so far (the accumulator
+// moves along when F rises), queries as fp16 q 2^(14 - e) with 2^e above the slot's largest (exact while they are normal).
+// One rounding of 2^-11 at most for every cached value, far below the 2^-8 of their int8 grid, and the scores' factor
+// 2^(e - 14 + E - 7) is one number per slot and block. Probabilities are fp16 there, kept 2^7 above what they are (2^15 at
+// most under kSlack), so that one as small as 2^-31 of the largest still counts. bf16 pages and the new tokens go in as
+// they are, with bf16 probabilities (2^-8 each, as the output's own rounding).
+//
+// The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first in the
+// next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
+constexpr int kBK = 64;
+constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
+
+template <int D>
+__device__ __forceinline__ int tk_off(int key, int chunk) {  // K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
+  return key * D + ((chunk ^ (D == 64 ? ((key >> 1) & 7) : (key & 15))) << 3);
+}
+template <int D>
+__device__ __forceinline__ int tv_chunk(int key, int chunk) {  // V rows: 4 consecutive keys' chunks of a transposing read 64 bytes apart
+  return D == 64 ? chunk ^ ((key & 2) << 1) : chunk ^ ((key & 3) << 2);
+}
+
+template <bool H>
+__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
+  if constexpr (H)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f zero16() { return v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
+
+// exponent e with x < 2^e for the bits of a finite x > 0; 0 for 0
+__device__ __forceinline__ int exp_above(uint32_t bits) { return bits ? (int)(bits >> 23) - 126 : 0; }
+
+// 16 int8 times f, each product rounded once to fp16: byte u = q + 128 becomes the fp16 1024 + u by its bits, and
+// (1024 + u) f - 1152 f is one fp32 fma per value (v_fma_mix). f has its last 4 bits clear (frame_scale), so that 1152 f is
+// exact and the result is q f rounded once, 0 for q = 0.
+__device__ __forceinline__ void i8x16_scaled(v4u w, float f, v4u& lo, v4u& hi) {
+  const float c = -1152.0f * f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = w[i] ^ 0x80808080u;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, k ? 0x04030402u : 0x04010400u));
+      const f16x2 r = {(_Float16)__builtin_fmaf((float)h.x, f, c), (_Float16)__builtin_fmaf((float)h.y, f, c)};
+      (i < 2 ? lo : hi)[2 * (i & 1) + k] = __builtin_bit_cast(uint32_t, r);
+    }
+  }
+}
+
+// s 2^e with 20 significant bits: within 2^-20 of it
+__device__ __forceinline__ float frame_scale(float s, int e) {
+  return __uint_as_float(__float_as_uint(__builtin_ldexpf(s, e)) & ~15u);
+}
+
+template <int D, int NW>
+struct alignas(16) TSmem {
+  uint16_t k[2][kBK * D];
+  uint16_t v[2][kBK * D];
+  int odd[2][NW];  // a wave found infinities or NaN among the block's new values
+  int lo[NW], hi[NW];
+};
+
+// One slot tile's constants per lane, and its state.
+template <int D>
+struct TSlot {
+  int ok, tok, head, begin;  // the slot exists; its token and head; the first new token that it sees
+  v4u q[D / 16];             // dims 16 ks + 8 h .. + 7
+  int qe;                    // fp16 queries: their exponent
+  float m, l;
+  v16f o[D == 256 ? 4 : D / 32];
+};
+
+template <int D>
+__device__ __forceinline__ void t_load_q(const AttnArgs& a, const Seq& s, TSlot<D>& t) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const uint16_t* qp = a.q + (int64_t)(s.s0 + t.tok) * a.sqt + (int64_t)t.head * a.sqh + 8 * h;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+    t.q[ks] = t.ok ? __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(qp + 16 * ks)) : v4u{0, 0, 0, 0};
+}
+// the queries as fp16 in the slot's frame
+template <int D>
+__device__ __forceinline__ void t_q_to_f16(TSlot<D>& t) {
+  uint32_t am = 0;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) am = od_absmax_bf16x2(am, t.q[ks][i]);
+  const float mx = od_xor32_max(od_absmax_bf16x2_value(am));
+  t.qe = mx < INFINITY ? exp_above(__float_as_uint(mx)) : 0;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = t.q[ks][i];
+      const f16x2 r = {(_Float16)__builtin_ldexpf(__uint_as_float(w << 16), 14 - t.qe),
+                       (_Float16)__builtin_ldexpf(__uint_as_float(w & 0xffff0000u), 14 - t.qe)};
+      t.q[ks][i] = __builtin_bit_cast(uint32_t, r);
+    }
+}
+
+// S^T of one block.
+template <int D, bool H>
+__device__ __forceinline__ void t_scores(const uint16_t* kb, const TSlot<D>& t, v16f (&s)[2]) {
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  constexpr int NQ = D / 16 * 2, RA = D == 256 ? 1 : 2;  // MFMA i: k-step i / 2, key tile i % 2; reads run RA ahead
+  s[0] = zero16();
+  s[1] = zero16();
+  v4u kf[RA + 1];
+  auto rd = [&](int i) {
+    kf[i % (RA + 1)] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(&kb[tk_off<D>((i % 2) * 32 + col, (i / 2) * 2 + h)]));
+  };
+#pragma unroll
+  for (int i = 0; i < RA; ++i) rd(i);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    if (i + RA < NQ) rd(i + RA);
+    s[i % 2] = mfma32<H>(kf[i % (RA + 1)], t.q[i / 2], s[i % 2]);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    if (i + RA < NQ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+  }
+}
+
+// The block's online softmax into P; c > 0: the scores' factor (log2 units), masked scores -inf.
+template <int D, bool H>
+__device__ __forceinline__ void t_softmax(v16f (&s)[2], float c, TSlot<D>& t, v4u (&pb)[4]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+  mx = od_xor32_max(mx) * c;
+  const bool move = mx > t.m + kSlack;
+  if (__builtin_amdgcn_ballot_w64(move) != 0) {
+    const float f = move ? __builtin_amdgcn_exp2f(t.m - mx) : 1.0f;  // m = -inf: 0
+#pragma unroll
+    for (auto& o : t.o)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[r] *= f;
+    t.l *= f;
+    if (move) t.m = mx;
+  }
+  const float ms = (t.m == -INFINITY ? 0.0f : t.m) - kLift;
+  float sum = 0.0f;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], c, -ms));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r + 1], c, -ms));
+      sum += p0;
+      sum += p1;
+      if constexpr (H) {
+        const f16x2 w = {(_Float16)p0, (_Float16)p1};
+        pb[kt * 2 + (r >> 3)][(r & 7) >> 1] = __builtin_bit_cast(uint32_t, w);
+      } else {
+        pb[kt * 2 + (r >> 3)][(r & 7) >> 1] = od_pack_bf16x2(p0, p1);
+      }
+    }
+  t.l += sum;  // this lane's share: keys of its half
+}
+
+// The A operand for value rows of d tile dt (vb: the lane's base there), keys 16 kk + 8 (i / 4) + 4 (lane / 32) + i % 4.
+template <int D>
+__device__ __forceinline__ v4u t_vfrag(const uint16_t* vblk, int vb, int kk) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  uint16_t* base = const_cast<uint16_t*>(vblk) + vb + kk * 16 * D;
+  const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)base);
+  const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(base + 8 * D));
+  return __builtin_bit_cast(v4u, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int D, bool H>
+__device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[D == 256 ? 4 : D / 32], const v4u (&pb)[4], TSlot<D>& t) {
+  constexpr int DT = D == 256 ? 4 : D / 32, NV = 4 * DT, RA = D == 256 ? 1 : 2;  // MFMA i: k-step i / DT, d tile i % DT
+  v4u vf[RA + 1];
+  auto rd = [&](int i) { vf[i % (RA + 1)] = t_vfrag<D>(vblk, vb[i % DT], i / DT); };
+#pragma unroll
+  for (int i = 0; i < RA; ++i) rd(i);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i + RA < NV) rd(i + RA);
+    t.o[i % DT] = mfma32<H>(vf[i % (RA + 1)], pb[i / DT], t.o[i % DT]);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x100, RA * 2, 0);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i + RA < NV) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+  }
+}
+// The same with infinities or NaN among the values: finite parts as usual, and the slots that see an infinity or NaN found
+// by products with 0 / 1 matrices, since 0 times one would reach the slots that do not.
+template <int D>
+__device__ __forceinline__ void t_values_odd(const uint16_t* vblk, const int (&vb)[D == 256 ? 4 : D / 32], const v4u (&pb)[4], TSlot<D>& t) {
+#pragma unroll
+  for (int dt = 0; dt < (D == 256 ? 4 : D / 32); ++dt) {
+    __builtin_amdgcn_sched_barrier(0);  // one d tile's operands at a time: this path must not cost the usual one registers
+    v16f pos = zero16(), neg = zero16();
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const v4u w = t_vfrag<D>(vblk, vb[dt], kk);
+      t.o[dt] = mfma32<false>(fin_bf16x8(w), pb[kk], t.o[dt]);
+      pos = mfma32<false>(inf_bf16x8(w, 0), pb[kk], pos);
+      neg = mfma32<false>(inf_bf16x8(w, 0x8000u), pb[kk], neg);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t.o[dt][r] += (pos[r] > 0.0f ? INFINITY : 0.0f) + (neg[r] > 0.0f ? -INFINITY : 0.0f);
+  }
+}
+
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
+  constexpr int NT = NW * 64, HALVES = D == 256 ? 2 : 1, SPT = 32 * NW / HALVES, DT = D == 256 ? 4 : D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
+  // work item -> (sequence, KV head, split, slot tile), tiles fastest: workgroups are dealt round-robin over the 8 XCDs, and
+  // each takes a contiguous range of the items, so that the slot tiles of one (sequence, head) read its keys through one L2
+  const int total = gridDim.x, per = total >> 3, rem = total & 7, xcd = blockIdx.x & 7, loc = blockIdx.x >> 3;
+  int w = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+  const int tile0 = w % a.tiles;
+  w /= a.tiles;
+  const int sp = w % a.nsplit;
+  w /= a.nsplit;
+  const int g = w % a.p.Hkv, b = w / a.p.Hkv;
+  const Seq s = seq_of(a, b);
+  const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
+  if (sp >= nv) return;
+  const int b_lo = sp * a.chunk, b_hi = sp == a.nsplit - 1 ? blocks : min(blocks, b_lo + a.chunk);
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave / (NW / HALVES);
+  int vb[DT];  // transposing-read bases
+  {
+    const int hh = lane >> 5, mh = (lane >> 4) & 1, e = (lane >> 2) & 3, c = lane & 3;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
+  }
+
+  for (int tile = tile0; tile * SPT < nslots; tile += a.tiles) {
+    __syncthreads();  // an earlier tile's readers are done
+    TSlot<D> t;
+    const int zw = tile * SPT + (wave % (NW / HALVES)) * 32, z = zw + col;
+    const bool live = zw < nslots;  // the wave has slots
+    t.ok = z < nslots;
+    t.tok = t.ok ? z / a.rep : s.n - 1;
+    t.head = g * a.rep + (t.ok ? z % a.rep : 0);
+    t.begin = a.row_begin && t.ok ? max(a.row_begin[s.s0 + t.tok], 0) : 0;
+    t.m = -INFINITY;
+    t.l = 0.0f;
+    t.qe = 0;
+#pragma unroll
+    for (auto& o : t.o) o = zero16();
+    t_load_q<D>(a, s, t);
+    int frame = 0;  // O is in units of 2^frame
+
+    // ---- the cached blocks b_lo .. b_hi - 1
+    if (b_lo < b_hi) {
+      if constexpr (Q8) t_q_to_f16<D>(t);
+      constexpr int E = Q8 ? 1 : 2;
+      constexpr int CPK = D * E / 16, CH = kBK * CPK, NC = 2 * CH / NT;  // 16-byte chunks per row, per side; per thread (K, then V)
+      v4u r[NC];
+      int pg = -1;             // lane l: the page of key l of the block whose loads come next
+      float ks = 0, vs = 0;    // lane l: the scales of key l of the loaded block
+      uint64_t there = 0;      // the loaded block's keys that exist
+      int pg_of = -1;          // the loaded block's pages
+      auto pages = [&](int blk) {
+        const int pos = blk * kBK + lane;
+        pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
+        if (pg >= a.p.n_pages) pg = -1;
+      };
+      auto load = [&](int blk) {
+        there = __builtin_amdgcn_ballot_w64(pg >= 0);
+        pg_of = pg;
+        const int mask = (1 << a.p.shift) - 1;
+        if constexpr (Q8) {
+          const int64_t at = (((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & mask);
+          ks = a.p.ks[at];
+          vs = a.p.vs[at];
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+          const int64_t row = (((int64_t)max(__shfl(pg, key, 64), 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + key) & mask);
+          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) + row * (D * E) + 16 * ch));
+        }
+      };
+      int kexp = 0, vexp = 0;  // the stored block's frames
+      bool vexp_set = false;
+      uint64_t seen = 0;
+      auto store = [&](int buf) {
+        seen = there;
+        float kf = 0, vf = 0;
+        if constexpr (Q8) {
+          // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not finite,
+          // leave them alone
+          const bool on = pg_of >= 0;
+          const uint32_t kb = on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u, vb2 = on && vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u;
+          kexp = exp_above(od_wave_umax_dpp(kb));
+          const uint32_t vm = od_wave_umax_dpp(vb2);
+          if (vm) vexp = vexp_set ? max(vexp, exp_above(vm)) : exp_above(vm);
+          if (vm) vexp_set = true;
+          kf = on ? frame_scale(ks, 7 - kexp) : 0.0f;
+          vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+          uint16_t* dst = side ? sm.v[buf] : sm.k[buf];
+          if constexpr (Q8) {
+            v4u lo, hi;
+            i8x16_scaled(r[i], __shfl(side ? vf : kf, key, 64), lo, hi);
+            const int o0 = side ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
+            const int o1 = side ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
+            *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
+            *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
+          } else {
+            const v4u x = (there >> key) & 1 ? r[i] : v4u{0, 0, 0, 0};
+            *reinterpret_cast<uint4*>(dst + (side ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch))) = __builtin_bit_cast(uint4, x);
+          }
+        }
+      };
+      pages(b_lo);
+      load(b_lo);
+      pages(b_lo + 1);
+      store(0);
+      if (b_lo + 1 < b_hi) {
+        load(b_lo + 1);
+        pages(b_lo + 2);
+      }
+      __syncthreads();
+      for (int blk = b_lo; blk < b_hi; ++blk) {
+        const int cur = (blk - b_lo) & 1;
+        const float c = Q8 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
+        const int f_new = Q8 ? vexp - 7 : 0;
+        const uint64_t mask = seen;
+        if (blk + 1 < b_hi) {
+          store(cur ^ 1);
+          if (blk + 2 < b_hi) {
+            load(blk + 2);
+            pages(blk + 3);
+          }
+        }
+        if (Q8 && f_new != frame) {  // the values' frame rose: uniform over the workgroup
+          const float f = __builtin_ldexpf(1.0f, frame - f_new);
+#pragma unroll
+          for (auto& o : t.o)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= f;
+          frame = f_new;
+        }
+        if (live) {
+          v16f sc[2];
+          v4u pb[4];
+          t_scores<D, Q8>(sm.k[cur], t, sc);
+          if (mask != ~0ull) {
+            const uint64_t m4 = mask >> (4 * h);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (!((m4 >> (kt * 32 + 8 * (i >> 2) + (i & 3))) & 1)) sc[kt][i] = -INFINITY;
+          }
+          t_softmax<D, Q8>(sc, c, t, pb);
+          t_values<D, Q8>(sm.v[cur], vb, pb, t);
+        }
+        __syncthreads();
+      }
+    }
+
+    // ---- the new tokens, in split 0
+    if (sp == 0 && a.k) {
+      if (Q8 && b_lo < b_hi) {  // back to bf16 queries and values as they are
+        t_load_q<D>(a, s, t);
+        if (frame != 0) {
+          const float f = __builtin_ldexpf(1.0f, frame);
+#pragma unroll
+          for (auto& o : t.o)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= f;
+          frame = 0;
+        }
+      }
+      // what the wave's slots see: tokens w_lo .. w_hi at most; all of them see all of w_in .. w_tok
+      const int w_tok = min(zw / a.rep, s.n - 1), w_hi = min((zw + 31) / a.rep, s.n - 1);
+      int w_lo = 0, w_in = 0;
+      if (a.row_begin) {
+        w_lo = t.ok ? t.begin : 0x7fffffff;
+        w_in = t.begin;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+          w_lo = min(w_lo, __shfl_xor(w_lo, o, 64));
+          w_in = max(w_in, __shfl_xor(w_in, o, 64));
+        }
+      }
+      w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+      w_in = __builtin_amdgcn_readfirstlane(w_in);
+      if (lane == 0) {
+        sm.lo[wave] = live ? w_lo : 0x7fffffff;
+        sm.hi[wave] = live ? w_in : 0;
+      }
+      __syncthreads();
+      int g_lo = 0x7fffffff, g_in = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        g_lo = min(g_lo, sm.lo[i]);
+        g_in = max(g_in, sm.hi[i]);
+      }
+      const int g_tok = min(tile * SPT / a.rep, s.n - 1), g_hi = min((tile * SPT + SPT - 1) / a.rep, s.n - 1);
+      const int o_lo = min(g_lo, g_hi + 1) / kBK, o_hi = g_hi / kBK + 1;
+      constexpr int CPK = D / 8, CH = kBK * CPK, NC = 2 * CH / NT;
+      v4u r[NC];
+      auto load = [&](int blk) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int cid = i * NT + tid, side = cid / CH, key = min(blk * kBK + cid % CH / CPK, s.n - 1), ch = cid % CPK;
+          const uint16_t* src = side ? a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh : a.k + (int64_t)(s.s0 + key) * a.skt + (int64_t)g * a.skh;
+          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(src + 8 * ch));
+        }
+      };
+      // a block that some slot of the workgroup sees only a part of
+      auto partial = [&](int blk) { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; };
+      auto store = [&](int blk, int buf) {
+        bool odd = false;
+        const bool part = partial(blk);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+          *reinterpret_cast<uint4*>((side ? sm.v[buf] : sm.k[buf]) + (side ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch))) =
+              __builtin_bit_cast(uint4, r[i]);
+          if (part && side) odd |= any_inf_bf16x8(r[i]);
+        }
+        if (part) {
+          const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+          if (lane == 0) sm.odd[buf][wave] = any;
+        }
+      };
+      if (o_lo < o_hi) {
+        load(o_lo);
+        __syncthreads();
+        store(o_lo, 0);
+        if (o_lo + 1 < o_hi) load(o_lo + 1);
+        __syncthreads();
+        for (int blk = o_lo; blk < o_hi; ++blk) {
+          const int cur = (blk - o_lo) & 1, j0 = blk * kBK;
+          if (blk + 1 < o_hi) {
+            store(blk + 1, cur ^ 1);
+            if (blk + 2 < o_hi) load(blk + 2);
+          }
+          if (live && j0 <= w_hi && j0 + kBK > w_lo) {
+            v16f sc[2];
+            v4u pb[4];
+            t_scores<D, false>(sm.k[cur], t, sc);
+            if (j0 + kBK - 1 > w_tok || j0 < w_in) {
+#pragma unroll
+              for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const int key = j0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+                  if (key > t.tok || key < t.begin) sc[kt][i] = -INFINITY;
+                }
+            }
+            t_softmax<D, false>(sc, a.scale_log2, t, pb);
+            int odd = 0;
+            if (partial(blk)) {
+#pragma unroll
+              for (int i = 0; i < NW; ++i) odd |= sm.odd[cur][i];
+            }
+            if (__builtin_amdgcn_readfirstlane(odd) == 0) t_values<D, false>(sm.v[cur], vb, pb, t);
+            else t_values_odd<D>(sm.v[cur], vb, pb, t);
+          }
+          __syncthreads();
+        }
+      }
+    }
+
+    // ---- out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
+    const float l = od_xor32_sum(t.l);
+    if (t.ok) {
+      const float inv = l == 0.0f ? 0.0f : __builtin_ldexpf(1.0f / l, frame), ls = t.m + __log2f(l) - kLift;
+      const int64_t n = s.s0 + t.tok;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const int d0 = half * 128 + dt * 32 + 8 * i4 + 4 * h;
+          const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv, t.o[dt][4 * i4 + 3] * inv);
+          if (nv == 1)
+            *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y), od_pack_bf16x2(y.z, y.w));
+          else
+            *reinterpret_cast<float4*>(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0) = y;
+        }
+      if (h == 0 && half == 0) {
+        if (nv > 1) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + ((int64_t)sp * a.p.N + n) * a.Hq + t.head] = ls;
+        else if (a.lse) a.lse[n * a.Hq + t.head] = ls * kLn2;
+      }
+    }
+  }
+}
+
+// How a call is split. Sequences' lengths are on the device; the host knows bounds.
+struct Plan {
+  bool stream;
+  int nw, tiles, width, chunk, nsplit;
+};
+Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx) {
+  Plan p;
+  const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
+  p.stream = slots <= 16;
+  p.nw = p.stream ? s_waves((int)D) : D == 256 || slots > 128 ? 8 : 4;
+  p.width = p.stream ? 32 : kBK;
+  const int64_t spt = p.stream ? 16 : D == 256 ? 128 : 32 * p.nw;
+  const int64_t tiles = (slots + spt - 1) / spt, keys = (max_ctx + p.width - 1) / p.width;
+  p.tiles = (int)tiles;
+  // workgroups without splits: every sequence's tiles, but no more than the tokens make
+  const int64_t all = N * rep / spt + B, wgs = (tiles * B < all ? tiles * B : all) * Hkv;
+  const int64_t fit = p.stream || p.nw == 4 ? 2 * cus : cus;  // how many run at once
+  const int64_t least = p.stream ? 2 * p.nw : 8;             // key tiles that are worth a workgroup of their own
+  int64_t n = fit / (wgs < 1 ? 1 : wgs);
+  if (n > keys / least) n = keys / least;
+  if (n > 128) n = 128;
+  if (n < 1) n = 1;
+  p.chunk = (int)((keys + n - 1) / n);
+  if (p.chunk < 1) p.chunk = 1;
+  p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
+  if (p.nsplit < 1) p.nsplit = 1;
+  return p;
 }
 
 bool aligned4(const void* p) { return (((uintptr_t)p) & 3u) == 0; }
@@ -299,6 +1273,23 @@ int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* 
   if (!od_aligned16(k_pages) || !od_aligned16(v_pages) || !aligned4(k_scale) || !aligned4(v_scale)) return OD_ERR_ALIGN;
   P = Paged{const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<float*>(k_scale), const_cast<float*>(v_scale),
             table, start, ctx, ld_table, n_pages, (int)cols, __builtin_ctzll(page), (int)B, (int)N, (int)Hkv};
+  return OD_OK;
+}
+
+// The tile kernel's LDS is above 64 KB at D >= 128, which a launch has to be allowed once per device.
+template <int D, bool Q8, int NW>
+int launch_tiles(const AttnArgs& a, unsigned groups, hipStream_t st) {
+  constexpr int bytes = (int)sizeof(TSmem<D, NW>);
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return OD_ERR_LAUNCH;
+  if (!((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_tile_kernel<D, Q8, NW>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            bytes) != hipSuccess)
+      return OD_ERR_LAUNCH;
+    allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  paged_tile_kernel<D, Q8, NW><<<dim3(groups), dim3(NW * 64), bytes, st>>>(a);
   return OD_OK;
 }
 
@@ -387,7 +1378,8 @@ extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, i
   if (!ws_floats) return OD_ERR_NULL;
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
   if (Hq % Hkv || (D != 64 && D != 128 && D != 256)) return OD_ERR_UNSUPPORTED;
-  *ws_floats = 0;
+  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx);
+  *ws_floats = p.nsplit > 1 ? p.nsplit * N * Hq * (D + 1) : 0;
   return OD_OK;
 }
 
@@ -427,11 +1419,39 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   a.Hq = (int)Hq;
   a.rep = (int)(Hq / Hkv);
   a.scale_log2 = scale * kLog2e;
+  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx);
+  if (p.nsplit > 1) {
+    if (!ws) return OD_ERR_NULL;
+    if (ws_floats < p.nsplit * N * Hq * (D + 1)) return OD_ERR_SHAPE;
+    if (!od_aligned16(ws)) return OD_ERR_ALIGN;
+  }
+  a.part = ws;
+  a.nsplit = p.nsplit;
+  a.chunk = p.chunk;
+  a.tiles = p.tiles;
+  if (n_pages == 0) a.p.cols = 0;
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t groups = (int64_t)p.tiles * p.nsplit * Hkv * B;
+  if (groups > 0x7fffffff || B > 65535) return OD_ERR_SHAPE;
+  int rc = OD_OK;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
-    const dim3 grid((unsigned)N, (unsigned)Hq);
-    if (k_scale) paged_attn_rows_kernel<DD, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(a);
-    else paged_attn_rows_kernel<DD, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(a);
+    auto launch = [&](auto QC) {
+      constexpr bool Q8 = decltype(QC)::value;
+      if (p.stream) {
+        paged_stream_kernel<DD, Q8><<<dim3((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B), dim3(s_waves(DD) * 64), 0, st>>>(a);
+      } else if (p.nw == 8) {
+        rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
+      } else if constexpr (DD != 256) {
+        rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
+      }
+    };
+    if (k_scale) launch(std::true_type{});
+    else launch(std::false_type{});
+    if (rc == OD_OK && p.nsplit > 1) {
+      const int heads = (kThreads / 64) * (64 / (DD / 8));
+      paged_combine_kernel<DD><<<dim3((unsigned)N, (unsigned)((Hq + heads - 1) / heads)), dim3(kThreads), 0, st>>>(a, p.width);
+    }
   });
-  return od_launch_status();
+  return rc == OD_OK ? od_launch_status() : rc;
 }
