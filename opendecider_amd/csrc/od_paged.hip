@@ -271,20 +271,11 @@ __device__ __forceinline__ uint32_t fin_bf16x2(uint32_t w) {  // infinities and 
   if ((w & 0x7f800000u) == 0x7f800000u) r &= 0xffffu;
   return r;
 }
-// 1 where a bf16 of the pair is NaN or the infinity of this sign (0: positive), else 0
-__device__ __forceinline__ uint32_t inf_bf16x2(uint32_t w, uint32_t sign) {
-  uint32_t r = 0;
-  const uint32_t lo = w & 0xffffu, hi = w >> 16;
-  if ((lo & 0x7fffu) > 0x7f80u || lo == (0x7f80u | sign)) r |= 0x3f80u;
-  if ((hi & 0x7fffu) > 0x7f80u || hi == (0x7f80u | sign)) r |= 0x3f800000u;
-  return r;
-}
 __device__ __forceinline__ v4u fin_bf16x8(v4u w) {
   return v4u{fin_bf16x2(w[0]), fin_bf16x2(w[1]), fin_bf16x2(w[2]), fin_bf16x2(w[3])};
 }
-__device__ __forceinline__ v4u inf_bf16x8(v4u w, uint32_t s) {
-  return v4u{inf_bf16x2(w[0], s), inf_bf16x2(w[1], s), inf_bf16x2(w[2], s), inf_bf16x2(w[3], s)};
-}
+// a bf16 that is infinite or NaN, as fp32; else 0
+__device__ __forceinline__ float odd_bf16(uint32_t b) { return (b & 0x7f80u) == 0x7f80u ? __uint_as_float(b << 16) : 0.0f; }
 __device__ __forceinline__ bool any_inf_bf16x8(v4u w) {
   uint32_t m = 0;
 #pragma unroll
@@ -603,23 +594,28 @@ __global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void 
         }
         v4u hi, lo;
         s_softmax<D, false>(y, f, x, hi, lo);
-        if (__builtin_amdgcn_ballot_w64(odd) == 0) {
+        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+          // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products take 0
+          // in their places, and the slots that see one get it added
 #pragma unroll
-          for (int dt = 0; dt < D / 16; ++dt) {
-            const v4u v8 = s_vfrag<D, false>(v, dt);
-            x.o[dt] = mfma16(v8, hi, x.o[dt]);
-            x.o[dt] = mfma16(v8, lo, x.o[dt]);
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) v[i][w] = fin_bf16x2(v[i][w]);
+#pragma unroll 1
+          for (int key = k0; key < k0 + left; ++key) {
+            if (z >= s.n * a.rep || key < begin || key > tok) continue;
+            const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + 4 * qd * (D / 16);
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.o[dt][i] += odd_bf16(vp[i * (D / 16) + dt]);
           }
-        } else {  // infinities or NaN among the values: 0 times one must not reach a slot that does not see it
+        }
 #pragma unroll
-          for (int dt = 0; dt < D / 16; ++dt) {
-            const v4u v8 = s_vfrag<D, false>(v, dt), fin = fin_bf16x8(v8);
-            x.o[dt] = mfma16(fin, hi, x.o[dt]);
-            x.o[dt] = mfma16(fin, lo, x.o[dt]);
-            const v4f pos = mfma16(inf_bf16x8(v8, 0), hi, v4f{0, 0, 0, 0}), neg = mfma16(inf_bf16x8(v8, 0x8000u), hi, v4f{0, 0, 0, 0});
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.o[dt][i] += (pos[i] > 0.0f ? INFINITY : 0.0f) + (neg[i] > 0.0f ? -INFINITY : 0.0f);
-          }
+        for (int dt = 0; dt < D / 16; ++dt) {
+          const v4u v8 = s_vfrag<D, false>(v, dt);
+          x.o[dt] = mfma16(v8, hi, x.o[dt]);
+          x.o[dt] = mfma16(v8, lo, x.o[dt]);
         }
       }
     }
@@ -781,8 +777,8 @@ template <int D, int NW>
 struct alignas(16) TSmem {
   uint16_t k[2][kBK * D];
   uint16_t v[2][kBK * D];
-  int odd[2][NW];  // a wave found infinities or NaN among the block's new values
   int lo[NW], hi[NW];
+  int odd;  // infinities or NaN among the new values of a block that some slot sees only a part of
 };
 
 // One slot tile's constants per lane, and its state.
@@ -919,26 +915,6 @@ __device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[D
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
   }
 }
-// The same with infinities or NaN among the values: finite parts as usual, and the slots that see an infinity or NaN found
-// by products with 0 / 1 matrices, since 0 times one would reach the slots that do not.
-template <int D>
-__device__ __forceinline__ void t_values_odd(const uint16_t* vblk, const int (&vb)[D == 256 ? 4 : D / 32], const v4u (&pb)[4], TSlot<D>& t) {
-#pragma unroll
-  for (int dt = 0; dt < (D == 256 ? 4 : D / 32); ++dt) {
-    __builtin_amdgcn_sched_barrier(0);  // one d tile's operands at a time: this path must not cost the usual one registers
-    v16f pos = zero16(), neg = zero16();
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const v4u w = t_vfrag<D>(vblk, vb[dt], kk);
-      t.o[dt] = mfma32<false>(fin_bf16x8(w), pb[kk], t.o[dt]);
-      pos = mfma32<false>(inf_bf16x8(w, 0), pb[kk], pos);
-      neg = mfma32<false>(inf_bf16x8(w, 0x8000u), pb[kk], neg);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) t.o[dt][r] += (pos[r] > 0.0f ? INFINITY : 0.0f) + (neg[r] > 0.0f ? -INFINITY : 0.0f);
-  }
-}
-
 template <int D, bool Q8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, HALVES = D == 256 ? 2 : 1, SPT = 32 * NW / HALVES, DT = D == 256 ? 4 : D / 32;
@@ -1125,6 +1101,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       }
       w_lo = __builtin_amdgcn_readfirstlane(w_lo);
       w_in = __builtin_amdgcn_readfirstlane(w_in);
+      if (tid == 0) sm.odd = 0;
       if (lane == 0) {
         sm.lo[wave] = live ? w_lo : 0x7fffffff;
         sm.hi[wave] = live ? w_in : 0;
@@ -1151,19 +1128,20 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       // a block that some slot of the workgroup sees only a part of
       auto partial = [&](int blk) { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; };
       auto store = [&](int blk, int buf) {
-        bool odd = false;
+        bool odd = false;  // 0 times an infinity must not reach a slot that does not see it: 0 goes in instead
         const bool part = partial(blk);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+          v4u x = r[i];
+          if (part && side && any_inf_bf16x8(x)) {
+            odd = true;
+            x = fin_bf16x8(x);
+          }
           *reinterpret_cast<uint4*>((side ? sm.v[buf] : sm.k[buf]) + (side ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch))) =
-              __builtin_bit_cast(uint4, r[i]);
-          if (part && side) odd |= any_inf_bf16x8(r[i]);
+              __builtin_bit_cast(uint4, x);
         }
-        if (part) {
-          const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-          if (lane == 0) sm.odd[buf][wave] = any;
-        }
+        if (odd) sm.odd = 1;
       };
       if (o_lo < o_hi) {
         load(o_lo);
@@ -1191,15 +1169,21 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
                 }
             }
             t_softmax<D, false>(sc, a.scale_log2, t, pb);
-            int odd = 0;
-            if (partial(blk)) {
-#pragma unroll
-              for (int i = 0; i < NW; ++i) odd |= sm.odd[cur][i];
-            }
-            if (__builtin_amdgcn_readfirstlane(odd) == 0) t_values<D, false>(sm.v[cur], vb, pb, t);
-            else t_values_odd<D>(sm.v[cur], vb, pb, t);
+            t_values<D, false>(sm.v[cur], vb, pb, t);
           }
           __syncthreads();
+        }
+        // infinities and NaN that went in as 0: the slots that see one get it added
+        if (sm.odd && t.ok) {
+#pragma unroll 1
+          for (int key = max(o_lo * kBK, t.begin); key <= t.tok; ++key) {
+            if (!partial(key / kBK)) continue;
+            const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + half * 128 + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) t.o[dt][i] += odd_bf16(vp[dt * 32 + 8 * (i >> 2) + (i & 3)]);
+          }
         }
       }
     }
