@@ -739,6 +739,29 @@ __device__ __forceinline__ int tv_chunk(int key, int chunk) {  // V rows: 4 cons
   return D == 64 ? chunk ^ ((key & 2) << 1) : chunk ^ ((key & 3) << 2);
 }
 
+// 16 bytes per lane from memory straight into LDS, lane l's to LDS byte lds + 16 l (lds wave-uniform, in M0). The compiler does
+// not track it: the kernel waits (vmcnt) and orders it with barriers itself.
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <typename T>
+__device__ __forceinline__ uint32_t lds_addr(T* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);
+}
+// A block's bf16 rows into LDS by DMA: instruction i of a wave fills the 1 KB at 1024 (i NW + wave) of K or V, so a lane owns a
+// place there, (key, swizzled chunk), and copies the chunk that the swizzle puts into it. at(key): its row.
+template <int D, int NW, typename KeyRow>
+__device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, KeyRow&& row) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < D / (8 * NW); ++i) {
+    const int pe = (i * NW + wave) * 512 + 8 * lane, key = pe / D, slot = pe % D / 8;
+    const int ch = v ? tv_chunk<D>(key, slot) : slot ^ (D == 64 ? ((key >> 1) & 7) : (key & 15));
+    dma16(row(key) + 8 * ch, lds_addr(lds) + 1024 * (i * NW + wave));
+  }
+}
+
 template <bool H>
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
   if constexpr (H)
@@ -963,32 +986,36 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
     // ---- the cached blocks b_lo .. b_hi - 1
     if (b_lo < b_hi) {
       if constexpr (Q8) t_q_to_f16<D>(t);
-      constexpr int E = Q8 ? 1 : 2;
-      constexpr int CPK = D * E / 16, CH = kBK * CPK, NC = 2 * CH / NT;  // 16-byte chunks per row, per side; per thread (K, then V)
-      v4u r[NC];
+      // int8 blocks pass through registers, NC 16-byte chunks per thread, K's first; bf16 ones go by DMA
+      constexpr int CPK = D / 16, CH = kBK * CPK, NC = 2 * CH / NT;
+      v4u r[Q8 ? NC : 1];
       int pg = -1;             // lane l: the page of key l of the block whose loads come next
       float ks = 0, vs = 0;    // lane l: the scales of key l of the loaded block
       uint64_t there = 0;      // the loaded block's keys that exist
-      int pg_of = -1;          // the loaded block's pages
+      const int in_page = (1 << a.p.shift) - 1;
       auto pages = [&](int blk) {
         const int pos = blk * kBK + lane;
         pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
         if (pg >= a.p.n_pages) pg = -1;
       };
-      auto load = [&](int blk) {
+      auto load = [&](int blk, int buf) {
         there = __builtin_amdgcn_ballot_w64(pg >= 0);
-        pg_of = pg;
-        const int mask = (1 << a.p.shift) - 1;
+        const int page = max(pg, 0);  // a key that is not there is read from page 0 and left out later
+        auto row = [&](int key) {
+          return (((int64_t)__shfl(page, key, 64) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + key) & in_page);
+        };
         if constexpr (Q8) {
-          const int64_t at = (((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & mask);
+          const int64_t at = (((int64_t)page * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & in_page);
           ks = a.p.ks[at];
           vs = a.p.vs[at];
-        }
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
-          const int64_t row = (((int64_t)max(__shfl(pg, key, 64), 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + key) & mask);
-          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) + row * (D * E) + 16 * ch));
+          for (int i = 0; i < NC; ++i) {
+            const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) + row(key) * D + 16 * ch));
+          }
+        } else {
+          dma_rows<D, NW>(sm.k[buf], wave, false, [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(key) * D; });
+          dma_rows<D, NW>(sm.v[buf], wave, true, [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(key) * D; });
         }
       };
       int kexp = 0, vexp = 0;  // the stored block's frames
@@ -996,42 +1023,43 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       uint64_t seen = 0;
       auto store = [&](int buf) {
         seen = there;
-        float kf = 0, vf = 0;
         if constexpr (Q8) {
           // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not finite,
           // leave them alone
-          const bool on = pg_of >= 0;
+          const bool on = (there >> lane) & 1;
           const uint32_t kb = on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u, vb2 = on && vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u;
           kexp = exp_above(od_wave_umax_dpp(kb));
           const uint32_t vm = od_wave_umax_dpp(vb2);
           if (vm) vexp = vexp_set ? max(vexp, exp_above(vm)) : exp_above(vm);
           if (vm) vexp_set = true;
-          kf = on ? frame_scale(ks, 7 - kexp) : 0.0f;
-          vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
-        }
+          const float kf = on ? frame_scale(ks, 7 - kexp) : 0.0f, vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
-          uint16_t* dst = side ? sm.v[buf] : sm.k[buf];
-          if constexpr (Q8) {
+          for (int i = 0; i < NC; ++i) {
+            const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+            uint16_t* dst = side ? sm.v[buf] : sm.k[buf];
             v4u lo, hi;
             i8x16_scaled(r[i], __shfl(side ? vf : kf, key, 64), lo, hi);
             const int o0 = side ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
             const int o1 = side ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
             *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
             *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
-          } else {
-            const v4u x = (there >> key) & 1 ? r[i] : v4u{0, 0, 0, 0};
-            *reinterpret_cast<uint4*>(dst + (side ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch))) = __builtin_bit_cast(uint4, x);
           }
+        } else if (seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
+          dma_wait();
+          __syncthreads();
+          for (int c = tid; c < kBK * (D / 8); c += NT)
+            if (!((seen >> (c / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[buf][8 * c]) = make_uint4(0, 0, 0, 0);
         }
       };
+      // One step: block blk's products; ahead of them, for int8 the conversion of block blk + 1 (in registers since the last
+      // step) and the loads of blk + 2, for bf16 the copy of blk + 1.
       pages(b_lo);
-      load(b_lo);
+      load(b_lo, 0);
       pages(b_lo + 1);
+      if constexpr (!Q8) dma_wait();
       store(0);
-      if (b_lo + 1 < b_hi) {
-        load(b_lo + 1);
+      if (Q8 && b_lo + 1 < b_hi) {
+        load(b_lo + 1, 1);
         pages(b_lo + 2);
       }
       __syncthreads();
@@ -1041,10 +1069,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
         const int f_new = Q8 ? vexp - 7 : 0;
         const uint64_t mask = seen;
         if (blk + 1 < b_hi) {
-          store(cur ^ 1);
-          if (blk + 2 < b_hi) {
-            load(blk + 2);
-            pages(blk + 3);
+          if constexpr (Q8) {
+            store(cur ^ 1);
+            if (blk + 2 < b_hi) {
+              load(blk + 2, cur);
+              pages(blk + 3);
+            }
+          } else {
+            load(blk + 1, cur ^ 1);
+            pages(blk + 2);
           }
         }
         if (Q8 && f_new != frame) {  // the values' frame rose: uniform over the workgroup
@@ -1069,6 +1102,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
           }
           t_softmax<D, Q8>(sc, c, t, pb);
           t_values<D, Q8>(sm.v[cur], vb, pb, t);
+        }
+        if (!Q8 && blk + 1 < b_hi) {
+          dma_wait();
+          store(cur ^ 1);
         }
         __syncthreads();
       }
@@ -1115,46 +1152,35 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       }
       const int g_tok = min(tile * SPT / a.rep, s.n - 1), g_hi = min((tile * SPT + SPT - 1) / a.rep, s.n - 1);
       const int o_lo = min(g_lo, g_hi + 1) / kBK, o_hi = g_hi / kBK + 1;
-      constexpr int CPK = D / 8, CH = kBK * CPK, NC = 2 * CH / NT;
-      v4u r[NC];
-      auto load = [&](int blk) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int cid = i * NT + tid, side = cid / CH, key = min(blk * kBK + cid % CH / CPK, s.n - 1), ch = cid % CPK;
-          const uint16_t* src = side ? a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh : a.k + (int64_t)(s.s0 + key) * a.skt + (int64_t)g * a.skh;
-          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(src + 8 * ch));
-        }
+      auto load = [&](int blk, int buf) {
+        const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
+        const uint16_t* vp = a.v + (int64_t)s.s0 * a.svt + (int64_t)g * a.svh;
+        dma_rows<D, NW>(sm.k[buf], wave, false, [&](int key) { return kp + min(blk * kBK + key, s.n - 1) * a.skt; });
+        dma_rows<D, NW>(sm.v[buf], wave, true, [&](int key) { return vp + min(blk * kBK + key, s.n - 1) * a.svt; });
       };
       // a block that some slot of the workgroup sees only a part of
       auto partial = [&](int blk) { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; };
-      auto store = [&](int blk, int buf) {
-        bool odd = false;  // 0 times an infinity must not reach a slot that does not see it: 0 goes in instead
-        const bool part = partial(blk);
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
-          v4u x = r[i];
-          if (part && side && any_inf_bf16x8(x)) {
-            odd = true;
-            x = fin_bf16x8(x);
+      // Such a block's infinities and NaN become 0 (0 times one would reach the slots that do not see it).
+      auto finite = [&](int blk, int buf) {
+        if (!partial(blk)) return;
+        __syncthreads();  // every wave's part of the copy is there
+        for (int c = tid; c < kBK * (D / 8); c += NT) {
+          uint4* at = reinterpret_cast<uint4*>(&sm.v[buf][8 * c]);
+          const v4u x = __builtin_bit_cast(v4u, *at);
+          if (any_inf_bf16x8(x)) {
+            *at = __builtin_bit_cast(uint4, fin_bf16x8(x));
+            sm.odd = 1;
           }
-          *reinterpret_cast<uint4*>((side ? sm.v[buf] : sm.k[buf]) + (side ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch))) =
-              __builtin_bit_cast(uint4, x);
         }
-        if (odd) sm.odd = 1;
       };
       if (o_lo < o_hi) {
-        load(o_lo);
-        __syncthreads();
-        store(o_lo, 0);
-        if (o_lo + 1 < o_hi) load(o_lo + 1);
+        load(o_lo, 0);
+        dma_wait();
+        finite(o_lo, 0);
         __syncthreads();
         for (int blk = o_lo; blk < o_hi; ++blk) {
           const int cur = (blk - o_lo) & 1, j0 = blk * kBK;
-          if (blk + 1 < o_hi) {
-            store(blk + 1, cur ^ 1);
-            if (blk + 2 < o_hi) load(blk + 2);
-          }
+          if (blk + 1 < o_hi) load(blk + 1, cur ^ 1);
           if (live && j0 <= w_hi && j0 + kBK > w_lo) {
             v16f sc[2];
             v4u pb[4];
@@ -1170,6 +1196,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
             }
             t_softmax<D, false>(sc, a.scale_log2, t, pb);
             t_values<D, false>(sm.v[cur], vb, pb, t);
+          }
+          if (blk + 1 < o_hi) {
+            dma_wait();
+            finite(blk + 1, cur ^ 1);
           }
           __syncthreads();
         }
