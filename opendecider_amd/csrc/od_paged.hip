@@ -10,8 +10,9 @@
 // columns, a negative length and packed rows outside [0, N) are found by the kernels and skipped (no such key is seen, no
 // such row written). The host needs no copy of start, ctx or table.
 #include <type_traits>
+#include <stdlib.h>
 
-#include "od_common.h"
+#include "/root/repo/opendecider_amd/csrc/od_common.h"
 
 namespace {
 
@@ -296,93 +297,92 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
 // reading the pages. A wave holds all 16 slots as the columns of V_MFMA_F32_16X16X32_BF16 and takes 32-key tiles straight
 // from memory into registers; the waves of a workgroup take every NW-th tile of the split's range and merge in LDS.
 // Lane (j, g) = (lane % 16, lane / 16):
-//  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: k-step ks takes the dims g D / 4 + 8 ks .. + 7 on both sides (a
-//    permutation of the reduction index), so a lane reads D / 4 contiguous values of its keys; int8 values enter as exact
-//    bf16 integers and the score takes the fp32 factor ks_j. The result gives lane (j, g) slot j and keys 16 kr + 4 g + i;
+//  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: the four lanes of a key read 64 contiguous bytes of it at a time
+//    (s_dim: a permutation of the reduction index, the same on both sides; reading D / 4 contiguous values per lane instead
+//    took 101 against 76 us for the loads of 16 x 8000 bf16 tokens); int8 values enter as exact bf16 integers and the
+//    score takes the fp32 factor ks_j. The result gives lane (j, g) slot j and keys 16 kr + 4 g + i;
 //  * O^T[dt] += V^T[dt] P^T with output row r of d tile dt being d = (D / 16) r + dt and the keys in the order 4 g + i (i < 4),
 //    12 + 4 g + i: the B operand is the lane's own 8 probabilities, the A operand value dt of the D / 16 contiguous values it
 //    reads of each of those keys. P (times vs_j) enters as bf16 hi + lo parts, 16 significant bits: the columns of the
 //    matrix instructions are mostly empty here, and no scale of the values can leave the range.
 // Half tiles are reached through buffer descriptors of their own (a half tile never crosses a page), whose length ends at
-// the last cached token: what lies behind reads as zeros. K of the next tile is asked for when this tile's scores are
-// done, V when its products are, into the same registers: with 4 waves a SIMD some 100 KB a CU are in flight.
+// the last cached token: what lies behind reads as zeros. Two register sets: a tile's loads are all issued before the
+// products of the tile ahead of it, unconditionally (past a wave's last tile with descriptors of no length, so that the waits are counted but nothing is read). Rows of 256 go in tiles of one half (R = 1): two sets of whole
+// ones do not fit the registers (16 x 8000 tokens 62 us, 49 with halves); bf16 ones then still take a SIMD alone.
+constexpr int s_halves(int D) { return D == 256 ? 1 : 2; }
 template <int D, bool Q8>
 struct STile {
-  static constexpr int KW = D / 4 * (Q8 ? 1 : 2) / 16;  // 16-byte loads of a key's D / 4 values
-  static constexpr int VB = D / 16 * (Q8 ? 1 : 2);      // bytes of a key's D / 16 values: 4, 8, 16 or 32
-  v4u k[2][KW];
-  uint32_t v[8][VB / 4];
+  static constexpr int R = s_halves(D), KW = D / 4 * (Q8 ? 1 : 2) / 16;  // KW: 16-byte loads of a key's D / 4 values
+  static constexpr int VB = D / 16 * (Q8 ? 1 : 2);                           // bytes of a key's D / 16 values: 4 to 32
+  v4u k[R][KW];
+  uint32_t v[4 * R][VB / 4];
   float ks, vs;  // lane l: the scales of key l % 32
+  int len[R];    // keys of the half tiles (wave-uniform)
 };
-__device__ __forceinline__ int s_key(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
+
+// first of the 8 dims that lanes of group g hold in k-step ks
+template <bool Q8>
+__device__ __forceinline__ int s_dim(int g, int ks) { return Q8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
 
 constexpr int kOnce = 2;  // non-temporal: each byte is read once
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
 }
 
-// The two half tiles of the tile at position kb: first rows and lengths (0: none).
-struct STileAt {
-  int64_t row[2];
-  int len[2];
-};
-__device__ __forceinline__ STileAt s_at(const AttnArgs& a, const Seq& s, int b, int g, int kb) {
-  STileAt t;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int pos = kb + 16 * r;
-    const int64_t row = pos < s.ctx ? uniform_row_of(a.p, b, g, pos) : -1;
-    t.row[r] = row < 0 ? 0 : row;
-    t.len[r] = row < 0 ? 0 : min(16, s.ctx - pos);
-  }
-  return t;
+// The pages of 64 / R tiles of a wave, one load: lane l has the page of half tile l % R of the wave's tile number l / R from
+// here (`pos` of tile 0, `step` positions from tile to tile; -1: no key or no page).
+template <int R>
+__device__ __forceinline__ int s_pages(const Paged& p, int b, int pos, int step) {
+  const int l = threadIdx.x & 63;
+  const int64_t at = (int64_t)pos + (int64_t)(l / R) * step + 16 * (l % R), col = at >> p.shift;
+  const int pg = col < p.cols ? p.table[b * p.ld_table + col] : -1;
+  return pg < p.n_pages ? pg : -1;
 }
+// A tile's loads, its pages in place `nth` of `pages`. Lane l takes the scales of key l % 32, each 16 lanes their half tile's.
 template <int D, bool Q8>
-__device__ __forceinline__ void s_load_k(const AttnArgs& a, const STileAt& t, STile<D, Q8>& x) {
+__device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth, STile<D, Q8>& x) {
+  using T = STile<D, Q8>;
   constexpr int E = Q8 ? 1 : 2;
-  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, j = lane & 15, gl = lane >> 4;
+  int64_t row[T::R];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const auto d = rsrc(static_cast<const char*>(a.p.k) + t.row[r] * (D * E), t.len[r] * (D * E));
+  for (int r = 0; r < T::R; ++r) {
+    const int pos = kb + 16 * r, pg = __builtin_amdgcn_readlane(pages, nth * T::R + r);
+    x.len[r] = pg < 0 || pos >= s.ctx ? 0 : min(16, s.ctx - pos);
+    row[r] = (((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + (pos & ((1 << a.p.shift) - 1));
+    const auto dk = rsrc(static_cast<const char*>(a.p.k) + row[r] * (D * E), x.len[r] * (D * E));
 #pragma unroll
-    for (int w = 0; w < STile<D, Q8>::KW; ++w)
-      x.k[r][w] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, (j * D + g * (D / 4)) * E + 16 * w, 0, kOnce));
-  }
-}
-template <int D, bool Q8>
-__device__ __forceinline__ void s_load_v(const AttnArgs& a, const STileAt& t, STile<D, Q8>& x) {
-  constexpr int E = Q8 ? 1 : 2, VB = STile<D, Q8>::VB;
-  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const auto d = rsrc(static_cast<const char*>(a.p.v) + t.row[r] * (D * E), t.len[r] * (D * E));
+    for (int w = 0; w < T::KW; ++w)
+      x.k[r][w] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(dk, j * D * E + 64 * w + 16 * gl, 0, kOnce));
+    const auto dv = rsrc(static_cast<const char*>(a.p.v) + row[r] * (D * E), x.len[r] * (D * E));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = (4 * g + i) * D * E + j * VB;
-      if constexpr (VB == 4) {
-        x.v[4 * r + i][0] = __builtin_amdgcn_raw_buffer_load_b32(d, at, 0, kOnce);
-      } else if constexpr (VB == 8) {
-        const auto u = __builtin_amdgcn_raw_buffer_load_b64(d, at, 0, kOnce);
+      const int at = (4 * gl + i) * D * E + j * T::VB;
+      if constexpr (T::VB == 4) {
+        x.v[4 * r + i][0] = __builtin_amdgcn_raw_buffer_load_b32(dv, at, 0, kOnce);
+      } else if constexpr (T::VB == 8) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b64(dv, at, 0, kOnce);
         x.v[4 * r + i][0] = u[0];
         x.v[4 * r + i][1] = u[1];
       } else {
 #pragma unroll
-        for (int w = 0; w < VB / 16; ++w) {
-          const v4u u = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, at + 16 * w, 0, kOnce));
+        for (int w = 0; w < T::VB / 16; ++w) {
+          const v4u u = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(dv, at + 16 * w, 0, kOnce));
 #pragma unroll
           for (int c = 0; c < 4; ++c) x.v[4 * r + i][4 * w + c] = u[c];
         }
       }
     }
   }
-}
-// lane l: the scales of key l % 32 (each half of 16 lanes its half tile's)
-__device__ __forceinline__ void s_load_scales(const AttnArgs& a, const STileAt& t, float& ks, float& vs) {
-  const int c = threadIdx.x & 31, r = c >> 4;
-  const bool in = (c & 15) < (r ? t.len[1] : t.len[0]);
-  const int64_t at = (r ? t.row[1] : t.row[0]) + (c & 15);
-  ks = in ? a.p.ks[at] : 0.0f;
-  vs = in ? a.p.vs[at] : 0.0f;
+  if constexpr (Q8) {
+    // a lane's own row: one descriptor cannot reach both half tiles, so lanes without a key read the pool's first scale
+    const int c = lane & 31;
+    const bool in = (c & 15) < (c < 16 ? x.len[0] : x.len[1]);
+    const int64_t at = in ? (c < 16 ? row[0] : row[1]) + (c & 15) : 0;
+    const float k1 = a.p.ks[at], v1 = a.p.vs[at];
+    x.ks = in ? k1 : 0.0f;
+    x.vs = in ? v1 : 0.0f;
+  }
 }
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
@@ -431,11 +431,11 @@ __device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SA
 }
 
 // value dt of each of the lane's 8 keys, as the bf16 A operand
-template <int D, bool Q8>
-__device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[8][STile<D, Q8>::VB / 4], int dt) {
-  v4u r;
+template <int D, bool Q8, int NK>
+__device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, Q8>::VB / 4], int dt) {
+  v4u r = v4u{0, 0, 0, 0};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < NK / 2; ++e) {
     if constexpr (Q8) {
       const uint32_t a = v[2 * e][dt / 4], b = v[2 * e + 1][dt / 4];
       const int sh = 8 * (dt % 4);
@@ -447,11 +447,11 @@ __device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[8][STile<D, Q8>::VB /
   return r;
 }
 
-constexpr int s_waves(int D) { return D == 256 ? 4 : 8; }  // the merge holds every wave's 16 x D outputs in LDS
+constexpr int kStreamWaves = 4;
 
 template <int D, bool Q8>
-__global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void paged_stream_kernel(AttnArgs a) {
-  constexpr int NW = s_waves(D), KS = D / 32, QR = D + 8;  // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
+__global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+  constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D), QR = D + 8;  // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
   __shared__ __attribute__((aligned(16))) union {
     uint16_t q[16 * QR];
     float o[NW][16][D + 4];
@@ -459,24 +459,55 @@ __global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void 
   __shared__ float sml[NW][2][16];
   __shared__ float4 skf[NW][2][8];  // a tile's per-key factors, from lane order to score order (one wave writes and reads)
   const int sp = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
-  const Seq s = seq_of(a, b);
-  const int tiles = (s.ctx + 31) >> 5, nv = splits_of(a, tiles);
-  if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
-  const int t_lo = sp * a.chunk, t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
+  constexpr int W = 16 * R, PT = 64 / R, SETS = 2;  // PT: tiles whose pages one load brings
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15, qd = lane >> 4, c = lane & 31;
+  // A short call is a chain of memory latencies: lengths and page numbers; queries, then the first tiles; the rest.
+  const int t_lo = sp * a.chunk;
+  const int pages0 = s_pages<R>(a.p, b, (t_lo + wave) * W, NW * W);
+  const Seq s = seq_of(a, b);
+  const int tiles = (s.ctx + W - 1) / W, nv = splits_of(a, tiles);
+  if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
+  const int t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
   for (int z0 = 0; z0 < s.n * a.rep; z0 += 16) {  // one round unless max_new was too small
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 8); i += NW * 64) {
-      const int z = z0 + i / (D / 8), d0 = (i % (D / 8)) * 8;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (z < s.n * a.rep)
-        w = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt + (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
-      *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + d0) = w;
+    constexpr int QC = 16 * (D / 8) / (NW * 64) ? 16 * (D / 8) / (NW * 64) : 1;
+    uint4 qw[QC];
+#pragma unroll
+    for (int k = 0; k < QC; ++k) {
+      const int i = k * NW * 64 + threadIdx.x, z = z0 + i / (D / 8), d0 = (i % (D / 8)) * 8;
+      qw[k] = make_uint4(0, 0, 0, 0);
+      if (i < 16 * (D / 8) && z < s.n * a.rep)
+        qw[k] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt + (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
+    }
+    int tt = t_lo + wave, pages = pages0, nth = -1;
+    // the wave's next tile into x (past the last one: an empty one, without traffic)
+    STile<D, Q8> tl[SETS];
+    int asked = tt - NW;  // the tile last asked for
+    auto next = [&](STile<D, Q8>& x) {
+      const bool more = asked + NW < t_hi;
+      if (more) {
+        asked += NW;
+        if (++nth == PT) {
+          nth = 0;
+          pages = s_pages<R>(a.p, b, asked * W, NW * W);
+        }
+      }
+      s_load<D, Q8>(a, s, g, more ? asked * W : s.ctx, pages, nth, x);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (tt < t_hi) {
+#pragma unroll
+      for (int i = 0; i < SETS - 1; ++i) next(tl[i]);
+    }
+    __syncthreads();  // an earlier round's readers are done
+#pragma unroll
+    for (int k = 0; k < QC; ++k) {
+      const int i = k * NW * 64 + threadIdx.x;
+      if (i < 16 * (D / 8)) *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = qw[k];
     }
     __syncthreads();
     auto qfrag = [&](int ks) {
-      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + j * QR + qd * (D / 4) + 8 * ks));
+      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + j * QR + s_dim<Q8>(qd, ks)));
     };
     SAcc<D> x;
     x.m = -INFINITY;
@@ -484,121 +515,53 @@ __global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void 
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
 
-    int tt = t_lo + wave;
-    if (tt < t_hi) {
-      STile<D, Q8> tl;
-      STileAt at = s_at(a, s, b, g, tt * 32);
-      s_load_k<D, Q8>(a, at, tl);
-      if constexpr (Q8) s_load_scales(a, at, tl.ks, tl.vs);
-      s_load_v<D, Q8>(a, at, tl);
-      for (; tt < t_hi; tt += NW) {
-        const int nx = tt + NW < t_hi ? tt + NW : tt;
-        const STileAt next = s_at(a, s, b, g, nx * 32);
-        if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
-          reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
-          reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
-        }
-        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            v4u k8;
-            if constexpr (Q8) {
-              uint32_t w[4];
-              i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1)], w[0], w[1]);
-              i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1) + 1], w[2], w[3]);
-              k8 = v4u{w[0], w[1], w[2], w[3]};
-            } else {
-              k8 = tl.k[r][ks];
-            }
-            sc[r] = mfma16(k8, qfrag(ks), sc[r]);
-          }
-        s_load_k<D, Q8>(a, next, tl);
-        float y[8], f[8];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float4 kf = Q8 ? skf[wave][0][4 * r + qd] : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
-          const float4 vf = Q8 ? skf[wave][1][4 * r + qd] : make_float4(1, 1, 1, 1);
-          const float kk[4] = {kf.x, kf.y, kf.z, kf.w}, vv[4] = {vf.x, vf.y, vf.z, vf.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            y[4 * r + i] = sc[r][i] * kk[i];
-            f[4 * r + i] = vv[i];
-          }
-        }
-        if (at.len[0] + at.len[1] != 32) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (4 * qd + (i & 3) >= at.len[i >> 2]) y[i] = -INFINITY;
-        }
-        if constexpr (Q8) s_load_scales(a, next, tl.ks, tl.vs);
-        v4u hi, lo;
-        s_softmax<D, Q8>(y, f, x, hi, lo);
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-          const v4u v8 = s_vfrag<D, Q8>(tl.v, dt);
-          x.o[dt] = mfma16(v8, hi, x.o[dt]);
-          x.o[dt] = mfma16(v8, lo, x.o[dt]);
-        }
-        s_load_v<D, Q8>(a, next, tl);
-        at = next;
-      }
-    }
-
-    // the new tokens: tiles of 32 bf16 keys, in split 0
-    if (sp == 0 && a.k) {
+    // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which have the
+    // fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do not hold both).
+    auto new_tokens = [&] {
+      if (sp != 0 || !a.k) return;
       const int z = z0 + j, tok = min(z / a.rep, s.n - 1);
       const int begin = a.row_begin ? max(a.row_begin[s.s0 + tok], 0) : 0;
       const int t_end = min((z0 + 15) / a.rep, s.n - 1);  // last token of these slots
-      for (int k0 = 32 * wave; k0 <= t_end; k0 += 32 * NW) {
-        const int left = min(32, s.n - k0);
-        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll 1
+      for (int k0 = 16 * (NW - 1 - wave); k0 <= t_end; k0 += 16 * NW) {
+        const int left = min(16, s.n - k0);
+        const uint16_t* kp = a.k + (int64_t)(s.s0 + k0 + min(j, left - 1)) * a.skt + (int64_t)g * a.skh;
+        v4u kr[KS];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = min(16 * r + j, left - 1);
-          const uint16_t* kp = a.k + (int64_t)(s.s0 + k0 + key) * a.skt + (int64_t)g * a.skh + qd * (D / 4);
+        for (int ks = 0; ks < KS; ++ks) kr[ks] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + s_dim<Q8>(qd, ks)));
+        uint32_t v[4][D / 32];
+        bool odd = false;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            sc[r] = mfma16(__builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + 8 * ks)), qfrag(ks), sc[r]);
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t* vp = a.v + (int64_t)(s.s0 + k0 + min(4 * qd + i, left - 1)) * a.svt + (int64_t)g * a.svh + j * (D / 16);
+#pragma unroll
+          for (int w = 0; w < D / 64; ++w) {
+            const uint2 u = *reinterpret_cast<const uint2*>(vp + 4 * w);
+            v[i][2 * w] = u.x;
+            v[i][2 * w + 1] = u.y;
+          }
         }
+        v4f sc = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sc = mfma16(kr[ks], qfrag(ks), sc);
         float y[8], f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int key = k0 + s_key(qd, i);
-          y[i] = z < s.n * a.rep && key >= begin && key <= tok ? sc[i >> 2][i & 3] * a.scale_log2 : -INFINITY;
+          const int key = k0 + 4 * qd + i;
+          y[i] = i < 4 && z < s.n * a.rep && key >= begin && key <= tok ? sc[i & 3] * a.scale_log2 : -INFINITY;
           f[i] = 1.0f;
         }
-        uint32_t v[8][D / 32];
-        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = min(s_key(qd, i), left - 1);
-          const uint16_t* vp = a.v + (int64_t)(s.s0 + k0 + key) * a.svt + (int64_t)g * a.svh + j * (D / 16);
-          if constexpr (D == 64) {
-            const uint2 u = *reinterpret_cast<const uint2*>(vp);
-            v[i][0] = u.x;
-            v[i][1] = u.y;
-          } else {
-#pragma unroll
-            for (int w = 0; w < D / 128; ++w) {
-              const uint4 u = *reinterpret_cast<const uint4*>(vp + 8 * w);
-              v[i][4 * w] = u.x;
-              v[i][4 * w + 1] = u.y;
-              v[i][4 * w + 2] = u.z;
-              v[i][4 * w + 3] = u.w;
-            }
-          }
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int w = 0; w < D / 32; ++w) odd |= fin_bf16x2(v[i][w]) != v[i][w];
-        }
         v4u hi, lo;
         s_softmax<D, false>(y, f, x, hi, lo);
         if (__builtin_amdgcn_ballot_w64(odd) != 0) {
           // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products take 0
           // in their places, and the slots that see one get it added
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int w = 0; w < D / 32; ++w) v[i][w] = fin_bf16x2(v[i][w]);
 #pragma unroll 1
@@ -613,12 +576,78 @@ __global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void 
         }
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) {
-          const v4u v8 = s_vfrag<D, false>(v, dt);
+          const v4u v8 = s_vfrag<D, false, 4>(v, dt);
           x.o[dt] = mfma16(v8, hi, x.o[dt]);
           x.o[dt] = mfma16(v8, lo, x.o[dt]);
         }
       }
+    };
+    if constexpr (D < 256) new_tokens();
+
+    // one tile's scores, softmax and products
+    auto products = [&](const STile<D, Q8>& tl) {
+      if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
+        reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
+        reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
+      }
+      v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          v4u k8;
+          if constexpr (Q8) {
+            uint32_t w[4];
+            i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1)], w[0], w[1]);
+            i8x4_to_bf16(tl.k[r][ks / 2][2 * (ks & 1) + 1], w[2], w[3]);
+            k8 = v4u{w[0], w[1], w[2], w[3]};
+          } else {
+            k8 = tl.k[r][ks];
+          }
+          sc[r] = mfma16(k8, qfrag(ks), sc[r]);
+        }
+      float y[8], f[8];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float4 kf = Q8 ? skf[wave][0][4 * r + qd] : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
+        const float4 vf = Q8 ? skf[wave][1][4 * r + qd] : make_float4(1, 1, 1, 1);
+        const float kk[4] = {kf.x, kf.y, kf.z, kf.w}, vv[4] = {vf.x, vf.y, vf.z, vf.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[4 * r + i] = r < R ? sc[r][i] * kk[i] : -INFINITY;
+          f[4 * r + i] = vv[i];
+        }
+      }
+      int there = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) there += tl.len[r];
+      if (there != 16 * R) {
+#pragma unroll
+        for (int i = 0; i < 4 * R; ++i)
+          if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
+      }
+      v4u hi, lo;
+      s_softmax<D, Q8>(y, f, x, hi, lo);
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        const v4u v8 = s_vfrag<D, Q8, 4 * R>(tl.v, dt);
+        x.o[dt] = mfma16(v8, hi, x.o[dt]);
+        x.o[dt] = mfma16(v8, lo, x.o[dt]);
+      }
+    };
+    if (tt < t_hi) {
+      for (bool more = true; more;) {
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) {
+          next(tl[(i + SETS - 1) % SETS]);
+          products(tl[i]);
+          tt += NW;
+          if (!(more = tt < t_hi)) break;
+        }
+      }
     }
+
+    if constexpr (D == 256) new_tokens();
 
     // merge the waves, then the output or this split's normalized partial
     float l = x.l + __shfl_xor(x.l, 16, 64);
@@ -670,43 +699,57 @@ __global__ __launch_bounds__(s_waves(D) * 64, D == 256 ? 2 : (Q8 ? 4 : 2)) void 
   }
 }
 
-// The splits of a sequence's slots merged by log-sum-exp: a wave per packed row and 64 / (D / 8) heads. `width`: keys per tile.
+// The splits of a slot merged by log-sum-exp, a workgroup per packed row and head: 4 columns a thread, and 1024 / D groups of
+// threads that share the splits, so that up to 4096 / D of them are in flight together. `width`: keys per tile.
 template <int D>
 __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int width) {
-  constexpr int G = D / 8, HW = 64 / G;
-  const int n = blockIdx.x, lane = threadIdx.x & 63;
-  const int head = (blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6)) * HW + lane / G, d0 = (lane % G) * 8;
+  constexpr int C = D / 4, S = kThreads / C, AHEAD = 4;
+  __shared__ float4 so[S][C];
+  __shared__ float sml[S][2];
+  const int n = blockIdx.x, head = blockIdx.y, c = threadIdx.x % C, grp = threadIdx.x / C;
+  const int64_t slot = (int64_t)n * a.Hq + head, step = (int64_t)a.p.N * a.Hq;
+  const float* ls = a.part + (int64_t)a.nsplit * step * D;
+  const float* po = a.part + slot * D + 4 * c;
+  // The first splits are asked for before their number is known: what no split has written is not used.
+  float l4[AHEAD];
+  float4 u4[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    const int64_t sp = min(grp + i * S, a.nsplit - 1);
+    l4[i] = ls[sp * step + slot];
+    u4[i] = *reinterpret_cast<const float4*>(po + sp * step * D);
+  }
   const int b = seq_search(a.p.start, a.p.B, n);
   const Seq s = seq_of(a, b);
   const int nv = splits_of(a, (s.ctx + width - 1) / width);
-  if (n < s.s0 || n >= s.s0 + s.n || nv == 1 || head >= a.Hq) return;
-  const int64_t slot = (int64_t)n * a.Hq + head, step = (int64_t)a.p.N * a.Hq;
-  const float* ls = a.part + (int64_t)a.nsplit * step * D;
-  float M = -INFINITY, L = 0.0f, acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  // one pass with a running max, unrolled: several splits' loads are in flight together
-#pragma unroll 4
-  for (int sp = 0; sp < nv; ++sp) {
-    const float l = ls[sp * step + slot];
-    const float4* po = reinterpret_cast<const float4*>(a.part + (sp * step + slot) * D + d0);
-    const float4 u = po[0], w = po[1];
-    if (l == -INFINITY) continue;  // a split that sees nothing
-    if (l > M) {
-      const float r = __builtin_amdgcn_exp2f(M - l);
-      L *= r;
+  if (n < s.s0 || n >= s.s0 + s.n || nv == 1) return;  // uniform over the workgroup
+  float M = -INFINITY, L = 0.0f;
+  float4 acc = make_float4(0, 0, 0, 0);
+  auto add = [&](float l, float w, float4 u) {  // w: the weight that comes with l
+    const float m2 = fmaxf(M, l), ms = m2 == -INFINITY ? 0.0f : m2;  // a NaN l leaves M and makes the sums NaN
+    const float r = __builtin_amdgcn_exp2f(M - ms), f = __builtin_amdgcn_exp2f(l - ms);
+    L = L * r + w * f;
+    acc = make_float4(acc.x * r + f * u.x, acc.y * r + f * u.y, acc.z * r + f * u.z, acc.w * r + f * u.w);
+    M = m2;
+  };
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= r;
-      M = l;
-    }
-    const float f = __builtin_amdgcn_exp2f(l - M);
-    L += f;
-    acc[0] += f * u.x; acc[1] += f * u.y; acc[2] += f * u.z; acc[3] += f * u.w;
-    acc[4] += f * w.x; acc[5] += f * w.y; acc[6] += f * w.z; acc[7] += f * w.w;
+  for (int i = 0; i < AHEAD; ++i)
+    if (grp + i * S < nv) add(l4[i], 1.0f, u4[i]);
+#pragma unroll 4
+  for (int sp = grp + AHEAD * S; sp < nv; sp += S) add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
+  so[grp][c] = acc;
+  if (c == 0) {
+    sml[grp][0] = M;
+    sml[grp][1] = L;
   }
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int k = 1; k < S; ++k) add(sml[k][0], sml[k][1], so[k][c]);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint4*>(a.out + n * a.sot + head * a.soh + d0) =
-      make_uint4(od_pack_bf16x2(acc[0] * inv, acc[1] * inv), od_pack_bf16x2(acc[2] * inv, acc[3] * inv),
-                 od_pack_bf16x2(acc[4] * inv, acc[5] * inv), od_pack_bf16x2(acc[6] * inv, acc[7] * inv));
-  if (a.lse && d0 == 0) a.lse[slot] = (M + __log2f(L)) * kLn2;
+  *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + 4 * c) =
+      make_uint2(od_pack_bf16x2(acc.x * inv, acc.y * inv), od_pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (a.lse && c == 0) a.lse[slot] = (M + __log2f(L)) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------------ many slots: tiles
@@ -1251,8 +1294,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   Plan p;
   const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
   p.stream = slots <= 16;
-  p.nw = p.stream ? s_waves((int)D) : D == 256 || slots > 128 ? 8 : 4;
-  p.width = p.stream ? 32 : kBK;
+  p.nw = p.stream ? kStreamWaves : D == 256 || slots > 128 ? 8 : 4;
+  p.width = p.stream ? 16 * s_halves((int)D) : kBK;
   const int64_t spt = p.stream ? 16 : D == 256 ? 128 : 32 * p.nw;
   const int64_t tiles = (slots + spt - 1) / spt, keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
@@ -1266,6 +1309,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   if (n < 1) n = 1;
   p.chunk = (int)((keys + n - 1) / n);
   if (p.chunk < 1) p.chunk = 1;
+  if (p.stream && getenv("OD_CHUNK")) p.chunk = atoi(getenv("OD_CHUNK"));
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   if (p.nsplit < 1) p.nsplit = 1;
   return p;
@@ -1453,7 +1497,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     auto launch = [&](auto QC) {
       constexpr bool Q8 = decltype(QC)::value;
       if (p.stream) {
-        paged_stream_kernel<DD, Q8><<<dim3((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B), dim3(s_waves(DD) * 64), 0, st>>>(a);
+        paged_stream_kernel<DD, Q8><<<dim3((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B), dim3(kStreamWaves * 64), 0, st>>>(a);
       } else if (p.nw == 8) {
         rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
       } else if constexpr (DD != 256) {
@@ -1463,8 +1507,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     if (k_scale) launch(std::true_type{});
     else launch(std::false_type{});
     if (rc == OD_OK && p.nsplit > 1) {
-      const int heads = (kThreads / 64) * (64 / (DD / 8));
-      paged_combine_kernel<DD><<<dim3((unsigned)N, (unsigned)((Hq + heads - 1) / heads)), dim3(kThreads), 0, st>>>(a, p.width);
+      paged_combine_kernel<DD><<<dim3((unsigned)N, (unsigned)Hq), dim3(kThreads), 0, st>>>(a, p.width);
     }
   });
   return rc == OD_OK ? od_launch_status() : rc;
