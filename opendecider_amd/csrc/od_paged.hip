@@ -699,14 +699,16 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
   }
 }
 
-// The splits of a slot merged by log-sum-exp, a workgroup per packed row and head: 4 columns a thread, and 1024 / D groups of
-// threads that share the splits, so that up to 4096 / D of them are in flight together. `width`: keys per tile.
-template <int D>
+// The splits of a slot merged by log-sum-exp: 4 columns a thread, S groups of threads share a slot's splits, 4 of them in flight in
+// each. One group where there are few splits (chunks: many slots), all of a workgroup where there are many (decode steps: few
+// slots; 8 tokens over 32768, 8 splits, 7 us with one group, 4.5 with 8). `width`: keys per tile.
+template <int D, int S>
 __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int width) {
-  constexpr int C = D / 4, S = kThreads / C, AHEAD = 4;
-  __shared__ float4 so[S][C];
-  __shared__ float sml[S][2];
-  const int n = blockIdx.x, head = blockIdx.y, c = threadIdx.x % C, grp = threadIdx.x / C;
+  constexpr int C = D / 4, SL = kThreads / (C * S), AHEAD = 4;
+  __shared__ float4 so[SL][S][C];
+  __shared__ float sml[SL][S][2];
+  const int c = threadIdx.x % C, grp = threadIdx.x / C % S, sl = threadIdx.x / (C * S);
+  const int n = blockIdx.x, my = blockIdx.y * SL + sl, head = min(my, a.Hq - 1);  // every lane takes part in the search
   const int64_t slot = (int64_t)n * a.Hq + head, step = (int64_t)a.p.N * a.Hq;
   const float* ls = a.part + (int64_t)a.nsplit * step * D;
   const float* po = a.part + slot * D + 4 * c;
@@ -737,15 +739,18 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
     if (grp + i * S < nv) add(l4[i], 1.0f, u4[i]);
 #pragma unroll 4
   for (int sp = grp + AHEAD * S; sp < nv; sp += S) add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
-  so[grp][c] = acc;
-  if (c == 0) {
-    sml[grp][0] = M;
-    sml[grp][1] = L;
-  }
-  __syncthreads();
-  if (grp != 0) return;
+  if constexpr (S > 1) {
+    so[sl][grp][c] = acc;
+    if (c == 0) {
+      sml[sl][grp][0] = M;
+      sml[sl][grp][1] = L;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int k = 1; k < S; ++k) add(sml[k][0], sml[k][1], so[k][c]);
+    for (int k = 1; k < S; ++k)
+      if (grp == 0) add(sml[sl][k][0], sml[sl][k][1], so[sl][k][c]);
+  }
+  if (grp != 0 || my >= a.Hq) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + 4 * c) =
       make_uint2(od_pack_bf16x2(acc.x * inv, acc.y * inv), od_pack_bf16x2(acc.z * inv, acc.w * inv));
@@ -1507,7 +1512,9 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     if (k_scale) launch(std::true_type{});
     else launch(std::false_type{});
     if (rc == OD_OK && p.nsplit > 1) {
-      paged_combine_kernel<DD><<<dim3((unsigned)N, (unsigned)Hq), dim3(kThreads), 0, st>>>(a, p.width);
+      constexpr int S = 4 * kThreads / DD, SL = S;  // groups when a workgroup has one slot; slots when a slot has one group
+      if (p.nsplit > 4) paged_combine_kernel<DD, S><<<dim3((unsigned)N, (unsigned)Hq), dim3(kThreads), 0, st>>>(a, p.width);
+      else paged_combine_kernel<DD, 1><<<dim3((unsigned)N, (unsigned)((Hq + SL - 1) / SL)), dim3(kThreads), 0, st>>>(a, p.width);
     }
   });
   return rc == OD_OK ? od_launch_status() : rc;
