@@ -10,9 +10,8 @@
 // columns, a negative length and packed rows outside [0, N) are found by the kernels and skipped (no such key is seen, no
 // such row written). The host needs no copy of start, ctx or table.
 #include <type_traits>
-#include <stdlib.h>
 
-#include "/root/repo/opendecider_amd/csrc/od_common.h"
+#include "od_common.h"
 
 namespace {
 
@@ -1307,14 +1306,27 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // workgroups without splits: every sequence's tiles, but no more than the tokens make
   const int64_t all = N * rep / spt + B, wgs = (tiles * B < all ? tiles * B : all) * Hkv;
   const int64_t fit = p.stream || p.nw == 4 ? 2 * cus : cus;  // how many run at once
-  const int64_t least = p.stream ? 2 * p.nw : 8;             // key tiles that are worth a workgroup of their own
-  int64_t n = fit / (wgs < 1 ? 1 : wgs);
-  if (n > keys / least) n = keys / least;
-  if (n > 128) n = 128;
-  if (n < 1) n = 1;
+  const int64_t least = 8;                                    // key tiles that are worth a workgroup of their own
+  int64_t most = keys / least < 128 ? keys / least : 128, n = 1;
+  if (p.stream) {
+    n = fit / (wgs < 1 ? 1 : wgs);
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+  } else {
+    // the n of least cost: rounds of workgroups times a workgroup's blocks and what it costs besides them, about 12 blocks (the
+    // queries, the first loads, the new tokens, the partials). One round filled once: a chunk of 512 over 16000 takes 583 us whole, 223 in 3, 192 in 4, 234
+    // in 6 parts; 304 workgroups of 256-wide heads in 2 rounds 739 us, 608 of half the keys in 3 rounds 620, 4 parts 709.
+    int64_t best = 0;
+    for (int64_t i = 1; i <= most || i == 1; ++i) {
+      const int64_t cost = ((wgs * i + fit - 1) / fit) * ((keys + i - 1) / i + 12);
+      if (best == 0 || cost < best) {
+        best = cost;
+        n = i;
+      }
+    }
+  }
   p.chunk = (int)((keys + n - 1) / n);
   if (p.chunk < 1) p.chunk = 1;
-  if (p.stream && getenv("OD_CHUNK")) p.chunk = atoi(getenv("OD_CHUNK"));
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   if (p.nsplit < 1) p.nsplit = 1;
   return p;
