@@ -236,6 +236,7 @@ struct AttnArgs {
   float scale_log2;
   int nsplit, chunk;  // split sp takes the key tiles sp chunk .. of a sequence, the last split all that are left
   int tiles;          // slot tiles of a sequence that the grid covers (the workgroups go on from there)
+  int run;            // tiles that lie together on one XCD
 };
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -990,15 +991,17 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, HALVES = D == 256 ? 2 : 1, SPT = 32 * NW / HALVES, DT = D == 256 ? 4 : D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
-  // work item -> (sequence, KV head, split, slot tile), tiles fastest: workgroups are dealt round-robin over the 8 XCDs, and
-  // each takes a contiguous range of the items, so that the slot tiles of one (sequence, head) read its keys through one L2
-  const int total = gridDim.x, per = total >> 3, rem = total & 7, xcd = blockIdx.x & 7, loc = blockIdx.x >> 3;
-  int w = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
-  const int tile0 = w % a.tiles;
-  w /= a.tiles;
-  const int sp = w % a.nsplit;
-  w /= a.nsplit;
-  const int g = w % a.p.Hkv, b = w / a.p.Hkv;
+  // Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of its own. A group is the slot tiles of one (sequence,
+  // KV head, split), which read the same keys; its tiles go to one XCD in runs of `run` (a whole group, or a part of it where
+  // there are few groups), and the runs are dealt round-robin, each turn of 8 shifted by 3 against the last (else the first of two
+  // sequences of 4 heads, or every first split, would stay with half of the XCDs): contiguous ranges of the groups gave each XCD the sequences of a
+  // ragged batch as they came (4 ragged chunks of 256-wide heads 618 us, so 466). A causal tile's work grows with its index:
+  // last first (both: 4 ragged first chunks of 2000, 199 us, 124).
+  const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3, runs = (a.tiles + a.run - 1) / a.run;
+  const int turn = loc / a.run, rid = turn * 8 + ((xcd + 3 * turn) & 7), tile0 = a.tiles - 1 - (rid % runs * a.run + loc % a.run);
+  const int pairs = a.p.B * a.p.Hkv, pair = rid / runs % pairs, sp = rid / runs / pairs;
+  if (tile0 < 0 || sp >= a.nsplit) return;
+  const int g = pair % a.p.Hkv, b = pair / a.p.Hkv;
   const Seq s = seq_of(a, b);
   const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
   if (sp >= nv) return;
@@ -1292,13 +1295,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
   bool stream;
-  int nw, tiles, width, chunk, nsplit;
+  int nw, tiles, run, width, chunk, nsplit;
 };
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx) {
   Plan p;
   const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
   p.stream = slots <= 16;
-  p.nw = p.stream ? kStreamWaves : D == 256 || slots > 128 ? 8 : 4;
+  // 8 waves share a block's conversion at D = 128 (a chunk of 2048 over 32768: 1316 us, 4 waves 1515); at D = 64 they only
+  // coarsen the work (bf16 chunks of 2048 over 16000 234 us, 4 waves 202; int8 ones the same).
+  p.nw = p.stream ? kStreamWaves : D == 256 || (D == 128 && slots > 128) ? 8 : 4;
   p.width = p.stream ? 16 * s_halves((int)D) : kBK;
   const int64_t spt = p.stream ? 16 : D == 256 ? 128 : 32 * p.nw;
   const int64_t tiles = (slots + spt - 1) / spt, keys = (max_ctx + p.width - 1) / p.width;
@@ -1329,6 +1334,11 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   if (p.chunk < 1) p.chunk = 1;
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   if (p.nsplit < 1) p.nsplit = 1;
+  // runs of tiles: as many as give every XCD the same number, or a few each
+  const int64_t groups = B * Hkv * p.nsplit;
+  int parts = 1;
+  while (parts < 8 && groups * parts % 8 && groups * parts < 64) parts *= 2;
+  p.run = (p.tiles + parts - 1) / parts;
   return p;
 }
 
@@ -1504,9 +1514,11 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
   a.tiles = p.tiles;
+  a.run = p.run;
   if (n_pages == 0) a.p.cols = 0;
   hipStream_t st = (hipStream_t)stream;
-  const int64_t groups = (int64_t)p.tiles * p.nsplit * Hkv * B;
+  // tiles: every run of every group, a multiple of 8 runs
+  const int64_t runs = (p.tiles + p.run - 1) / p.run, groups = (p.nsplit * Hkv * B * runs + 7) / 8 * 8 * p.run;
   if (groups > 0x7fffffff || B > 65535) return OD_ERR_SHAPE;
   int rc = OD_OK;
   by_head_dim(D, [&](auto DC) {
@@ -1515,9 +1527,13 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
       constexpr bool Q8 = decltype(QC)::value;
       if (p.stream) {
         paged_stream_kernel<DD, Q8><<<dim3((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B), dim3(kStreamWaves * 64), 0, st>>>(a);
+      } else if constexpr (DD == 64) {
+        rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
+      } else if constexpr (DD == 256) {
+        rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
       } else if (p.nw == 8) {
         rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
-      } else if constexpr (DD != 256) {
+      } else {
         rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
       }
     };

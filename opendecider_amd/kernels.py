@@ -1022,38 +1022,55 @@ def gdn_norm_quant(o: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
 
 # ------------------------------------------------------------------------------------------------ paged K/V cache
 def _paged(cache, table, start, ctx_len, name):
-    """The arguments of a paged batch that every entry point takes, checked: (pages, table) and the sequence count."""
-    k = cache.k
+    """The arguments of a paged batch that every entry point takes, checked: the sequence count and (pages, table)."""
+    k, i32 = cache.k, torch.int32
     B = ctx_len.numel()
-    if table.dtype != torch.int32 or ctx_len.dtype != torch.int32 or (start is not None and start.dtype != torch.int32):
+    if table.dtype != i32 or ctx_len.dtype != i32 or (start is not None and start.dtype != i32):
         raise TypeError(f"{name}: table, start and the lengths must be int32")
     if table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{name}: table must be (sequences, pages per sequence) with contiguous rows, one row per length")
     if not ctx_len.is_contiguous() or (start is not None and (start.numel() != B + 1 or not start.is_contiguous())):
         raise ValueError(f"{name}: start must be (sequences + 1,) and the lengths (sequences,), contiguous")
-    dev = k.device
-    for t in (cache.v, table, ctx_len, start):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: all tensors must be on one device")
+    dev = k.get_device()
+    if table.get_device() != dev or ctx_len.get_device() != dev or cache.v.get_device() != dev or \
+            (start is not None and start.get_device() != dev):
+        raise ValueError(f"{name}: all tensors must be on one device")
     cols = table.shape[1]
     return B, (k.data_ptr(), ptr(cache.k_scale), cache.v.data_ptr(), ptr(cache.v_scale), k.shape[0], k.shape[2],
                table.data_ptr(), max(table.stride(0), cols) if B > 1 else cols, cols)
 
 
 def _new_rows(x, N, H, D, cache, name):
-    """bf16 rows (N, H, D) whose strides the 16-byte loads take (else a contiguous copy)."""
-    _lib.bf16_bits(x)
+    """bf16 rows (N, H, D), as they are where their strides and address suit the 16-byte loads, else copied; and the
+    pointer and strides (token, head) that the library takes."""
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected bfloat16, got {x.dtype}")
     if x.shape != (N, H, D):
         raise ValueError(f"{name}: expected {(N, H, D)}, got {tuple(x.shape)}")
-    if x.device != cache.k.device:
+    if x.get_device() != cache.k.get_device():
         raise ValueError(f"{name}: all tensors must be on one device")
-    x = _rows_aligned(x)
-    return x.clone() if x.data_ptr() % 16 else x  # contiguous rows at an odd address stay where they are above
+    st, sh, sd = x.stride()
+    if sd != 1 or st % 8 or sh % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st, sh = H * D, D
+    return x, (x.data_ptr(), st, sh)
 
 
-def _on_device(t: torch.Tensor):
-    """The tensor's device as the current one, for a library call (a launch goes to the current device)."""
-    return torch.cuda.device(t.device)
+class _OnDevice:
+    """The tensor's device as the current one for a library call (a launch goes to the current device); a switch only where
+    it is not (torch.cuda.device itself takes 1.3 us more)."""
+
+    def __init__(self, t: torch.Tensor):
+        i = t.get_device()
+        self.guard = None if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, start: torch.Tensor,
@@ -1067,9 +1084,10 @@ def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, st
     B, pages = _paged(cache, table, start, ctx_len, "page_append")
     _, H, _, D = cache.k.shape
     N = k.shape[0]
-    k, v = _new_rows(k, N, H, D, cache, "page_append: k"), _new_rows(v, N, H, D, cache, "page_append: v")
-    with _on_device(k):
-        check(lib().od_page_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *pages,
+    k, ka = _new_rows(k, N, H, D, cache, "page_append: k")
+    v, va = _new_rows(v, N, H, D, cache, "page_append: v")
+    with _OnDevice(k):
+        check(lib().od_page_append(*ka, *va, *pages,
                                    start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
 
 
@@ -1090,7 +1108,7 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
     ks = vs = None
     if dtype == torch.int8:
         ks, vs = (torch.empty(B, H, T, dtype=torch.float32, device=dev) for _ in range(2))
-    with _on_device(k):
+    with _OnDevice(k):
         check(lib().od_page_read(*pages, length.data_ptr(), B, T, H, D, forms[dtype], k.data_ptr(), ptr(ks), v.data_ptr(),
                                  ptr(vs), stream_of(k)), "od_page_read")
     if ks is None:
@@ -1129,31 +1147,36 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     B, pages = _paged(cache, table, start, ctx_len, "paged_attn")
     n_pages, H, page, D = cache.k.shape
     N, Hq = q.shape[0], q.shape[1]
-    q = _new_rows(q, N, Hq, D, cache, "paged_attn: q")
+    q, qa = _new_rows(q, N, Hq, D, cache, "paged_attn: q")
     if (k is None) != (v is None):
         raise ValueError("paged_attn: k and v come together")
     if Hq % H:
         raise ValueError(f"paged_attn: {Hq} query heads over {H} K/V heads")
     if not 0.0 < float(scale) < float("inf"):
         raise ValueError(f"paged_attn: the scale must be positive and finite, got {scale}")
-    kst = vst = (None, 0, 0)
+    ka = va = (None, 0, 0)
     if k is not None:
-        k, v = _new_rows(k, N, H, D, cache, "paged_attn: k"), _new_rows(v, N, H, D, cache, "paged_attn: v")
-        kst, vst = (k.data_ptr(), k.stride(0), k.stride(1)), (v.data_ptr(), v.stride(0), v.stride(1))
+        k, ka = _new_rows(k, N, H, D, cache, "paged_attn: k")
+        v, va = _new_rows(v, N, H, D, cache, "paged_attn: v")
     if row_begin is not None and (row_begin.dtype != torch.int32 or row_begin.numel() != N or
-                                  not row_begin.is_contiguous() or row_begin.device != q.device):
+                                  not row_begin.is_contiguous() or row_begin.get_device() != q.get_device()):
         raise ValueError("paged_attn: row_begin must be int32 (N,), contiguous, on the queries' device")
     most = table.shape[1] * page
     max_new = N if max_new is None else min(max(int(max_new), 0), N)
     max_ctx = most if max_ctx is None else min(max(int(max_ctx), 0), most)
-    given, out = out, _check_out(out, (N, Hq, D), q.device, "paged_attn")
-    dst = out if given is None or (not out.data_ptr() % 16 and not any(s % 8 for s in out.stride()[:2])) else \
-        torch.empty(N, Hq, D, dtype=out.dtype, device=out.device).copy_(out)
+    if out is None:
+        out = dst = torch.empty(N, Hq, D, dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, (N, Hq, D), q.device, "paged_attn")
+        if out.get_device() != q.get_device():
+            raise ValueError("paged_attn: all tensors must be on one device")
+        aligned = not (out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8)
+        dst = out if aligned else out.clone(memory_format=torch.contiguous_format)
     lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    with _on_device(q):
-        check(lib().od_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), *kst, *vst, *pages, start.data_ptr(),
+    with _OnDevice(q):
+        check(lib().od_paged_attn(*qa, *ka, *va, *pages, start.data_ptr(),
                                   ctx_len.data_ptr(), ptr(row_begin), dst.data_ptr(), dst.stride(0), dst.stride(1),
                                   ptr(lse), B, N, Hq, H, D, max_new, max_ctx, float(scale), ptr(ws), n, stream_of(q)),
               "od_paged_attn")
