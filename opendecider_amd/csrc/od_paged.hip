@@ -801,7 +801,8 @@ __device__ __forceinline__ uint32_t lds_addr(T* p) {
 // place there, (key, swizzled chunk), and copies the chunk that the swizzle puts into it. at(key): its row.
 template <int D, int NW, typename KeyRow>
 __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, KeyRow&& row) {
-  const int lane = threadIdx.x & 63;
+  int lane = threadIdx.x & 63;
+  if constexpr (D > 64) asm volatile("" : "+v"(lane));  // places are formed here each time, not kept in registers over the block loop
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i) {
     const int pe = (i * NW + wave) * 512 + 8 * lane, key = pe / D, slot = pe % D / 8;
@@ -986,22 +987,142 @@ __device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[D
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
   }
 }
+// Where a workgroup's work lies (sp < 0: nowhere). Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of its own.
+// A group is the slot tiles of one (sequence, KV head, split), which read the same keys; its tiles go to one XCD in runs of
+// `run` (a whole group, or a part of it where there are few groups), and the runs are dealt round-robin, each turn of 8 shifted by 3
+// against the last (else the first of two sequences of 4 heads, or every first split, would stay with half of the XCDs):
+// contiguous ranges of the groups gave each XCD the sequences of a ragged batch as they came (4 ragged chunks of 256-wide
+// heads 618 us, so 446). A causal tile's work grows with its index: last first (both: 4 ragged first chunks of 2000, 199
+// us, 124). Of up to 64 sequences the longest come first, so that the last workgroups to run are short ones (option rows of 8 ragged requests 158 us, 140).
+struct TilePlace {
+  int b, g, sp, tile;
+};
+__device__ __forceinline__ TilePlace tile_place(const AttnArgs& a) {
+  const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3, runs = (a.tiles + a.run - 1) / a.run, turn = loc / a.run;
+  const int rid = turn * 8 + ((xcd + 3 * turn) & 7), pairs = a.p.B * a.p.Hkv, pair = rid / runs % pairs;
+  TilePlace w;
+  w.tile = a.tiles - 1 - (rid % runs * a.run + loc % a.run);
+  w.sp = rid / runs / pairs;
+  w.g = pair % a.p.Hkv;
+  w.b = pair / a.p.Hkv;
+  if (w.tile < 0 || w.sp >= a.nsplit) w.sp = -1;
+  if (a.p.B > 1 && a.p.B <= 64) {  // the place among the sequences, longest first -> the sequence
+    const int lane = threadIdx.x & 63;
+    int64_t size = -1;
+    if (lane < a.p.B) size = (int64_t)max(a.p.ctx[lane], 0) + a.p.start[lane + 1] - a.p.start[lane];
+    const int key = (int)min(max(size, (int64_t)0), (int64_t)0x7fffffff);
+    int ahead = 0;
+    for (int i = 0; i < a.p.B; ++i) {
+      const int other = __builtin_amdgcn_readlane(key, i);
+      ahead += other > key || (other == key && i < lane);
+    }
+    w.b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.p.B && ahead == w.b));
+  }
+  return w;
+}
+
+// The new tokens that a slot tile sees: blocks lo .. hi - 1 of them. Of the wave's slots (w_) and the workgroup's (g_): the first
+// and last token that any sees (w_lo, w_hi), and the span that all see whole, w_in .. w_tok.
+struct NewSpan {
+  int lo, hi, w_lo, w_hi, w_in, w_tok, g_in, g_tok;
+  // a block that some slot of the workgroup sees only a part of
+  __device__ __forceinline__ bool partial(int blk) const { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; }
+};
+template <int D>
+__device__ __forceinline__ NewSpan new_span(const AttnArgs& a, const Seq& s, int tile, int spt, int zw, bool live, const TSlot<D>& t,
+                                            int* lo, int* hi, int* odd, int nw, int wave) {
+  const int lane = threadIdx.x & 63;
+  NewSpan n;
+  n.w_tok = min(zw / a.rep, s.n - 1);
+  n.w_hi = min((zw + 31) / a.rep, s.n - 1);
+  n.w_lo = n.w_in = 0;
+  if (a.row_begin) {
+    n.w_lo = t.ok ? t.begin : 0x7fffffff;
+    n.w_in = t.begin;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      n.w_lo = min(n.w_lo, __shfl_xor(n.w_lo, o, 64));
+      n.w_in = max(n.w_in, __shfl_xor(n.w_in, o, 64));
+    }
+  }
+  n.w_lo = __builtin_amdgcn_readfirstlane(n.w_lo);
+  n.w_in = __builtin_amdgcn_readfirstlane(n.w_in);
+  if (threadIdx.x == 0) *odd = 0;
+  if (lane == 0) {
+    lo[wave] = live ? n.w_lo : 0x7fffffff;
+    hi[wave] = live ? n.w_in : 0;
+  }
+  __syncthreads();
+  int g_lo = 0x7fffffff;
+  n.g_in = 0;
+  for (int i = 0; i < nw; ++i) {
+    g_lo = min(g_lo, lo[i]);
+    n.g_in = max(n.g_in, hi[i]);
+  }
+  n.g_tok = min(tile * spt / a.rep, s.n - 1);
+  const int g_hi = min((tile * spt + spt - 1) / a.rep, s.n - 1);
+  n.lo = min(g_lo, g_hi + 1) / kBK;
+  n.hi = g_hi / kBK + 1;
+  return n;
+}
+// A partly seen block's infinities and NaN become 0 (0 times one would reach the slots that do not see it) ...
+template <int D, int NT>
+__device__ __forceinline__ void make_finite(uint16_t* v, int* odd) {
+  for (int c = threadIdx.x; c < kBK * (D / 8); c += NT) {
+    uint4* at = reinterpret_cast<uint4*>(&v[8 * c]);
+    const v4u x = __builtin_bit_cast(v4u, *at);
+    if (any_inf_bf16x8(x)) {
+      *at = __builtin_bit_cast(uint4, fin_bf16x8(x));
+      *odd = 1;
+    }
+  }
+}
+// ... and the slots that see one get it added.
+template <int D>
+__device__ __forceinline__ void add_odd(const AttnArgs& a, const Seq& s, int g, int half, const NewSpan& n, TSlot<D>& t) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+  for (int key = max(n.lo * kBK, t.begin); key <= t.tok; ++key) {
+    if (!n.partial(key / kBK)) continue;
+    const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + half * 128 + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < (D == 256 ? 4 : D / 32); ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t.o[dt][i] += odd_bf16(vp[dt * 32 + 8 * (i >> 2) + (i & 3)]);
+  }
+}
+// out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
+template <int D, int DT>
+__device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, int frame, int sp, int nv, int half) {
+  if (!t.ok) return;
+  const int h = (threadIdx.x & 63) >> 5;
+  const float inv = l == 0.0f ? 0.0f : __builtin_ldexpf(1.0f / l, frame), ls = t.m + __log2f(l) - kLift;
+  const int64_t n = s.s0 + t.tok;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const int d0 = half * 128 + dt * 32 + 8 * i4 + 4 * h;
+      const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv, t.o[dt][4 * i4 + 3] * inv);
+      if (nv == 1)
+        *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y), od_pack_bf16x2(y.z, y.w));
+      else
+        *reinterpret_cast<float4*>(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0) = y;
+    }
+  if (h == 0 && half == 0) {
+    if (nv > 1) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + ((int64_t)sp * a.p.N + n) * a.Hq + t.head] = ls;
+    else if (a.lse) a.lse[n * a.Hq + t.head] = ls * kLn2;
+  }
+}
+
 template <int D, bool Q8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   constexpr int NT = NW * 64, HALVES = D == 256 ? 2 : 1, SPT = 32 * NW / HALVES, DT = D == 256 ? 4 : D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
-  // Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of its own. A group is the slot tiles of one (sequence,
-  // KV head, split), which read the same keys; its tiles go to one XCD in runs of `run` (a whole group, or a part of it where
-  // there are few groups), and the runs are dealt round-robin, each turn of 8 shifted by 3 against the last (else the first of two
-  // sequences of 4 heads, or every first split, would stay with half of the XCDs): contiguous ranges of the groups gave each XCD the sequences of a
-  // ragged batch as they came (4 ragged chunks of 256-wide heads 618 us, so 466). A causal tile's work grows with its index:
-  // last first (both: 4 ragged first chunks of 2000, 199 us, 124).
-  const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3, runs = (a.tiles + a.run - 1) / a.run;
-  const int turn = loc / a.run, rid = turn * 8 + ((xcd + 3 * turn) & 7), tile0 = a.tiles - 1 - (rid % runs * a.run + loc % a.run);
-  const int pairs = a.p.B * a.p.Hkv, pair = rid / runs % pairs, sp = rid / runs / pairs;
-  if (tile0 < 0 || sp >= a.nsplit) return;
-  const int g = pair % a.p.Hkv, b = pair / a.p.Hkv;
+  const TilePlace at = tile_place(a);
+  if (at.sp < 0) return;
+  const int sp = at.sp, g = at.g, b = at.b;
   const Seq s = seq_of(a, b);
   const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
   if (sp >= nv) return;
@@ -1016,7 +1137,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
-  for (int tile = tile0; tile * SPT < nslots; tile += a.tiles) {
+  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
     __syncthreads();  // an earlier tile's readers are done
     TSlot<D> t;
     const int zw = tile * SPT + (wave % (NW / HALVES)) * 32, z = zw + col;
@@ -1174,68 +1295,31 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
           frame = 0;
         }
       }
-      // what the wave's slots see: tokens w_lo .. w_hi at most; all of them see all of w_in .. w_tok
-      const int w_tok = min(zw / a.rep, s.n - 1), w_hi = min((zw + 31) / a.rep, s.n - 1);
-      int w_lo = 0, w_in = 0;
-      if (a.row_begin) {
-        w_lo = t.ok ? t.begin : 0x7fffffff;
-        w_in = t.begin;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-          w_lo = min(w_lo, __shfl_xor(w_lo, o, 64));
-          w_in = max(w_in, __shfl_xor(w_in, o, 64));
-        }
-      }
-      w_lo = __builtin_amdgcn_readfirstlane(w_lo);
-      w_in = __builtin_amdgcn_readfirstlane(w_in);
-      if (tid == 0) sm.odd = 0;
-      if (lane == 0) {
-        sm.lo[wave] = live ? w_lo : 0x7fffffff;
-        sm.hi[wave] = live ? w_in : 0;
-      }
-      __syncthreads();
-      int g_lo = 0x7fffffff, g_in = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        g_lo = min(g_lo, sm.lo[i]);
-        g_in = max(g_in, sm.hi[i]);
-      }
-      const int g_tok = min(tile * SPT / a.rep, s.n - 1), g_hi = min((tile * SPT + SPT - 1) / a.rep, s.n - 1);
-      const int o_lo = min(g_lo, g_hi + 1) / kBK, o_hi = g_hi / kBK + 1;
+      const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load = [&](int blk, int buf) {
         const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
         const uint16_t* vp = a.v + (int64_t)s.s0 * a.svt + (int64_t)g * a.svh;
         dma_rows<D, NW>(sm.k[buf], wave, false, [&](int key) { return kp + min(blk * kBK + key, s.n - 1) * a.skt; });
         dma_rows<D, NW>(sm.v[buf], wave, true, [&](int key) { return vp + min(blk * kBK + key, s.n - 1) * a.svt; });
       };
-      // a block that some slot of the workgroup sees only a part of
-      auto partial = [&](int blk) { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; };
-      // Such a block's infinities and NaN become 0 (0 times one would reach the slots that do not see it).
       auto finite = [&](int blk, int buf) {
-        if (!partial(blk)) return;
+        if (!n.partial(blk)) return;
         __syncthreads();  // every wave's part of the copy is there
-        for (int c = tid; c < kBK * (D / 8); c += NT) {
-          uint4* at = reinterpret_cast<uint4*>(&sm.v[buf][8 * c]);
-          const v4u x = __builtin_bit_cast(v4u, *at);
-          if (any_inf_bf16x8(x)) {
-            *at = __builtin_bit_cast(uint4, fin_bf16x8(x));
-            sm.odd = 1;
-          }
-        }
+        make_finite<D, NT>(sm.v[buf], &sm.odd);
       };
-      if (o_lo < o_hi) {
-        load(o_lo, 0);
+      if (n.lo < n.hi) {
+        load(n.lo, 0);
         dma_wait();
-        finite(o_lo, 0);
+        finite(n.lo, 0);
         __syncthreads();
-        for (int blk = o_lo; blk < o_hi; ++blk) {
-          const int cur = (blk - o_lo) & 1, j0 = blk * kBK;
-          if (blk + 1 < o_hi) load(blk + 1, cur ^ 1);
-          if (live && j0 <= w_hi && j0 + kBK > w_lo) {
+        for (int blk = n.lo; blk < n.hi; ++blk) {
+          const int cur = (blk - n.lo) & 1, j0 = blk * kBK;
+          if (blk + 1 < n.hi) load(blk + 1, cur ^ 1);
+          if (live && j0 <= n.w_hi && j0 + kBK > n.w_lo) {
             v16f sc[2];
             v4u pb[4];
             t_scores<D, false>(sm.k[cur], t, sc);
-            if (j0 + kBK - 1 > w_tok || j0 < w_in) {
+            if (j0 + kBK - 1 > n.w_tok || j0 < n.w_in) {
 #pragma unroll
               for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -1247,48 +1331,357 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
             t_softmax<D, false>(sc, a.scale_log2, t, pb);
             t_values<D, false>(sm.v[cur], vb, pb, t);
           }
-          if (blk + 1 < o_hi) {
+          if (blk + 1 < n.hi) {
             dma_wait();
             finite(blk + 1, cur ^ 1);
           }
           __syncthreads();
         }
-        // infinities and NaN that went in as 0: the slots that see one get it added
-        if (sm.odd && t.ok) {
-#pragma unroll 1
-          for (int key = max(o_lo * kBK, t.begin); key <= t.tok; ++key) {
-            if (!partial(key / kBK)) continue;
-            const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + half * 128 + 4 * h;
+        if (sm.odd && t.ok) add_odd<D>(a, s, g, half, n, t);
+      }
+    }
+
+    t_out<D, DT>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, half);
+  }
+}
+
+// ------------------------------------------------------------------------------------- many slots, heads of 256
+// 256 value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots: each
+// accumulates 128 of the columns. In the kernel above each of them takes all the scores; here each takes those of 32 of the
+// block's 64 keys, and its half of the softmax, and they exchange the maximum and the probabilities through LDS (as the
+// fragments that the products want): 32 instead of 48 matrix instructions a block and wave, half the exponentials. For that the
+// waves meet twice a block. K runs a block ahead of V, so that both meetings also order the buffers:
+//   scores(b) | maxima out, barrier | K(b + 2), V(b + 1) into the buffers of blocks that all are done with; softmax, probabilities
+//   out, barrier | products(b), scores(b + 1) ...
+struct alignas(16) WSmem {
+  uint16_t k[2][kBK * 256];
+  uint16_t v[2][kBK * 256];
+  v4u p[4][4][64];     // [slot group][k-step][lane]
+  float mx[2][4][32];  // [half][slot group][slot]
+  int lo[8], hi[8];
+  int odd;
+};
+
+template <bool Q8>
+__global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
+  constexpr int D = 256, NW = 8, NT = 512, SPT = 128, DT = 4;
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  WSmem& sm = *reinterpret_cast<WSmem*>(smem_raw);
+  const TilePlace at = tile_place(a);
+  if (at.sp < 0) return;
+  const int sp = at.sp, g = at.g, b = at.b;
+  const Seq s = seq_of(a, b);
+  const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
+  if (sp >= nv) return;
+  const int b_lo = sp * a.chunk, b_hi = sp == a.nsplit - 1 ? blocks : min(blocks, b_lo + a.chunk);
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, grp = wave & 3;
+  int vb[DT];  // transposing-read bases
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+  for (int dt = 0; dt < DT; ++dt) {
+    const int hh = lane >> 5, mh = (lane >> 4) & 1, e = (lane >> 2) & 3, c = lane & 3;
+    vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
+  }
+
+  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
+    __syncthreads();  // an earlier tile's readers are done
+    TSlot<D> t;
+    const int zw = tile * SPT + grp * 32, z = zw + col;
+    const bool live = zw < nslots;  // the wave has slots
+    t.ok = z < nslots;
+    t.tok = t.ok ? z / a.rep : s.n - 1;
+    t.head = g * a.rep + (t.ok ? z % a.rep : 0);
+    t.begin = a.row_begin && t.ok ? max(a.row_begin[s.s0 + t.tok], 0) : 0;
+    t.m = -INFINITY;
+    t.l = 0.0f;
+    t.qe = 0;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) t.o[dt][i] += odd_bf16(vp[dt * 32 + 8 * (i >> 2) + (i & 3)]);
+    for (auto& o : t.o) o = zero16();
+    t_load_q<D>(a, s, t);
+    int frame = 0;  // O is in units of 2^frame
+
+    // this wave's half of a block's scores: keys 32 half + 8 (i / 4) + 4 h + i % 4
+    auto scores = [&](auto H, const uint16_t* kb) {
+      v16f x = zero16();
+      v4u kf[2];
+      auto rd = [&](int i) {
+        kf[i % 2] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(&kb[tk_off<D>(half * 32 + col, 2 * i + h)]));
+      };
+      rd(0);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        if (i + 1 < D / 16) rd(i + 1);
+        x = mfma32<decltype(H)::value>(kf[i % 2], t.q[i], x);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // reads stay one ahead
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        if (i + 1 < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      return x;
+    };
+    // maxima out; after the barrier: the common maximum decides, the probabilities go out
+    auto put_max = [&](const v16f& x, float c) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[r]);
+      mx = od_xor32_max(mx) * c;
+      if (h == 0) sm.mx[half][grp][col] = mx;
+      return mx;
+    };
+    auto softmax = [&](auto H, const v16f& x, float c, float mine, v4u (&pb)[4]) {
+      const float mx = fmaxf(mine, sm.mx[half ^ 1][grp][col]);
+      const bool move = mx > t.m + kSlack;
+      if (__builtin_amdgcn_ballot_w64(move) != 0) {
+        const float f = move ? __builtin_amdgcn_exp2f(t.m - mx) : 1.0f;  // m = -inf: 0
+#pragma unroll
+        for (auto& o : t.o)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] *= f;
+        t.l *= f;
+        if (move) t.m = mx;
+      }
+      const float ms = (t.m == -INFINITY ? 0.0f : t.m) - kLift;
+      float sum = 0.0f;
+      v4u mp[2];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -ms));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r + 1], c, -ms));
+        sum += p0;
+        sum += p1;
+        if constexpr (decltype(H)::value) {
+          const f16x2 w = {(_Float16)p0, (_Float16)p1};
+          mp[r >> 3][(r & 7) >> 1] = __builtin_bit_cast(uint32_t, w);
+        } else {
+          mp[r >> 3][(r & 7) >> 1] = od_pack_bf16x2(p0, p1);
+        }
+      }
+      t.l += sum;  // this lane's share: its keys of this wave's half
+      sm.p[grp][2 * half][lane] = mp[0];
+      sm.p[grp][2 * half + 1][lane] = mp[1];
+    };
+    auto get_p = [&](v4u (&pb)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) pb[k] = sm.p[grp][k][lane];
+    };
+    auto rescale = [&](int f_new) {  // uniform over the workgroup
+      if (f_new == frame) return;
+      const float f = __builtin_ldexpf(1.0f, frame - f_new);
+#pragma unroll
+      for (auto& o : t.o)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] *= f;
+      frame = f_new;
+    };
+    using HT = std::integral_constant<bool, Q8>;
+
+    // ---- the cached blocks b_lo .. b_hi - 1
+    if (b_lo < b_hi) {
+      if constexpr (Q8) t_q_to_f16<D>(t);
+      constexpr int CPK = D / 16, NC = kBK * CPK / NT;  // int8: 16-byte chunks per row; per thread and side
+      const int in_page = (1 << a.p.shift) - 1;
+      // lane l: the page of key l of a block, or -1
+      auto pages = [&](int blk) {
+        const int pos = blk * kBK + lane;
+        const int pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
+        return pg < a.p.n_pages ? pg : -1;
+      };
+      auto row = [&](int blk, int pg, int key) {  // a key that is not there is read from page 0 and left out later
+        return (((int64_t)max(__shfl(pg, key, 64), 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + key) & in_page);
+      };
+      // int8: a block's K or V into registers, and lane l the scale of key l
+      // (the places below are formed each time: kept over the block loop they cost the kernel 60 spilled registers)
+      auto load8 = [&](int blk, int pg, const void* pool, const float* scales, v4u (&r)[NC], float& sc) {
+        int ti = tid;
+        asm volatile("" : "+v"(ti));
+        sc = scales[(((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & in_page)];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int key = (i * NT + ti) / CPK, ch = (i * NT + ti) % CPK;
+          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(pool) + row(blk, pg, key) * D + 16 * ch));
+        }
+      };
+      auto scale_bits = [&](int pg, float sc) {  // the largest scale of the block's keys that is a number, as bits
+        return od_wave_umax_dpp(pg >= 0 && sc < INFINITY && sc > 0 ? __float_as_uint(sc) : 0u);
+      };
+      auto put8 = [&](uint16_t* dst, bool v, const v4u (&r)[NC], float f) {
+        int ti = tid;
+        asm volatile("" : "+v"(ti));
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int key = (i * NT + ti) / CPK, ch = (i * NT + ti) % CPK;
+          v4u lo, hi;
+          __builtin_amdgcn_sched_barrier(0);
+          i8x16_scaled(r[i], __shfl(f, key, 64), lo, hi);
+          const int o0 = v ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
+          const int o1 = v ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
+          *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
+          *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
+        }
+      };
+      v4u rk[Q8 ? NC : 1], rv[Q8 ? NC : 1];
+      float ks = 0, vs = 0;
+      int ke0 = 0, ke1 = 0;  // the frames of the K blocks in the two buffers
+      int vexp = 0;          // the frame of the last V block stored
+      bool vexp_set = false;
+      auto store_k = [&](int blk, int pg) {
+        if constexpr (Q8) {
+          const int e = exp_above(scale_bits(pg, ks));
+          put8(sm.k[blk & 1], false, rk, pg >= 0 ? frame_scale(ks, 7 - e) : 0.0f);
+          if (blk & 1) ke1 = e;
+          else ke0 = e;
+        }
+      };
+      auto store_v = [&](int blk, int pg) {
+        if constexpr (Q8) {
+          const uint32_t bits = scale_bits(pg, vs);
+          if (bits) vexp = vexp_set ? max(vexp, exp_above(bits)) : exp_above(bits);
+          if (bits) vexp_set = true;
+          put8(sm.v[blk & 1], true, rv, pg >= 0 ? frame_scale(vs, 7 - vexp) : 0.0f);
+        }
+      };
+      auto load_k = [&](int blk, int pg) {
+        if constexpr (Q8) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
+        else dma_rows<D, NW>(sm.k[blk & 1], wave, false, [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(blk, pg, key) * D; });
+      };
+      auto load_v = [&](int blk, int pg) {
+        if constexpr (Q8) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
+        else dma_rows<D, NW>(sm.v[blk & 1], wave, true, [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(blk, pg, key) * D; });
+      };
+      // pages of the blocks blk (the current one), blk + 1, blk + 2, blk + 3; past the last block: none
+      int p0 = pages(b_lo), p1 = pages(b_lo + 1), p2 = pages(b_lo + 2), p3 = pages(b_lo + 3);
+      load_k(b_lo, p0);
+      load_v(b_lo, p0);
+      if constexpr (Q8) {
+        v4u rn[NC];
+        float sn;
+        load8(b_lo + 1, p1, a.p.k, a.p.ks, rn, sn);
+        store_k(b_lo, p0);
+        store_v(b_lo, p0);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) rk[i] = rn[i];
+        ks = sn;
+        store_k(b_lo + 1, p1);
+        load_k(b_lo + 2, p2);
+        load_v(b_lo + 1, p1);
+      } else {
+        load_k(b_lo + 1, p1);
+        dma_wait();
+      }
+      int f_cur = vexp - 7;
+      __syncthreads();
+      for (int blk = b_lo; blk < b_hi; ++blk) {
+        const float c = Q8 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + (blk & 1 ? ke1 : ke0) - 7) : a.scale_log2;
+        const uint64_t seen = __builtin_amdgcn_ballot_w64(p0 >= 0);
+        v16f x;
+        float mine = -INFINITY;
+        if (live) {
+          x = scores(HT{}, sm.k[blk & 1]);
+          if (seen != ~0ull) {
+            const uint64_t m4 = seen >> (32 * half + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!((m4 >> (8 * (i >> 2) + (i & 3))) & 1)) x[i] = -INFINITY;
           }
+          mine = put_max(x, c);
+        }
+        if constexpr (!Q8) dma_wait();  // this wave's part of V(blk) and K(blk + 1)
+        __syncthreads();
+        if (!Q8 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
+          for (int i = tid; i < kBK * (D / 8); i += NT)
+            if (!((seen >> (i / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
+        }
+        const int f_now = f_cur;
+        if constexpr (Q8) {
+          if (blk + 2 < b_hi) store_k(blk + 2, p2);
+          if (blk + 1 < b_hi) store_v(blk + 1, p1);
+          f_cur = vexp - 7;
+          if (blk + 3 < b_hi) load_k(blk + 3, p3);
+          if (blk + 2 < b_hi) load_v(blk + 2, p2);
+        } else {
+          if (blk + 2 < b_hi) load_k(blk + 2, p2);
+          if (blk + 1 < b_hi) load_v(blk + 1, p1);
+        }
+        p0 = p1;
+        p1 = p2;
+        p2 = p3;
+        p3 = pages(blk + 4);
+        v4u pb[4];
+        if (live) {
+          if constexpr (Q8) rescale(f_now);
+          softmax(HT{}, x, c, mine, pb);
+        }
+        __syncthreads();
+        if (live) {
+          get_p(pb);
+          t_values<D, Q8>(sm.v[blk & 1], vb, pb, t);
         }
       }
     }
 
-    // ---- out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
-    const float l = od_xor32_sum(t.l);
-    if (t.ok) {
-      const float inv = l == 0.0f ? 0.0f : __builtin_ldexpf(1.0f / l, frame), ls = t.m + __log2f(l) - kLift;
-      const int64_t n = s.s0 + t.tok;
+    // ---- the new tokens, in split 0
+    if (sp == 0 && a.k) {
+      if (Q8 && b_lo < b_hi) {  // back to bf16 queries and values as they are
+        t_load_q<D>(a, s, t);
+        rescale(0);
+      }
+      const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
+      auto load_k = [&](int blk) {
+        const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
+        dma_rows<D, NW>(sm.k[blk & 1], wave, false, [&](int key) { return kp + min(blk * kBK + key, s.n - 1) * a.skt; });
+      };
+      auto load_v = [&](int blk) {
+        const uint16_t* vp = a.v + (int64_t)s.s0 * a.svt + (int64_t)g * a.svh;
+        dma_rows<D, NW>(sm.v[blk & 1], wave, true, [&](int key) { return vp + min(blk * kBK + key, s.n - 1) * a.svt; });
+      };
+      if (n.lo < n.hi) {
+        load_k(n.lo);
+        load_v(n.lo);
+        if (n.lo + 1 < n.hi) load_k(n.lo + 1);
+        dma_wait();
+        __syncthreads();
+        for (int blk = n.lo; blk < n.hi; ++blk) {
+          const int j0 = blk * kBK;
+          const bool work = live && j0 <= n.w_hi && j0 + kBK > n.w_lo;
+          v16f x;
+          float mine = -INFINITY;
+          if (work) {
+            x = scores(std::false_type{}, sm.k[blk & 1]);
+            if (j0 + kBK - 1 > n.w_tok || j0 < n.w_in) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int d0 = half * 128 + dt * 32 + 8 * i4 + 4 * h;
-          const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv, t.o[dt][4 * i4 + 3] * inv);
-          if (nv == 1)
-            *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y), od_pack_bf16x2(y.z, y.w));
-          else
-            *reinterpret_cast<float4*>(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0) = y;
+              for (int i = 0; i < 16; ++i) {
+                const int key = j0 + half * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+                if (key > t.tok || key < t.begin) x[i] = -INFINITY;
+              }
+            }
+            mine = put_max(x, a.scale_log2);
+          }
+          dma_wait();
+          __syncthreads();
+          if (n.partial(blk)) make_finite<D, NT>(sm.v[blk & 1], &sm.odd);
+          if (blk + 2 < n.hi) load_k(blk + 2);
+          if (blk + 1 < n.hi) load_v(blk + 1);
+          v4u pb[4];
+          if (work) softmax(std::false_type{}, x, a.scale_log2, mine, pb);
+          __syncthreads();
+          if (work) {
+            get_p(pb);
+            t_values<D, false>(sm.v[blk & 1], vb, pb, t);
+          }
         }
-      if (h == 0 && half == 0) {
-        if (nv > 1) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + ((int64_t)sp * a.p.N + n) * a.Hq + t.head] = ls;
-        else if (a.lse) a.lse[n * a.Hq + t.head] = ls * kLn2;
+        if (sm.odd && t.ok) add_odd<D>(a, s, g, half, n, t);
       }
     }
+
+    // ---- the sum of both halves, then as above
+    float l = od_xor32_sum(t.l);
+    __syncthreads();  // the last block's maxima are read
+    if (h == 0) sm.mx[half][grp][col] = l;
+    __syncthreads();
+    l += sm.mx[half ^ 1][grp][col];
+    t_out<D, DT>(a, s, t, l, frame, sp, nv, half);
   }
 }
 
@@ -1361,21 +1754,23 @@ int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* 
   return OD_OK;
 }
 
-// The tile kernel's LDS is above 64 KB at D >= 128, which a launch has to be allowed once per device.
-template <int D, bool Q8, int NW>
-int launch_tiles(const AttnArgs& a, unsigned groups, hipStream_t st) {
-  constexpr int bytes = (int)sizeof(TSmem<D, NW>);
+// A launch with more than 64 KB of LDS, which a kernel has to be allowed once per device.
+template <auto* Kernel>
+int launch_big(const AttnArgs& a, unsigned groups, int threads, int bytes, hipStream_t st) {
   static std::atomic<uint64_t> allowed{0};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return OD_ERR_LAUNCH;
   if (!((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_tile_kernel<D, Q8, NW>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            bytes) != hipSuccess)
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
       return OD_ERR_LAUNCH;
     allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  paged_tile_kernel<D, Q8, NW><<<dim3(groups), dim3(NW * 64), bytes, st>>>(a);
+  Kernel<<<dim3(groups), dim3(threads), bytes, st>>>(a);
   return OD_OK;
+}
+template <int D, bool Q8, int NW>
+int launch_tiles(const AttnArgs& a, unsigned groups, hipStream_t st) {
+  return launch_big<&paged_tile_kernel<D, Q8, NW>>(a, groups, NW * 64, (int)sizeof(TSmem<D, NW>), st);
 }
 
 template <class F>
@@ -1530,7 +1925,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
       } else if constexpr (DD == 64) {
         rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
       } else if constexpr (DD == 256) {
-        rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
+        rc = launch_big<&paged_wide_kernel<Q8>>(a, (unsigned)groups, 512, (int)sizeof(WSmem), st);
       } else if (p.nw == 8) {
         rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
       } else {
