@@ -22,6 +22,7 @@ import torch
 
 from . import _lib, kernels
 from .kv_cache import GDNState, HybridState, Int8KVCache, StateKV
+from .paged_cache import PagedStates
 
 
 @dataclass
@@ -477,9 +478,95 @@ class DenseDecoder:
                 st.length = n0 + S
         return h
 
-    def _embed(self, ids: torch.Tensor) -> torch.Tensor:
-        """The tokens' embeddings, gathered straight into the residual buffer of their workspace (returned)."""
-        h = self.workspace(ids.numel())["h"][0]
+    # ---------------------------------------------------------------- paged states
+    def new_paged_states(self, batch: int, n_pages: int, max_tokens: int, page: int = 64,
+                         quantized: bool = True) -> PagedStates:
+        """`batch` empty states in pages (n_pages pages of `page` tokens per layer, at most max_tokens tokens a state): each
+        has its own length, takes pages as it grows (extend) and gives them back (PagedStates.release)."""
+        if self.hybrid:
+            raise ValueError("paged states hold attention layers only (a Gated DeltaNet layer's state has no tokens)")
+        cfg = self.cfg
+        return PagedStates(len(self.layers), batch, cfg.n_kv_heads, cfg.head_dim, n_pages, max_tokens, page, self.dev,
+                           quantized)
+
+    def _check_paged(self, states: PagedStates) -> None:
+        if not isinstance(states, PagedStates) or len(states) != len(self.layers) or states.batch < 1:
+            raise ValueError(f"expected the paged states of {len(self.layers)} layers (new_paged_states)")
+
+    def _paged_pass(self, ids: torch.Tensor, ws: dict, states: PagedStates, pos, start, max_new: int, row_begin=None,
+                    write: bool = False) -> torch.Tensor:
+        """Packed tokens ids (N,) through every layer, in ws of N rows: each attends its state's pages and the new tokens
+        of its state (from row_begin on) up to itself. write: their K and V go into the pages."""
+        cfg = self.cfg
+        D, Hq, Hk = cfg.head_dim, cfg.n_heads, cfg.n_kv_heads
+        N = ids.numel()
+        h, mid = ws["h"]
+        self._embed(ids, h)
+        max_ctx = max(states.lengths)
+        for li in range(len(self.layers)):
+            qkv = self._attn_in(li, h, ws, pos)
+            q, k, v = (qkv[:, a * D:b * D].view(N, b - a, D) for a, b in ((0, Hq), (Hq, Hq + Hk), (Hq + Hk, Hq + 2 * Hk)))
+            kernels.paged_attn(q, k, v, states[li], states.table, start, states.ctx, D ** -0.5, row_begin=row_begin,
+                               max_new=max_new, max_ctx=max_ctx, out=ws["attn"].view(N, Hq, D))
+            if write:
+                kernels.page_append(k, v, states[li], states.table, start, states.ctx)
+            self._attn_out_mlp(li, h, mid, ws)
+        return h
+
+    def extend(self, ids: torch.Tensor, counts, states: PagedStates) -> torch.Tensor:
+        """Appends counts[b] (0 or more, any length) new tokens to every state b: ids (sum of counts,) on the GPU, state
+        after state. The new tokens attend their state's cached tokens and each other causally, whatever the states hold;
+        their K and V go into pages taken from the pool. Returns their final hidden states (N, hidden), in a buffer that
+        a later call overwrites. MemoryError, with the states unchanged, where the pool has too few pages."""
+        self._check_paged(states)
+        counts = [int(n) for n in counts]
+        if ids.dim() != 1 or ids.numel() != sum(counts):
+            raise ValueError("extend: ids must be (sum of counts,)")
+        longest = max((t + n for t, n in zip(states.lengths, counts)), default=0)
+        if longest > self.cos.shape[0]:
+            raise ValueError(f"extend: positions up to {longest} exceed the rotary tables ({self.cos.shape[0]})")
+        states.reserve(counts)
+        N = ids.numel()
+        if N == 0:
+            return torch.empty(0, self.cfg.hidden, dtype=torch.bfloat16, device=self.dev)
+        start, max_new = kernels.row_start_of(counts, self.dev)
+        first = states.ctx - start[:-1]  # a token's position is its packed row plus this
+        pos = torch.arange(N, dtype=torch.int32, device=self.dev)
+        pos += torch.repeat_interleave(first, start[1:] - start[:-1], output_size=N)
+        # N is any number, call by call: buffers of the next power of two, so that few are kept
+        ws = {k: [x[:N] for x in b] if isinstance(b, list) else b[:N]
+              for k, b in self.workspace(1 << (N - 1).bit_length()).items() if k != "M"}
+        h = self._paged_pass(ids, ws, states, pos, start, max_new, write=True)
+        states.advance(counts)
+        return h
+
+    def score_paged(self, ids: torch.Tensor, states: PagedStates, pool_last: int | None = None) -> torch.Tensor:
+        """score over paged states of any lengths: ids (B, n_opt, t) option-row token ids on the GPU; a row's tokens follow
+        its state's own last one, and see the state and their own row. Nothing is written. Returns (B, n_opt + 1)
+        log-probabilities over the options and 'none'. Captured into a graph (after one eager call of the same sizes), it
+        scores whatever the states hold at the replay."""
+        self._check_paged(states)
+        B, n_opt, t = ids.shape
+        if B != states.batch or n_opt < 1 or t < 1:
+            raise ValueError(f"score_paged: ids must be ({states.batch}, options, tokens), got {tuple(ids.shape)}")
+        captured = torch.cuda.is_current_stream_capturing()  # then the states may grow to all that their table holds
+        longest = (states.cols * states.page if captured else max(states.lengths)) + t
+        if longest > self.cos.shape[0]:
+            raise ValueError(f"score_paged: positions up to {longest} exceed the rotary tables ({self.cos.shape[0]})")
+        per = n_opt * t
+        key = ("paged", B, n_opt, t)
+        if key not in self._rows:
+            i = torch.arange(per, dtype=torch.int32)
+            self._rows[key] = ((i % t).repeat(B).to(self.dev), (i // t * t).repeat(B).to(self.dev),
+                               kernels.row_start_of([per] * B, self.dev, kept=True)[0])
+        in_row, row_begin, start = self._rows[key]
+        pos = in_row + states.ctx.repeat_interleave(per, output_size=B * per)
+        h = self._paged_pass(ids, self.workspace(B * per), states, pos, start, per, row_begin)
+        return self.readout(h, B, n_opt, t, pool_last)
+
+    def _embed(self, ids: torch.Tensor, h: torch.Tensor | None = None) -> torch.Tensor:
+        """The tokens' embeddings, gathered straight into the residual buffer of their workspace (returned) or into h."""
+        h = self.workspace(ids.numel())["h"][0] if h is None else h
         if self.embed.dtype == h.dtype and not self.embed.requires_grad and _lib.unwatched(self.embed):
             return torch.index_select(self.embed, 0, ids.reshape(-1), out=h)
         return h.copy_(self.embed.index_select(0, ids.reshape(-1)))

@@ -418,6 +418,16 @@ def row_start_of(row_counts, device, kept: bool = False) -> tuple[torch.Tensor, 
     return out, max(counts)
 
 
+def fill_i32(values, out: torch.Tensor) -> None:
+    """Host ints into a contiguous int32 tensor, as kernel arguments on the current stream (no host-to-device copy, which
+    waits for the stream's earlier work)."""
+    if out.dtype != torch.int32 or not out.is_contiguous() or out.numel() != len(values):
+        raise ValueError("fill_i32: out must be contiguous int32 with one element per value")
+    host = torch.tensor(values, dtype=torch.int32)
+    with _OnDevice(out):
+        check(lib().od_fill_i32(host.data_ptr(), len(values), out.data_ptr(), stream_of(out)), "od_fill_i32")
+
+
 def split_count(slot_tiles: int, T: int, n_cu: int = 256, wg_per_cu: int = 2, min_blocks: int = 4) -> int:
     """Key-range splits for the block-image paths (od_branched_attn_split / _staged / _staged2): with few slot tiles
     over a long state, n splits of `slot_tiles` workgroups cost ceil(slot_tiles n / (n_cu wg_per_cu)) rounds of

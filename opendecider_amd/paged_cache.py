@@ -113,7 +113,7 @@ class PagedStates:
                 got = [self.free.pop() for _ in range(n)]
                 at = len(self.pages[b])
                 self.pages[b] += got
-                self.table[b, at:at + n] = torch.tensor(got, dtype=torch.int32).to(self.table.device)
+                self._put(self.table[b, at:at + n], got)
 
     def advance(self, counts) -> None:
         """Counts the tokens that every layer has written since reserve."""
@@ -135,7 +135,14 @@ class PagedStates:
         self._write_ctx()
 
     def _write_ctx(self) -> None:
-        self.ctx.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+        self._put(self.ctx, self.lengths)
+
+    @staticmethod
+    def _put(out: torch.Tensor, values: list) -> None:
+        if out.is_cuda:
+            kernels.fill_i32(values, out)
+        else:
+            out.copy_(torch.tensor(values, dtype=torch.int32))
 
     def read(self, li: int, dtype=torch.bfloat16):
         """Layer li's cached K and V as dense (batch, Hkv, T, D), T the longest state (kernels.page_read)."""

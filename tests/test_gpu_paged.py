@@ -403,6 +403,139 @@ def test_on_another_stream(gpu_lib):
     assert torch.equal(got, want)
 
 
+# ------------------------------------------------------------------------------------------------ in the decoder
+CFG = dict(hidden=256, ffn=512, n_heads=8, n_kv_heads=2, head_dim=64, n_layers=2, vocab=300)
+
+
+def recorded(monkeypatch, name):
+    """Every call of a kernels function with its arguments and result, tensors copied."""
+    from opendecider_amd import kernels
+    calls, fn = [], getattr(kernels, name)
+    keep = lambda x: x.clone() if isinstance(x, torch.Tensor) else x
+
+    def wrap(*a, **kw):
+        held = [keep(x) for x in a], {k: keep(v) for k, v in kw.items()}
+        if name == "paged_attn":
+            c = a[3]
+            held[0][3] = [keep(x) for x in (c.k, c.v, c.k_scale, c.v_scale)]
+        res = fn(*a, **kw)
+        calls.append((*held, keep(res)))
+        return res
+
+    monkeypatch.setattr(kernels, name, wrap)
+    return calls
+
+
+def check_calls(calls):
+    for (q, k, v, pages, table, start, ctx, scale), kw, out in calls:
+        cpu = lambda x: None if x is None else x.cpu()
+        c = dict(q=q.cpu(), k=k.cpu(), v=v.cpu(), pages=[cpu(pages[0]), cpu(pages[1])], scales=[cpu(pages[2]), cpu(pages[3])],
+                 table=table.cpu(), start=start.cpu(), ctx=ctx.cpu(), scale=scale, row_begin=cpu(kw["row_begin"]))
+        _, lse, _, _, _ = op.attention(c["q"], c["k"], c["v"], (*c["pages"], *c["scales"]), c["table"], c["start"], c["ctx"], scale,
+                                       c["row_begin"])
+        check_attn(c, out, lse)
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("gated", [False, True])
+def test_decoder_over_pages(gpu_lib, monkeypatch, quantized, gated):
+    """Ragged states grow in chunks of any length, end, and score their options. Layer 0's inputs to the attention and the bytes
+    in its pages equal the rectangular path's for the same tokens at the same positions; every attention call is right for
+    its own inputs (the rest of a layer is the rectangular path's code); a state that another one's end made room for works."""
+    from opendecider_amd import kernels
+    from opendecider_amd.decoder import DecoderConfig, random_decoder
+    dec = random_decoder(DecoderConfig(gated=gated, **CFG), seed=1, max_pos=512)
+    g = torch.Generator().manual_seed(2)
+    tok = lambda n: torch.randint(0, 300, (n,), generator=g).to(DEV)
+    states = dec.new_paged_states(3, n_pages=15, max_tokens=400, page=32, quantized=quantized)
+    calls = recorded(monkeypatch, "paged_attn")
+    parts = [[tok(70), tok(0), tok(5)], [tok(1), tok(1), tok(1)], [tok(0), tok(40), tok(300)]]
+    for part in parts:
+        h = dec.extend(torch.cat(part), [p.numel() for p in part], states)
+        assert h.shape == (sum(p.numel() for p in part), 256) and torch.isfinite(h.float()).all()
+    assert states.lengths == [71, 41, 306] and states.ctx.tolist() == [71, 41, 306]
+    ids = torch.randint(0, 300, (3, 4, 5), generator=g).to(DEV)
+    before = states[1].k.clone()
+    lp = dec.score_paged(ids, states)
+    assert lp.shape == (3, 5) and torch.allclose(lp.exp().sum(1), torch.ones(3, device=DEV), atol=1e-5)
+    assert torch.equal(states[1].k, before)
+    check_calls(calls)
+    # layer 0 against the rectangular path, state by state
+    old = recorded(monkeypatch, "branched_attn")
+    for b in range(3):
+        whole = torch.cat([p[b] for p in parts])
+        flat = dec.new_state_caches(1, 400)
+        dec.prefill(whole[None], flat)
+        T = whole.numel()
+        if quantized:
+            k, v = kernels.page_read(states[0], states.table, states.ctx, 306, dtype=torch.int8)
+            for x, c in ((k, flat[0][0]), (v, flat[0][1])):
+                assert torch.equal(x.q[b, :, :T], c.q[0, :, :T]) and torch.equal(x.scale[b, :, :T, 0], c.scale[0, :, :T])
+        old.clear()
+        dec.score(ids[b:b + 1], flat)
+        (q, k, v), score0 = old[0][0][:3], calls[-2][0]
+        for want, got in ((q, score0[0]), (k, score0[1]), (v, score0[2])):
+            assert torch.equal(want.transpose(1, 2).reshape(20, -1, 64), got[20 * b:20 * b + 20])
+    # no room: nothing changes; after a state's end there is
+    with pytest.raises(MemoryError):
+        dec.extend(tok(50), [50, 0, 0], states)
+    assert states.lengths == [71, 41, 306]
+    states.release(2)
+    dec.extend(tok(80), [50, 0, 30], states)
+    assert states.lengths == [121, 41, 30] and torch.isfinite(dec.score_paged(ids, states)).all()
+    del calls[:-4]
+    check_calls(calls)
+    for bad in (lambda: dec.extend(tok(3), [1, 1, 2], states), lambda: dec.extend(tok(500), [500, 0, 0], states),
+                lambda: dec.score_paged(ids[:2], states)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_captured_scoring_follows_the_states(gpu_lib, monkeypatch):
+    """One graph of a scoring pass over paged states, replayed as they grow, end and start anew: bit for bit the eager calls
+    with the graph's hint of the lengths (by which the keys are split, and so summed)."""
+    from opendecider_amd import kernels
+    from opendecider_amd.decoder import DecoderConfig, random_decoder
+    dec = random_decoder(DecoderConfig(**CFG), seed=3, max_pos=512)
+    g = torch.Generator().manual_seed(4)
+    tok = lambda n: torch.randint(0, 300, (n,), generator=g).to(DEV)
+    states = dec.new_paged_states(2, n_pages=20, max_tokens=448, page=32)
+    ids = tok(2 * 3 * 4).view(2, 3, 4)
+    dec.extend(tok(40), [33, 7], states)
+    dec.score_paged(ids, states)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lp = dec.score_paged(ids, states)
+    for counts in ([0, 0], [1, 200], [90, 1], None, [60, 0]):
+        if counts is None:
+            states.release(0)
+        else:
+            dec.extend(tok(sum(counts)), counts, states)
+        ids.copy_(tok(24).view(2, 3, 4))
+        graph.replay()
+        got = lp.clone()
+        with monkeypatch.context() as m:
+            fn = kernels.paged_attn
+            m.setattr(kernels, "paged_attn", lambda *a, max_ctx, **kw: fn(*a, max_ctx=33, **kw))
+            want = dec.score_paged(ids, states)
+        assert torch.equal(got, want) and torch.isfinite(got).all()
+        graph.replay()
+        assert torch.equal(lp, got)
+    small = dec.new_paged_states(2, n_pages=4, max_tokens=512, page=32)  # its table holds more than the rotary tables
+    dec.score_paged(ids, small)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError):
+        dec.score_paged(ids, small)
+
+
+def test_hybrid_has_no_paged_states(gpu_lib):
+    from opendecider_amd.decoder import DecoderConfig, random_decoder
+    dec = random_decoder(DecoderConfig(hidden=256, ffn=512, n_heads=4, n_kv_heads=2, head_dim=64, n_layers=2, vocab=50,
+                                       full_attention_interval=2, lin_k_heads=2, lin_v_heads=2), max_pos=64)
+    with pytest.raises(ValueError):
+        dec.new_paged_states(1, 2, 32)
+
+
 def test_refusals(gpu_lib):
     from opendecider_amd import PagedKVCache, kernels
     c = make(52, [4, 3], [20, 5])
