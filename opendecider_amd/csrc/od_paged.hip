@@ -1,14 +1,14 @@
 // A paged K/V cache, for gfx950: new tokens written into pages, sequences read back, attention over pages.
 //
-// Layout. A layer's K and V are two pools of n_pages pages; page p holds `page` (a power of two >= 16) token rows of every
-// KV head, [n_pages, Hkv, page, D], int8 with one fp32 scale per row ([n_pages, Hkv, page]) or bf16. Position j of sequence
-// b is row j % page of page table[b, j / page]. A (page, head) block is contiguous, so that an attention workgroup of one
-// head reads whole runs of `page` rows. Batches are packed and ragged: sequence b's new tokens are the packed rows
-// start[b] .. start[b + 1] - 1, at the positions ctx[b], ctx[b] + 1, ...
+// Layout. A layer's K and V are two pools of n_pages pages; page p holds `page` (a power of two >= 16) token rows of
+// every KV head, [n_pages, Hkv, page, D], int8 with one fp32 scale per row ([n_pages, Hkv, page]) or bf16. Position j
+// of sequence b is row j % page of page table[b, j / page]. A (page, head) block is contiguous, so that an attention
+// workgroup of one head reads whole runs of `page` rows. Batches are packed and ragged: sequence b's new tokens are the
+// packed rows start[b] .. start[b + 1] - 1, at the positions ctx[b], ctx[b] + 1, ...
 //
 // Nothing on the device is trusted to stay in bounds: a table entry outside [0, n_pages), a position past the table's
-// columns, a negative length and packed rows outside [0, N) are found by the kernels and skipped (no such key is seen, no
-// such row written). The host needs no copy of start, ctx or table.
+// columns, a negative length and packed rows outside [0, N) are found by the kernels and skipped (no such key is seen,
+// no such row written). The host needs no copy of start, ctx or table.
 #include <type_traits>
 
 #include "od_common.h"
@@ -32,23 +32,12 @@ struct Paged {
   int cols, shift, B, N, Hkv;  // page = 1 << shift
 };
 
-// First row (over all heads of the pool) of the page that holds position `pos` of sequence b for head h, plus the row in
-// the page: the index of a token row of D values and of its scale. -1: no such page.
+// First row (over all heads of the pool) of the page that holds position `pos` of sequence b for head h, plus the row
+// in the page: the index of a token row of D values and of its scale. -1: no such page.
 __device__ __forceinline__ int64_t row_of(const Paged& p, int b, int h, int64_t pos) {
   const int64_t col = pos >> p.shift;
   if (pos < 0 || col >= p.cols) return -1;
   const int pg = p.table[b * p.ld_table + col];
-  if (pg < 0 || pg >= p.n_pages) return -1;
-  return (((int64_t)pg * p.Hkv + h) << p.shift) + (pos & ((1 << p.shift) - 1));
-}
-
-// A load at a wave-uniform address through the scalar path, whose wait does not include the vector loads in flight.
-__device__ __forceinline__ int uniform_load(const int32_t* p) {
-  return *(__attribute__((address_space(4))) const int32_t*)(uintptr_t)p;
-}
-// row_of for wave-uniform arguments
-__device__ __forceinline__ int64_t uniform_row_of(const Paged& p, int b, int h, int pos) {
-  const int pg = uniform_load(p.table + b * p.ld_table + (pos >> p.shift));
   if (pg < 0 || pg >= p.n_pages) return -1;
   return (((int64_t)pg * p.Hkv + h) << p.shift) + (pos & ((1 << p.shift) - 1));
 }
@@ -135,8 +124,8 @@ __global__ __launch_bounds__(kThreads) void page_append_kernel(AppendArgs a) {
 
 // --------------------------------------------------------------------------------------------------------- read
 // Dense (B, Hkv, T, D) K and V of every sequence's first ctx[b] tokens, zeros behind them: the values q * s (one fp32
-// product, rounded once to bf16 where that is asked), bf16 rows as they are, or the int8 rows with their scales. A group
-// of G = D / 16 lanes takes one token row of K and the same of V (16 values per lane). Bound by memory.
+// product, rounded once to bf16 where that is asked), bf16 rows as they are, or the int8 rows with their scales. A
+// group of G = D / 16 lanes takes one token row of K and the same of V (16 values per lane). Bound by memory.
 struct ReadArgs {
   Paged p;
   void* k;
@@ -219,9 +208,9 @@ __global__ __launch_bounds__(kThreads) void page_read_kernel(ReadArgs a) {
 // row_begin[n] .. i of its own sequence (row_begin null: from 0), bf16 as they come: o = sum_j p_j v_j / sum_j p_j with
 // p_j = exp(scale q.k_j - max), lse = max + log sum p; a token that sees nothing has o = 0 and lse = -inf.
 //
-// A "slot" is a (new token, head of the KV group) pair: slot z of a sequence is token z / rep, head g rep + z % rep. Both
-// kernels go over the keys once with a running maximum m and sum l in fp32 (log2 units). m moves only when a block's maximum
-// lies more than 2^kSlack above it, so most blocks do not rescale the output: p <= 2^kSlack.
+// A "slot" is a (new token, head of the KV group) pair: slot z of a sequence is token z / rep, head g rep + z % rep.
+// Both kernels go over the keys once with a running maximum m and sum l in fp32 (log2 units). m moves only when a
+// block's maximum lies more than 2^kSlack above it, so most blocks do not rescale the output: p <= 2^kSlack.
 struct AttnArgs {
   Paged p;
   const uint16_t* q;
@@ -276,7 +265,9 @@ __device__ __forceinline__ v4u fin_bf16x8(v4u w) {
   return v4u{fin_bf16x2(w[0]), fin_bf16x2(w[1]), fin_bf16x2(w[2]), fin_bf16x2(w[3])};
 }
 // a bf16 that is infinite or NaN, as fp32; else 0
-__device__ __forceinline__ float odd_bf16(uint32_t b) { return (b & 0x7f80u) == 0x7f80u ? __uint_as_float(b << 16) : 0.0f; }
+__device__ __forceinline__ float odd_bf16(uint32_t b) {
+  return (b & 0x7f80u) == 0x7f80u ? __uint_as_float(b << 16) : 0.0f;
+}
 __device__ __forceinline__ bool any_inf_bf16x8(v4u w) {
   uint32_t m = 0;
 #pragma unroll
@@ -286,29 +277,33 @@ __device__ __forceinline__ bool any_inf_bf16x8(v4u w) {
 
 // 4 int8 -> 4 exact bf16: |q| <= 128 has at most 8 significant bits, so the top half of the fp32 value is it
 __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t f0 = __float_as_uint((float)(int8_t)(w & 0xffu)), f1 = __float_as_uint((float)(int8_t)((w >> 8) & 0xffu));
-  const uint32_t f2 = __float_as_uint((float)(int8_t)((w >> 16) & 0xffu)), f3 = __float_as_uint((float)(int8_t)(w >> 24));
+  const uint32_t f0 = __float_as_uint((float)(int8_t)(w & 0xffu)),
+      f1 = __float_as_uint((float)(int8_t)((w >> 8) & 0xffu));
+  const uint32_t f2 = __float_as_uint((float)(int8_t)((w >> 16) & 0xffu)),
+      f3 = __float_as_uint((float)(int8_t)(w >> 24));
   lo = __builtin_amdgcn_perm(f1, f0, 0x07060302u);
   hi = __builtin_amdgcn_perm(f3, f2, 0x07060302u);
 }
 
 // ------------------------------------------------------------------------------------------ few slots: streaming
-// Up to 16 slots of a (sequence, KV head): decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of int8 K and V: bound by
-// reading the pages. A wave holds all 16 slots as the columns of V_MFMA_F32_16X16X32_BF16 and takes 32-key tiles straight
-// from memory into registers; the waves of a workgroup take every NW-th tile of the split's range and merge in LDS.
-// Lane (j, g) = (lane % 16, lane / 16):
-//  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: the four lanes of a key read 64 contiguous bytes of it at a time
-//    (s_dim: a permutation of the reduction index, the same on both sides; reading D / 4 contiguous values per lane instead
-//    took 101 against 76 us for the loads of 16 x 8000 bf16 tokens); int8 values enter as exact bf16 integers and the
-//    score takes the fp32 factor ks_j. The result gives lane (j, g) slot j and keys 16 kr + 4 g + i;
-//  * O^T[dt] += V^T[dt] P^T with output row r of d tile dt being d = (D / 16) r + dt and the keys in the order 4 g + i (i < 4),
-//    12 + 4 g + i: the B operand is the lane's own 8 probabilities, the A operand value dt of the D / 16 contiguous values it
-//    reads of each of those keys. P (times vs_j) enters as bf16 hi + lo parts, 16 significant bits: the columns of the
-//    matrix instructions are mostly empty here, and no scale of the values can leave the range.
-// Half tiles are reached through buffer descriptors of their own (a half tile never crosses a page), whose length ends at
-// the last cached token: what lies behind reads as zeros. Two register sets: a tile's loads are all issued before the
-// products of the tile ahead of it, unconditionally (past a wave's last tile with descriptors of no length, so that the waits are counted but nothing is read). Rows of 256 go in tiles of one half (R = 1): two sets of whole
-// ones do not fit the registers (16 x 8000 tokens 62 us, 49 with halves); bf16 ones then still take a SIMD alone.
+// Up to 16 slots of a (sequence, KV head): decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of int8 K and V:
+// bound by reading the pages. A wave holds all 16 slots as the columns of V_MFMA_F32_16X16X32_BF16 and takes 32-key
+// tiles straight from memory into registers; the waves of a workgroup take every NW-th tile of the split's range and
+// merge in LDS. Lane (j, g) = (lane % 16, lane / 16):
+//  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: the four lanes of a key read 64 contiguous bytes of it at
+//    a time (s_dim: a permutation of the reduction index, the same on both sides; reading D / 4 contiguous values per
+//    lane instead took 101 against 76 us for the loads of 16 x 8000 bf16 tokens); int8 values enter as exact bf16
+//    integers and the score takes the fp32 factor ks_j. The result gives lane (j, g) slot j and keys 16 kr + 4 g + i;
+//  * O^T[dt] += V^T[dt] P^T with output row r of d tile dt being d = (D / 16) r + dt and the keys in the order 4 g + i
+//    (i < 4), 12 + 4 g + i: the B operand is the lane's own 8 probabilities, the A operand value dt of the D / 16
+//    contiguous values it reads of each of those keys. P (times vs_j) enters as bf16 hi + lo parts, 16 significant
+//    bits: the columns of the matrix instructions are mostly empty here, and no scale of the values can leave the
+//    range.
+// Half tiles are reached through buffer descriptors of their own (a half tile never crosses a page), whose length ends
+// at the last cached token: what lies behind reads as zeros. Two register sets: a tile's loads are all issued before
+// the products of the tile ahead of it, unconditionally (past a wave's last tile with descriptors of no length, so that
+// the waits are counted but nothing is read). Rows of 256 go in tiles of one half (R = 1): two sets of whole ones do
+// not fit the registers (16 x 8000 tokens 62 us, 49 with halves); bf16 ones then still take a SIMD alone.
 constexpr int s_halves(int D) { return D == 256 ? 1 : 2; }
 template <int D, bool Q8>
 struct STile {
@@ -322,15 +317,17 @@ struct STile {
 
 // first of the 8 dims that lanes of group g hold in k-step ks
 template <bool Q8>
-__device__ __forceinline__ int s_dim(int g, int ks) { return Q8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
+__device__ __forceinline__ int s_dim(int g, int ks) {
+  return Q8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
+}
 
 constexpr int kOnce = 2;  // non-temporal: each byte is read once
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
 }
 
-// The pages of 64 / R tiles of a wave, one load: lane l has the page of half tile l % R of the wave's tile number l / R from
-// here (`pos` of tile 0, `step` positions from tile to tile; -1: no key or no page).
+// The pages of 64 / R tiles of a wave, one load: lane l has the page of half tile l % R of the wave's tile number l / R
+// from here (`pos` of tile 0, `step` positions from tile to tile; -1: no key or no page).
 template <int R>
 __device__ __forceinline__ int s_pages(const Paged& p, int b, int pos, int step) {
   const int l = threadIdx.x & 63;
@@ -338,9 +335,11 @@ __device__ __forceinline__ int s_pages(const Paged& p, int b, int pos, int step)
   const int pg = col < p.cols ? p.table[b * p.ld_table + col] : -1;
   return pg < p.n_pages ? pg : -1;
 }
-// A tile's loads, its pages in place `nth` of `pages`. Lane l takes the scales of key l % 32, each 16 lanes their half tile's.
+// A tile's loads, its pages in place `nth` of `pages`. Lane l takes the scales of key l % 32, each 16 lanes their half
+// tile's.
 template <int D, bool Q8>
-__device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth, STile<D, Q8>& x) {
+__device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth,
+                                       STile<D, Q8>& x) {
   using T = STile<D, Q8>;
   constexpr int E = Q8 ? 1 : 2;
   const int lane = threadIdx.x & 63, j = lane & 15, gl = lane >> 4;
@@ -353,7 +352,8 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
     const auto dk = rsrc(static_cast<const char*>(a.p.k) + row[r] * (D * E), x.len[r] * (D * E));
 #pragma unroll
     for (int w = 0; w < T::KW; ++w)
-      x.k[r][w] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(dk, j * D * E + 64 * w + 16 * gl, 0, kOnce));
+      x.k[r][w] = __builtin_bit_cast(
+          v4u, __builtin_amdgcn_raw_buffer_load_b128(dk, j * D * E + 64 * w + 16 * gl, 0, kOnce));
     const auto dv = rsrc(static_cast<const char*>(a.p.v) + row[r] * (D * E), x.len[r] * (D * E));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -376,9 +376,10 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
   }
   if constexpr (Q8) {
     // a lane's own row: one descriptor cannot reach both half tiles, so lanes without a key read the pool's first scale
+    constexpr int kUpper = T::R - 1;  // tiles of one half: lanes 16 .. 31 take the same keys as 0 .. 15
     const int c = lane & 31;
-    const bool in = (c & 15) < (c < 16 ? x.len[0] : x.len[1]);
-    const int64_t at = in ? (c < 16 ? row[0] : row[1]) + (c & 15) : 0;
+    const bool in = (c & 15) < (c < 16 ? x.len[0] : x.len[kUpper]);
+    const int64_t at = in ? (c < 16 ? row[0] : row[kUpper]) + (c & 15) : 0;
     const float k1 = a.p.ks[at], v1 = a.p.vs[at];
     x.ks = in ? k1 : 0.0f;
     x.vs = in ? v1 : 0.0f;
@@ -386,7 +387,8 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
 }
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
 }
 
 // The slot state of a lane: column j's running max and its share of the sum, output rows 4 g + i of every d tile.
@@ -396,8 +398,8 @@ struct SAcc {
   v4f o[D / 16];
 };
 
-// One tile's online softmax into bf16 hi and lo parts: y the lane's 8 scores (log2 units, -inf masked), f a factor on p for
-// the P.V product only (the V scales).
+// One tile's online softmax into bf16 hi and lo parts: y the lane's 8 scores (log2 units, -inf masked), f a factor on p
+// for the P.V product only (the V scales).
 template <int D, bool F>
 __device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
   float mx = y[0];
@@ -439,7 +441,8 @@ __device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, Q8>::VB 
     if constexpr (Q8) {
       const uint32_t a = v[2 * e][dt / 4], b = v[2 * e + 1][dt / 4];
       const int sh = 8 * (dt % 4);
-      r[e] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(b >> sh)), __float_as_uint((float)(int8_t)(a >> sh)), 0x07060302u);
+      r[e] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(b >> sh)),
+          __float_as_uint((float)(int8_t)(a >> sh)), 0x07060302u);
     } else {
       r[e] = __builtin_amdgcn_perm(v[2 * e + 1][dt / 2], v[2 * e][dt / 2], dt % 2 ? 0x07060302u : 0x05040100u);
     }
@@ -451,13 +454,15 @@ constexpr int kStreamWaves = 4;
 
 template <int D, bool Q8>
 __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
-  constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D), QR = D + 8;  // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
+  // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
+  constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D), QR = D + 8;
   __shared__ __attribute__((aligned(16))) union {
     uint16_t q[16 * QR];
     float o[NW][16][D + 4];
   } sm;
   __shared__ float sml[NW][2][16];
-  __shared__ float4 skf[NW][2][8];  // a tile's per-key factors, from lane order to score order (one wave writes and reads)
+  // a tile's per-key factors, from lane order to score order (one wave writes and reads)
+  __shared__ float4 skf[NW][2][8];
   const int sp = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
   constexpr int W = 16 * R, PT = 64 / R, SETS = 2;  // PT: tiles whose pages one load brings
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -477,7 +482,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
       const int i = k * NW * 64 + threadIdx.x, z = z0 + i / (D / 8), d0 = (i % (D / 8)) * 8;
       qw[k] = make_uint4(0, 0, 0, 0);
       if (i < 16 * (D / 8) && z < s.n * a.rep)
-        qw[k] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt + (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
+        qw[k] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt +
+                                                (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
     }
     int tt = t_lo + wave, pages = pages0, nth = -1;
     // the wave's next tile into x (past the last one: an empty one, without traffic)
@@ -515,8 +521,9 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
 
-    // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which have the
-    // fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do not hold both).
+    // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which
+    // have the fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do
+    // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
       const int z = z0 + j, tok = min(z / a.rep, s.n - 1);
@@ -528,12 +535,14 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
         const uint16_t* kp = a.k + (int64_t)(s.s0 + k0 + min(j, left - 1)) * a.skt + (int64_t)g * a.skh;
         v4u kr[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kr[ks] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + s_dim<Q8>(qd, ks)));
+        for (int ks = 0; ks < KS; ++ks)
+          kr[ks] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + s_dim<Q8>(qd, ks)));
         uint32_t v[4][D / 32];
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint16_t* vp = a.v + (int64_t)(s.s0 + k0 + min(4 * qd + i, left - 1)) * a.svt + (int64_t)g * a.svh + j * (D / 16);
+          const uint16_t* vp =
+              a.v + (int64_t)(s.s0 + k0 + min(4 * qd + i, left - 1)) * a.svt + (int64_t)g * a.svh + j * (D / 16);
 #pragma unroll
           for (int w = 0; w < D / 64; ++w) {
             const uint2 u = *reinterpret_cast<const uint2*>(vp + 4 * w);
@@ -558,8 +567,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
         v4u hi, lo;
         s_softmax<D, false>(y, f, x, hi, lo);
         if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-          // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products take 0
-          // in their places, and the slots that see one get it added
+          // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products
+          // take 0 in their places, and the slots that see one get it added
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -609,7 +618,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
       float y[8], f[8];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float4 kf = Q8 ? skf[wave][0][4 * r + qd] : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
+        const float4 kf = Q8 ? skf[wave][0][4 * r + qd]
+                             : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
         const float4 vf = Q8 ? skf[wave][1][4 * r + qd] : make_float4(1, 1, 1, 1);
         const float kk[4] = {kf.x, kf.y, kf.z, kf.w}, vv[4] = {vf.x, vf.y, vf.z, vf.w};
 #pragma unroll
@@ -688,7 +698,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
       const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
       acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
       if (nv == 1) {
-        *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(acc.x, acc.y), od_pack_bf16x2(acc.z, acc.w));
+        *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(acc.x, acc.y),
+            od_pack_bf16x2(acc.z, acc.w));
         if (a.lse && d0 == 0) a.lse[n * a.Hq + head] = ls * kLn2;
       } else {
         const int64_t slot = ((int64_t)sp * a.p.N + n) * a.Hq + head;
@@ -699,9 +710,9 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
   }
 }
 
-// The splits of a slot merged by log-sum-exp: 4 columns a thread, S groups of threads share a slot's splits, 4 of them in flight in
-// each. One group where there are few splits (chunks: many slots), all of a workgroup where there are many (decode steps: few
-// slots; 8 tokens over 32768, 8 splits, 7 us with one group, 4.5 with 8). `width`: keys per tile.
+// The splits of a slot merged by log-sum-exp: 4 columns a thread, S groups of threads share a slot's splits, 4 of them
+// in flight in each. One group where there are few splits (chunks: many slots), all of a workgroup where there are many
+// (decode steps: few slots; 8 tokens over 32768, 8 splits, 7 us with one group, 4.5 with 8). `width`: keys per tile.
 template <int D, int S>
 __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int width) {
   constexpr int C = D / 4, SL = kThreads / (C * S), AHEAD = 4;
@@ -738,7 +749,8 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
   for (int i = 0; i < AHEAD; ++i)
     if (grp + i * S < nv) add(l4[i], 1.0f, u4[i]);
 #pragma unroll 4
-  for (int sp = grp + AHEAD * S; sp < nv; sp += S) add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
+  for (int sp = grp + AHEAD * S; sp < nv; sp += S)
+    add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
   if constexpr (S > 1) {
     so[sl][grp][c] = acc;
     if (c == 0) {
@@ -758,37 +770,39 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 }
 
 // ------------------------------------------------------------------------------------------------ many slots: tiles
-// Chunks and option rows: bound by the matrix cores and the softmax's vector work. A workgroup of NW waves owns 32 slots per
-// wave of one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'. Scores are taken
-// transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so that a slot's softmax is
-// lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them; V^T comes from row-major LDS
-// by transposing reads. At D = 256 a wave accumulates 128 of the value columns and two waves share 32 slots (each takes the
-// scores again): 256 columns of accumulators beside 256-wide queries do not fit its registers.
+// Chunks and option rows: bound by the matrix cores and the softmax's vector work. A workgroup of NW waves owns 32
+// slots per wave of one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'.
+// Scores are taken transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so
+// that a slot's softmax is lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them;
+// V^T comes from row-major LDS by transposing reads. The kernel here is for heads of 64 and 128; heads of 256 have one
+// of their own below, of the same parts.
 //
-// int8 blocks are converted once per workgroup on the way into LDS, to fp16 in power-of-two frames: K' = fp16(q ks_j 2^(7 - E))
-// with 2^E above the block's largest scale, V' = fp16(q vs_j 2^(7 - F)) with 2^F above the largest so far (the accumulator
-// moves along when F rises), queries as fp16 q 2^(14 - e) with 2^e above the slot's largest (exact while they are normal).
-// One rounding of 2^-11 at most for every cached value, far below the 2^-8 of their int8 grid, and the scores' factor
-// 2^(e - 14 + E - 7) is one number per slot and block. Probabilities are fp16 there, kept 2^7 above what they are (2^15 at
-// most under kSlack), so that one as small as 2^-31 of the largest still counts. bf16 pages and the new tokens go in as
-// they are, with bf16 probabilities (2^-8 each, as the output's own rounding).
+// int8 blocks are converted once per workgroup on the way into LDS, to fp16 in power-of-two frames: K' = fp16(q ks_j
+// 2^(7 - E)) with 2^E above the block's largest scale, V' = fp16(q vs_j 2^(7 - F)) with 2^F above the largest so far
+// (the accumulator moves along when F rises), queries as fp16 q 2^(14 - e) with 2^e above the slot's largest (exact
+// while they are normal). One rounding of 2^-11 at most for every cached value, far below the 2^-8 of their int8 grid,
+// and the scores' factor 2^(e - 14 + E - 7) is one number per slot and block. Probabilities are fp16 there, kept 2^7
+// above what they are (2^15 at most under kSlack), so that one as small as 2^-31 of the largest still counts. bf16
+// pages and the new tokens go in as they are, with bf16 probabilities (2^-8 each, as the output's own rounding).
 //
-// The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first in the
-// next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
+// The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first
+// in the next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
 constexpr int kBK = 64;
 constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
 
 template <int D>
-__device__ __forceinline__ int tk_off(int key, int chunk) {  // K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
+// K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
+__device__ __forceinline__ int tk_off(int key, int chunk) {
   return key * D + ((chunk ^ (D == 64 ? ((key >> 1) & 7) : (key & 15))) << 3);
 }
 template <int D>
-__device__ __forceinline__ int tv_chunk(int key, int chunk) {  // V rows: 4 consecutive keys' chunks of a transposing read 64 bytes apart
+// V rows: 4 consecutive keys' chunks of a transposing read 64 bytes apart
+__device__ __forceinline__ int tv_chunk(int key, int chunk) {
   return D == 64 ? chunk ^ ((key & 2) << 1) : chunk ^ ((key & 3) << 2);
 }
 
-// 16 bytes per lane from memory straight into LDS, lane l's to LDS byte lds + 16 l (lds wave-uniform, in M0). The compiler does
-// not track it: the kernel waits (vmcnt) and orders it with barriers itself.
+// 16 bytes per lane from memory straight into LDS, lane l's to LDS byte lds + 16 l (lds wave-uniform, in M0). The
+// compiler does not track it: the kernel waits (vmcnt) and orders it with barriers itself.
 __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
@@ -797,12 +811,13 @@ template <typename T>
 __device__ __forceinline__ uint32_t lds_addr(T* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);
 }
-// A block's bf16 rows into LDS by DMA: instruction i of a wave fills the 1 KB at 1024 (i NW + wave) of K or V, so a lane owns a
-// place there, (key, swizzled chunk), and copies the chunk that the swizzle puts into it. at(key): its row.
+// A block's bf16 rows into LDS by DMA: instruction i of a wave fills the 1 KB at 1024 (i NW + wave) of K or V, so a
+// lane owns a place there, (key, swizzled chunk), and copies the chunk that the swizzle puts into it. at(key): its row.
 template <int D, int NW, typename KeyRow>
 __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, KeyRow&& row) {
   int lane = threadIdx.x & 63;
-  if constexpr (D > 64) asm volatile("" : "+v"(lane));  // places are formed here each time, not kept in registers over the block loop
+  // places are formed here each time, not kept in registers over the block loop
+  if constexpr (D > 64) asm volatile("" : "+v"(lane));
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i) {
     const int pe = (i * NW + wave) * 512 + 8 * lane, key = pe / D, slot = pe % D / 8;
@@ -814,17 +829,19 @@ __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, 
 template <bool H>
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
   if constexpr (H)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                  0, 0);
   else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                   0, 0, 0);
 }
 __device__ __forceinline__ v16f zero16() { return v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
 
 // exponent e with x < 2^e for the bits of a finite x > 0; 0 for 0
 __device__ __forceinline__ int exp_above(uint32_t bits) { return bits ? (int)(bits >> 23) - 126 : 0; }
 
-// 16 int8 times f, each product rounded once to fp16: byte u = q + 128 becomes the fp16 1024 + u by its bits, and
-// (1024 + u) f - 1152 f is one fp32 fma per value (v_fma_mix). f has its last 4 bits clear (frame_scale), so that 1152 f is
+// 16 int8 times f, each product rounded once to fp16: byte u = q + 128 becomes the fp16 1024 + u by its bits, and (1024
+// + u) f - 1152 f is one fp32 fma per value (v_fma_mix). f has its last 4 bits clear (frame_scale), so that 1152 f is
 // exact and the result is q f rounded once, 0 for q = 0.
 __device__ __forceinline__ void i8x16_scaled(v4u w, float f, v4u& lo, v4u& hi) {
   const float c = -1152.0f * f;
@@ -853,6 +870,8 @@ struct alignas(16) TSmem {
   int odd;  // infinities or NaN among the new values of a block that some slot sees only a part of
 };
 
+// Value tiles of 32 columns that a wave accumulates (D = 256: half of the columns).
+constexpr int t_cols(int D) { return D == 256 ? 4 : D / 32; }
 // One slot tile's constants per lane, and its state.
 template <int D>
 struct TSlot {
@@ -860,7 +879,7 @@ struct TSlot {
   v4u q[D / 16];             // dims 16 ks + 8 h .. + 7
   int qe;                    // fp16 queries: their exponent
   float m, l;
-  v16f o[D == 256 ? 4 : D / 32];
+  v16f o[t_cols(D)];
 };
 
 template <int D>
@@ -896,12 +915,13 @@ __device__ __forceinline__ void t_q_to_f16(TSlot<D>& t) {
 template <int D, bool H>
 __device__ __forceinline__ void t_scores(const uint16_t* kb, const TSlot<D>& t, v16f (&s)[2]) {
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-  constexpr int NQ = D / 16 * 2, RA = D == 256 ? 1 : 2;  // MFMA i: k-step i / 2, key tile i % 2; reads run RA ahead
+  constexpr int NQ = D / 16 * 2, RA = 2;  // MFMA i: k-step i / 2, key tile i % 2; reads run RA ahead
   s[0] = zero16();
   s[1] = zero16();
   v4u kf[RA + 1];
   auto rd = [&](int i) {
-    kf[i % (RA + 1)] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(&kb[tk_off<D>((i % 2) * 32 + col, (i / 2) * 2 + h)]));
+    const uint16_t* at = &kb[tk_off<D>((i % 2) * 32 + col, (i / 2) * 2 + h)];
+    kf[i % (RA + 1)] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(at));
   };
 #pragma unroll
   for (int i = 0; i < RA; ++i) rd(i);
@@ -957,7 +977,8 @@ __device__ __forceinline__ void t_softmax(v16f (&s)[2], float c, TSlot<D>& t, v4
   t.l += sum;  // this lane's share: keys of its half
 }
 
-// The A operand for value rows of d tile dt (vb: the lane's base there), keys 16 kk + 8 (i / 4) + 4 (lane / 32) + i % 4.
+// The A operand for value rows of d tile dt (vb: the lane's base there), keys 16 kk + 8 (i / 4) + 4 (lane / 32) + i %
+// 4.
 template <int D>
 __device__ __forceinline__ v4u t_vfrag(const uint16_t* vblk, int vb, int kk) {
   typedef short v4s __attribute__((ext_vector_type(4)));
@@ -969,8 +990,9 @@ __device__ __forceinline__ v4u t_vfrag(const uint16_t* vblk, int vb, int kk) {
 }
 
 template <int D, bool H>
-__device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[D == 256 ? 4 : D / 32], const v4u (&pb)[4], TSlot<D>& t) {
-  constexpr int DT = D == 256 ? 4 : D / 32, NV = 4 * DT, RA = D == 256 ? 1 : 2;  // MFMA i: k-step i / DT, d tile i % DT
+__device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[t_cols(D)], const v4u (&pb)[4],
+    TSlot<D>& t) {
+  constexpr int DT = t_cols(D), NV = 4 * DT, RA = D == 256 ? 1 : 2;  // MFMA i: k-step i / DT, d tile i % DT
   v4u vf[RA + 1];
   auto rd = [&](int i) { vf[i % (RA + 1)] = t_vfrag<D>(vblk, vb[i % DT], i / DT); };
 #pragma unroll
@@ -987,13 +1009,14 @@ __device__ __forceinline__ void t_values(const uint16_t* vblk, const int (&vb)[D
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
   }
 }
-// Where a workgroup's work lies (sp < 0: nowhere). Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of its own.
-// A group is the slot tiles of one (sequence, KV head, split), which read the same keys; its tiles go to one XCD in runs of
-// `run` (a whole group, or a part of it where there are few groups), and the runs are dealt round-robin, each turn of 8 shifted by 3
-// against the last (else the first of two sequences of 4 heads, or every first split, would stay with half of the XCDs):
-// contiguous ranges of the groups gave each XCD the sequences of a ragged batch as they came (4 ragged chunks of 256-wide
-// heads 618 us, so 446). A causal tile's work grows with its index: last first (both: 4 ragged first chunks of 2000, 199
-// us, 124). Of up to 64 sequences the longest come first, so that the last workgroups to run are short ones (option rows of 8 ragged requests 158 us, 140).
+// Where a workgroup's work lies (sp < 0: nowhere). Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of
+// its own. A group is the slot tiles of one (sequence, KV head, split), which read the same keys; its tiles go to one
+// XCD in runs of `run` (a whole group, or a part of it where there are few groups), and the runs are dealt round-robin,
+// each turn of 8 shifted by 3 against the last (else the first of two sequences of 4 heads, or every first split, would
+// stay with half of the XCDs): contiguous ranges of the groups gave each XCD the sequences of a ragged batch as they
+// came (4 ragged chunks of 256-wide heads 618 us, so 446). A causal tile's work grows with its index: last first (both:
+// 4 ragged first chunks of 2000, 199 us, 124). Of up to 64 sequences the longest come first, so that the last
+// workgroups to run are short ones (option rows of 8 ragged requests 158 us, 140).
 struct TilePlace {
   int b, g, sp, tile;
 };
@@ -1021,16 +1044,16 @@ __device__ __forceinline__ TilePlace tile_place(const AttnArgs& a) {
   return w;
 }
 
-// The new tokens that a slot tile sees: blocks lo .. hi - 1 of them. Of the wave's slots (w_) and the workgroup's (g_): the first
-// and last token that any sees (w_lo, w_hi), and the span that all see whole, w_in .. w_tok.
+// The new tokens that a slot tile sees: blocks lo .. hi - 1 of them. Of the wave's slots (w_) and the workgroup's (g_):
+// the first and last token that any sees (w_lo, w_hi), and the span that all see whole, w_in .. w_tok.
 struct NewSpan {
   int lo, hi, w_lo, w_hi, w_in, w_tok, g_in, g_tok;
   // a block that some slot of the workgroup sees only a part of
   __device__ __forceinline__ bool partial(int blk) const { return blk * kBK + kBK - 1 > g_tok || blk * kBK < g_in; }
 };
 template <int D>
-__device__ __forceinline__ NewSpan new_span(const AttnArgs& a, const Seq& s, int tile, int spt, int zw, bool live, const TSlot<D>& t,
-                                            int* lo, int* hi, int* odd, int nw, int wave) {
+__device__ __forceinline__ NewSpan new_span(const AttnArgs& a, const Seq& s, int tile, int spt, int zw, bool live,
+                                            const TSlot<D>& t, int* lo, int* hi, int* odd, int nw, int wave) {
   const int lane = threadIdx.x & 63;
   NewSpan n;
   n.w_tok = min(zw / a.rep, s.n - 1);
@@ -1079,33 +1102,37 @@ __device__ __forceinline__ void make_finite(uint16_t* v, int* odd) {
 }
 // ... and the slots that see one get it added.
 template <int D>
-__device__ __forceinline__ void add_odd(const AttnArgs& a, const Seq& s, int g, int half, const NewSpan& n, TSlot<D>& t) {
+__device__ __forceinline__ void add_odd(const AttnArgs& a, const Seq& s, int g, int half, const NewSpan& n,
+    TSlot<D>& t) {
   const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
   for (int key = max(n.lo * kBK, t.begin); key <= t.tok; ++key) {
     if (!n.partial(key / kBK)) continue;
     const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + half * 128 + 4 * h;
 #pragma unroll
-    for (int dt = 0; dt < (D == 256 ? 4 : D / 32); ++dt)
+    for (int dt = 0; dt < t_cols(D); ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) t.o[dt][i] += odd_bf16(vp[dt * 32 + 8 * (i >> 2) + (i & 3)]);
   }
 }
 // out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
-template <int D, int DT>
-__device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, int frame, int sp, int nv, int half) {
+template <int D>
+__device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, int frame, int sp,
+    int nv, int half) {
   if (!t.ok) return;
   const int h = (threadIdx.x & 63) >> 5;
   const float inv = l == 0.0f ? 0.0f : __builtin_ldexpf(1.0f / l, frame), ls = t.m + __log2f(l) - kLift;
   const int64_t n = s.s0 + t.tok;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int dt = 0; dt < t_cols(D); ++dt)
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {
       const int d0 = half * 128 + dt * 32 + 8 * i4 + 4 * h;
-      const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv, t.o[dt][4 * i4 + 3] * inv);
+      const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv,
+          t.o[dt][4 * i4 + 3] * inv);
       if (nv == 1)
-        *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y), od_pack_bf16x2(y.z, y.w));
+        *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y),
+            od_pack_bf16x2(y.z, y.w));
       else
         *reinterpret_cast<float4*>(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0) = y;
     }
@@ -1117,7 +1144,7 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
 
 template <int D, bool Q8, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
-  constexpr int NT = NW * 64, HALVES = D == 256 ? 2 : 1, SPT = 32 * NW / HALVES, DT = D == 256 ? 4 : D / 32;
+  constexpr int NT = NW * 64, SPT = 32 * NW, DT = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
   const TilePlace at = tile_place(a);
@@ -1128,19 +1155,19 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   if (sp >= nv) return;
   const int b_lo = sp * a.chunk, b_hi = sp == a.nsplit - 1 ? blocks : min(blocks, b_lo + a.chunk);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave / (NW / HALVES);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int vb[DT];  // transposing-read bases
   {
     const int hh = lane >> 5, mh = (lane >> 4) & 1, e = (lane >> 2) & 3, c = lane & 3;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
+      vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
   for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
     __syncthreads();  // an earlier tile's readers are done
     TSlot<D> t;
-    const int zw = tile * SPT + (wave % (NW / HALVES)) * 32, z = zw + col;
+    const int zw = tile * SPT + wave * 32, z = zw + col;
     const bool live = zw < nslots;  // the wave has slots
     t.ok = z < nslots;
     t.tok = t.ok ? z / a.rep : s.n - 1;
@@ -1182,11 +1209,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
-            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) + row(key) * D + 16 * ch));
+            const char* pool = static_cast<const char*>(side ? a.p.v : a.p.k);
+            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(pool + row(key) * D + 16 * ch));
           }
         } else {
-          dma_rows<D, NW>(sm.k[buf], wave, false, [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(key) * D; });
-          dma_rows<D, NW>(sm.v[buf], wave, true, [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(key) * D; });
+          dma_rows<D, NW>(sm.k[buf], wave, false,
+                          [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(key) * D; });
+          dma_rows<D, NW>(sm.v[buf], wave, true,
+                          [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(key) * D; });
         }
       };
       int kexp = 0, vexp = 0;  // the stored block's frames
@@ -1195,10 +1225,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       auto store = [&](int buf) {
         seen = there;
         if constexpr (Q8) {
-          // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not finite,
-          // leave them alone
+          // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not
+          // finite, leave them alone
           const bool on = (there >> lane) & 1;
-          const uint32_t kb = on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u, vb2 = on && vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u;
+          const uint32_t kb = on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u,
+              vb2 = on && vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u;
           kexp = exp_above(od_wave_umax_dpp(kb));
           const uint32_t vm = od_wave_umax_dpp(vb2);
           if (vm) vexp = vexp_set ? max(vexp, exp_above(vm)) : exp_above(vm);
@@ -1222,8 +1253,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
             if (!((seen >> (c / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[buf][8 * c]) = make_uint4(0, 0, 0, 0);
         }
       };
-      // One step: block blk's products; ahead of them, for int8 the conversion of block blk + 1 (in registers since the last
-      // step) and the loads of blk + 2, for bf16 the copy of blk + 1.
+      // One step: block blk's products; ahead of them, for int8 the conversion of block blk + 1 (in registers since the
+      // last step) and the loads of blk + 2, for bf16 the copy of blk + 1.
       pages(b_lo);
       load(b_lo, 0);
       pages(b_lo + 1);
@@ -1337,22 +1368,23 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
           }
           __syncthreads();
         }
-        if (sm.odd && t.ok) add_odd<D>(a, s, g, half, n, t);
+        if (sm.odd && t.ok) add_odd<D>(a, s, g, 0, n, t);
       }
     }
 
-    t_out<D, DT>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, half);
+    t_out<D>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, 0);
   }
 }
 
 // ------------------------------------------------------------------------------------- many slots, heads of 256
-// 256 value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots: each
-// accumulates 128 of the columns. In the kernel above each of them takes all the scores; here each takes those of 32 of the
-// block's 64 keys, and its half of the softmax, and they exchange the maximum and the probabilities through LDS (as the
-// fragments that the products want): 32 instead of 48 matrix instructions a block and wave, half the exponentials. For that the
-// waves meet twice a block. K runs a block ahead of V, so that both meetings also order the buffers:
-//   scores(b) | maxima out, barrier | K(b + 2), V(b + 1) into the buffers of blocks that all are done with; softmax, probabilities
-//   out, barrier | products(b), scores(b + 1) ...
+// 256 value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots:
+// each accumulates 128 of the columns. Each takes the scores of 32 of the block's 64 keys, and its half of the softmax,
+// and they exchange the maximum and the probabilities through LDS (as the fragments that the products want); taking all
+// the scores in both instead, 48 matrix instructions a block and wave for 32, a chunk of 2048 over 16000 bf16 tokens
+// took 840 us, now 718 (4 ragged first chunks of 2000: 333, 216). For that the waves meet twice a block. K runs a block
+// ahead of V, so that both meetings also order the buffers:
+//   scores(b) | maxima out, barrier | K(b + 2), V(b + 1) into the buffers of blocks that all are done with; softmax,
+//   probabilities out, barrier | products(b), scores(b + 1) ...
 struct alignas(16) WSmem {
   uint16_t k[2][kBK * 256];
   uint16_t v[2][kBK * 256];
@@ -1405,7 +1437,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       v16f x = zero16();
       v4u kf[2];
       auto rd = [&](int i) {
-        kf[i % 2] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(&kb[tk_off<D>(half * 32 + col, 2 * i + h)]));
+        const uint16_t* at = &kb[tk_off<D>(half * 32 + col, 2 * i + h)];
+        kf[i % 2] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(at));
       };
       rd(0);
 #pragma unroll
@@ -1500,7 +1533,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           const int key = (i * NT + ti) / CPK, ch = (i * NT + ti) % CPK;
-          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(pool) + row(blk, pg, key) * D + 16 * ch));
+          const char* at = static_cast<const char*>(pool) + row(blk, pg, key) * D + 16 * ch;
+          r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(at));
         }
       };
       auto scale_bits = [&](int pg, float sc) {  // the largest scale of the block's keys that is a number, as bits
@@ -1544,11 +1578,13 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       };
       auto load_k = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
-        else dma_rows<D, NW>(sm.k[blk & 1], wave, false, [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(blk, pg, key) * D; });
+        else dma_rows<D, NW>(sm.k[blk & 1], wave, false,
+            [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(blk, pg, key) * D; });
       };
       auto load_v = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
-        else dma_rows<D, NW>(sm.v[blk & 1], wave, true, [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(blk, pg, key) * D; });
+        else dma_rows<D, NW>(sm.v[blk & 1], wave, true,
+            [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(blk, pg, key) * D; });
       };
       // pages of the blocks blk (the current one), blk + 1, blk + 2, blk + 3; past the last block: none
       int p0 = pages(b_lo), p1 = pages(b_lo + 1), p2 = pages(b_lo + 2), p3 = pages(b_lo + 3);
@@ -1591,7 +1627,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         __syncthreads();
         if (!Q8 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
           for (int i = tid; i < kBK * (D / 8); i += NT)
-            if (!((seen >> (i / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
+            if (!((seen >> (i / (D / 8))) & 1))
+              *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
         }
         const int f_now = f_cur;
         if constexpr (Q8) {
@@ -1630,7 +1667,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load_k = [&](int blk) {
         const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
-        dma_rows<D, NW>(sm.k[blk & 1], wave, false, [&](int key) { return kp + min(blk * kBK + key, s.n - 1) * a.skt; });
+        dma_rows<D, NW>(sm.k[blk & 1], wave, false,
+                        [&](int key) { return kp + min(blk * kBK + key, s.n - 1) * a.skt; });
       };
       auto load_v = [&](int blk) {
         const uint16_t* vp = a.v + (int64_t)s.s0 * a.svt + (int64_t)g * a.svh;
@@ -1681,7 +1719,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     if (h == 0) sm.mx[half][grp][col] = l;
     __syncthreads();
     l += sm.mx[half ^ 1][grp][col];
-    t_out<D, DT>(a, s, t, l, frame, sp, nv, half);
+    t_out<D>(a, s, t, l, frame, sp, nv, half);
   }
 }
 
@@ -1692,10 +1730,13 @@ struct Plan {
 };
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx) {
   Plan p;
+  // hints past any call's own size say nothing; below 2^30 no split begins past the positions an int holds
+  max_new = max_new < N ? max_new : N;
+  max_ctx = max_ctx < (1 << 30) ? max_ctx : 1 << 30;
   const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
   p.stream = slots <= 16;
-  // 8 waves share a block's conversion at D = 128 (a chunk of 2048 over 32768: 1316 us, 4 waves 1515); at D = 64 they only
-  // coarsen the work (bf16 chunks of 2048 over 16000 234 us, 4 waves 202; int8 ones the same).
+  // 8 waves share a block's conversion at D = 128 (a chunk of 2048 over 32768: 1316 us, 4 waves 1515); at D = 64 they
+  // only coarsen the work (bf16 chunks of 2048 over 16000 234 us, 4 waves 202; int8 ones the same).
   p.nw = p.stream ? kStreamWaves : D == 256 || (D == 128 && slots > 128) ? 8 : 4;
   p.width = p.stream ? 16 * s_halves((int)D) : kBK;
   const int64_t spt = p.stream ? 16 : D == 256 ? 128 : 32 * p.nw;
@@ -1711,9 +1752,10 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     if (n > most) n = most;
     if (n < 1) n = 1;
   } else {
-    // the n of least cost: rounds of workgroups times a workgroup's blocks and what it costs besides them, about 12 blocks (the
-    // queries, the first loads, the new tokens, the partials). One round filled once: a chunk of 512 over 16000 takes 583 us whole, 223 in 3, 192 in 4, 234
-    // in 6 parts; 304 workgroups of 256-wide heads in 2 rounds 739 us, 608 of half the keys in 3 rounds 620, 4 parts 709.
+    // the n of least cost: rounds of workgroups times a workgroup's blocks and what it costs besides them, about 12
+    // blocks (the queries, the first loads, the new tokens, the partials). One round filled once: a chunk of 512 over
+    // 16000 takes 583 us whole, 223 in 3, 192 in 4, 234 in 6 parts; 304 workgroups of 256-wide heads in 2 rounds 739
+    // us, 608 of half the keys in 3 rounds 620, 4 parts 709.
     int64_t best = 0;
     for (int64_t i = 1; i <= most || i == 1; ++i) {
       const int64_t cost = ((wgs * i + fit - 1) / fit) * ((keys + i - 1) / i + 12);
@@ -1735,12 +1777,15 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   return p;
 }
 
+// slots of a KV head, so that an int holds them and a stride of tiles past them
+constexpr int64_t kMaxSlots = 0x3fff0000;
+
 bool aligned4(const void* p) { return (((uintptr_t)p) & 3u) == 0; }
 
 // Checks of the pages that every entry point makes; fills P.
-int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale, int64_t n_pages,
-               int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx,
-               int64_t B, int64_t N, int64_t Hkv, int64_t D) {
+int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
+               int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
+               const int32_t* start, const int32_t* ctx, int64_t B, int64_t N, int64_t Hkv, int64_t D) {
   if (B < 0 || N < 0 || Hkv < 1 || n_pages < 0 || cols < 0 || ld_table < cols) return OD_ERR_SHAPE;
   if (D != 64 && D != 128 && D != 256) return OD_ERR_UNSUPPORTED;
   if (page < 16 || page > (1 << 20) || (page & (page - 1))) return OD_ERR_UNSUPPORTED;
@@ -1749,8 +1794,9 @@ int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* 
   if (!k_scale != !v_scale) return OD_ERR_NULL;
   if (n_pages > 0 && (!k_pages || !v_pages)) return OD_ERR_NULL;
   if (!od_aligned16(k_pages) || !od_aligned16(v_pages) || !aligned4(k_scale) || !aligned4(v_scale)) return OD_ERR_ALIGN;
-  P = Paged{const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<float*>(k_scale), const_cast<float*>(v_scale),
-            table, start, ctx, ld_table, n_pages, (int)cols, __builtin_ctzll(page), (int)B, (int)N, (int)Hkv};
+  P = Paged{const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<float*>(k_scale),
+            const_cast<float*>(v_scale), table, start, ctx, ld_table, n_pages, (int)cols, __builtin_ctzll(page), (int)B,
+            (int)N, (int)Hkv};
   return OD_OK;
 }
 
@@ -1761,7 +1807,8 @@ int launch_big(const AttnArgs& a, unsigned groups, int threads, int bytes, hipSt
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return OD_ERR_LAUNCH;
   if (!((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+        bytes) != hipSuccess)
       return OD_ERR_LAUNCH;
     allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
@@ -1783,12 +1830,13 @@ void by_head_dim(int64_t D, F&& f) {
 }  // namespace
 
 extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh,
-                              void* k_pages, float* k_scale, void* v_pages, float* v_scale, int64_t n_pages, int64_t page,
-                              const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
-                              const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D, od_stream_t stream) {
+                              void* k_pages, float* k_scale, void* v_pages, float* v_scale, int64_t n_pages,
+                              int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                              const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D,
+                              od_stream_t stream) {
   AppendArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table, cols, start, ctx_len,
-                                B, N, Hkv, D))
+  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+                                cols, start, ctx_len, B, N, Hkv, D))
     return rc;
   if (B == 0 || N == 0 || cols == 0 || n_pages == 0) return OD_OK;
   if (!k || !v || !table || !start || !ctx_len) return OD_ERR_NULL;
@@ -1802,7 +1850,8 @@ extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const
   a.skh = skh;
   a.svt = svt;
   a.svh = svh;
-  const int64_t per_block = (int64_t)(kThreads / 64) * (64 / (D / 16)), blocks = (N * 2 * Hkv + per_block - 1) / per_block;
+  const int64_t per_block = (int64_t)(kThreads / 64) * (64 / (D / 16));
+  const int64_t blocks = (N * 2 * Hkv + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return OD_ERR_SHAPE;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
@@ -1818,8 +1867,8 @@ extern "C" int od_page_read(const void* k_pages, const float* k_scale, const voi
                             const int32_t* length, int64_t B, int64_t T, int64_t Hkv, int64_t D, int form, void* k_out,
                             float* ks_out, void* v_out, float* vs_out, od_stream_t stream) {
   ReadArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table, cols, nullptr, length,
-                                B, 0, Hkv, D))
+  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+                                cols, nullptr, length, B, 0, Hkv, D))
     return rc;
   if (T < 0 || T > 0x3fffffff) return OD_ERR_SHAPE;
   if (form != OD_READ_BF16 && form != OD_READ_FP32 && form != OD_READ_INT8) return OD_ERR_UNSUPPORTED;
@@ -1853,11 +1902,12 @@ extern "C" int od_page_read(const void* k_pages, const float* k_scale, const voi
   return od_launch_status();
 }
 
-extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx,
-                                int64_t* ws_floats) {
+extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                                int64_t max_ctx, int64_t* ws_floats) {
   if (!ws_floats) return OD_ERR_NULL;
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
   if (Hq % Hkv || (D != 64 && D != 128 && D != 256)) return OD_ERR_UNSUPPORTED;
+  if (B > 65535 || Hq > 65535 || N > kMaxSlots / (Hq / Hkv)) return OD_ERR_SHAPE;
   const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx);
   *ws_floats = p.nsplit > 1 ? p.nsplit * N * Hq * (D + 1) : 0;
   return OD_OK;
@@ -1865,23 +1915,25 @@ extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, i
 
 extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
                              const uint16_t* v, int64_t svt, int64_t svh, const void* k_pages, const float* k_scale,
-                             const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page, const int32_t* table,
-                             int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx_len,
-                             const int32_t* row_begin, uint16_t* out, int64_t sot, int64_t soh, float* lse, int64_t B,
-                             int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx, float scale,
-                             float* ws, int64_t ws_floats, od_stream_t stream) {
+                             const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page,
+                             const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                             const int32_t* ctx_len, const int32_t* row_begin, uint16_t* out, int64_t sot, int64_t soh,
+                             float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                             int64_t max_ctx, float scale, float* ws, int64_t ws_floats, od_stream_t stream) {
   AttnArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table, cols, start, ctx_len,
-                                B, N, Hkv, D))
+  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+                                cols, start, ctx_len, B, N, Hkv, D))
     return rc;
-  if (Hq < 1 || Hq > 65535 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
+  if (Hq < 1 || Hq > 65535 || B > 65535 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
+  if (Hq >= Hkv && N > kMaxSlots / (Hq / Hkv)) return OD_ERR_SHAPE;
   if (Hq % Hkv || !(scale > 0.0f) || !(scale < INFINITY)) return OD_ERR_UNSUPPORTED;
   if (B == 0 || N == 0) return OD_OK;
   if (!q || !out || !start || !ctx_len || !k != !v || (cols > 0 && !table)) return OD_ERR_NULL;
   const int64_t strides[] = {sqt, sqh, skt, skh, svt, svh, sot, soh};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return OD_ERR_ALIGN;
-  if (!od_aligned16(q) || !od_aligned16(k) || !od_aligned16(v) || !od_aligned16(out) || !aligned4(lse)) return OD_ERR_ALIGN;
+  if (!od_aligned16(q) || !od_aligned16(k) || !od_aligned16(v) || !od_aligned16(out) || !aligned4(lse))
+    return OD_ERR_ALIGN;
   a.q = q;
   a.k = k;
   a.v = v;
@@ -1914,14 +1966,15 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   hipStream_t st = (hipStream_t)stream;
   // tiles: every run of every group, a multiple of 8 runs
   const int64_t runs = (p.tiles + p.run - 1) / p.run, groups = (p.nsplit * Hkv * B * runs + 7) / 8 * 8 * p.run;
-  if (groups > 0x7fffffff || B > 65535) return OD_ERR_SHAPE;
+  if (groups > 0x7fffffff) return OD_ERR_SHAPE;
   int rc = OD_OK;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
     auto launch = [&](auto QC) {
       constexpr bool Q8 = decltype(QC)::value;
       if (p.stream) {
-        paged_stream_kernel<DD, Q8><<<dim3((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B), dim3(kStreamWaves * 64), 0, st>>>(a);
+        const dim3 grid((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B);
+        paged_stream_kernel<DD, Q8><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
       } else if constexpr (DD == 64) {
         rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
       } else if constexpr (DD == 256) {
@@ -1935,9 +1988,11 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     if (k_scale) launch(std::true_type{});
     else launch(std::false_type{});
     if (rc == OD_OK && p.nsplit > 1) {
-      constexpr int S = 4 * kThreads / DD, SL = S;  // groups when a workgroup has one slot; slots when a slot has one group
-      if (p.nsplit > 4) paged_combine_kernel<DD, S><<<dim3((unsigned)N, (unsigned)Hq), dim3(kThreads), 0, st>>>(a, p.width);
-      else paged_combine_kernel<DD, 1><<<dim3((unsigned)N, (unsigned)((Hq + SL - 1) / SL)), dim3(kThreads), 0, st>>>(a, p.width);
+      // groups when a workgroup has one slot; slots when a slot has one group
+      constexpr int S = 4 * kThreads / DD, SL = S;
+      const dim3 one((unsigned)N, (unsigned)Hq), many((unsigned)N, (unsigned)((Hq + SL - 1) / SL)), block(kThreads);
+      if (p.nsplit > 4) paged_combine_kernel<DD, S><<<one, block, 0, st>>>(a, p.width);
+      else paged_combine_kernel<DD, 1><<<many, block, 0, st>>>(a, p.width);
     }
   });
   return rc == OD_OK ? od_launch_status() : rc;

@@ -146,3 +146,21 @@ def test_no_cpu_path():
         kernels.page_read(c, i[None], i[:1], 4)
     with pytest.raises(RuntimeError):
         kernels.paged_attn(x, x, x, c, i[None], i, i[:1], 0.1)
+
+
+def test_workspace_of_any_hint():
+    """The lengths are hints: past any call's own size they ask for no more (what a split holds stays countable), and a call
+    with more slots of a KV head than an int counts is refused."""
+    import ctypes
+    from opendecider_amd._lib import lib
+
+    def ws(*sizes, want=0):
+        n = ctypes.c_int64(-1)
+        assert (lib().od_paged_attn_ws(*sizes, ctypes.byref(n)) == 0) == (want == 0)
+        return n.value
+    for n, rep in ((1, 1), (8, 4), (700, 4), (4096, 8)):
+        most = ws(2, n, 8 * rep, 8, 128, n, 1 << 30)
+        for new, ctx in ((1 << 40, 1 << 30), (n, 1 << 31), (1 << 62, (1 << 62) + 1)):
+            assert ws(2, n, 8 * rep, 8, 128, new, ctx) == most
+        assert most % (n * 8 * rep * 129) == 0 and most <= 128 * n * 8 * rep * 129
+    ws(1, 1 << 29, 64, 1, 128, 1, 100, want="refused")
