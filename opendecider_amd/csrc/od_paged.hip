@@ -285,11 +285,12 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
   hi = __builtin_amdgcn_perm(f3, f2, 0x07060302u);
 }
 
-// ------------------------------------------------------------------------------------------ few slots: streaming
-// Up to 16 slots of a (sequence, KV head): decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of int8 K and V:
-// bound by reading the pages. A wave holds all 16 slots as the columns of V_MFMA_F32_16X16X32_BF16 and takes 32-key
-// tiles straight from memory into registers; the waves of a workgroup take every NW-th tile of the split's range and
-// merge in LDS. Lane (j, g) = (lane % 16, lane / 16):
+// ------------------------------------------------------------------------------------------ few slots: streaming Up to
+// 16 or 32 slots of a (sequence, KV head) in a workgroup: decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of
+// int8 K and V: bound by reading the pages (64 x 4096 tokens of 8 heads of 128 in 70 us, 5.4 TB/s). A wave holds 16
+// slots as the columns of V_MFMA_F32_16X16X32_BF16, or 32 as two of them, and takes 32-key tiles straight from memory
+// into registers; the waves of a workgroup take every NW-th tile of the split's range and merge in LDS. Lane (j, g) =
+// (lane % 16, lane / 16):
 //  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: the four lanes of a key read 64 contiguous bytes of it at
 //    a time (s_dim: a permutation of the reduction index, the same on both sides; reading D / 4 contiguous values per
 //    lane instead took 101 against 76 us for the loads of 16 x 8000 bf16 tokens); int8 values enter as exact bf16
@@ -451,19 +452,21 @@ __device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, Q8>::VB 
 }
 
 constexpr int kStreamWaves = 4;
+// whether a wave has a SIMD's registers to itself
+constexpr bool s_alone(int D, bool q8, int columns) { return D * columns >= (q8 ? 512 : 256); }
 
-template <int D, bool Q8>
-__global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+template <int D, bool Q8, int CT>
+__global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
   // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
   constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D), QR = D + 8;
   __shared__ __attribute__((aligned(16))) union {
-    uint16_t q[16 * QR];
+    uint16_t q[16 * CT * QR];
     float o[NW][16][D + 4];
   } sm;
   __shared__ float sml[NW][2][16];
   // a tile's per-key factors, from lane order to score order (one wave writes and reads)
   __shared__ float4 skf[NW][2][8];
-  const int sp = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int sp = blockIdx.x, g = blockIdx.y % a.p.Hkv, b = blockIdx.z;
   constexpr int W = 16 * R, PT = 64 / R, SETS = 2;  // PT: tiles whose pages one load brings
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane & 15, qd = lane >> 4, c = lane & 31;
@@ -474,14 +477,15 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
   const int tiles = (s.ctx + W - 1) / W, nv = splits_of(a, tiles);
   if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
   const int t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
-  for (int z0 = 0; z0 < s.n * a.rep; z0 += 16) {  // one round unless max_new was too small
-    constexpr int QC = 16 * (D / 8) / (NW * 64) ? 16 * (D / 8) / (NW * 64) : 1;
+  // one round unless max_new was too small
+  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep; z0 += a.tiles * 16 * CT) {
+    constexpr int QN = 16 * CT * (D / 8), QC = QN / (NW * 64) ? QN / (NW * 64) : 1;
     uint4 qw[QC];
 #pragma unroll
     for (int k = 0; k < QC; ++k) {
       const int i = k * NW * 64 + threadIdx.x, z = z0 + i / (D / 8), d0 = (i % (D / 8)) * 8;
       qw[k] = make_uint4(0, 0, 0, 0);
-      if (i < 16 * (D / 8) && z < s.n * a.rep)
+      if (i < QN && z < s.n * a.rep)
         qw[k] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt +
                                                 (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
     }
@@ -509,28 +513,36 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
 #pragma unroll
     for (int k = 0; k < QC; ++k) {
       const int i = k * NW * 64 + threadIdx.x;
-      if (i < 16 * (D / 8)) *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = qw[k];
+      if (i < QN) *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = qw[k];
     }
     __syncthreads();
-    auto qfrag = [&](int ks) {
-      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + j * QR + s_dim<Q8>(qd, ks)));
+    auto qfrag = [&](int ct, int ks) {
+      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + (16 * ct + j) * QR + s_dim<Q8>(qd, ks)));
     };
-    SAcc<D> x;
-    x.m = -INFINITY;
-    x.l = 0.0f;
+    SAcc<D> acc[CT];
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
+    for (auto& x : acc) {
+      x.m = -INFINITY;
+      x.l = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
+    }
 
     // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which
     // have the fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do
     // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
-      const int z = z0 + j, tok = min(z / a.rep, s.n - 1);
-      const int begin = a.row_begin ? max(a.row_begin[s.s0 + tok], 0) : 0;
-      const int t_end = min((z0 + 15) / a.rep, s.n - 1);  // last token of these slots
+      const int t_end = min((z0 + 16 * CT - 1) / a.rep, s.n - 1);  // last token of these slots
+      int k_lo = 0;                                                // the first one that any of them sees
+      if (a.row_begin) {
+        k_lo = max(a.row_begin[s.s0 + min((z0 + c) / a.rep, t_end)], 0);  // c: the slots of both columns
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) k_lo = min(k_lo, __shfl_xor(k_lo, o, 64));
+        k_lo = __builtin_amdgcn_readfirstlane(min(k_lo, t_end + 1)) & ~15;
+      }
 #pragma unroll 1
-      for (int k0 = 16 * (NW - 1 - wave); k0 <= t_end; k0 += 16 * NW) {
+      for (int k0 = k_lo + 16 * (NW - 1 - wave); k0 <= t_end; k0 += 16 * NW) {
         const int left = min(16, s.n - k0);
         const uint16_t* kp = a.k + (int64_t)(s.s0 + k0 + min(j, left - 1)) * a.skt + (int64_t)g * a.skh;
         v4u kr[KS];
@@ -550,44 +562,50 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
             v[i][2 * w + 1] = u.y;
           }
         }
-        v4f sc = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) sc = mfma16(kr[ks], qfrag(ks), sc);
-        float y[8], f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = k0 + 4 * qd + i;
-          y[i] = i < 4 && z < s.n * a.rep && key >= begin && key <= tok ? sc[i & 3] * a.scale_log2 : -INFINITY;
-          f[i] = 1.0f;
-        }
+        // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products
+        // take 0 in their places, and the slots that see one get it added
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) odd |= fin_bf16x2(v[i][w]) != v[i][w];
-        v4u hi, lo;
-        s_softmax<D, false>(y, f, x, hi, lo);
-        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
-          // infinities or NaN among the values: 0 times one must not reach a slot that does not see it, so the products
-          // take 0 in their places, and the slots that see one get it added
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w) v[i][w] = fin_bf16x2(v[i][w]);
-#pragma unroll 1
-          for (int key = k0; key < k0 + left; ++key) {
-            if (z >= s.n * a.rep || key < begin || key > tok) continue;
-            const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + 4 * qd * (D / 16);
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x.o[dt][i] += odd_bf16(vp[i * (D / 16) + dt]);
+          for (int w = 0; w < D / 32; ++w) {
+            const uint32_t f = fin_bf16x2(v[i][w]);
+            odd |= f != v[i][w];
+            v[i][w] = f;
           }
-        }
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-          const v4u v8 = s_vfrag<D, false, 4>(v, dt);
-          x.o[dt] = mfma16(v8, hi, x.o[dt]);
-          x.o[dt] = mfma16(v8, lo, x.o[dt]);
+        for (int ct = 0; ct < CT; ++ct) {
+          const int z = z0 + 16 * ct + j, tok = min(z / a.rep, s.n - 1);
+          const int begin = a.row_begin ? max(a.row_begin[s.s0 + tok], 0) : 0;
+          SAcc<D>& x = acc[ct];
+          v4f sc = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) sc = mfma16(kr[ks], qfrag(ct, ks), sc);
+          float y[8], f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = k0 + 4 * qd + i;
+            y[i] = i < 4 && z < s.n * a.rep && key >= begin && key <= tok ? sc[i & 3] * a.scale_log2 : -INFINITY;
+            f[i] = 1.0f;
+          }
+          v4u hi, lo;
+          s_softmax<D, false>(y, f, x, hi, lo);
+          if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+#pragma unroll 1
+            for (int key = k0; key < k0 + left; ++key) {
+              if (z >= s.n * a.rep || key < begin || key > tok) continue;
+              const uint16_t* vp = a.v + (int64_t)(s.s0 + key) * a.svt + (int64_t)g * a.svh + 4 * qd * (D / 16);
+#pragma unroll
+              for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.o[dt][i] += odd_bf16(vp[i * (D / 16) + dt]);
+            }
+          }
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) {
+            const v4u v8 = s_vfrag<D, false, 4>(v, dt);
+            x.o[dt] = mfma16(v8, hi, x.o[dt]);
+            x.o[dt] = mfma16(v8, lo, x.o[dt]);
+          }
         }
       }
     };
@@ -599,7 +617,9 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
         reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
         reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
       }
-      v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+      v4f sc[CT][2];
+#pragma unroll
+      for (auto& c2 : sc) c2[0] = c2[1] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -613,36 +633,46 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
           } else {
             k8 = tl.k[r][ks];
           }
-          sc[r] = mfma16(k8, qfrag(ks), sc[r]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) sc[ct][r] = mfma16(k8, qfrag(ct, ks), sc[ct][r]);
         }
-      float y[8], f[8];
+      float kk[8], f[8];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float4 kf = Q8 ? skf[wave][0][4 * r + qd]
                              : make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
         const float4 vf = Q8 ? skf[wave][1][4 * r + qd] : make_float4(1, 1, 1, 1);
-        const float kk[4] = {kf.x, kf.y, kf.z, kf.w}, vv[4] = {vf.x, vf.y, vf.z, vf.w};
+        const float k4[4] = {kf.x, kf.y, kf.z, kf.w}, v4[4] = {vf.x, vf.y, vf.z, vf.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          y[4 * r + i] = r < R ? sc[r][i] * kk[i] : -INFINITY;
-          f[4 * r + i] = vv[i];
+          kk[4 * r + i] = k4[i];
+          f[4 * r + i] = v4[i];
         }
       }
       int there = 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) there += tl.len[r];
-      if (there != 16 * R) {
+      v4u hi[CT], lo[CT];
 #pragma unroll
-        for (int i = 0; i < 4 * R; ++i)
-          if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
+      for (int ct = 0; ct < CT; ++ct) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = i < 4 * R ? sc[ct][i >> 2][i & 3] * kk[i] : -INFINITY;
+        if (there != 16 * R) {
+#pragma unroll
+          for (int i = 0; i < 4 * R; ++i)
+            if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
+        }
+        s_softmax<D, Q8>(y, f, acc[ct], hi[ct], lo[ct]);
       }
-      v4u hi, lo;
-      s_softmax<D, Q8>(y, f, x, hi, lo);
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
         const v4u v8 = s_vfrag<D, Q8, 4 * R>(tl.v, dt);
-        x.o[dt] = mfma16(v8, hi, x.o[dt]);
-        x.o[dt] = mfma16(v8, lo, x.o[dt]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          acc[ct].o[dt] = mfma16(v8, hi[ct], acc[ct].o[dt]);
+          acc[ct].o[dt] = mfma16(v8, lo[ct], acc[ct].o[dt]);
+        }
       }
     };
     if (tt < t_hi) {
@@ -660,51 +690,55 @@ __global__ __launch_bounds__(kStreamWaves * 64, D == 256 && !Q8 ? 1 : 2) void pa
     if constexpr (D == 256) new_tokens();
 
     // merge the waves, then the output or this split's normalized partial
-    float l = x.l + __shfl_xor(x.l, 16, 64);
-    l = od_xor32_sum(l);
-    __syncthreads();  // every wave is done with the queries
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int ct = 0; ct < CT; ++ct) {
+      const SAcc<D>& x = acc[ct];
+      float l = x.l + __shfl_xor(x.l, 16, 64);
+      l = od_xor32_sum(l);
+      __syncthreads();  // every wave is done with the queries, or the columns before
 #pragma unroll
-      for (int d4 = 0; d4 < D / 64; ++d4)
-        *reinterpret_cast<float4*>(&sm.o[wave][j][(4 * qd + i) * (D / 16) + 4 * d4]) =
-            make_float4(x.o[4 * d4][i], x.o[4 * d4 + 1][i], x.o[4 * d4 + 2][i], x.o[4 * d4 + 3][i]);
-    if (qd == 0) {
-      sml[wave][0][j] = x.m;
-      sml[wave][1][j] = l;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
-      const int zz = i / (D / 4), d0 = (i % (D / 4)) * 4, z = z0 + zz;
-      if (z >= s.n * a.rep) continue;
-      float M = -INFINITY;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][0][zz]);
-      float L = 0.0f;
-      float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float mw = sml[w][0][zz];
-        const float e = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-        const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][zz][d0]);
-        L += e * sml[w][1][zz];
-        acc.x += e * v.x;
-        acc.y += e * v.y;
-        acc.z += e * v.z;
-        acc.w += e * v.w;
+        for (int d4 = 0; d4 < D / 64; ++d4)
+          *reinterpret_cast<float4*>(&sm.o[wave][j][(4 * qd + i) * (D / 16) + 4 * d4]) =
+              make_float4(x.o[4 * d4][i], x.o[4 * d4 + 1][i], x.o[4 * d4 + 2][i], x.o[4 * d4 + 3][i]);
+      if (qd == 0) {
+        sml[wave][0][j] = x.m;
+        sml[wave][1][j] = l;
       }
-      // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L);
-      const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
-      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      if (nv == 1) {
-        *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(acc.x, acc.y),
-            od_pack_bf16x2(acc.z, acc.w));
-        if (a.lse && d0 == 0) a.lse[n * a.Hq + head] = ls * kLn2;
-      } else {
-        const int64_t slot = ((int64_t)sp * a.p.N + n) * a.Hq + head;
-        *reinterpret_cast<float4*>(a.part + slot * D + d0) = acc;
-        if (d0 == 0) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + slot] = ls;
+      __syncthreads();
+      for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+        const int zz = i / (D / 4), d0 = (i % (D / 4)) * 4, z = z0 + 16 * ct + zz;
+        if (z >= s.n * a.rep) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][0][zz]);
+        float L = 0.0f;
+        float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float mw = sml[w][0][zz];
+          const float e = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+          const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][zz][d0]);
+          L += e * sml[w][1][zz];
+          sum.x += e * v.x;
+          sum.y += e * v.y;
+          sum.z += e * v.z;
+          sum.w += e * v.w;
+        }
+        // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L);
+        const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
+        sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        if (nv == 1) {
+          *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(sum.x, sum.y),
+              od_pack_bf16x2(sum.z, sum.w));
+          if (a.lse && d0 == 0) a.lse[n * a.Hq + head] = ls * kLn2;
+        } else {
+          const int64_t slot = ((int64_t)sp * a.p.N + n) * a.Hq + head;
+          *reinterpret_cast<float4*>(a.part + slot * D + d0) = sum;
+          if (d0 == 0) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + slot] = ls;
+        }
       }
     }
   }
@@ -1726,26 +1760,39 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
   bool stream;
+  int ct;  // stream: columns of 16 slots, 1 or 2
   int nw, tiles, run, width, chunk, nsplit;
 };
-Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx) {
+Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx, bool q8) {
   Plan p;
   // hints past any call's own size say nothing; below 2^30 no split begins past the positions an int holds
   max_new = max_new < N ? max_new : N;
   max_ctx = max_ctx < (1 << 30) ? max_ctx : 1 << 30;
   const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
-  p.stream = slots <= 16;
+  // Up to 32 slots stream: 8 tokens of 4 heads a group over 16 ragged x 4000 int8 tokens 37 us, 51 as tiles of 128
+  // slots (bf16 42 and 45; over 1 x 4000 15 and 29, bf16 15 and 25). More of them, 32 a workgroup, where there is
+  // little work: a step of the tile kernel is a chain of some 2 us that needs company on its CU, a streaming one has
+  // nothing to wait for but memory. The workgroups fit in at once and have no more than 128 KB of K a CU to read, from
+  // the L2 mostly: 16 tokens over 1 x 4000 16 us, 30 as tiles; 256 over 1 x 100 15 and 24; 32 over 2 x 4000 21 and 32;
+  // above it 32 over 1 x 32000 62 and 50, bf16 80 and 42, 120 of one head over 1 x 8000 bf16 tokens 37 and 34.
+  const int64_t few = B * Hkv * ((slots + 31) / 32);
+  p.stream = slots <= 32 || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
+  p.ct = slots <= 16 ? 1 : 2;
   // 8 waves share a block's conversion at D = 128 (a chunk of 2048 over 32768: 1316 us, 4 waves 1515); at D = 64 they
   // only coarsen the work (bf16 chunks of 2048 over 16000 234 us, 4 waves 202; int8 ones the same).
   p.nw = p.stream ? kStreamWaves : D == 256 || (D == 128 && slots > 128) ? 8 : 4;
   p.width = p.stream ? 16 * s_halves((int)D) : kBK;
-  const int64_t spt = p.stream ? 16 : D == 256 ? 128 : 32 * p.nw;
+  const int64_t spt = p.stream ? 16 * p.ct : D == 256 ? 128 : 32 * p.nw;
   const int64_t tiles = (slots + spt - 1) / spt, keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
   // workgroups without splits: every sequence's tiles, but no more than the tokens make
   const int64_t all = N * rep / spt + B, wgs = (tiles * B < all ? tiles * B : all) * Hkv;
-  const int64_t fit = p.stream || p.nw == 4 ? 2 * cus : cus;  // how many run at once
-  const int64_t least = 8;                                    // key tiles that are worth a workgroup of their own
+  // how many run at once: two a CU, one where a wave or the shared memory needs it whole
+  const bool one = p.stream ? s_alone((int)D, q8, p.ct) : p.nw == 8;
+  const int64_t fit = one ? cus : 2 * cus;
+  // key tiles that are worth a workgroup of their own (128 tokens over 1 x 1000: 37 us with 8 blocks at least, 35 with
+  // 2)
+  const int64_t least = p.stream ? 8 : 2;
   int64_t most = keys / least < 128 ? keys / least : 128, n = 1;
   if (p.stream) {
     n = fit / (wgs < 1 ? 1 : wgs);
@@ -1908,8 +1955,9 @@ extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, i
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
   if (Hq % Hkv || (D != 64 && D != 128 && D != 256)) return OD_ERR_UNSUPPORTED;
   if (B > 65535 || Hq > 65535 || N > kMaxSlots / (Hq / Hkv)) return OD_ERR_SHAPE;
-  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx);
-  *ws_floats = p.nsplit > 1 ? p.nsplit * N * Hq * (D + 1) : 0;
+  const int n8 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, true).nsplit;
+  const int n16 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, false).nsplit, n = n8 > n16 ? n8 : n16;
+  *ws_floats = n > 1 ? n * N * Hq * (D + 1) : 0;
   return OD_OK;
 }
 
@@ -1951,7 +1999,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   a.Hq = (int)Hq;
   a.rep = (int)(Hq / Hkv);
   a.scale_log2 = scale * kLog2e;
-  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx);
+  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, k_scale != nullptr);
   if (p.nsplit > 1) {
     if (!ws) return OD_ERR_NULL;
     if (ws_floats < p.nsplit * N * Hq * (D + 1)) return OD_ERR_SHAPE;
@@ -1973,8 +2021,9 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     auto launch = [&](auto QC) {
       constexpr bool Q8 = decltype(QC)::value;
       if (p.stream) {
-        const dim3 grid((unsigned)p.nsplit, (unsigned)Hkv, (unsigned)B);
-        paged_stream_kernel<DD, Q8><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+        const dim3 grid((unsigned)p.nsplit, (unsigned)(Hkv * p.tiles), (unsigned)B);
+        if (p.ct == 1) paged_stream_kernel<DD, Q8, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+        else paged_stream_kernel<DD, Q8, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
       } else if constexpr (DD == 64) {
         rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
       } else if constexpr (DD == 256) {

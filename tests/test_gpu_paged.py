@@ -280,6 +280,84 @@ def test_same_calls_same_bits_and_order(gpu_lib, new, ctx):
     assert torch.equal(o, a[rows.to(DEV)]) and torch.equal(ol, al[rows.to(DEV)])
 
 
+# ------------------------------------------------------------------------ the same, by the kernel for many slots
+MANY = [([20], [0]), ([9, 17, 3], [70, 0, 300]), ([33, 64, 7], [64, 65, 130]), ([130], [200]), ([70, 1, 150], [0, 300, 31]),
+        ([300], [0]), ([1, 1], [700, 3]), ([0, 12, 0], [9, 500, 0])]
+
+
+@pytest.fixture(params=["rows", "table"])
+def tiled(request, monkeypatch):
+    """Small calls that the library takes for large ones, by rows of no sequence or by a table with room for 2^20 tokens."""
+    small = make
+
+    def large(*a, **kw):
+        c = small(*a, **dict(kw, pad=kw.get("pad", 0) + (1100 if request.param == "rows" else 0)))
+        if request.param == "table":
+            wide = torch.full((c["table"].shape[0], 2 ** 20 // c["pages"][0].shape[2]), -1, dtype=torch.int32)
+            wide[:, :c["table"].shape[1]] = c["table"]
+            c["table"] = wide
+        return c
+
+    monkeypatch.setitem(globals(), "make", large)
+    return request.param
+
+
+@pytest.mark.parametrize("d,heads,kv", [(64, 4, 4), (128, 8, 2), (256, 4, 1), (128, 7, 1)])
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("shape", range(len(MANY)))
+def test_many_slots(gpu_lib, tiled, shape, int8, d, heads, kv):
+    new, ctx = MANY[shape]
+    c = make(shape, new, ctx, heads, kv, d, page=[16, 64, 32][shape % 3], int8=int8)
+    check_attn(c, *run_attn(c))
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new,ctx,rows", [([24, 40, 1], [50, 0, 129], 8), ([150, 90], [33, 64], 30), ([260], [10], 100)])
+def test_many_slots_option_rows(gpu_lib, tiled, new, ctx, rows, d, int8):
+    test_option_rows(gpu_lib, new, ctx, rows, d, int8)
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_many_slots_masks(gpu_lib, tiled, int8):
+    test_cached_tokens_only(gpu_lib, [100, 60], [0, 90], int8)
+    test_no_pages_and_short_tables(gpu_lib, [40, 1, 100], [200, 90, 33], int8)
+    test_what_is_masked_does_not_matter(gpu_lib, [100], [70], int8)
+    test_sharp_scores(gpu_lib, [64, 90], [400, 10], int8)
+
+
+def test_many_slots_values(gpu_lib, tiled):
+    c = make(6, [70], [20], heads=2, kv=1, d=64, int8=False)
+    c["v"][30, 0, 5] = float("inf")
+    out, _ = run_attn(c)
+    assert torch.isfinite(out[:30].float()).all() and (out[30:70, :, 5] == float("inf")).all()
+    assert torch.isfinite(torch.cat([out[30:70, :, :5], out[30:70, :, 6:]], 2).float()).all()
+    for k_exp, v_exp in [(-100, 60), (60, -100), (0, -20), (20, 100)]:
+        test_sizes_of_the_rows(gpu_lib, [90], [300], k_exp, v_exp)
+    test_bounds_do_not_change_what_is_computed(gpu_lib, [3, 60, 1])
+
+
+def test_many_slots_same_bits(gpu_lib):
+    test_same_calls_same_bits_and_order(gpu_lib, [300, 3], [900, 64])
+    test_same_calls_same_bits_and_order(gpu_lib, [8, 3, 5], [9, 900, 64])  # two columns of 16
+
+
+@pytest.mark.parametrize("new", [[7, 8, 3], [60, 2]])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_infinite_values_of_new_tokens(gpu_lib, new, d):
+    """Each later token sees an infinite value, and nothing else is infinite: bit for bit the rest of the outputs."""
+    c = make(14, new, [40, 0, 9][:len(new)], heads=4, kv=1, d=d)
+    want, _ = run_attn(c)
+    c["v"][2, 0, 5], c["v"][new[0], 0, d - 1] = float("inf"), float("-inf")
+    out, _ = run_attn(c)
+    hit = torch.zeros(out.shape, dtype=torch.bool)
+    hit[2:new[0], :, 5] = True
+    hit[new[0]:new[0] + new[1], :, d - 1] = True
+    hit = hit.to(DEV)
+    assert torch.equal(out[~hit], want[~hit])
+    assert (out[2:new[0], :, 5] == float("inf")).all() and (out[new[0]:new[0] + new[1], :, d - 1] == float("-inf")).all()
+
+
 # ------------------------------------------------------------------------------------------------ append, read
 @pytest.mark.parametrize("d,kv", [(64, 1), (64, 5), (128, 2), (128, 8), (256, 3)])
 @pytest.mark.parametrize("int8", [True, False])
