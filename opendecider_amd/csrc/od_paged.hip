@@ -221,6 +221,17 @@ struct AttnArgs {
   int nsplit, chunk;  // split sp takes the key tiles sp chunk .. of a sequence, the last split all that are left
   int tiles;          // slot tiles of a sequence that the grid covers (the workgroups go on from there)
   int run;            // tiles that lie together on one XCD
+  // the image of int8 pages, img_blocks blocks of every (sequence, KV head): 64 rows of K, then of V, fp16 in frames
+  uint16_t* img;
+  struct ImageBlock* img_heads;
+  int* img_vexp;       // the frame of all of a (sequence, KV head)'s V
+  int img_blocks;      // 0: no image
+  bool rest;           // the kernel without the image, for the sequences that have none
+};
+// Of one block of the image: its keys that exist, the frame of its K.
+struct ImageBlock {
+  uint64_t seen;
+  int kexp, unused;
 };
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -805,17 +816,19 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 // V^T comes from row-major LDS by transposing reads. The kernel here is for heads of 64 and 128; heads of 256 have one
 // of their own below, of the same parts.
 //
-// int8 blocks are converted once per workgroup on the way into LDS, to fp16 in power-of-two frames: K' = fp16(q ks_j
-// 2^(7 - E)) with 2^E above the block's largest scale, V' = fp16(q vs_j 2^(7 - F)) with 2^F above the largest so far
-// (the accumulator moves along when F rises), queries as fp16 q 2^(14 - e) with 2^e above the slot's largest (exact
-// while they are normal). One rounding of 2^-11 at most for every cached value, far below the 2^-8 of their int8 grid,
-// and the scores' factor 2^(e - 14 + E - 7) is one number per slot and block. Probabilities are fp16 there, kept 2^7
-// above what they are (2^15 at most under kSlack), so that one as small as 2^-31 of the largest still counts. bf16
-// pages and the new tokens go in as they are, with bf16 probabilities (2^-8 each, as the output's own rounding).
+// int8 blocks are converted once per workgroup on the way into LDS, or once for all of them ahead (the image, below),
+// to fp16 in power-of-two frames: K' = fp16(q ks_j 2^(7 - E)) with 2^E above the block's largest scale, V' = fp16(q
+// vs_j 2^(7 - F)) with 2^F above the largest so far (the accumulator moves along when F rises), queries as fp16 q 2^(14
+// - e) with 2^e above the slot's largest (exact while they are normal). One rounding of 2^-11 at most for every cached
+// value, far below the 2^-8 of their int8 grid, and the scores' factor 2^(e - 14 + E - 7) is one number per slot and
+// block. Probabilities are fp16 there, kept 2^7 above what they are (2^15 at most under kSlack), so that one as small
+// as 2^-31 of the largest still counts. bf16 pages and the new tokens go in as they are, with bf16 probabilities (2^-8
+// each, as the output's own rounding).
 //
 // The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first
 // in the next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
 constexpr int kBK = 64;
+enum { kBf16 = 0, kInt8 = 1, kImage = 2 };  // what the tile kernels read: bf16 pages, int8 pages, their image
 constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
 
 template <int D>
@@ -852,6 +865,14 @@ __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, 
     const int ch = v ? tv_chunk<D>(key, slot) : slot ^ (D == 64 ? ((key >> 1) & 7) : (key & 15));
     dma16(row(key) + 8 * ch, lds_addr(lds) + 1024 * (i * NW + wave));
   }
+}
+
+// The same from a block of the image, which lies in memory as it does in LDS.
+template <int D, int NW>
+__device__ __forceinline__ void dma_block(const uint16_t* lds, int wave, const uint16_t* src) {
+#pragma unroll
+  for (int i = 0; i < D / (8 * NW); ++i)
+    dma16(src + (i * NW + wave) * 512 + 8 * (threadIdx.x & 63), lds_addr(lds) + 1024 * (i * NW + wave));
 }
 
 template <bool H>
@@ -1170,8 +1191,9 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
   }
 }
 
-template <int D, bool Q8, int NW>
+template <int D, int SRC, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
+  constexpr bool Q8 = SRC == kInt8, IMG = SRC == kImage, H16 = SRC != kBf16;
   constexpr int NT = NW * 64, SPT = 32 * NW, DT = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
@@ -1180,7 +1202,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   const int sp = at.sp, g = at.g, b = at.b;
   const Seq s = seq_of(a, b);
   const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
-  if (sp >= nv) return;
+  if (sp >= nv || (IMG ? blocks > a.img_blocks : a.rest && blocks <= a.img_blocks)) return;
   const int b_lo = sp * a.chunk, b_hi = sp == a.nsplit - 1 ? blocks : min(blocks, b_lo + a.chunk);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1211,7 +1233,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
 
     // ---- the cached blocks b_lo .. b_hi - 1
     if (b_lo < b_hi) {
-      if constexpr (Q8) t_q_to_f16<D>(t);
+      if constexpr (H16) t_q_to_f16<D>(t);
+      const int64_t first = ((int64_t)b * a.p.Hkv + g) * a.img_blocks;  // image: the sequence's first block
+      if constexpr (IMG) frame = a.img_vexp[b * a.p.Hkv + g] - 7;
       // int8 blocks pass through registers, NC 16-byte chunks per thread, K's first; bf16 ones go by DMA
       constexpr int CPK = D / 16, CH = kBK * CPK, NC = 2 * CH / NT;
       v4u r[Q8 ? NC : 1];
@@ -1220,11 +1244,21 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       uint64_t there = 0;      // the loaded block's keys that exist
       const int in_page = (1 << a.p.shift) - 1;
       auto pages = [&](int blk) {
+        if constexpr (IMG) return;
         const int pos = blk * kBK + lane;
         pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
         if (pg >= a.p.n_pages) pg = -1;
       };
+      int kexp_in = 0;  // image: the loaded block's frame
       auto load = [&](int blk, int buf) {
+        if constexpr (IMG) {
+          const uint16_t* src = a.img + (first + blk) * (2 * kBK * D);
+          dma_block<D, NW>(sm.k[buf], wave, src);
+          dma_block<D, NW>(sm.v[buf], wave, src + kBK * D);
+          there = a.img_heads[first + blk].seen;
+          kexp_in = a.img_heads[first + blk].kexp;
+          return;
+        }
         there = __builtin_amdgcn_ballot_w64(pg >= 0);
         const int page = max(pg, 0);  // a key that is not there is read from page 0 and left out later
         auto row = [&](int key) {
@@ -1252,7 +1286,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       uint64_t seen = 0;
       auto store = [&](int buf) {
         seen = there;
-        if constexpr (Q8) {
+        if constexpr (IMG) {
+          kexp = kexp_in;
+        } else if constexpr (Q8) {
           // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not
           // finite, leave them alone
           const bool on = (there >> lane) & 1;
@@ -1295,7 +1331,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
       __syncthreads();
       for (int blk = b_lo; blk < b_hi; ++blk) {
         const int cur = (blk - b_lo) & 1;
-        const float c = Q8 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
+        const float c = H16 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
         const int f_new = Q8 ? vexp - 7 : 0;
         const uint64_t mask = seen;
         if (blk + 1 < b_hi) {
@@ -1321,7 +1357,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
         if (live) {
           v16f sc[2];
           v4u pb[4];
-          t_scores<D, Q8>(sm.k[cur], t, sc);
+          t_scores<D, H16>(sm.k[cur], t, sc);
           if (mask != ~0ull) {
             const uint64_t m4 = mask >> (4 * h);
 #pragma unroll
@@ -1330,8 +1366,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
               for (int i = 0; i < 16; ++i)
                 if (!((m4 >> (kt * 32 + 8 * (i >> 2) + (i & 3))) & 1)) sc[kt][i] = -INFINITY;
           }
-          t_softmax<D, Q8>(sc, c, t, pb);
-          t_values<D, Q8>(sm.v[cur], vb, pb, t);
+          t_softmax<D, H16>(sc, c, t, pb);
+          t_values<D, H16>(sm.v[cur], vb, pb, t);
         }
         if (!Q8 && blk + 1 < b_hi) {
           dma_wait();
@@ -1343,7 +1379,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
 
     // ---- the new tokens, in split 0
     if (sp == 0 && a.k) {
-      if (Q8 && b_lo < b_hi) {  // back to bf16 queries and values as they are
+      if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
         if (frame != 0) {
           const float f = __builtin_ldexpf(1.0f, frame);
@@ -1422,8 +1458,9 @@ struct alignas(16) WSmem {
   int odd;
 };
 
-template <bool Q8>
+template <int SRC>
 __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
+  constexpr bool Q8 = SRC == kInt8, IMG = SRC == kImage, H16 = SRC != kBf16;
   constexpr int D = 256, NW = 8, NT = 512, SPT = 128, DT = 4;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   WSmem& sm = *reinterpret_cast<WSmem*>(smem_raw);
@@ -1432,7 +1469,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
   const int sp = at.sp, g = at.g, b = at.b;
   const Seq s = seq_of(a, b);
   const int nslots = s.n * a.rep, blocks = (s.ctx + kBK - 1) / kBK, nv = splits_of(a, blocks);
-  if (sp >= nv) return;
+  if (sp >= nv || (IMG ? blocks > a.img_blocks : a.rest && blocks <= a.img_blocks)) return;
   const int b_lo = sp * a.chunk, b_hi = sp == a.nsplit - 1 ? blocks : min(blocks, b_lo + a.chunk);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, grp = wave & 3;
@@ -1536,15 +1573,18 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         for (int i = 0; i < 16; ++i) o[i] *= f;
       frame = f_new;
     };
-    using HT = std::integral_constant<bool, Q8>;
+    using HT = std::integral_constant<bool, H16>;
 
     // ---- the cached blocks b_lo .. b_hi - 1
     if (b_lo < b_hi) {
-      if constexpr (Q8) t_q_to_f16<D>(t);
+      if constexpr (H16) t_q_to_f16<D>(t);
+      const int64_t first = ((int64_t)b * a.p.Hkv + g) * a.img_blocks;  // image: the sequence's first block
+      if constexpr (IMG) frame = a.img_vexp[b * a.p.Hkv + g] - 7;
       constexpr int CPK = D / 16, NC = kBK * CPK / NT;  // int8: 16-byte chunks per row; per thread and side
       const int in_page = (1 << a.p.shift) - 1;
       // lane l: the page of key l of a block, or -1
       auto pages = [&](int blk) {
+        if constexpr (IMG) return -1;
         const int pos = blk * kBK + lane;
         const int pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
         return pg < a.p.n_pages ? pg : -1;
@@ -1606,11 +1646,13 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       };
       auto load_k = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
+        else if constexpr (IMG) dma_block<D, NW>(sm.k[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D));
         else dma_rows<D, NW>(sm.k[blk & 1], wave, false,
             [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(blk, pg, key) * D; });
       };
       auto load_v = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
+        else if constexpr (IMG) dma_block<D, NW>(sm.v[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D) + kBK * D);
         else dma_rows<D, NW>(sm.v[blk & 1], wave, true,
             [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(blk, pg, key) * D; });
       };
@@ -1631,14 +1673,18 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         load_k(b_lo + 2, p2);
         load_v(b_lo + 1, p1);
       } else {
-        load_k(b_lo + 1, p1);
+        if (!IMG || b_lo + 1 < b_hi) load_k(b_lo + 1, p1);
         dma_wait();
       }
       int f_cur = vexp - 7;
       __syncthreads();
+      ImageBlock head = {};
+      if constexpr (IMG) head = a.img_heads[first + b_lo];
       for (int blk = b_lo; blk < b_hi; ++blk) {
-        const float c = Q8 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + (blk & 1 ? ke1 : ke0) - 7) : a.scale_log2;
-        const uint64_t seen = __builtin_amdgcn_ballot_w64(p0 >= 0);
+        const int kexp = IMG ? head.kexp : blk & 1 ? ke1 : ke0;
+        const float c = H16 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
+        const uint64_t seen = IMG ? head.seen : __builtin_amdgcn_ballot_w64(p0 >= 0);
+        if (IMG && blk + 1 < b_hi) head = a.img_heads[first + blk + 1];
         v16f x;
         float mine = -INFINITY;
         if (live) {
@@ -1653,7 +1699,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         }
         if constexpr (!Q8) dma_wait();  // this wave's part of V(blk) and K(blk + 1)
         __syncthreads();
-        if (!Q8 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
+        if (!H16 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
           for (int i = tid; i < kBK * (D / 8); i += NT)
             if (!((seen >> (i / (D / 8))) & 1))
               *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
@@ -1681,14 +1727,14 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         __syncthreads();
         if (live) {
           get_p(pb);
-          t_values<D, Q8>(sm.v[blk & 1], vb, pb, t);
+          t_values<D, H16>(sm.v[blk & 1], vb, pb, t);
         }
       }
     }
 
     // ---- the new tokens, in split 0
     if (sp == 0 && a.k) {
-      if (Q8 && b_lo < b_hi) {  // back to bf16 queries and values as they are
+      if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
         rescale(0);
       }
@@ -1751,11 +1797,79 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------ the image of int8 pages
+// Where many slot tiles read the same int8 pages, converting them in each costs more than once for all: the two kernels
+// here write the blocks that the tile kernels want, fp16 in frames and in the order of LDS, into the workspace. V's
+// frame is that of its largest scale over the whole (sequence, KV head), K's that of the block. Sequences longer than
+// img_blocks (the caller's bound was too low) have none; sequences without new tokens need none.
+__global__ __launch_bounds__(1024) void page_frame_kernel(AttnArgs a) {
+  __shared__ uint32_t sm[16];
+  const int g = blockIdx.x % a.p.Hkv, b = blockIdx.x / a.p.Hkv;
+  const Seq s = seq_of(a, b);
+  if (s.n == 0 || (s.ctx + kBK - 1) / kBK > a.img_blocks) return;
+  uint32_t m = 0;
+#pragma unroll 8
+  for (int pos = threadIdx.x; pos < s.ctx; pos += 1024) {
+    const int64_t row = row_of(a.p, b, g, pos);
+    const float vs = row >= 0 ? a.p.vs[row] : 0.0f;
+    if (vs < INFINITY && vs > 0) m = max(m, __float_as_uint(vs));
+  }
+  m = od_wave_umax_dpp(m);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = max(m, sm[i]);
+    a.img_vexp[blockIdx.x] = exp_above(m);
+  }
+}
+template <int D>
+__global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
+  constexpr int CPK = D / 16, CH = kBK * CPK, NC = 2 * CH / kThreads;
+  const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+  const Seq s = seq_of(a, b);
+  const int blocks = (s.ctx + kBK - 1) / kBK;
+  if (s.n == 0 || blk >= blocks || blocks > a.img_blocks) return;
+  const int64_t at = ((int64_t)b * a.p.Hkv + g) * a.img_blocks + blk;
+  const int pos = blk * kBK + lane;
+  const int64_t mine = pos < s.ctx ? row_of(a.p, b, g, pos) : -1, row = max(mine, (int64_t)0);
+  const bool on = mine >= 0;  // a key that is not there: the pool's first row, times 0
+  const float ks = a.p.ks[row], vs = a.p.vs[row];
+  const uint64_t seen = __builtin_amdgcn_ballot_w64(on);
+  const int kexp = exp_above(od_wave_umax_dpp(on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u));
+  const int vexp = a.img_vexp[b * a.p.Hkv + g];
+  const float kf = on ? frame_scale(ks, 7 - kexp) : 0.0f, vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
+  if (threadIdx.x == 0) a.img_heads[at] = ImageBlock{seen, kexp, 0};
+  v4u r[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int cid = i * kThreads + threadIdx.x, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+    const int64_t from = ((int64_t)__shfl((int)(row >> 32), key, 64) << 32) | (uint32_t)__shfl((int)row, key, 64);
+    r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) +
+                                                                  from * D + 16 * ch));
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int cid = i * kThreads + threadIdx.x, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+    uint16_t* dst = a.img + at * (2 * kBK * D) + side * (kBK * D);
+    v4u lo, hi;
+    i8x16_scaled(r[i], __shfl(side ? vf : kf, key, 64), lo, hi);
+    const int o0 = side ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
+    const int o1 = side ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
+    *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
+    *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
+  }
+}
+
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
   bool stream;
   int ct;  // stream: columns of 16 slots, 1 or 2
   int nw, tiles, run, width, chunk, nsplit;
+  int64_t img_blocks;  // of every (sequence, KV head); 0: no image
+  // the workspace, in floats: partials, then the image's V frames, heads and blocks
+  int64_t part, vexp, heads, img;
+  int64_t floats() const { return part + vexp + heads + img; }
 };
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx, bool q8) {
   Plan p;
@@ -1815,6 +1929,17 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   int parts = 1;
   while (parts < 8 && groups * parts % 8 && groups * parts < 64) parts *= 2;
   p.run = (p.tiles + parts - 1) / parts;
+  p.part = p.nsplit > 1 ? (p.nsplit * N * Hq * (D + 1) + 3) / 4 * 4 : 0;
+  // The image, up to 1 GB of it, where 4 slot tiles or more share a block and the conversions that it saves are worth
+  // its launches: counted in values a slot they are wgs keys D / spt. Chunks of 2048 over 32768 1364 us, with it 1190;
+  // 256-wide heads, 4 ragged 900 over 6000 416, 300; 1 x 256 over 6000 (3000 blocks in all) 92, 86; 8 x 64 (2 tiles)
+  // 121, 126; heads of 128, 8 x 256 over 6000 (4 tiles) 219, 203, 8 x 128 (2 tiles) 132, 146, 4 x 1024 over 1000 (8000
+  // blocks) 84, 89, 4 x 256 over 6000 (12000) 132, 124.
+  p.img_blocks = !p.stream && q8 && tiles >= 4 && wgs * keys * D / spt > 5 << 10 ? keys : 0;
+  if (p.img_blocks * B * Hkv > (1ll << 28) / (kBK * D)) p.img_blocks = 0;
+  p.vexp = p.img_blocks ? (B * Hkv + 3) / 4 * 4 : 0;
+  p.heads = p.img_blocks * B * Hkv * 4;
+  p.img = p.img_blocks * B * Hkv * kBK * D;
   return p;
 }
 
@@ -1856,9 +1981,9 @@ int launch_big(const AttnArgs& a, unsigned groups, int threads, int bytes, hipSt
   Kernel<<<dim3(groups), dim3(threads), bytes, st>>>(a);
   return OD_OK;
 }
-template <int D, bool Q8, int NW>
+template <int D, int SRC, int NW>
 int launch_tiles(const AttnArgs& a, unsigned groups, hipStream_t st) {
-  return launch_big<&paged_tile_kernel<D, Q8, NW>>(a, groups, NW * 64, (int)sizeof(TSmem<D, NW>), st);
+  return launch_big<&paged_tile_kernel<D, SRC, NW>>(a, groups, NW * 64, (int)sizeof(TSmem<D, NW>), st);
 }
 
 template <class F>
@@ -1948,9 +2073,9 @@ extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, i
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
   if (Hq % Hkv || (D != 64 && D != 128 && D != 256)) return OD_ERR_UNSUPPORTED;
   if (B > 65535 || Hq > 65535 || N > kMaxSlots / (Hq / Hkv)) return OD_ERR_SHAPE;
-  const int n8 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, true).nsplit;
-  const int n16 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, false).nsplit, n = n8 > n16 ? n8 : n16;
-  *ws_floats = n > 1 ? n * N * Hq * (D + 1) : 0;
+  const int64_t n8 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, true).floats();
+  const int64_t n16 = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, false).floats();
+  *ws_floats = n8 > n16 ? n8 : n16;
   return OD_OK;
 }
 
@@ -1993,12 +2118,17 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   a.rep = (int)(Hq / Hkv);
   a.scale_log2 = scale * kLog2e;
   const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, k_scale != nullptr);
-  if (p.nsplit > 1) {
+  if (p.floats()) {
     if (!ws) return OD_ERR_NULL;
-    if (ws_floats < p.nsplit * N * Hq * (D + 1)) return OD_ERR_SHAPE;
+    if (ws_floats < p.floats()) return OD_ERR_SHAPE;
     if (!od_aligned16(ws)) return OD_ERR_ALIGN;
   }
   a.part = ws;
+  a.img_vexp = reinterpret_cast<int*>(ws + p.part);
+  a.img_heads = reinterpret_cast<ImageBlock*>(ws + p.part + p.vexp);
+  a.img = reinterpret_cast<uint16_t*>(ws + p.part + p.vexp + p.heads);
+  a.img_blocks = (int)p.img_blocks;
+  a.rest = false;
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
   a.tiles = p.tiles;
@@ -2011,24 +2141,37 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   int rc = OD_OK;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
-    auto launch = [&](auto QC) {
-      constexpr bool Q8 = decltype(QC)::value;
-      if (p.stream) {
-        const dim3 grid((unsigned)p.nsplit, (unsigned)(Hkv * p.tiles), (unsigned)B);
-        if (p.ct == 1) paged_stream_kernel<DD, Q8, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
-        else paged_stream_kernel<DD, Q8, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
-      } else if constexpr (DD == 64) {
-        rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
-      } else if constexpr (DD == 256) {
-        rc = launch_big<&paged_wide_kernel<Q8>>(a, (unsigned)groups, 512, (int)sizeof(WSmem), st);
-      } else if (p.nw == 8) {
-        rc = launch_tiles<DD, Q8, 8>(a, (unsigned)groups, st);
-      } else {
-        rc = launch_tiles<DD, Q8, 4>(a, (unsigned)groups, st);
-      }
+    auto tiles = [&](auto SC) {
+      constexpr int SRC = decltype(SC)::value;
+      if constexpr (DD == 64) rc = launch_tiles<DD, SRC, 4>(a, (unsigned)groups, st);
+      else if constexpr (DD == 256) rc = launch_big<&paged_wide_kernel<SRC>>(a, (unsigned)groups, 512,
+          (int)sizeof(WSmem), st);
+      else if (p.nw == 8) rc = launch_tiles<DD, SRC, 8>(a, (unsigned)groups, st);
+      else rc = launch_tiles<DD, SRC, 4>(a, (unsigned)groups, st);
     };
-    if (k_scale) launch(std::true_type{});
-    else launch(std::false_type{});
+    auto stream = [&](auto QC) {
+      constexpr bool Q8 = decltype(QC)::value;
+      const dim3 grid((unsigned)p.nsplit, (unsigned)(Hkv * p.tiles), (unsigned)B);
+      if (p.ct == 1) paged_stream_kernel<DD, Q8, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+      else paged_stream_kernel<DD, Q8, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+    };
+    if (p.stream) {
+      if (k_scale) stream(std::true_type{});
+      else stream(std::false_type{});
+    } else if (!k_scale) {
+      tiles(std::integral_constant<int, kBf16>{});
+    } else {
+      if (p.img_blocks) {
+        const dim3 grid((unsigned)p.img_blocks, (unsigned)Hkv, (unsigned)B);
+        page_frame_kernel<<<dim3((unsigned)(B * Hkv)), dim3(1024), 0, st>>>(a);
+        page_image_kernel<DD><<<grid, dim3(kThreads), 0, st>>>(a);
+        tiles(std::integral_constant<int, kImage>{});
+        a.rest = true;
+      }
+      // the sequences without an image, if the table can hold any
+      if (rc == OD_OK && p.img_blocks * kBK < ((int64_t)a.p.cols << a.p.shift)) tiles(std::integral_constant<int,
+          kInt8>{});
+    }
     if (rc == OD_OK && p.nsplit > 1) {
       // groups when a workgroup has one slot; slots when a slot has one group
       constexpr int S = 4 * kThreads / DD, SL = S;

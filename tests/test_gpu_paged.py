@@ -337,6 +337,63 @@ def test_many_slots_values(gpu_lib, tiled):
     test_bounds_do_not_change_what_is_computed(gpu_lib, [3, 60, 1])
 
 
+@pytest.fixture
+def imaged(monkeypatch):
+    """Small calls with the bounds of large ones: their int8 pages go through the image (rows of no sequence, a table with room
+    for 2^16 tokens)."""
+    small = make
+
+    def large(*a, **kw):
+        c = small(*a, **dict(kw, pad=kw.get("pad", 0) + 1100))
+        B, (_, kv, page, d) = c["table"].shape[0], c["pages"][0].shape
+        wide = torch.full((B, 2 ** 16 // page), -1, dtype=torch.int32)
+        wide[:, :c["table"].shape[1]] = c["table"]
+        c["table"] = wide
+        if c["scales"][0] is not None:
+            from opendecider_amd import kernels
+            N, heads, _ = c["q"].shape
+            dev = torch.device(DEV, torch.cuda.current_device())
+            assert kernels.paged_attn_workspace_floats(B, N, heads, kv, d, N, 2 ** 16, dev) > B * kv * 2 ** 16 * d
+        return c
+
+    monkeypatch.setitem(globals(), "make", large)
+
+
+@pytest.mark.parametrize("d,heads,kv", [(64, 4, 4), (128, 8, 2), (256, 4, 1), (128, 7, 1)])
+@pytest.mark.parametrize("shape", range(len(MANY)))
+def test_image(gpu_lib, imaged, shape, d, heads, kv):
+    new, ctx = MANY[shape]
+    c = make(shape, new, ctx, heads, kv, d, page=[16, 64, 32][shape % 3])
+    check_attn(c, *run_attn(c))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_image_option_rows(gpu_lib, imaged, d):
+    test_option_rows(gpu_lib, [150, 90], [33, 64], 30, d, True)
+
+
+def test_image_masks_and_values(gpu_lib, imaged):
+    test_cached_tokens_only(gpu_lib, [100, 60], [0, 90], True)
+    c = make(11, [40, 1, 100], [200, 90, 33])
+    n = c["pages"][0].shape[0]
+    c["table"][0, 1], c["table"][0, 3], c["table"][1, 0], c["table"][2, 0], c["table"][2, 1] = -1, n, 2 ** 31 - 1, -7, n + 5
+    check_attn(c, *run_attn(c))
+    test_what_is_masked_does_not_matter(gpu_lib, [100], [70], True)
+    test_sharp_scores(gpu_lib, [64, 90], [400, 10], True)
+    for k_exp, v_exp in [(-100, 60), (60, -100), (0, -20), (20, 100)]:
+        test_sizes_of_the_rows(gpu_lib, [90], [300], k_exp, v_exp)
+
+
+@pytest.mark.parametrize("d,heads,kv,pad", [(256, 4, 1, 6000), (128, 8, 1, 24000)])
+def test_image_of_some(gpu_lib, d, heads, kv, pad):
+    """max_ctx below one state's length: the others go through the image, that one as it is."""
+    c = make(15, [70, 40, 30], [500, 3000, 1024], heads, kv, d, page=64, pad=pad)
+    from opendecider_amd import kernels
+    dev = torch.device(DEV, torch.cuda.current_device())
+    assert kernels.paged_attn_workspace_floats(3, pad + 140, heads, kv, d, pad + 140, 1024, dev) > 3 * kv * 1024 * d
+    check_attn(c, *run_attn(c, max_ctx=1024))
+
+
 def test_many_slots_same_bits(gpu_lib):
     test_same_calls_same_bits_and_order(gpu_lib, [300, 3], [900, 64])
     test_same_calls_same_bits_and_order(gpu_lib, [8, 3, 5], [9, 900, 64])  # two columns of 16
