@@ -1886,15 +1886,22 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   const int64_t few = B * Hkv * ((slots + 31) / 32);
   p.stream = slots <= 32 || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
   p.ct = slots <= 16 ? 1 : 2;
-  // 8 waves share a block's conversion at D = 128 (a chunk of 2048 over 32768: 1316 us, 4 waves 1515); at D = 64 they
-  // only coarsen the work (bf16 chunks of 2048 over 16000 234 us, 4 waves 202; int8 ones the same).
-  p.nw = p.stream ? kStreamWaves : D == 256 || (D == 128 && slots > 128) ? 8 : 4;
+  // workgroups without splits for tiles of spt slots: every sequence's, but no more than the tokens make
+  auto wgs_of = [&](int64_t spt) {
+    const int64_t each = (slots + spt - 1) / spt * B, all = N * rep / spt + B;
+    return (each < all ? each : all) * Hkv;
+  };
+  // Heads of 128 take 8 waves, which share a block (chunk of 2048 over 32768 1140 us, 4 waves 1193; bf16 1137 and
+  // 1304), or 4 for few slots and for several sequences that leave CUs without work: the longest of them decides then,
+  // and its workgroups run faster where they have a CU to themselves (2 ragged x 1024 over 8000 244 us with 8, 195 with
+  // 4; bf16 271 and 244; 3 x 700 over 4000 142 and 123; but 2 x 2000 over 500, 432 of 8, 90 and 98). Heads of 64: 4
+  // (bf16 chunks of 2048 over 16000 234 and 202).
+  const bool wide8 = D == 128 && slots > 128 && (B == 1 || wgs_of(256) >= cus);
+  p.nw = p.stream ? kStreamWaves : D == 256 || wide8 ? 8 : 4;
   p.width = p.stream ? 16 * s_halves((int)D) : kBK;
   const int64_t spt = p.stream ? 16 * p.ct : D == 256 ? 128 : 32 * p.nw;
-  const int64_t tiles = (slots + spt - 1) / spt, keys = (max_ctx + p.width - 1) / p.width;
+  const int64_t tiles = (slots + spt - 1) / spt, wgs = wgs_of(spt), keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
-  // workgroups without splits: every sequence's tiles, but no more than the tokens make
-  const int64_t all = N * rep / spt + B, wgs = (tiles * B < all ? tiles * B : all) * Hkv;
   // how many run at once: two a CU, one where a wave or the shared memory needs it whole
   const bool one = p.stream ? s_alone((int)D, q8, p.ct) : p.nw == 8;
   const int64_t fit = one ? cus : 2 * cus;
@@ -1907,13 +1914,15 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     if (n > most) n = most;
     if (n < 1) n = 1;
   } else {
-    // the n of least cost: rounds of workgroups times a workgroup's blocks and what it costs besides them, about 12
-    // blocks (the queries, the first loads, the new tokens, the partials). One round filled once: a chunk of 512 over
-    // 16000 takes 583 us whole, 223 in 3, 192 in 4, 234 in 6 parts; 304 workgroups of 256-wide heads in 2 rounds 739
-    // us, 608 of half the keys in 3 rounds 620, 4 parts 709.
+    // The n of least cost: rounds of workgroups times a workgroup's blocks and what it costs besides them, about 12
+    // blocks (the queries, the first loads, the new tokens, the partials). x > 1 rounds count as x + 1/2, 1.6 at least:
+    // a workgroup starts where another ends, and the last ones leave CUs idle. A chunk of 512 over 16000 takes 583 us
+    // whole, 223 in 3, 192 in 4 (one round), 234 in 6 parts; 5 ragged bf16 600 over 2000 (592 workgroups) whole rounds
+    // chose 2 parts, 108 us, and this takes 3, 91; 8 x 384 over 6000 272 and 251.
     int64_t best = 0;
     for (int64_t i = 1; i <= most || i == 1; ++i) {
-      const int64_t cost = ((wgs * i + fit - 1) / fit) * ((keys + i - 1) / i + 12);
+      const int64_t x10 = 10 * wgs * i / fit + 5, rounds10 = wgs * i <= fit ? 10 : x10 < 16 ? 16 : x10;
+      const int64_t cost = rounds10 * ((keys + i - 1) / i + 12);
       if (best == 0 || cost < best) {
         best = cost;
         n = i;
