@@ -228,10 +228,11 @@ struct AttnArgs {
   int img_blocks;      // 0: no image
   bool rest;           // the kernel without the image, for the sequences that have none
 };
-// Of one block of the image: its keys that exist, the frame of its K.
+// Of one block of the image: its keys that exist, the frame of its K, the largest of its V scales (as bits).
 struct ImageBlock {
   uint64_t seen;
-  int kexp, unused;
+  int kexp;
+  uint32_t v_bits;
 };
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -1801,27 +1802,18 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 // Where many slot tiles read the same int8 pages, converting them in each costs more than once for all: the two kernels
 // here write the blocks that the tile kernels want, fp16 in frames and in the order of LDS, into the workspace. V's
 // frame is that of its largest scale over the whole (sequence, KV head), K's that of the block. Sequences longer than
-// img_blocks (the caller's bound was too low) have none; sequences without new tokens need none.
-__global__ __launch_bounds__(1024) void page_frame_kernel(AttnArgs a) {
-  __shared__ uint32_t sm[16];
-  const int g = blockIdx.x % a.p.Hkv, b = blockIdx.x / a.p.Hkv;
+// img_blocks (the caller's bound was too low) have none; sequences without new tokens need none. A wave takes the frame
+// of one block's V (of all of them in a workgroup per (sequence, KV head), 32768 tokens took 20 us).
+__global__ __launch_bounds__(kThreads) void page_frame_kernel(AttnArgs a) {
+  const int blk = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), g = blockIdx.y, b = blockIdx.z;
   const Seq s = seq_of(a, b);
-  if (s.n == 0 || (s.ctx + kBK - 1) / kBK > a.img_blocks) return;
-  uint32_t m = 0;
-#pragma unroll 8
-  for (int pos = threadIdx.x; pos < s.ctx; pos += 1024) {
-    const int64_t row = row_of(a.p, b, g, pos);
-    const float vs = row >= 0 ? a.p.vs[row] : 0.0f;
-    if (vs < INFINITY && vs > 0) m = max(m, __float_as_uint(vs));
-  }
-  m = od_wave_umax_dpp(m);
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) m = max(m, sm[i]);
-    a.img_vexp[blockIdx.x] = exp_above(m);
-  }
+  const int blocks = (s.ctx + kBK - 1) / kBK, pos = blk * kBK + (threadIdx.x & 63);
+  if (s.n == 0 || blk >= blocks || blocks > a.img_blocks) return;
+  const int64_t row = pos < s.ctx ? row_of(a.p, b, g, pos) : -1;
+  const float vs = row >= 0 ? a.p.vs[row] : 0.0f;
+  const uint32_t m = od_wave_umax_dpp(vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u);
+  if ((threadIdx.x & 63) == 0)
+    a.img_heads[((int64_t)b * a.p.Hkv + g) * a.img_blocks + blk].v_bits = m;
 }
 template <int D>
 __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
@@ -1837,9 +1829,17 @@ __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
   const float ks = a.p.ks[row], vs = a.p.vs[row];
   const uint64_t seen = __builtin_amdgcn_ballot_w64(on);
   const int kexp = exp_above(od_wave_umax_dpp(on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u));
-  const int vexp = a.img_vexp[b * a.p.Hkv + g];
+  // the largest of all blocks, by every wave
+  uint32_t vm = 0;
+#pragma unroll 4
+  for (int i = lane; i < blocks; i += 64) vm = max(vm, a.img_heads[at - blk + i].v_bits);
+  const int vexp = exp_above(od_wave_umax_dpp(vm));
   const float kf = on ? frame_scale(ks, 7 - kexp) : 0.0f, vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
-  if (threadIdx.x == 0) a.img_heads[at] = ImageBlock{seen, kexp, 0};
+  if (threadIdx.x == 0) {
+    a.img_heads[at].seen = seen;
+    a.img_heads[at].kexp = kexp;
+    if (blk == 0) a.img_vexp[b * a.p.Hkv + g] = vexp;
+  }
   v4u r[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -2172,7 +2172,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     } else {
       if (p.img_blocks) {
         const dim3 grid((unsigned)p.img_blocks, (unsigned)Hkv, (unsigned)B);
-        page_frame_kernel<<<dim3((unsigned)(B * Hkv)), dim3(1024), 0, st>>>(a);
+        page_frame_kernel<<<dim3((unsigned)((p.img_blocks + 3) / 4), grid.y, grid.z), dim3(kThreads), 0, st>>>(a);
         page_image_kernel<DD><<<grid, dim3(kThreads), 0, st>>>(a);
         tiles(std::integral_constant<int, kImage>{});
         a.rest = true;
