@@ -592,7 +592,8 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
  *   ones only). q, out bf16 [N, Hq, D], lse fp32 [N, Hq] or NULL (natural log, of the scaled scores); a token that sees
  *   nothing gets 0 and -inf. The pages are read, not written: append before or after. scale > 0 and finite. max_new and
  *   max_ctx are the caller's bounds on a sequence's new and cached tokens; they size the grid, the key splits and the
- *   workspace (od_paged_attn_ws floats, 16-byte aligned, NULL where that is 0), not the result.
+ *   workspace (od_paged_attn_ws floats, 16-byte aligned, NULL where that is 0; one call's at a time), not the result. out
+ *   must not overlap the inputs. B <= 65535, N Hq / Hkv < 2^30.
  */
 #define OD_READ_BF16 0
 #define OD_READ_FP32 1

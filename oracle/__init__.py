@@ -18,6 +18,9 @@ Modules
              gates, the gated delta rule, the gated RMSNorm. Reference: transformers' Qwen3.5 modules, which the
              reference runs (src/opendecider/backbone.py:256-289, skipkv.py:208-231).
 
+  paged      The paged K/V cache: where a packed token lies, writing, reading back, and attention over pages in float64.
+             No counterpart in the reference (its caches are rectangular); written from the layout.
+
 Pinning (how each function is checked, in tests/test_oracle_*.py)
   quant.quantize_rows      brute-force per-element IEEE float32 arithmetic with numpy and round-half-even, hand
                            known answers (ties, zero rows, absmax -> +-127), error bound |q*s - x| <= s/2,
@@ -27,6 +30,8 @@ Pinning (how each function is checked, in tests/test_oracle_*.py)
   quant.smooth_*           the reference test test_int8_gemm.py:70-88 restated (float64 exactness, formula).
   attention.*              float64 brute-force softmax loops on tiny shapes; merge == one softmax over the
                            concatenated keys; permutation equivariance; empty key set; torch.logsumexp.
+  paged.*                  per-token float64 softmax loops over tables with bad entries and empty states; written tokens read
+                           back as quant.quantize_rows has them (tests/test_paged_cache.py).
   gdn.*                    transformers' own functions (causal_conv1d_fn / _update, l2norm, the recurrent and
                            chunked gated delta rule, Qwen3_5RMSNormGated), a pure-decay closed form, continuation ==
                            whole sequence, decimal rsqrt.
