@@ -608,6 +608,9 @@ int od_page_read(const void* k_pages, const float* k_scale, const void* v_pages,
                  od_stream_t stream);
 int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx,
                      int64_t* ws_floats);
+/* for int8 pages (int8 != 0) or bf16 ones; od_paged_attn_ws is enough for either */
+int od_paged_attn_ws_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx,
+                        int int8_pages, int64_t* ws_floats);
 int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
                   const uint16_t* v, int64_t svt, int64_t svh, const void* k_pages, const float* k_scale,
                   const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page, const int32_t* table,

@@ -96,6 +96,7 @@ SIGNATURES = {
     "od_page_read": [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _i64, _i64,
                      ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     "od_paged_attn_ws": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_ptr],
+    "od_paged_attn_ws_of": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _c_ptr],
     "od_paged_attn": [_c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64,
                       _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _i64, _i64, _i64,
                       _i64, _i64, ctypes.c_float, _c_ptr, _i64, _c_ptr],

@@ -519,6 +519,8 @@ class DenseDecoder:
         their K and V go into pages taken from the pool. Returns their final hidden states (N, hidden), in a buffer that
         a later call overwrites. MemoryError, with the states unchanged, where the pool has too few pages."""
         self._check_paged(states)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("extend cannot be captured: a replay would not take pages or advance the states")
         counts = [int(n) for n in counts]
         if ids.dim() != 1 or ids.numel() != sum(counts):
             raise ValueError("extend: ids must be (sum of counts,)")

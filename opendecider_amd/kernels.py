@@ -1032,7 +1032,8 @@ def gdn_norm_quant(o: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
 
 # ------------------------------------------------------------------------------------------------ paged K/V cache
 def _paged(cache, table, start, ctx_len, name):
-    """The arguments of a paged batch that every entry point takes, checked: the sequence count and (pages, table)."""
+    """The arguments of a paged batch that every entry point takes, checked: the sequence count, (pages, table) and the table
+    that they point to (a copy of rows that share memory: hold it until the call is made)."""
     k, i32 = cache.k, torch.int32
     B = ctx_len.numel()
     if table.dtype != i32 or ctx_len.dtype != i32 or (start is not None and start.dtype != i32):
@@ -1046,8 +1047,10 @@ def _paged(cache, table, start, ctx_len, name):
             (start is not None and start.get_device() != dev):
         raise ValueError(f"{name}: all tensors must be on one device")
     cols = table.shape[1]
+    if B > 1 and table.stride(0) < cols:
+        table = table.contiguous()
     return B, (k.data_ptr(), ptr(cache.k_scale), cache.v.data_ptr(), ptr(cache.v_scale), k.shape[0], k.shape[2],
-               table.data_ptr(), max(table.stride(0), cols) if B > 1 else cols, cols)
+               table.data_ptr(), table.stride(0) if B > 1 else cols, cols), table
 
 
 def _new_rows(x, N, H, D, cache, name):
@@ -1091,7 +1094,7 @@ def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, st
     before, which is where they go. Tokens without a page are not written. The lengths stay: advance them once every layer
     has its tokens."""
     require_gpu(k, v, cache.k, table, start, ctx_len, name="page_append")
-    B, pages = _paged(cache, table, start, ctx_len, "page_append")
+    B, pages, table = _paged(cache, table, start, ctx_len, "page_append")
     _, H, _, D = cache.k.shape
     N = k.shape[0]
     k, ka = _new_rows(k, N, H, D, cache, "page_append: k")
@@ -1106,7 +1109,7 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
     them. dtype bfloat16 or float32: the values q * s, one fp32 product (Int8Tensor.dequantize rounds the scale to bf16
     first). int8 (int8 pages only): two Int8Tensors, the stored bytes and scales (scales (B, Hkv, T, 1))."""
     require_gpu(cache.k, table, length, name="page_read")
-    B, pages = _paged(cache, table, None, length, "page_read")
+    B, pages, table = _paged(cache, table, None, length, "page_read")
     if T < 0:
         raise ValueError(f"page_read: T must not be negative, got {T}")
     forms = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
@@ -1130,16 +1133,18 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
 _PAGED_WS: dict = {}
 
 
-def paged_attn_workspace_floats(B: int, N: int, Hq: int, Hkv: int, D: int, max_new: int, max_ctx: int, device) -> int:
-    """Floats of od_paged_attn's workspace for these sizes on the device (0: the keys are not split)."""
-    key = (device.index, B, N, Hq, Hkv, D, max_new, max_ctx)
+def paged_attn_workspace_floats(B: int, N: int, Hq: int, Hkv: int, D: int, max_new: int, max_ctx: int, device,
+                                quantized: bool = True) -> int:
+    """Floats of od_paged_attn's workspace for these sizes and pages on the device (0: none)."""
+    key = (device.index, B, N, Hq, Hkv, D, max_new, max_ctx, quantized)
     n = _PAGED_WS.get(key)
     if n is None:
         if len(_PAGED_WS) >= 65536:  # the sizes are cheap to ask for again
             _PAGED_WS.clear()
         w = ctypes.c_int64(0)
         with torch.cuda.device(device):
-            check(lib().od_paged_attn_ws(B, N, Hq, Hkv, D, max_new, max_ctx, ctypes.byref(w)), "od_paged_attn_ws")
+            check(lib().od_paged_attn_ws_of(B, N, Hq, Hkv, D, max_new, max_ctx, int(quantized), ctypes.byref(w)),
+                  "od_paged_attn_ws_of")
         n = _PAGED_WS[key] = w.value
     return n
 
@@ -1154,7 +1159,7 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     read; int8 rows count as the exact q * s. Returns out (N, Hq, D) bf16 [, lse (N, Hq) fp32]; a token that sees nothing
     gets 0 and -inf, rows of no sequence are left as they were."""
     require_gpu(q, k, v, cache.k, table, start, ctx_len, row_begin, out, name="paged_attn")
-    B, pages = _paged(cache, table, start, ctx_len, "paged_attn")
+    B, pages, table = _paged(cache, table, start, ctx_len, "paged_attn")
     n_pages, H, page, D = cache.k.shape
     N, Hq = q.shape[0], q.shape[1]
     q, qa = _new_rows(q, N, Hq, D, cache, "paged_attn: q")
@@ -1183,7 +1188,7 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
         aligned = not (out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8)
         dst = out if aligned else out.clone(memory_format=torch.contiguous_format)
     lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device)
+    n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device, cache.k_scale is not None)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     with _OnDevice(q):
         check(lib().od_paged_attn(*qa, *ka, *va, *pages, start.data_ptr(),

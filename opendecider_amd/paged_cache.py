@@ -48,6 +48,8 @@ class PagedKVCache:
             raise TypeError(f"PagedKVCache: pages are int8 or bfloat16, got {k.dtype}")
         elif ks is not None or vs is not None:
             raise TypeError("PagedKVCache: bf16 pages have no scales")
+        if any(x is not None and x.device != k.device for x in (v, ks, vs)):
+            raise ValueError("PagedKVCache: the pages and scales must be on one device")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("PagedKVCache: the pages must be contiguous")
         if shape[2] < 16 or shape[2] & (shape[2] - 1):

@@ -415,6 +415,60 @@ def test_infinite_values_of_new_tokens(gpu_lib, new, d):
     assert (out[2:new[0], :, 5] == float("inf")).all() and (out[new[0]:new[0] + new[1], :, d - 1] == float("-inf")).all()
 
 
+@pytest.mark.parametrize("new,pad", [(2, 0), (60, 0), (60, 6000)])
+def test_one_table_row_for_all(gpu_lib, new, pad):
+    """An expanded table: every sequence reads the same pages."""
+    from opendecider_amd import kernels
+    c = make(16, [new] * 3, [500, 300, 500], 8, 2, pad=pad, page=32)
+    row = gpu(c["table"][:1])
+    c["table"] = c["table"][:1].repeat(3, 1)
+    want, wl = run_attn(c)
+    cache = cache_of(c)
+    got, gl = kernels.paged_attn(gpu(c["q"]), gpu(c["k"]), gpu(c["v"]), cache, row.expand(3, -1), gpu(c["start"]), gpu(c["ctx"]),
+                                 c["scale"], return_lse=True)
+    N = 3 * new
+    assert torch.equal(got[:N], want[:N]) and torch.equal(gl[:N], wl[:N])
+    for x, y in zip(kernels.page_read(cache, row.expand(3, -1), gpu(c["ctx"]), 500),
+                    kernels.page_read(cache, gpu(c["table"]), gpu(c["ctx"]), 500)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_many_sequences(gpu_lib, int8):
+    """More sequences than are put in order by their lengths."""
+    new = [(37 * b) % 50 for b in range(70)]
+    c = make(17, new, [(61 * b) % 300 for b in range(70)], 8, 2, int8=int8, page=32)
+    check_attn(c, *run_attn(c, max_new=max(new), max_ctx=300))
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("new,pad", [(1, 0), (70, 1100), (70, 6000)])
+def test_a_pool_past_32_bits(gpu_lib, int8, new, pad):
+    """Pages behind the first 2^31 values of the pool: bit for bit what the same pages do in a small one."""
+    from opendecider_amd import PagedKVCache, kernels
+    c = make(18, [new, new], [900, 333], 8, 2, page=64, int8=int8, pad=pad)
+    want, wl = run_attn(c)
+    n, kv, page, d = c["pages"][0].shape
+    total = 2 ** 31 // (kv * page * d) + n
+    big = []
+    for x in (*c["pages"], *c["scales"]):
+        big.append(None if x is None else torch.zeros(total, *x.shape[1:], dtype=x.dtype, device=DEV))
+        if x is not None:
+            big[-1][-n:] = gpu(x)
+    cache = PagedKVCache.from_tensors(*big)
+    table = torch.where(c["table"] >= 0, c["table"] + (total - n), -1).to(torch.int32)
+    got, gl = run_attn(dict(c, table=table), cache=cache)
+    N = 2 * new
+    assert torch.equal(got[:N], want[:N]) and torch.equal(gl[:N], wl[:N])
+    args = gpu(c["start"]), gpu(c["ctx"])
+    small = cache_of(c)
+    kernels.page_append(gpu(c["k"]), gpu(c["v"]), cache, gpu(table), *args)
+    kernels.page_append(gpu(c["k"]), gpu(c["v"]), small, gpu(c["table"]), *args)
+    assert torch.equal(cache.k[-n:], small.k) and torch.equal(cache.v[-n:], small.v) and not cache.k[:-n].any()
+    for x, y in zip(kernels.page_read(cache, gpu(table), args[1], 900), kernels.page_read(small, gpu(c["table"]), args[1], 900)):
+        assert torch.equal(x, y)
+
+
 # ------------------------------------------------------------------------------------------------ append, read
 @pytest.mark.parametrize("d,kv", [(64, 1), (64, 5), (128, 2), (128, 8), (256, 3)])
 @pytest.mark.parametrize("int8", [True, False])

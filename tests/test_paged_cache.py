@@ -164,3 +164,23 @@ def test_workspace_of_any_hint():
             assert ws(2, n, 8 * rep, 8, 128, new, ctx) == most
         assert most % (n * 8 * rep * 129) == 0 and most <= 128 * n * 8 * rep * 129
     ws(1, 1 << 29, 64, 1, 128, 1, 100, want="refused")
+
+
+def test_cache_on_one_device():
+    from opendecider_amd import PagedKVCache
+    k, sc = torch.zeros(2, 1, 16, 64, dtype=torch.int8), torch.zeros(2, 1, 16)
+    for bad in ((k, k.to("meta"), sc, sc), (k, k, sc, sc.to("meta"))):
+        with pytest.raises(ValueError):
+            PagedKVCache.from_tensors(*bad)
+
+
+def test_workspace_by_page_type():
+    """bf16 pages have no image; a workspace for either type is the larger one."""
+    import ctypes
+    from opendecider_amd._lib import lib
+    n = [ctypes.c_int64(-1) for _ in range(3)]
+    sizes = (1, 2048, 32, 8, 128, 2048, 32768)
+    assert lib().od_paged_attn_ws_of(*sizes, 1, ctypes.byref(n[0])) == lib().od_paged_attn_ws_of(*sizes, 0, ctypes.byref(n[1])) == 0
+    assert lib().od_paged_attn_ws(*sizes, ctypes.byref(n[2])) == 0
+    assert n[0].value >= 32768 * 8 * 128 > n[1].value and n[2].value == max(n[0].value, n[1].value)
+    assert lib().od_paged_attn_ws_of(*sizes, 1, None) == NULL
