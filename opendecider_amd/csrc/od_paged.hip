@@ -1878,13 +1878,17 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   max_ctx = max_ctx < (1 << 30) ? max_ctx : 1 << 30;
   const int64_t rep = Hq / Hkv, slots = (max_new < 1 ? 1 : max_new) * rep, cus = od_cu_count();
   // Up to 32 slots stream: 8 tokens of 4 heads a group over 16 ragged x 4000 int8 tokens 37 us, 51 as tiles of 128
-  // slots (bf16 42 and 45; over 1 x 4000 15 and 29, bf16 15 and 25). More of them, 32 a workgroup, where there is
-  // little work: a step of the tile kernel is a chain of some 2 us that needs company on its CU, a streaming one has
-  // nothing to wait for but memory. The workgroups fit in at once and have no more than 128 KB of K a CU to read, from
-  // the L2 mostly: 16 tokens over 1 x 4000 16 us, 30 as tiles; 256 over 1 x 100 15 and 24; 32 over 2 x 4000 21 and 32;
-  // above it 32 over 1 x 32000 62 and 50, bf16 80 and 42, 120 of one head over 1 x 8000 bf16 tokens 37 and 34.
+  // slots (bf16 42 and 45; over 1 x 4000 15 and 29, bf16 15 and 25). Up to 64, as two workgroups of 32, over int8 pages
+  // of heads of 64 and 128, where half of a tile's waves would idle beside its conversions (16 tokens over 32 x 8000
+  // 146 and 201 us, heads of 64 over 16 x 4000 35 and 44; but bf16 235 and 185, int8 heads of 256 140 and 139, 80 slots
+  // 90 and 78). More of them where there is little work: a step of the tile kernel is a chain of some 2 us that needs
+  // company on its CU, a streaming one has nothing to wait for but memory. The workgroups fit in at once and have no
+  // more than 128 KB of K a CU to read, from the L2 mostly: 16 tokens over 1 x 4000 16 us, 30 as tiles; 256 over 1 x
+  // 100 15 and 24; 32 over 2 x 4000 21 and 32; above it 32 over 1 x 32000 62 and 50, bf16 80 and 42, 120 of one head
+  // over 1 x 8000 bf16 tokens 37 and 34.
   const int64_t few = B * Hkv * ((slots + 31) / 32);
-  p.stream = slots <= 32 || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
+  const int64_t always = q8 && D <= 128 && Hkv < (1 << 15) ? 64 : 32;  // (a grid has 65535 rows)
+  p.stream = slots <= always || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
   p.ct = slots <= 16 ? 1 : 2;
   // workgroups without splits for tiles of spt slots: every sequence's, but no more than the tokens make
   auto wgs_of = [&](int64_t spt) {
