@@ -592,6 +592,34 @@ def test_on_another_stream(gpu_lib):
     assert torch.equal(got, want)
 
 
+def test_a_graph_of_a_long_chunk(gpu_lib):
+    """The image, the tiles and the merge of splits captured on a stream of their own, replayed with new contents between eager
+    calls on another stream."""
+    from opendecider_amd import kernels
+    c = make(19, [70, 40, 30], [500, 3000, 1024], 4, 1, 256, page=64, pad=6000)
+    cache, meta = cache_of(c), (gpu(c["table"]), gpu(c["start"]), gpu(c["ctx"]), c["scale"])
+    q, k, v = gpu(c["q"]), gpu(c["k"]), gpu(c["v"])
+    out = torch.zeros_like(q)
+    call = lambda o: kernels.paged_attn(q, k, v, cache, *meta, max_ctx=3000, out=o)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(torch.zeros_like(q))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call(out)
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        q.copy_(torch.randn(q.shape, generator=g))
+        cache.v_scale.mul_(1.5)
+        meta[2].copy_(torch.tensor([500 - seed, 3000 - 700 * seed, 1024 - 64 * seed]))
+        graph.replay()
+        want = call(torch.zeros_like(q))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.isfinite(out.float()).all() and out[:140].any(2).all()
+
+
 # ------------------------------------------------------------------------------------------------ in the decoder
 CFG = dict(hidden=256, ffn=512, n_heads=8, n_kv_heads=2, head_dim=64, n_layers=2, vocab=300)
 
