@@ -868,12 +868,36 @@ __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, 
   }
 }
 
+// The same at a wave-uniform address plus the lane's offset in bytes. (Five wait states between a vector instruction
+// that writes a scalar register and a load that reads it: the compiler does not see the load.)
+__device__ __forceinline__ void dma16_at(const void* src, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(src)
+               : "memory", "m0");
+}
+// A block's bf16 rows from the pages; lane l has the page of key l. An instruction's 1 KB is 512 / D keys, which never
+// cross a page, so its address is one of the wave.
+template <int D, int NW>
+__device__ __forceinline__ void dma_pages(const uint16_t* lds, int wave, bool v, const Paged& p, int g, int blk,
+    int pg) {
+  int lane = threadIdx.x & 63;
+  if constexpr (D > 64) asm volatile("" : "+v"(lane));
+  const uint16_t* pool = static_cast<const uint16_t*>(v ? p.v : p.k);
+#pragma unroll
+  for (int i = 0; i < D / (8 * NW); ++i) {
+    const int first = (i * NW + wave) * (512 / D), page = max(__builtin_amdgcn_readlane(pg, first), 0);
+    const int64_t row = (((int64_t)page * p.Hkv + g) << p.shift) + ((blk * kBK + first) & ((1 << p.shift) - 1));
+    const int key = lane / (D / 8), slot = lane % (D / 8);
+    const int ch = v ? tv_chunk<D>(first + key, slot)
+                     : slot ^ (D == 64 ? (((first + key) >> 1) & 7) : ((first + key) & 15));
+    dma16_at(pool + row * D, 2 * (key * D + 8 * ch), lds_addr(lds) + 1024 * (i * NW + wave));
+  }
+}
 // The same from a block of the image, which lies in memory as it does in LDS.
 template <int D, int NW>
 __device__ __forceinline__ void dma_block(const uint16_t* lds, int wave, const uint16_t* src) {
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i)
-    dma16(src + (i * NW + wave) * 512 + 8 * (threadIdx.x & 63), lds_addr(lds) + 1024 * (i * NW + wave));
+    dma16_at(src + (i * NW + wave) * 512, 16 * (threadIdx.x & 63), lds_addr(lds) + 1024 * (i * NW + wave));
 }
 
 template <bool H>
@@ -1276,10 +1300,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
             r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(pool + row(key) * D + 16 * ch));
           }
         } else {
-          dma_rows<D, NW>(sm.k[buf], wave, false,
-                          [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(key) * D; });
-          dma_rows<D, NW>(sm.v[buf], wave, true,
-                          [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(key) * D; });
+          dma_pages<D, NW>(sm.k[buf], wave, false, a.p, g, blk, pg);
+          dma_pages<D, NW>(sm.v[buf], wave, true, a.p, g, blk, pg);
         }
       };
       int kexp = 0, vexp = 0;  // the stored block's frames
@@ -1648,14 +1670,12 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       auto load_k = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
         else if constexpr (IMG) dma_block<D, NW>(sm.k[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D));
-        else dma_rows<D, NW>(sm.k[blk & 1], wave, false,
-            [&](int key) { return static_cast<const uint16_t*>(a.p.k) + row(blk, pg, key) * D; });
+        else dma_pages<D, NW>(sm.k[blk & 1], wave, false, a.p, g, blk, pg);
       };
       auto load_v = [&](int blk, int pg) {
         if constexpr (Q8) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
         else if constexpr (IMG) dma_block<D, NW>(sm.v[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D) + kBK * D);
-        else dma_rows<D, NW>(sm.v[blk & 1], wave, true,
-            [&](int key) { return static_cast<const uint16_t*>(a.p.v) + row(blk, pg, key) * D; });
+        else dma_pages<D, NW>(sm.v[blk & 1], wave, true, a.p, g, blk, pg);
       };
       // pages of the blocks blk (the current one), blk + 1, blk + 2, blk + 3; past the last block: none
       int p0 = pages(b_lo), p1 = pages(b_lo + 1), p2 = pages(b_lo + 2), p3 = pages(b_lo + 3);
