@@ -66,7 +66,8 @@ __device__ __forceinline__ int seq_search(const int32_t* start, int B, int t) {
 // Rows of D values, 16 per lane (two 16-byte loads), G = D / 16 lanes per row. A wave takes 64 / G consecutive items of
 // the packed (token, K heads then V heads) order, so it reads whole runs of the projection's row. int8 pages take the
 // bytes and the scale of the row quantizer (od_q8_words: absmax / 127, round half to even), bf16 pages the values.
-// Bound by launch latency for a decode step and by memory for chunks: 2 bytes read and 1 written per value.
+// Bound by launch latency for a decode step (a token for each of 64 sequences 4.7 us) and by vector work and memory for
+// chunks, 2 bytes read and 1 written per value (64 x 900 tokens of 8 heads of 128 55 us, 4.4 TB/s; bf16 pages 58, 5.6).
 struct AppendArgs {
   Paged p;
   const uint16_t* k;
@@ -810,12 +811,13 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 }
 
 // ------------------------------------------------------------------------------------------------ many slots: tiles
-// Chunks and option rows: bound by the matrix cores and the softmax's vector work. A workgroup of NW waves owns 32
-// slots per wave of one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'.
-// Scores are taken transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so
-// that a slot's softmax is lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them;
-// V^T comes from row-major LDS by transposing reads. The kernel here is for heads of 64 and 128; heads of 256 have one
-// of their own below, of the same parts.
+// Chunks and option rows: bound by the matrix cores and the softmax's vector work (a chunk of 2048 over 32768 tokens,
+// 32 heads of 128, 1130 us, 1000 TFLOP/s, 56 and 44% of the cycles). A workgroup of NW waves owns 32 slots per wave of
+// one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'. Scores are taken
+// transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so that a slot's
+// softmax is lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them; V^T comes from
+// row-major LDS by transposing reads. The kernel here is for heads of 64 and 128; heads of 256 have one of their own
+// below, of the same parts.
 //
 // int8 blocks are converted once per workgroup on the way into LDS, or once for all of them ahead (the image, below),
 // to fp16 in power-of-two frames: K' = fp16(q ks_j 2^(7 - E)) with 2^E above the block's largest scale, V' = fp16(q
@@ -1463,13 +1465,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
   }
 }
 
-// ------------------------------------------------------------------------------------- many slots, heads of 256
-// 256 value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots:
+// ------------------------------------------------------------------------------------- many slots, heads of 256 256
+// value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots:
 // each accumulates 128 of the columns. Each takes the scores of 32 of the block's 64 keys, and its half of the softmax,
 // and they exchange the maximum and the probabilities through LDS (as the fragments that the products want); taking all
-// the scores in both instead, 48 matrix instructions a block and wave for 32, a chunk of 2048 over 16000 bf16 tokens
-// took 840 us, now 718 (4 ragged first chunks of 2000: 333, 216). For that the waves meet twice a block. K runs a block
-// ahead of V, so that both meetings also order the buffers:
+// the scores in both instead, 48 matrix instructions a block and wave for 32, cost a chunk of 2048 over 16000 bf16
+// tokens 17% more, and 4 ragged first chunks of 2000 54%. Now: 686 us (830 TFLOP/s), over an image of int8 pages 680,
+// 217 us. For that the waves meet twice a block. K runs a block ahead of V, so that both meetings also order the
+// buffers:
 //   scores(b) | maxima out, barrier | K(b + 2), V(b + 1) into the buffers of blocks that all are done with; softmax,
 //   probabilities out, barrier | products(b), scores(b + 1) ...
 struct alignas(16) WSmem {
@@ -1823,7 +1826,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 // here write the blocks that the tile kernels want, fp16 in frames and in the order of LDS, into the workspace. V's
 // frame is that of its largest scale over the whole (sequence, KV head), K's that of the block. Sequences longer than
 // img_blocks (the caller's bound was too low) have none; sequences without new tokens need none. A wave takes the frame
-// of one block's V (of all of them in a workgroup per (sequence, KV head), 32768 tokens took 20 us).
+// of one block's V (5 us; of all of them in a workgroup per (sequence, KV head), 32768 tokens took 20). The
+// image of 32768 tokens, 8 heads of 128, takes 47 us, 4.3 TB/s.
 __global__ __launch_bounds__(kThreads) void page_frame_kernel(AttnArgs a) {
   const int blk = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), g = blockIdx.y, b = blockIdx.z;
   const Seq s = seq_of(a, b);
