@@ -992,11 +992,13 @@ template <int D, bool H>
 __device__ __forceinline__ void t_scores(const uint16_t* kb, const TSlot<D>& t, v16f (&s)[2]) {
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   constexpr int NQ = D / 16 * 2, RA = 2;  // MFMA i: k-step i / 2, key tile i % 2; reads run RA ahead
+  int place = tk_off<D>(col, h);
+  asm volatile("" : "+v"(place));  // the places are formed here each time, not kept in registers
   s[0] = zero16();
   s[1] = zero16();
   v4u kf[RA + 1];
   auto rd = [&](int i) {
-    const uint16_t* at = &kb[tk_off<D>((i % 2) * 32 + col, (i / 2) * 2 + h)];
+    const uint16_t* at = &kb[(place ^ (i / 2 << 4)) + (i % 2) * 32 * D];  // tk_off<D>(key, 2 (i / 2) + h)
     kf[i % (RA + 1)] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(at));
   };
 #pragma unroll
@@ -1218,8 +1220,10 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
   }
 }
 
+// Waves a SIMD: heads of 64 leave the registers for three, but for the conversion of int8 blocks.
+constexpr int t_waves(int D, int src) { return D == 64 && src != kInt8 ? 3 : 2; }
 template <int D, int SRC, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(AttnArgs a) {
   constexpr bool Q8 = SRC == kInt8, IMG = SRC == kImage, H16 = SRC != kBf16;
   constexpr int NT = NW * 64, SPT = 32 * NW, DT = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -1525,10 +1529,12 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 
     // this wave's half of a block's scores: keys 32 half + 8 (i / 4) + 4 h + i % 4
     auto scores = [&](auto H, const uint16_t* kb) {
+      int place = tk_off<D>(half * 32 + col, h);
+      asm volatile("" : "+v"(place));  // the places are formed here each time, not kept in registers
       v16f x = zero16();
       v4u kf[2];
       auto rd = [&](int i) {
-        const uint16_t* at = &kb[tk_off<D>(half * 32 + col, 2 * i + h)];
+        const uint16_t* at = &kb[place ^ (i << 4)];  // tk_off<D>(key, 2 i + h): chunks are 8 values, rows 256
         kf[i % 2] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(at));
       };
       rd(0);
@@ -1949,10 +1955,13 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     // blocks (the queries, the first loads, the new tokens, the partials). x > 1 rounds count as x + 1/2, 1.6 at least:
     // a workgroup starts where another ends, and the last ones leave CUs idle. A chunk of 512 over 16000 takes 583 us
     // whole, 223 in 3, 192 in 4 (one round), 234 in 6 parts; 5 ragged bf16 600 over 2000 (592 workgroups) whole rounds
-    // chose 2 parts, 108 us, and this takes 3, 91; 8 x 384 over 6000 272 and 251.
+    // chose 2 parts, 108 us, and this takes 3, 91; 8 x 384 over 6000 272 and 251. Heads of 64: three workgroups a CU
+    // where that takes 4 parts at most (ragged bf16 chunks of 700 over 3000 in 3 parts 44 us, in 2 50; 2048 over 16000
+    // 187 and 204; but 4 x 256 over 6000 in 7 parts 66, in 5 53).
     int64_t best = 0;
     for (int64_t i = 1; i <= most || i == 1; ++i) {
-      const int64_t x10 = 10 * wgs * i / fit + 5, rounds10 = wgs * i <= fit ? 10 : x10 < 16 ? 16 : x10;
+      const int64_t at_once = D == 64 && tiles >= 4 && i <= 4 ? 3 * cus : fit;
+      const int64_t x10 = 10 * wgs * i / at_once + 5, rounds10 = wgs * i <= at_once ? 10 : x10 < 16 ? 16 : x10;
       const int64_t cost = rounds10 * ((keys + i - 1) / i + 12);
       if (best == 0 || cost < best) {
         best = cost;
