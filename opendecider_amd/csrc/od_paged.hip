@@ -1474,8 +1474,8 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
 // each accumulates 128 of the columns. Each takes the scores of 32 of the block's 64 keys, and its half of the softmax,
 // and they exchange the maximum and the probabilities through LDS (as the fragments that the products want); taking all
 // the scores in both instead, 48 matrix instructions a block and wave for 32, cost a chunk of 2048 over 16000 bf16
-// tokens 17% more, and 4 ragged first chunks of 2000 54%. Now: 686 us (830 TFLOP/s), over an image of int8 pages 680,
-// 217 us. For that the waves meet twice a block. K runs a block ahead of V, so that both meetings also order the
+// tokens 17% more, and 4 ragged first chunks of 2000 54%. Now: 661 us (860 TFLOP/s), over an image of int8 pages 652,
+// 197 us. For that the waves meet twice a block. K runs a block ahead of V, so that both meetings also order the
 // buffers:
 //   scores(b) | maxima out, barrier | K(b + 2), V(b + 1) into the buffers of blocks that all are done with; softmax,
 //   probabilities out, barrier | products(b), scores(b + 1) ...
@@ -1833,7 +1833,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 // frame is that of its largest scale over the whole (sequence, KV head), K's that of the block. Sequences longer than
 // img_blocks (the caller's bound was too low) have none; sequences without new tokens need none. A wave takes the frame
 // of one block's V (5 us; of all of them in a workgroup per (sequence, KV head), 32768 tokens took 20). The
-// image of 32768 tokens, 8 heads of 128, takes 47 us, 4.3 TB/s.
+// image of 32768 tokens, 8 heads of 128, takes 35 to 47 us, 4.3 to 5.6 TB/s.
 __global__ __launch_bounds__(kThreads) void page_frame_kernel(AttnArgs a) {
   const int blk = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), g = blockIdx.y, b = blockIdx.z;
   const Seq s = seq_of(a, b);
