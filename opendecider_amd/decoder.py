@@ -490,8 +490,8 @@ class DenseDecoder:
                            quantized)
 
     def _check_paged(self, states: PagedStates) -> None:
-        if not isinstance(states, PagedStates) or len(states) != len(self.layers) or states.batch < 1:
-            raise ValueError(f"expected the paged states of {len(self.layers)} layers (new_paged_states)")
+        if self.hybrid or not isinstance(states, PagedStates) or len(states) != len(self.layers) or states.batch < 1:
+            raise ValueError(f"expected the paged states of {len(self.layers)} attention layers (new_paged_states)")
 
     def _paged_pass(self, ids: torch.Tensor, ws: dict, states: PagedStates, pos, start, max_new: int, row_begin=None,
                     write: bool = False) -> torch.Tensor:

@@ -753,6 +753,25 @@ def test_hybrid_has_no_paged_states(gpu_lib):
         dec.new_paged_states(1, 2, 32)
 
 
+def test_states_of_another_decoder(gpu_lib):
+    from opendecider_amd import PagedStates
+    from opendecider_amd.decoder import DecoderConfig, random_decoder
+    hybrid = random_decoder(DecoderConfig(hidden=256, ffn=512, n_heads=4, n_kv_heads=2, head_dim=64, n_layers=2, vocab=50,
+                                          full_attention_interval=2, lin_k_heads=2, lin_v_heads=2), max_pos=64)
+    dec = random_decoder(DecoderConfig(**CFG), max_pos=64)
+    ids = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for d, states in ((hybrid, PagedStates(2, 1, 2, 64, 2, 32, 16)), (dec, PagedStates(3, 1, 2, 64, 2, 32, 16)),
+                      (dec, PagedStates(2, 0, 2, 64, 2, 32, 16)), (dec, dec.new_state_caches(1, 32))):
+        with pytest.raises(ValueError):
+            d.extend(ids, [1], states)
+        with pytest.raises(ValueError):
+            d.score_paged(ids.view(1, 1, 1), states)
+    narrow = PagedStates(2, 1, 4, 64, 2, 32, 16)  # of other heads: refused by the kernels, and nothing is counted
+    with pytest.raises(ValueError):
+        dec.extend(ids, [1], narrow)
+    assert narrow.lengths == [0]
+
+
 def test_refusals(gpu_lib):
     from opendecider_amd import PagedKVCache, kernels
     c = make(52, [4, 3], [20, 5])
