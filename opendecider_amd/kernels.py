@@ -1042,10 +1042,6 @@ def _paged(cache, table, start, ctx_len, name):
         raise ValueError(f"{name}: table must be (sequences, pages per sequence) with contiguous rows, one row per length")
     if not ctx_len.is_contiguous() or (start is not None and (start.numel() != B + 1 or not start.is_contiguous())):
         raise ValueError(f"{name}: start must be (sequences + 1,) and the lengths (sequences,), contiguous")
-    dev = k.get_device()
-    if table.get_device() != dev or ctx_len.get_device() != dev or cache.v.get_device() != dev or \
-            (start is not None and start.get_device() != dev):
-        raise ValueError(f"{name}: all tensors must be on one device")
     cols = table.shape[1]
     if B > 1 and table.stride(0) < cols:
         table = table.contiguous()
@@ -1053,20 +1049,31 @@ def _paged(cache, table, start, ctx_len, name):
                table.data_ptr(), table.stride(0) if B > 1 else cols, cols), table
 
 
-def _new_rows(x, N, H, D, cache, name):
+def _one_device(name: str, first: torch.Tensor, *tensors) -> int:
+    """The device index that all the tensors (None: left out) are on. RuntimeError where one is not on a GPU."""
+    dev = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            require_gpu(first, *tensors, name=name)
+            raise ValueError(f"{name}: all tensors must be on one device")
+    if dev < 0:
+        require_gpu(first, name=name)
+    return dev
+
+
+def _new_rows(x, N, H, D, name):
     """bf16 rows (N, H, D), as they are where their strides and address suit the 16-byte loads, else copied; and the
     pointer and strides (token, head) that the library takes."""
     if x.dtype != torch.bfloat16:
         raise TypeError(f"{name}: expected bfloat16, got {x.dtype}")
     if x.shape != (N, H, D):
         raise ValueError(f"{name}: expected {(N, H, D)}, got {tuple(x.shape)}")
-    if x.get_device() != cache.k.get_device():
-        raise ValueError(f"{name}: all tensors must be on one device")
     st, sh, sd = x.stride()
-    if sd != 1 or st % 8 or sh % 8 or x.data_ptr() % 16:
+    at = x.data_ptr()
+    if sd != 1 or st % 8 or sh % 8 or at % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-        st, sh = H * D, D
-    return x, (x.data_ptr(), st, sh)
+        at, st, sh = x.data_ptr(), H * D, D
+    return x, (at, st, sh)
 
 
 class _OnDevice:
@@ -1093,12 +1100,12 @@ def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, st
     (B + 1,): sequence b's tokens are the rows start[b] .. start[b + 1] - 1; ctx_len int32 (B,): the tokens it holds
     before, which is where they go. Tokens without a page are not written. The lengths stay: advance them once every layer
     has its tokens."""
-    require_gpu(k, v, cache.k, table, start, ctx_len, name="page_append")
+    _one_device("page_append", k, v, cache.k, cache.v, table, start, ctx_len)
     B, pages, table = _paged(cache, table, start, ctx_len, "page_append")
     _, H, _, D = cache.k.shape
     N = k.shape[0]
-    k, ka = _new_rows(k, N, H, D, cache, "page_append: k")
-    v, va = _new_rows(v, N, H, D, cache, "page_append: v")
+    k, ka = _new_rows(k, N, H, D, "page_append: k")
+    v, va = _new_rows(v, N, H, D, "page_append: v")
     with _OnDevice(k):
         check(lib().od_page_append(*ka, *va, *pages,
                                    start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
@@ -1108,7 +1115,7 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
     """od_page_read: the first length[b] (at most T) tokens of every sequence as dense (B, Hkv, T, D) K and V, zeros behind
     them. dtype bfloat16 or float32: the values q * s, one fp32 product (Int8Tensor.dequantize rounds the scale to bf16
     first). int8 (int8 pages only): two Int8Tensors, the stored bytes and scales (scales (B, Hkv, T, 1))."""
-    require_gpu(cache.k, table, length, name="page_read")
+    _one_device("page_read", cache.k, cache.v, table, length)
     B, pages, table = _paged(cache, table, None, length, "page_read")
     if T < 0:
         raise ValueError(f"page_read: T must not be negative, got {T}")
@@ -1158,11 +1165,11 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     tokens that the caller knows on the host (the work is split by them; the result is right for any). The pages are only
     read; int8 rows count as the exact q * s. Returns out (N, Hq, D) bf16 [, lse (N, Hq) fp32]; a token that sees nothing
     gets 0 and -inf, rows of no sequence are left as they were."""
-    require_gpu(q, k, v, cache.k, table, start, ctx_len, row_begin, out, name="paged_attn")
+    dev = _one_device("paged_attn", q, k, v, cache.k, cache.v, table, start, ctx_len, row_begin, out)
     B, pages, table = _paged(cache, table, start, ctx_len, "paged_attn")
     n_pages, H, page, D = cache.k.shape
     N, Hq = q.shape[0], q.shape[1]
-    q, qa = _new_rows(q, N, Hq, D, cache, "paged_attn: q")
+    q, qa = _new_rows(q, N, Hq, D, "paged_attn: q")
     if (k is None) != (v is None):
         raise ValueError("paged_attn: k and v come together")
     if Hq % H:
@@ -1171,30 +1178,32 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
         raise ValueError(f"paged_attn: the scale must be positive and finite, got {scale}")
     ka = va = (None, 0, 0)
     if k is not None:
-        k, ka = _new_rows(k, N, H, D, cache, "paged_attn: k")
-        v, va = _new_rows(v, N, H, D, cache, "paged_attn: v")
+        k, ka = _new_rows(k, N, H, D, "paged_attn: k")
+        v, va = _new_rows(v, N, H, D, "paged_attn: v")
     if row_begin is not None and (row_begin.dtype != torch.int32 or row_begin.numel() != N or
-                                  not row_begin.is_contiguous() or row_begin.get_device() != q.get_device()):
-        raise ValueError("paged_attn: row_begin must be int32 (N,), contiguous, on the queries' device")
+                                  not row_begin.is_contiguous()):
+        raise ValueError("paged_attn: row_begin must be int32 (N,), contiguous")
     most = table.shape[1] * page
     max_new = N if max_new is None else min(max(int(max_new), 0), N)
     max_ctx = most if max_ctx is None else min(max(int(max_ctx), 0), most)
     if out is None:
         out = dst = torch.empty(N, Hq, D, dtype=torch.bfloat16, device=q.device)
+        oa = (out.data_ptr(), Hq * D, D)
     else:
         _check_out(out, (N, Hq, D), q.device, "paged_attn")
-        if out.get_device() != q.get_device():
-            raise ValueError("paged_attn: all tensors must be on one device")
         aligned = not (out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8)
         dst = out if aligned else out.clone(memory_format=torch.contiguous_format)
+        oa = (dst.data_ptr(), dst.stride(0), dst.stride(1))
     lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device, cache.k_scale is not None)
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    with _OnDevice(q):
-        check(lib().od_paged_attn(*qa, *ka, *va, *pages, start.data_ptr(),
-                                  ctx_len.data_ptr(), ptr(row_begin), dst.data_ptr(), dst.stride(0), dst.stride(1),
-                                  ptr(lse), B, N, Hq, H, D, max_new, max_ctx, float(scale), ptr(ws), n, stream_of(q)),
-              "od_paged_attn")
+    args = (*qa, *ka, *va, *pages, start.data_ptr(), ctx_len.data_ptr(), ptr(row_begin), *oa, ptr(lse), B, N, Hq, H, D, max_new,
+            max_ctx, float(scale), ptr(ws), n, torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        check(lib().od_paged_attn(*args), "od_paged_attn")
+    else:
+        with torch.cuda.device(dev):
+            check(lib().od_paged_attn(*args), "od_paged_attn")
     if dst is not out:
         out.copy_(dst)
     return (out, lse) if return_lse else out
