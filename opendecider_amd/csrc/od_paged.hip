@@ -619,7 +619,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
     if constexpr (D < 256) new_tokens();
 
     // one tile's scores, softmax and products
-    auto products = [&](const STile<D, Q8>& tl) {
+    auto products = [&](STile<D, Q8>& tl) {
       if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
         reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
         reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
@@ -671,6 +671,27 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
             if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
         s_softmax<D, Q8>(y, f, acc[ct], hi[ct], lo[ct]);
+      }
+      if constexpr (!Q8) {
+        // The low part of a probability may be 0 or negative: infinities and NaN among the values are taken by the high
+        // part alone, ahead of the products, which take 0 in their places.
+        uint32_t m = 0;
+#pragma unroll
+        for (auto& key : tl.v)
+#pragma unroll
+          for (const uint32_t w : key) m = od_absmax_bf16x2(m, w);
+        if (__builtin_amdgcn_ballot_w64((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) != 0) {
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) {
+            const v4u v8 = s_vfrag<D, Q8, 4 * R>(tl.v, dt), fin = fin_bf16x8(v8);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) acc[ct].o[dt] = mfma16(v8 ^ fin, hi[ct], acc[ct].o[dt]);
+          }
+#pragma unroll
+          for (auto& key : tl.v)
+#pragma unroll
+            for (uint32_t& w : key) w = fin_bf16x2(w);
+        }
       }
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {

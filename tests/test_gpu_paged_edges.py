@@ -1,0 +1,62 @@
+"""The paged K/V cache at the edges of its range, on the GPU against its float64 restatement: values and scales that are not
+finite, sizes near the ends of the formats, offsets outside the packed rows. Batches, bounds and checks are
+test_gpu_paged.py's; every case runs through each kernel that it can reach."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged as op
+from test_gpu_paged import BF, DEV, check_attn, gpu, make, run_attn
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(64, 4, 4), (128, 8, 2), (256, 4, 1)]  # head dim, query heads, K/V heads
+
+
+def through(path, seed, new, ctx, heads, kv, d, **kw):
+    """A batch that the library takes by the kernels of `path`: "stream" (up to 32 slots), "tiles" (rows of no sequence
+    make the call a large one), "image" (and a table with room for 2^16 tokens)."""
+    page = kw.get("page", 16)
+    c = make(seed, new, ctx, heads, kv, d, **dict(kw, pad=0 if path == "stream" else 1100))
+    if path == "stream":
+        assert c["q"].shape[0] * heads // kv <= 32
+    if path == "image":
+        wide = torch.full((len(new), 2 ** 16 // page), -1, dtype=torch.int32)
+        wide[:, :c["table"].shape[1]] = c["table"]
+        c["table"] = wide
+    return c
+
+
+def place(c, b, pos):
+    """(page, row) of a cached position."""
+    page = c["pages"][0].shape[2]
+    return int(c["table"][b, pos // page]), pos % page
+
+
+# ------------------------------------------------------------------------------------------------ not finite
+@pytest.mark.parametrize("d,heads,kv", HEADS)
+@pytest.mark.parametrize("path", ["stream", "tiles"])
+def test_infinite_values_in_bf16_pages(gpu_lib, path, d, heads, kv):
+    """A cached infinity arrives at every token of its sequence in its column, both signs and NaN as NaN, and every other
+    output keeps its bits."""
+    c = through(path, 60, [1, 2, 1], [40, 2500, 70], heads, kv, d, int8=False)
+    at = [place(c, 0, 3), place(c, 0, 39), place(c, 1, 1200), place(c, 1, 2499)]
+    for page, row in at:  # of ordinary weight: no score is far below the others
+        c["pages"][0][page, 0, row] = 0
+    want, wl = run_attn(c)
+    inf, rep = float("inf"), heads // kv
+    c["pages"][1][at[0][0], 0, at[0][1], 5] = inf
+    c["pages"][1][at[1][0], 0, at[1][1], d - 1] = -inf
+    c["pages"][1][at[2][0], 0, at[2][1], 0] = -inf
+    c["pages"][1][at[2][0], 0, at[2][1], 17] = inf
+    c["pages"][1][at[3][0], 0, at[3][1], 17] = -inf
+    c["pages"][1][at[3][0], 0, at[3][1], 18] = float("nan")
+    got, gl = run_attn(c)
+    assert torch.equal(gl[:4], wl[:4])
+    hit = torch.zeros(4, heads, d, dtype=torch.bool)
+    hit[0, :rep, [5, d - 1]] = True
+    hit[1:3, :rep, [0, 17, 18]] = True
+    assert torch.equal(got[:4].cpu()[~hit], want[:4].cpu()[~hit])
+    assert (got[0, :rep, 5] == inf).all() and (got[0, :rep, d - 1] == -inf).all()
+    assert (got[1:3, :rep, 0] == -inf).all() and got[1:3, :rep, 17:19].isnan().all()
