@@ -573,7 +573,9 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
  * src/opendecider/backbone.py:435-468). A layer's K and V are two pools of n_pages pages of `page` token rows (a power of
  * two >= 16) for every KV head:
  *   k_pages, v_pages  int8 [n_pages, Hkv, page, D] with k_scale, v_scale fp32 [n_pages, Hkv, page], or bf16 with both
- *                     scales NULL; contiguous, 16-byte aligned; D in {64, 128, 256}
+ *                     scales NULL; contiguous, 16-byte aligned; D in {64, 128, 256}. To the attention an int8 row whose
+ *                     scale is not finite is a row of NaN (the append writes such scales for rows that hold an infinity or
+ *                     NaN, with bytes of 0)
  *   table             int32 [B, cols], row stride ld_table: position j of sequence b is row j % page of page
  *                     table[b, j / page]. An entry outside [0, n_pages) is no page: no key is there, nothing is written
  *   start             int32 [B + 1]: sequence b's new tokens are the packed rows start[b] .. start[b + 1] - 1 (ascending;

@@ -621,7 +621,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
     // one tile's scores, softmax and products
     auto products = [&](STile<D, Q8>& tl) {
       if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
-        reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks * a.scale_log2;
+        // (an infinite scale as NaN: a score of -inf would be no key)
+        reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks < INFINITY ? tl.ks * a.scale_log2 : NAN;
         reinterpret_cast<float*>(skf[wave][1])[c] = tl.vs;
       }
       v4f sc[CT][2];

@@ -60,3 +60,21 @@ def test_infinite_values_in_bf16_pages(gpu_lib, path, d, heads, kv):
     assert torch.equal(got[:4].cpu()[~hit], want[:4].cpu()[~hit])
     assert (got[0, :rep, 5] == inf).all() and (got[0, :rep, d - 1] == -inf).all()
     assert (got[1:3, :rep, 0] == -inf).all() and got[1:3, :rep, 17:19].isnan().all()
+
+
+@pytest.mark.parametrize("d,heads,kv", HEADS)
+@pytest.mark.parametrize("path", ["stream", "tiles", "image"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_scales_that_are_not_finite(gpu_lib, bad, path, d, heads, kv):
+    """An int8 row with such a scale counts as NaN: K's in the whole outputs and the LSE of the tokens that see it, V's in the
+    outputs. Other heads and sequences keep their bits."""
+    c = through(path, 61, [1, 2, 1], [40, 700, 70], heads, kv, d)
+    want, wl = run_attn(c)
+    rep = heads // kv
+    for i, b, pos in ((0, 0, 9), (1, 1, 650)):
+        page, row = place(c, b, pos)
+        c["scales"][i][page, 0, row] = bad
+    got, gl = run_attn(c)
+    assert got[:3, :rep].isnan().all() and gl[0, :rep].isnan().all()
+    assert torch.equal(gl[1:4], wl[1:4]) and torch.equal(got[3], want[3])
+    assert torch.equal(got[:3, rep:], want[:3, rep:]) and torch.equal(gl[0, rep:], wl[0, rep:])
