@@ -1009,6 +1009,12 @@ __device__ __forceinline__ void t_q_to_f16(TSlot<D>& t) {
     }
 }
 
+// The factor scale 2^e of a block's fp16 scores (of 2^36 at most), a number above 0 whatever the exponents: the scores of
+// masked keys are -inf ahead of it, and 2^-126 makes any score as good as 0.
+__device__ __forceinline__ float score_factor(float scale_log2, int e) {
+  return __builtin_amdgcn_fmed3f(__builtin_ldexpf(scale_log2, e), 0x1p-126f, 0x1.fffffep127f);
+}
+
 // S^T of one block.
 template <int D, bool H>
 __device__ __forceinline__ void t_scores(const uint16_t* kb, const TSlot<D>& t, v16f (&s)[2]) {
@@ -1382,7 +1388,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       __syncthreads();
       for (int blk = b_lo; blk < b_hi; ++blk) {
         const int cur = (blk - b_lo) & 1;
-        const float c = H16 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
+        const float c = H16 ? score_factor(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
         const int f_new = Q8 ? vexp - 7 : 0;
         const uint64_t mask = seen;
         if (blk + 1 < b_hi) {
@@ -1734,7 +1740,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       if constexpr (IMG) head = a.img_heads[first + b_lo];
       for (int blk = b_lo; blk < b_hi; ++blk) {
         const int kexp = IMG ? head.kexp : blk & 1 ? ke1 : ke0;
-        const float c = H16 ? __builtin_ldexpf(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
+        const float c = H16 ? score_factor(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
         const uint64_t seen = IMG ? head.seen : __builtin_amdgcn_ballot_w64(p0 >= 0);
         if (IMG && blk + 1 < b_hi) head = a.img_heads[first + blk + 1];
         v16f x;

@@ -78,3 +78,22 @@ def test_scales_that_are_not_finite(gpu_lib, bad, path, d, heads, kv):
     assert got[:3, :rep].isnan().all() and gl[0, :rep].isnan().all()
     assert torch.equal(gl[1:4], wl[1:4]) and torch.equal(got[3], want[3])
     assert torch.equal(got[:3, rep:], want[:3, rep:]) and torch.equal(gl[0, rep:], wl[0, rep:])
+
+
+# ------------------------------------------------------------------------------------------------ small numbers
+@pytest.mark.parametrize("d,heads,kv", HEADS)
+@pytest.mark.parametrize("path", ["stream", "tiles", "image"])
+@pytest.mark.parametrize("q_exp,k_exp", [(-66, -66), (-126, 0), (-100, None)])
+def test_small_queries_and_keys(gpu_lib, q_exp, k_exp, path, d, heads, kv):
+    """Scores that vanish: the mean of the values, also where a block's last keys are none. k_exp None: keys of zeros, with the
+    scale that the append gives them."""
+    c = through(path, 62, [1, 3], [300, 70], heads, kv, d)
+    c["q"] = (c["q"].float() * 2.0 ** q_exp).to(BF)
+    if k_exp is None:
+        c["pages"][0].zero_()
+        c["scales"][0].fill_(1e-8 / 127)
+        c["k"].zero_()
+    else:
+        c["scales"][0] = c["scales"][0] * 2.0 ** k_exp
+        c["k"] = (c["k"].float() * 2.0 ** k_exp).to(BF)
+    check_attn(c, *run_attn(c))
