@@ -1227,15 +1227,16 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
     int nv, int half) {
   if (!t.ok) return;
   const int h = (threadIdx.x & 63) >> 5;
-  const float inv = l == 0.0f ? 0.0f : __builtin_ldexpf(1.0f / l, frame), ls = t.m + __log2f(l) - kLift;
+  // 2^frame may be subnormal, so it comes last
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = __builtin_ldexpf(1.0f, frame), ls = t.m + __log2f(l) - kLift;
   const int64_t n = s.s0 + t.tok;
 #pragma unroll
   for (int dt = 0; dt < t_cols(D); ++dt)
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {
       const int d0 = half * 128 + dt * 32 + 8 * i4 + 4 * h;
-      const float4 y = make_float4(t.o[dt][4 * i4] * inv, t.o[dt][4 * i4 + 1] * inv, t.o[dt][4 * i4 + 2] * inv,
-          t.o[dt][4 * i4 + 3] * inv);
+      const float4 y = make_float4(t.o[dt][4 * i4] * inv * unit, t.o[dt][4 * i4 + 1] * inv * unit,
+          t.o[dt][4 * i4 + 2] * inv * unit, t.o[dt][4 * i4 + 3] * inv * unit);
       if (nv == 1)
         *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y),
             od_pack_bf16x2(y.z, y.w));
@@ -1381,6 +1382,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       pages(b_lo + 1);
       if constexpr (!Q8) dma_wait();
       store(0);
+      if constexpr (Q8) frame = vexp - 7;  // O is 0 still: no rescaling, by what may be no fp32 number
       if (Q8 && b_lo + 1 < b_hi) {
         load(b_lo + 1, 1);
         pages(b_lo + 2);
@@ -1735,6 +1737,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         dma_wait();
       }
       int f_cur = vexp - 7;
+      if constexpr (Q8) frame = f_cur;  // O is 0 still: no rescaling, by what may be no fp32 number
       __syncthreads();
       ImageBlock head = {};
       if constexpr (IMG) head = a.img_heads[first + b_lo];

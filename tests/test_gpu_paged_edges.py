@@ -97,3 +97,25 @@ def test_small_queries_and_keys(gpu_lib, q_exp, k_exp, path, d, heads, kv):
         c["scales"][0] = c["scales"][0] * 2.0 ** k_exp
         c["k"] = (c["k"].float() * 2.0 ** k_exp).to(BF)
     check_attn(c, *run_attn(c))
+
+
+@pytest.mark.parametrize("d,heads,kv", HEADS)
+@pytest.mark.parametrize("path", ["tiles", "image"])
+@pytest.mark.parametrize("own", [False, True])
+def test_small_values(gpu_lib, own, path, d, heads, kv):
+    """int8 values around 2^-120, whose frames' reciprocals no fp32 number holds. The outputs are partly subnormal: half of
+    their step, 2^-134, more than the relative bounds."""
+    c = through(path, 63, [1, 40], [300, 130], heads, kv, d)
+    c["scales"][1] = c["scales"][1] * 2.0 ** -120
+    c["v"] = (c["v"].float() * 2.0 ** -120).to(BF)
+    assert c["scales"][1].max() < 2.0 ** -121
+    out, lse = run_attn(c, own=own)
+    live = 41
+    ref, rl, mean, size, total = op.attention(c["q"][:live], c["k"][:live] if own else None, c["v"][:live] if own else None,
+                                              (*c["pages"], *c["scales"]), c["table"], c["start"], c["ctx"], c["scale"])
+    e = (2.0 ** -11 + 2.0 ** -24 * (d + 8)) * size
+    bound = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -11 + 2 * e[..., None] + 2.0 ** -22 * 400) * 1.02 * mean + \
+        2.0 ** -31 * total[..., None] + 2.0 ** -134
+    out = out[:live].double().cpu()
+    assert ((out - ref).abs() <= bound).all(), ((out - ref).abs() / bound).max()
+    assert ((lse[:live].double().cpu() - rl).abs() <= e + 2.0 ** -20 * (1 + rl.abs() + size)).all()
