@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) void page_append_kernel(AppendArgs a) {
   while (b < p.B && p.start[b + 1] <= t) ++b;
   if (item >= items || b >= p.B) return;  // whole G-lane groups leave together
   const int s0 = p.start[b];
-  if (t < s0) return;
+  if (t < s0 || s0 < 0 || p.start[b + 1] > p.N) return;  // (a range outside the packed rows: no sequence, as seq_of)
   const bool isv = h >= p.Hkv;
   const int kh = isv ? h - p.Hkv : h;
   const int64_t row = row_of(p, b, kh, (int64_t)max(p.ctx[b], 0) + (t - s0));
@@ -251,9 +251,9 @@ struct Seq {
 };
 __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int b) {
   Seq s;
+  const int end = a.p.start[b + 1];
   s.s0 = a.p.start[b];
-  s.n = a.p.start[b + 1] - s.s0;
-  if (s.s0 < 0 || s.n < 0 || s.s0 > a.p.N - s.n) s.n = 0;  // not a range of packed rows
+  s.n = s.s0 < 0 || end < s.s0 || end > a.p.N ? 0 : end - s.s0;  // 0: not a range of packed rows
   s.ctx = min(max(a.p.ctx[b], 0), a.p.cols << a.p.shift);
   return s;
 }

@@ -119,3 +119,30 @@ def test_small_values(gpu_lib, own, path, d, heads, kv):
     out = out[:live].double().cpu()
     assert ((out - ref).abs() <= bound).all(), ((out - ref).abs() / bound).max()
     assert ((lse[:live].double().cpu() - rl).abs() <= e + 2.0 ** -20 * (1 + rl.abs() + size)).all()
+
+
+# ------------------------------------------------------------------------------------------------ offsets
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("pad", [0, 1100])
+def test_sequences_outside_the_packed_rows(gpu_lib, pad, int8):
+    """A sequence that begins before the first packed row, or ends behind the last one, has no tokens: nothing of it is
+    written, and its rows stay as they were."""
+    from opendecider_amd import kernels
+    from test_gpu_paged import cache_of
+    c = make(64, [5, 4, 6], [20, 3, 40], int8=int8, pad=pad)
+    N = c["q"].shape[0]
+    for first, last in ((-3, N), (0, N + 5), (-1, N + 1), (-(2 ** 31), 2 ** 31 - 1)):
+        c["start"] = torch.tensor([first, 5, 9, last], dtype=torch.int32)
+        cache = cache_of(c)
+        kernels.page_append(gpu(c["k"]), gpu(c["v"]), cache, gpu(c["table"]), gpu(c["start"]), gpu(c["ctx"]))
+        for i, (x, got, gs) in enumerate(((c["k"], cache.k, cache.k_scale), (c["v"], cache.v, cache.v_scale))):
+            want, ws = op.append(c["pages"][i], c["scales"][i], x, c["table"], c["start"], c["ctx"])
+            assert torch.equal(got.cpu(), want), (first, last)
+            assert ws is None or torch.equal(gs.cpu(), ws)
+        out = torch.full(c["q"].shape, 7.0, dtype=BF, device=DEV)
+        _, lse = run_attn(c, out=out)
+        check_attn(c, out, lse)
+        if first < 0:
+            assert (out[:5] == 7).all()
+        if last > N:
+            assert (out[9:] == 7).all()
