@@ -1922,6 +1922,9 @@ __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
   }
 }
 
+// A launch has fewer than 2^32 threads: workgroups of 256.
+constexpr int64_t kMaxGroups = (1 << 24) - 1;
+
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
   bool stream;
@@ -1974,6 +1977,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // 2)
   const int64_t least = p.stream ? 8 : 2;
   int64_t most = keys / least < 128 ? keys / least : 128, n = 1;
+  if (N > kMaxGroups) most = 1;  // no merge, which has a workgroup a token
   // two streams of that size take as long as one (a token over 500: 9.9 us, 10.1 whole), with a launch more for the
   // host
   if (p.stream && most < 3) most = 1;
@@ -2004,8 +2008,11 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   if (p.chunk < 1) p.chunk = 1;
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   if (p.nsplit < 1) p.nsplit = 1;
+  // (Bounds far above a batch's own lengths could ask for more slot tiles than a launch holds: its workgroups go on to the
+  // tiles behind the grid's.)
+  const int64_t groups = B * Hkv * p.nsplit, room = kMaxGroups / 8 / groups;
+  if (!p.stream && p.tiles > room) p.tiles = room < 1 ? 1 : (int)room;
   // runs of tiles: as many as give every XCD the same number, or a few each
-  const int64_t groups = B * Hkv * p.nsplit;
   int parts = 1;
   while (parts < 8 && groups * parts % 8 && groups * parts < 64) parts *= 2;
   p.run = (p.tiles + parts - 1) / parts;
@@ -2098,7 +2105,7 @@ extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const
   a.svh = svh;
   const int64_t per_block = (int64_t)(kThreads / 64) * (64 / (D / 16));
   const int64_t blocks = (N * 2 * Hkv + per_block - 1) / per_block;
-  if (blocks > 0x7fffffff) return OD_ERR_SHAPE;
+  if (blocks > kMaxGroups) return OD_ERR_SHAPE;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
     const dim3 grid((unsigned)blocks);
@@ -2129,7 +2136,7 @@ extern "C" int od_page_read(const void* k_pages, const float* k_scale, const voi
   a.vs = vs_out;
   a.T = (int)T;
   const int64_t per_block = kThreads / (D / read_values(form)), tiles = (T + per_block - 1) / per_block;
-  if (B * Hkv > 0x7fffffff / tiles) return OD_ERR_SHAPE;
+  if (B * Hkv > kMaxGroups / tiles) return OD_ERR_SHAPE;
   a.tiles = (int)tiles;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
@@ -2224,7 +2231,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   hipStream_t st = (hipStream_t)stream;
   // tiles: every run of every group, a multiple of 8 runs
   const int64_t runs = (p.tiles + p.run - 1) / p.run, groups = (p.nsplit * Hkv * B * runs + 7) / 8 * 8 * p.run;
-  if (groups > 0x7fffffff) return OD_ERR_SHAPE;
+  if (!p.stream && groups * p.nw > 4 * kMaxGroups) return OD_ERR_SHAPE;
   int rc = OD_OK;
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;

@@ -146,3 +146,21 @@ def test_sequences_outside_the_packed_rows(gpu_lib, pad, int8):
             assert (out[:5] == 7).all()
         if last > N:
             assert (out[9:] == 7).all()
+
+
+# ------------------------------------------------------------------------------------------------ many
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("bounds", [{}, dict(max_new=1, max_ctx=1)])
+def test_many_states_without_bounds(gpu_lib, bounds, int8):
+    """20000 states of a token each, for bounds that ask for more slot tiles than a launch holds. Queries of 0: the token's value,
+    or half of it beside a cached token of zeros."""
+    from opendecider_amd import PagedKVCache, kernels
+    B, heads, d = 20000, 8, 128
+    cache = PagedKVCache(1, 1, d, 16, DEV, quantized=int8)
+    i32 = lambda x: x.to(torch.int32).to(DEV)
+    v = torch.randn(B, 1, d, generator=torch.Generator().manual_seed(65)).to(BF).to(DEV)
+    ctx = torch.arange(B) % 2
+    out = kernels.paged_attn(torch.zeros(B, heads, d, dtype=BF, device=DEV), v, v, cache, i32(torch.zeros(B, 1)), i32(torch.arange(B + 1)),
+                             i32(ctx), d ** -0.5, **bounds)
+    want = torch.where(ctx.to(DEV).bool()[:, None, None], v / 2, v).expand(B, heads, d)
+    assert torch.equal(out, want)
