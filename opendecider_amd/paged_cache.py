@@ -73,7 +73,8 @@ class PagedKVCache:
 class PagedStates:
     """Every layer's pages of `batch` states: one pool of n_pages pages per layer, one table (batch, max_tokens / page) for
     all layers on the device (-1: no page), the states' lengths on the host (`lengths`) and on the device (`ctx`). Indexing
-    and iteration give the layers' PagedKVCache. reserve -> write (every layer) -> advance appends tokens."""
+    and iteration give the layers' PagedKVCache. reserve -> write (every layer) -> advance appends tokens; these steps, and
+    release, change the host's side too and are refused while a graph is captured."""
 
     def __init__(self, n_layers: int, batch: int, n_heads: int, head_dim: int, n_pages: int, max_tokens: int, page: int = 64,
                  device="cuda", quantized: bool = True):
@@ -101,6 +102,7 @@ class PagedStates:
 
     def reserve(self, counts) -> None:
         """Pages for counts[b] more tokens of every state b. MemoryError (nothing taken) where the pool has too few."""
+        self._not_captured("reserve")
         counts = [int(n) for n in counts]
         if len(counts) != self.batch or min(counts, default=0) < 0:
             raise ValueError("PagedStates: one count of new tokens per state")
@@ -119,6 +121,7 @@ class PagedStates:
 
     def advance(self, counts) -> None:
         """Counts the tokens that every layer has written since reserve."""
+        self._not_captured("advance")
         counts = [int(n) for n in counts]
         if len(counts) != self.batch or min(counts, default=0) < 0:
             raise ValueError("PagedStates: one count of new tokens per state")
@@ -130,11 +133,17 @@ class PagedStates:
 
     def release(self, b: int) -> None:
         """State b ends: its pages go back to the pool and it is empty."""
+        self._not_captured("release")
         self.free += self.pages[b][::-1]
         self.pages[b] = []
         self.table[b].fill_(-1)
         self.lengths[b] = 0
         self._write_ctx()
+
+    def _not_captured(self, name: str) -> None:
+        if self.ctx.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"PagedStates.{name} cannot be captured: a replay would write the lengths and pages of the capture "
+                               "again, whatever the states have come to since")
 
     def _write_ctx(self) -> None:
         self._put(self.ctx, self.lengths)

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oracle import paged as op
+from oracle.quant import quantize_rows
 from test_gpu_paged import BF, DEV, check_attn, gpu, make, run_attn
 
 pytestmark = pytest.mark.gpu
@@ -14,13 +15,11 @@ pytestmark = pytest.mark.gpu
 HEADS = [(64, 4, 4), (128, 8, 2), (256, 4, 1)]  # head dim, query heads, K/V heads
 
 
-def through(path, seed, new, ctx, heads, kv, d, **kw):
-    """A batch that the library takes by the kernels of `path`: "stream" (up to 32 slots), "tiles" (rows of no sequence
-    make the call a large one), "image" (and a table with room for 2^16 tokens)."""
+def through(path, seed, new, ctx, heads, kv, d, of=make, **kw):
+    """A batch that the library takes by the kernels of `path`: "stream" (small calls), "tiles" (rows of no sequence make the
+    call a large one), "image" (and a table with room for 2^16 tokens)."""
     page = kw.get("page", 16)
-    c = make(seed, new, ctx, heads, kv, d, **dict(kw, pad=0 if path == "stream" else 1100))
-    if path == "stream":
-        assert c["q"].shape[0] * heads // kv <= 32
+    c = of(seed, new, ctx, heads, kv, d, **dict(kw, pad=0 if path == "stream" else 1100))
     if path == "image":
         wide = torch.full((len(new), 2 ** 16 // page), -1, dtype=torch.int32)
         wide[:, :c["table"].shape[1]] = c["table"]
@@ -164,3 +163,50 @@ def test_many_states_without_bounds(gpu_lib, bounds, int8):
                              i32(ctx), d ** -0.5, **bounds)
     want = torch.where(ctx.to(DEV).bool()[:, None, None], v / 2, v).expand(B, heads, d)
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------------ states
+def test_states_do_not_change_in_a_capture(gpu_lib, monkeypatch):
+    """What changes the host's lengths and free pages is refused while a graph is captured, with nothing changed."""
+    from opendecider_amd import PagedStates
+    s = PagedStates(1, 2, 1, 64, n_pages=4, max_tokens=64, page=16)
+    s.reserve([20, 3])
+    s.advance([20, 3])
+    held = lambda: (list(s.lengths), [list(p) for p in s.pages], list(s.free), s.table.tolist(), s.ctx.tolist())
+    before = held()
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for step in (lambda: s.reserve([1, 20]), lambda: s.advance([1, 1]), lambda: s.release(0)):
+            with pytest.raises(RuntimeError):
+                step()
+    assert held() == before
+    s.reserve([1, 20])
+    s.release(0)
+    assert s.lengths == [0, 3] and s.ctx.tolist() == [0, 3]
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+def test_states_read(gpu_lib, quantized):
+    """PagedStates.read: every layer's own pages through the common table, as long as the longest state."""
+    from opendecider_amd import PagedStates, kernels
+    s = PagedStates(2, 3, 2, 64, n_pages=9, max_tokens=64, page=16, quantized=quantized)
+    counts = [20, 0, 33]
+    x = torch.randn(4, 53, 2, 64, generator=torch.Generator().manual_seed(66)).to(BF)
+    s.reserve(counts)
+    start = torch.tensor([0, 20, 20, 53], dtype=torch.int32)
+    for li in range(2):
+        kernels.page_append(gpu(x[2 * li]), gpu(x[2 * li + 1]), s[li], s.table, gpu(start), s.ctx)
+    s.advance(counts)
+    for li in range(2):
+        for dtype in (BF, torch.float32):
+            for side, got in enumerate(s.read(li, dtype=dtype)):
+                want = torch.zeros(3, 2, 33, 64, dtype=dtype)
+                for b in (0, 2):
+                    rows = x[2 * li + side][start[b]:start[b + 1]].transpose(0, 1)
+                    if quantized:
+                        q, sc = quantize_rows(rows)
+                        rows = q.float() * sc
+                    want[b, :, :counts[b]] = rows.to(dtype)
+                assert torch.equal(got.cpu(), want)
+    none = PagedStates(1, 0, 2, 64, n_pages=1, max_tokens=16, page=16, quantized=quantized)
+    assert [t.shape for t in none.read(0)] == [(0, 2, 0, 64)] * 2
