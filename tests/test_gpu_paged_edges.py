@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import paged_exact
 from oracle import paged as op
 from oracle.quant import quantize_rows
 from test_gpu_paged import BF, DEV, check_attn, gpu, make, run_attn
@@ -118,6 +119,28 @@ def test_small_values(gpu_lib, own, path, d, heads, kv):
     out = out[:live].double().cpu()
     assert ((out - ref).abs() <= bound).all(), ((out - ref).abs() / bound).max()
     assert ((lse[:live].double().cpu() - rl).abs() <= e + 2.0 ** -20 * (1 + rl.abs() + size)).all()
+
+
+# ------------------------------------------------------------------------------------------------ every key
+@pytest.mark.parametrize("d,heads,kv", [*HEADS, (128, 7, 1)])
+@pytest.mark.parametrize("path", ["stream", "tiles", "image"])
+@pytest.mark.parametrize("shape", range(len(paged_exact.SHAPES)))
+def test_every_key_counts(gpu_lib, shape, path, d, heads, kv):
+    """Narrow bounds (paged_exact.py) at the borders of tiles and blocks, for the bounds that the call knows and for a max_ctx that
+    leaves the last split all keys but the first 64."""
+    new, ctx = paged_exact.SHAPES[shape]
+    c = through(path, shape, new, ctx, heads, kv, d, of=paged_exact.batch, page=[16, 64, 32][shape % 3])
+    for own in (True, False):
+        paged_exact.check(c, *run_attn(c, own=own), path == "stream", own)
+    if path != "image":
+        paged_exact.check(c, *run_attn(c, max_ctx=64), path == "stream")
+
+
+@pytest.mark.parametrize("d,heads,kv", HEADS)
+@pytest.mark.parametrize("path", ["stream", "tiles", "image"])
+def test_every_key_counts_in_option_rows(gpu_lib, path, d, heads, kv):
+    c = through(path, 67, [24, 40, 1], [63, 65, 128], heads, kv, d, of=paged_exact.batch, rows=8, page=32)
+    paged_exact.check(c, *run_attn(c), path == "stream")
 
 
 # ------------------------------------------------------------------------------------------------ offsets
