@@ -125,8 +125,8 @@ __global__ __launch_bounds__(kThreads) void page_append_kernel(AppendArgs a) {
   }
 }
 
-// --------------------------------------------------------------------------------------------------------- read Dense
-// (B, Hkv, T, D) K and V of every sequence's first ctx[b] tokens, zeros behind them: the values q * s (one fp32
+// ---------------------------------------------------------------------------------------------------------- read
+// Dense (B, Hkv, T, D) K and V of every sequence's first ctx[b] tokens, zeros behind them: the values q * s (one fp32
 // product, rounded once to bf16 where that is asked), bf16 rows as they are, or the int8 rows with their scales. Bound
 // by memory: 64 sequences of 8192 tokens, 8 heads of 128, 1.1 GB read and 2.1 GB written in 505 us, 5.7 TB/s. A lane
 // takes the V values of a row of K, and of V, that make 16 bytes there, so that a wave's stores are whole lines (16
@@ -292,10 +292,10 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
   hi = __builtin_amdgcn_perm(f3, f2, 0x07060302u);
 }
 
-// ------------------------------------------------------------------------------------------ few slots: streaming Up to
-// 16 or 32 slots of a (sequence, KV head) in a workgroup: decode steps. 4 rep D FLOP per key against 2 D (+ 8) bytes of
-// int8 K and V: bound by reading the pages (64 x 4096 tokens of 8 heads of 128 in 70 us, 5.4 TB/s). A wave holds 16
-// slots as the columns of V_MFMA_F32_16X16X32_BF16, or 32 as two of them, and takes 32-key tiles straight from memory
+// ------------------------------------------------------------------------------------------ few slots: streaming
+// Up to 16 or 32 slots of a (sequence, KV head) in a workgroup: decode steps. 4 rep D FLOP per key against 2 D (+ 8)
+// bytes of int8 K and V: bound by reading the pages (64 x 4096 tokens of 8 heads of 128 in 70 us, 5.4 TB/s). A wave holds
+// 16 slots as the columns of V_MFMA_F32_16X16X32_BF16, or 32 as two of them, and takes 32-key tiles straight from memory
 // into registers; the waves of a workgroup take every NW-th tile of the split's range and merge in LDS. Lane (j, g) =
 // (lane % 16, lane / 16):
 //  * scores S^T[kr] = K[kr] Q^T for the 16-key half tiles kr: the four lanes of a key read 64 contiguous bytes of it at
@@ -305,8 +305,8 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
 //  * O^T[dt] += V^T[dt] P^T with output row r of d tile dt being d = (D / 16) r + dt and the keys in the order 4 g + i
 //    (i < 4), 12 + 4 g + i: the B operand is the lane's own 8 probabilities, the A operand value dt of the D / 16
 //    contiguous values it reads of each of those keys. P (times vs_j) enters as bf16 hi + lo parts, 16 significant
-//    bits: the columns of the matrix instructions are mostly empty here, and no scale of the values can leave the
-//    range.
+//    bits: the columns of the matrix instructions are mostly empty here, and it takes no frames (the low part of a
+//    product below 2^-117 begins to be lost under bf16's range).
 // Half tiles are reached through buffer descriptors of their own (a half tile never crosses a page), whose length ends
 // at the last cached token: what lies behind reads as zeros. Two register sets: a tile's loads are all issued before
 // the products of the tile ahead of it, unconditionally (past a wave's last tile with descriptors of no length, so that
@@ -856,13 +856,13 @@ constexpr int kBK = 64;
 enum { kBf16 = 0, kInt8 = 1, kImage = 2 };  // what the tile kernels read: bf16 pages, int8 pages, their image
 constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
 
-template <int D>
 // K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
+template <int D>
 __device__ __forceinline__ int tk_off(int key, int chunk) {
   return key * D + ((chunk ^ (D == 64 ? ((key >> 1) & 7) : (key & 15))) << 3);
 }
-template <int D>
 // V rows: 4 consecutive keys' chunks of a transposing read 64 bytes apart
+template <int D>
 __device__ __forceinline__ int tv_chunk(int key, int chunk) {
   return D == 64 ? chunk ^ ((key & 2) << 1) : chunk ^ ((key & 3) << 2);
 }
@@ -1499,8 +1499,8 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
   }
 }
 
-// ------------------------------------------------------------------------------------- many slots, heads of 256 256
-// value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots:
+// ------------------------------------------------------------------------------------------ many slots, heads of 256
+// 256 value columns of accumulators do not fit a wave's registers beside 256-wide queries, so two waves share 32 slots:
 // each accumulates 128 of the columns. Each takes the scores of 32 of the block's 64 keys, and its half of the softmax,
 // and they exchange the maximum and the probabilities through LDS (as the fragments that the products want); taking all
 // the scores in both instead, 48 matrix instructions a block and wave for 32, cost a chunk of 2048 over 16000 bf16
@@ -1590,7 +1590,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       if (h == 0) sm.mx[half][grp][col] = mx;
       return mx;
     };
-    auto softmax = [&](auto H, const v16f& x, float c, float mine, v4u (&pb)[4]) {
+    auto softmax = [&](auto H, const v16f& x, float c, float mine) {
       const float mx = fmaxf(mine, sm.mx[half ^ 1][grp][col]);
       const bool move = mx > t.m + kSlack;
       if (__builtin_amdgcn_ballot_w64(move) != 0) {
@@ -1783,7 +1783,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         v4u pb[4];
         if (live) {
           if constexpr (Q8) rescale(f_now);
-          softmax(HT{}, x, c, mine, pb);
+          softmax(HT{}, x, c, mine);
         }
         __syncthreads();
         if (live) {
@@ -1837,7 +1837,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
           if (blk + 2 < n.hi) load_k(blk + 2);
           if (blk + 1 < n.hi) load_v(blk + 1);
           v4u pb[4];
-          if (work) softmax(std::false_type{}, x, a.scale_log2, mine, pb);
+          if (work) softmax(std::false_type{}, x, a.scale_log2, mine);
           __syncthreads();
           if (work) {
             get_p(pb);
