@@ -425,21 +425,6 @@ __device__ __forceinline__ BlockInfo read_info(const int* info) {
   return bi;
 }
 
-// One global_load_lds_dwordx4: lane l copies 16 bytes from its `src` to LDS byte lds_base + 16 l (lds_base is
-// wave-uniform, passed in M0). Written as inline asm so that the compiler does not track it: the caller waits for it
-// (vmcnt) and orders it with barriers, whereas the compiler would wait for it before every LDS read that it cannot
-// prove disjoint from the copy, which is every read of the other image buffer. The compiler keeps nothing in M0 in
-// these kernels (no LDS DMA, movrel or sendmsg of its own), so setting it here disturbs no live value.
-__device__ __forceinline__ void dma16(const void* src, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src)
-               : "memory", "m0");
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t lds_addr(T* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);
-}
-
 // Copies NBYTES (a multiple of 16) of a staged image into LDS, 16 bytes per lane and no registers: round i moves
 // bytes [4096 i, 4096 (i + 1)), wave w the 1 KiB at 1024 w of it; the tail round has every wave copy the last
 // 1 KiB (bytes already copied are written again with the same values), so that no round branches on the lane or
@@ -461,12 +446,12 @@ __device__ __forceinline__ void copy_round(const void* src, void* dst, int i) {
   const int tid = threadIdx.x;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const char* s = reinterpret_cast<const char*>(src);
-  const uint32_t d = __builtin_amdgcn_readfirstlane(lds_addr(dst));
+  const uint32_t d = __builtin_amdgcn_readfirstlane(od_lds_addr(dst));
   const int lane = tid & 63;
   if (i < C::kFull)
-    dma16(s + i * C::kRound + tid * 16, d + i * C::kRound + wave * 1024);
+    od_dma16(s + i * C::kRound + tid * 16, d + i * C::kRound + wave * 1024);
   else
-    dma16(s + NBYTES - 1024 + lane * 16, d + NBYTES - 1024);
+    od_dma16(s + NBYTES - 1024 + lane * 16, d + NBYTES - 1024);
 }
 
 template <int NBYTES>

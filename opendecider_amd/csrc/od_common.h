@@ -129,6 +129,21 @@ __device__ __forceinline__ float od_group_max(float v) {
   return v;
 }
 
+// One global_load_lds_dwordx4: lane l copies 16 bytes from its `src` to LDS byte lds_base + 16 l (lds_base is
+// wave-uniform, passed in M0). Written as inline asm so that the compiler does not track it: the caller waits for it
+// (vmcnt) and orders it with barriers, whereas the compiler would wait for it before every LDS read that it cannot
+// prove disjoint from the copy, which is every read of another buffer. The compiler keeps nothing in M0 in the kernels
+// that use it (no LDS DMA, movrel or sendmsg of its own), so setting it here disturbs no live value.
+__device__ __forceinline__ void od_dma16(const void* src, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src)
+               : "memory", "m0");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t od_lds_addr(T* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);
+}
+
 static inline int od_launch_status() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? OD_OK : OD_ERR_LAUNCH;

@@ -867,16 +867,7 @@ __device__ __forceinline__ int tv_chunk(int key, int chunk) {
   return D == 64 ? chunk ^ ((key & 2) << 1) : chunk ^ ((key & 3) << 2);
 }
 
-// 16 bytes per lane from memory straight into LDS, lane l's to LDS byte lds + 16 l (lds wave-uniform, in M0). The
-// compiler does not track it: the kernel waits (vmcnt) and orders it with barriers itself.
-__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
-}
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <typename T>
-__device__ __forceinline__ uint32_t lds_addr(T* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);
-}
 // A block's bf16 rows into LDS by DMA: instruction i of a wave fills the 1 KB at 1024 (i NW + wave) of K or V, so a
 // lane owns a place there, (key, swizzled chunk), and copies the chunk that the swizzle puts into it. at(key): its row.
 template <int D, int NW, typename KeyRow>
@@ -888,11 +879,11 @@ __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, 
   for (int i = 0; i < D / (8 * NW); ++i) {
     const int pe = (i * NW + wave) * 512 + 8 * lane, key = pe / D, slot = pe % D / 8;
     const int ch = v ? tv_chunk<D>(key, slot) : slot ^ (D == 64 ? ((key >> 1) & 7) : (key & 15));
-    dma16(row(key) + 8 * ch, lds_addr(lds) + 1024 * (i * NW + wave));
+    od_dma16(row(key) + 8 * ch, od_lds_addr(lds) + 1024 * (i * NW + wave));
   }
 }
 
-// The same at a wave-uniform address plus the lane's offset in bytes. (Five wait states between a vector instruction
+// od_dma16 at a wave-uniform address plus the lane's offset in bytes. (Five wait states between a vector instruction
 // that writes a scalar register and a load that reads it: the compiler does not see the load.)
 __device__ __forceinline__ void dma16_at(const void* src, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(src)
@@ -913,7 +904,7 @@ __device__ __forceinline__ void dma_pages(const uint16_t* lds, int wave, bool v,
     const int key = lane / (D / 8), slot = lane % (D / 8);
     const int ch = v ? tv_chunk<D>(first + key, slot)
                      : slot ^ (D == 64 ? (((first + key) >> 1) & 7) : ((first + key) & 15));
-    dma16_at(pool + row * D, 2 * (key * D + 8 * ch), lds_addr(lds) + 1024 * (i * NW + wave));
+    dma16_at(pool + row * D, 2 * (key * D + 8 * ch), od_lds_addr(lds) + 1024 * (i * NW + wave));
   }
 }
 // The same from a block of the image, which lies in memory as it does in LDS.
@@ -921,7 +912,7 @@ template <int D, int NW>
 __device__ __forceinline__ void dma_block(const uint16_t* lds, int wave, const uint16_t* src) {
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i)
-    dma16_at(src + (i * NW + wave) * 512, 16 * (threadIdx.x & 63), lds_addr(lds) + 1024 * (i * NW + wave));
+    dma16_at(src + (i * NW + wave) * 512, 16 * (threadIdx.x & 63), od_lds_addr(lds) + 1024 * (i * NW + wave));
 }
 
 template <bool H>
