@@ -579,7 +579,8 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
  *   table             int32 [B, cols], row stride ld_table: position j of sequence b is row j % page of page
  *                     table[b, j / page]. An entry outside [0, n_pages) is no page: no key is there, nothing is written
  *   start             int32 [B + 1]: sequence b's new tokens are the packed rows start[b] .. start[b + 1] - 1 (ascending;
- *                     rows of no sequence, e.g. behind start[B], are neither read as tokens nor written)
+ *                     rows of no sequence, e.g. behind start[B], are neither read as tokens nor written; a sequence that
+ *                     reaches outside 0 .. N has no tokens)
  *   ctx_len           int32 [B]: sequence b's cached tokens (negative: 0; past the table: the table's end)
  * All on the device; the host needs none of them.
  *
@@ -589,6 +590,8 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
  * od_page_read: the first `length[b]` (<= T) tokens of every sequence into contiguous [B, Hkv, T, D], zeros behind them and
  *   where there is no page: form OD_READ_BF16 or OD_READ_FP32 the values q * s (an fp32 product, rounded once to bf16), or
  *   OD_READ_INT8 the rows with their scales [B, Hkv, T] (int8 pages only; ks_out and vs_out NULL otherwise).
+ * An append takes fewer than 2^35 values of K (N Hkv D); a read writes fewer than 2^34 of K (B Hkv T D) in fp32, 2^35 in bf16,
+ * 2^36 in int8, T counted in whole workgroups (else OD_ERR_SHAPE).
  * od_paged_attn: every new token of a sequence attends that sequence's ctx_len[b] cached tokens and its new tokens from
  *   row_begin[n] (int32 [N], counted from start[b]; NULL: 0) up to itself, as they come in bf16 (k and v NULL: the cached
  *   ones only). q, out bf16 [N, Hq, D], lse fp32 [N, Hq] or NULL (natural log, of the scaled scores); a token that sees

@@ -202,7 +202,9 @@ __global__ __launch_bounds__(kThreads) void page_read_kernel(ReadArgs a) {
 // ---------------------------------------------------------------------------------------------------- attention
 // New token i of sequence b (packed row n = start[b] + i) sees the cached positions 0 .. ctx[b] - 1 and the new tokens
 // row_begin[n] .. i of its own sequence (row_begin null: from 0), bf16 as they come: o = sum_j p_j v_j / sum_j p_j with
-// p_j = exp(scale q.k_j - max), lse = max + log sum p; a token that sees nothing has o = 0 and lse = -inf.
+// p_j = exp(scale q.k_j - max), lse = max + log sum p; a token that sees nothing has o = 0 and lse = -inf. An int8 row whose
+// scale is not finite counts as NaN. A value that is infinite gives an infinite output where it is seen (NaN beside one of
+// the other sign, and where a cached one's probability is 0 in fp32).
 //
 // A "slot" is a (new token, head of the KV group) pair: slot z of a sequence is token z / rep, head g rep + z % rep.
 // Both kernels go over the keys once with a running maximum m and sum l in fp32 (log2 units). m moves only when a
@@ -834,7 +836,7 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 
 // ------------------------------------------------------------------------------------------------ many slots: tiles
 // Chunks and option rows: bound by the matrix cores and the softmax's vector work (a chunk of 2048 over 32768 tokens,
-// 32 heads of 128, 1130 us, 1000 TFLOP/s, 56 and 44% of the cycles). A workgroup of NW waves owns 32 slots per wave of
+// 32 heads of 128, 1130 to 1180 us by the card, 960 to 1000 TFLOP/s, 59 and 47% of the cycles). A workgroup of NW waves owns 32 slots per wave of
 // one (sequence, KV head) and goes over 64-key blocks: first the cached ones, then the new tokens'. Scores are taken
 // transposed, S^T = K Q^T on 32 x 32 x 16 matrix instructions (64 keys by the wave's 32 slots), so that a slot's
 // softmax is lane-local but for one exchange, and the probabilities sit where O^T += V^T P^T wants them; V^T comes from
@@ -2009,10 +2011,10 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   p.run = (p.tiles + parts - 1) / parts;
   p.part = p.nsplit > 1 ? (p.nsplit * N * Hq * (D + 1) + 3) / 4 * 4 : 0;
   // The image, up to 1 GB of it, where 4 slot tiles or more share a block and the conversions that it saves are worth
-  // its launches: counted in values a slot they are wgs keys D / spt. Chunks of 2048 over 32768 1364 us, with it 1190;
-  // 256-wide heads, 4 ragged 900 over 6000 416, 300; 1 x 256 over 6000 (3000 blocks in all) 92, 86; 8 x 64 (2 tiles)
-  // 121, 126; heads of 128, 8 x 256 over 6000 (4 tiles) 219, 203, 8 x 128 (2 tiles) 132, 146, 4 x 1024 over 1000 (8000
-  // blocks) 84, 89, 4 x 256 over 6000 (12000) 132, 124.
+  // its launches: counted in values a slot they are wgs keys D / spt. Chunks of 2048 over 32768 1382 us, with it 1183;
+  // 256-wide heads, 4 ragged 900 over 6000 402, 284; 1 x 256 over 6000 (3000 blocks in all) 82, 76; 8 x 64 (2 tiles)
+  // 115, 121; heads of 128, 8 x 256 over 6000 (4 tiles) 217, 183, 8 x 128 (2 tiles) 150, 139, 4 x 1024 over 1000 (8000
+  // blocks) 85, 87, 4 x 256 over 6000 (12000) 152, 115.
   p.img_blocks = !p.stream && q8 && tiles >= 4 && wgs * keys * D / spt > 5 << 10 ? keys : 0;
   if (p.img_blocks * B * Hkv > (1ll << 28) / (kBK * D)) p.img_blocks = 0;
   p.vexp = p.img_blocks ? (B * Hkv + 3) / 4 * 4 : 0;

@@ -546,7 +546,8 @@ class DenseDecoder:
         """score over paged states of any lengths: ids (B, n_opt, t) option-row token ids on the GPU; a row's tokens follow
         its state's own last one, and see the state and their own row. Nothing is written. Returns (B, n_opt + 1)
         log-probabilities over the options and 'none'. Captured into a graph (after one eager call of the same sizes), it
-        scores whatever the states hold at the replay."""
+        scores whatever the states hold at the replay, with its work split for their lengths at the capture: capture it over
+        states as long as they will be."""
         self._check_paged(states)
         B, n_opt, t = ids.shape
         if B != states.batch or n_opt < 1 or t < 1:

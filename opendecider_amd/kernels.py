@@ -1163,7 +1163,8 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     page_append. row_begin int32 (N,): the first new token that a token sees, counted from its sequence's first (option
     rows and packed documents see their own tokens only); None: 0. max_new, max_ctx: bounds on a sequence's new and cached
     tokens that the caller knows on the host (the work is split by them; the result is right for any). The pages are only
-    read; int8 rows count as the exact q * s. Returns out (N, Hq, D) bf16 [, lse (N, Hq) fp32]; a token that sees nothing
+    read; an int8 row stands for q * s (exact with few slots a sequence, else each value rounded once to fp16; NaN where the
+    scale is not finite). Returns out (N, Hq, D) bf16 [, lse (N, Hq) fp32]; a token that sees nothing
     gets 0 and -inf, rows of no sequence are left as they were."""
     dev = _one_device("paged_attn", q, k, v, cache.k, cache.v, table, start, ctx_len, row_begin, out)
     B, pages, table = _paged(cache, table, start, ctx_len, "paged_attn")

@@ -1,8 +1,8 @@
 """A paged K/V cache: states of different lengths that grow and end on their own, in one pool of pages.
 
 Int8KVCache holds every state of a batch at one common length in a rectangle of its own; here a state is a row of page
-numbers, so a batch may be ragged in what it holds and in what it adds, memory is taken page by page, and states may share
-the pages of a common beginning. The operators over it (kernels.page_append, page_read, paged_attn) take a batch's new
+numbers, so a batch may be ragged in what it holds and in what it adds, and memory is taken page by page. (Tables of a caller's
+own may name a page in several sequences, for reading; PagedStates gives each state pages of its own.) The operators over it (kernels.page_append, page_read, paged_attn) take a batch's new
 tokens packed, sequence after sequence, with the offsets `start`.
 """
 from __future__ import annotations
