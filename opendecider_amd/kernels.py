@@ -1200,7 +1200,7 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     args = (*qa, *ka, *va, *pages, start.data_ptr(), ctx_len.data_ptr(), ptr(row_begin), *oa, ptr(lse), B, N, Hq, H, D, max_new,
             max_ctx, float(scale), ptr(ws), n, torch._C._cuda_getCurrentRawStream(dev))
-    if dev == torch._C._cuda_getDevice():
+    if dev == torch._C._cuda_getDevice():  # as _OnDevice, without its calls: the host bounds a token over a short state
         check(lib().od_paged_attn(*args), "od_paged_attn")
     else:
         with torch.cuda.device(dev):
