@@ -3,9 +3,10 @@ new tokens into pages with the q/k norm and the rotation on the way, and attenti
 
 Formats. Weights (N, K) in blocks of 32 along a row: w = (u - 8) d with u in 0..15 and one fp16 d a block; a block's 16 bytes
 hold values 0-15 in their low halves, 16-31 in the high ones. Pages of 4 bits hold token rows of D values in blocks of 32:
-value (u - 8) d with one bf16 d a block, byte i of a row values 2 i (low half) and 2 i + 1. A row x is written as: m the value
-of the largest |x| of the block (the first of several), d = bf16(m / -8), u = floor(x / d + 8.5) within 0..15; a block below
-2^-100 is d = 0, u = 8. Pages may also hold int8 rows with one fp32 scale, or bf16 rows.
+value (u - 8) d with one bf16 d a block; four bytes hold 8 values, the even ones 0, 2, 4, 6 in the halves of the first two bytes
+(low half first), the odd ones in those of the last two. A row x is written as: m the value of the largest |x| of the block (the
+first of several), d = bf16(m / -8), u = floor(x / d + 8.5) within 0..15; a block below 2^-100 is d = 0, u = 8. Pages may also
+hold int8 rows with one fp32 scale, or bf16 rows.
 
 Batches are packed and ragged: sequence b's new tokens are the rows start[b] .. start[b + 1] - 1, at the positions ctx[b],
 ctx[b] + 1, ...; position j of sequence b lies in row j % page of page table[b, j // page]. Kinds:
@@ -27,6 +28,7 @@ own = False
 DEV = "cuda"
 BF = torch.bfloat16
 EPS = 1e-6
+ORDER = [0, 2, 4, 6, 1, 3, 5, 7]  # the values of 8 in the order of their four bits
 
 
 def listed():
@@ -165,6 +167,7 @@ def _q4(x):
     d = torch.where(m.abs() < 2.0 ** -100, 0.0, m / -8.0).to(BF)
     inv = torch.where(d == 0, 0.0, 1.0).double()
     u = torch.floor(g.double() * inv / torch.where(d == 0, 1.0, d.double()) + 8.5).clamp_(0, 15).to(torch.uint8).flatten(-2)
+    u = u.unflatten(-1, (-1, 8))[..., ORDER].flatten(-2)
     return u[..., 0::2] | (u[..., 1::2] << 4), d[..., 0]
 
 
@@ -174,7 +177,8 @@ def _values(rows, scale):
         return rows.float()
     if rows.dtype == torch.int8:
         return rows * scale[..., None]
-    u = torch.stack([rows & 15, rows >> 4], -1).flatten(-2)
+    u = torch.stack([rows & 15, rows >> 4], -1).flatten(-2).unflatten(-1, (-1, 8))
+    u = u.unflatten(-1, (2, 4)).transpose(-1, -2).flatten(-4)  # even and odd ones side by side
     return ((u.float() - 8.0).unflatten(-1, (-1, 32)) * scale.float()[..., None]).flatten(-2)
 
 
@@ -356,7 +360,9 @@ def _exact_rows(pages, scales):
     if pages.dtype == torch.int8:
         return pages.double() * scales.double()[..., None]
     y = torch.empty(*pages.shape[:-1], 2 * pages.shape[-1], dtype=torch.float64, device=DEV)
-    y[..., 0::2], y[..., 1::2] = (pages % 16).double() - 8, (pages // 16).double() - 8
+    for byte in range(4):
+        for half, part in enumerate((pages[..., byte::4] % 16, pages[..., byte::4] // 16)):
+            y[..., ORDER[2 * byte + half]::8] = part.double() - 8
     return y * scales.double().repeat_interleave(32, -1)
 
 
