@@ -178,7 +178,7 @@ def _values(rows, scale):
     if rows.dtype == torch.int8:
         return rows * scale[..., None]
     u = torch.stack([rows & 15, rows >> 4], -1).flatten(-2).unflatten(-1, (-1, 8))
-    u = u.unflatten(-1, (2, 4)).transpose(-1, -2).flatten(-4)  # even and odd ones side by side
+    u = u.unflatten(-1, (2, 4)).transpose(-1, -2).flatten(-3)  # even and odd ones side by side
     return ((u.float() - 8.0).unflatten(-1, (-1, 32)) * scale.float()[..., None]).flatten(-2)
 
 
