@@ -624,6 +624,51 @@ int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k
                   int64_t D, int64_t max_new, int64_t max_ctx, float scale, float* ws, int64_t ws_floats,
                   od_stream_t stream);
 
+/*
+ * The same over pages of any format. OD_PAGE_BF16 (scales NULL) and OD_PAGE_INT8 (fp32 scales) as above. OD_PAGE_INT4:
+ *   k_pages, v_pages  uint8 [n_pages, Hkv, page, D / 2] with k_scale, v_scale bf16 [n_pages, Hkv, page, D / 32], contiguous,
+ *                     16-byte aligned: blocks of 32 values (u - 8) d along a row, u in 0 .. 15. Four bytes (a little-endian
+ *                     word) hold 8 values: value 2 i at bit 4 i, value 2 i + 1 at bit 16 + 4 i. A block is written as: m its
+ *                     value of the largest magnitude (the first of several), d = m / -8, u = floor(x / d + 8.5) within
+ *                     0 .. 15; below 2^-100 d = 0 and u = 8; with an infinity or NaN d = NaN (its u mean nothing). To the
+ *                     attention a block whose d is not finite holds NaN.
+ * od_page_read_ex: no OD_READ_INT8 of 4-bit pages.
+ */
+#define OD_PAGE_BF16 0
+#define OD_PAGE_INT8 1
+#define OD_PAGE_INT4 2
+int od_page_append_ex(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh, int format,
+                      void* k_pages, void* k_scale, void* v_pages, void* v_scale, int64_t n_pages, int64_t page,
+                      const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx_len,
+                      int64_t B, int64_t N, int64_t Hkv, int64_t D, od_stream_t stream);
+int od_page_read_ex(int format, const void* k_pages, const void* k_scale, const void* v_pages, const void* v_scale,
+                    int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
+                    const int32_t* length, int64_t B, int64_t T, int64_t Hkv, int64_t D, int form, void* k_out,
+                    float* ks_out, void* v_out, float* vs_out, od_stream_t stream);
+int od_paged_attn_ws_ex(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx,
+                        int format, int64_t* ws_floats);
+int od_paged_attn_ex(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
+                     const uint16_t* v, int64_t svt, int64_t svh, int format, const void* k_pages, const void* k_scale,
+                     const void* v_pages, const void* v_scale, int64_t n_pages, int64_t page, const int32_t* table,
+                     int64_t ld_table, int64_t cols, const int32_t* start, const int32_t* ctx_len, const int32_t* row_begin,
+                     uint16_t* out, int64_t sot, int64_t soh, float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+                     int64_t D, int64_t max_new, int64_t max_ctx, float scale, float* ws, int64_t ws_floats,
+                     od_stream_t stream);
+
+/*
+ * od_qk_norm_rope_ex and od_page_append_ex in one pass: qkv bf16 [N, ld >= (n_heads_q + 2 Hkv) D], per row its q, key and value
+ * heads. Every row's q and key heads, normed and rotated at pos[n], go to out bf16 [N, ldo >= (n_heads_q + Hkv) D] (qkv
+ * itself, with ldo = ld: in place; else they must not overlap); the tokens of sequences have their rotated keys and their values
+ * written into the pages, the bytes of the two calls. Rows 16-byte aligned; cos_t, sin_t bf16 [n_pos, rot_dim / 2], rot_dim D or
+ * D / 4. N (n_heads_q + 2 Hkv) D < 2^36.
+ */
+int od_qk_norm_rope_page_append(const uint16_t* qkv, int64_t ld, uint16_t* out, int64_t ldo, int64_t n_heads_q,
+                                int64_t rot_dim, int weight_offset, const uint16_t* q_w, const uint16_t* k_w,
+                                const uint16_t* cos_t, const uint16_t* sin_t, int64_t n_pos, const int32_t* pos, float eps,
+                                int format, void* k_pages, void* k_scale, void* v_pages, void* v_scale, int64_t n_pages,
+                                int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                                const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D, od_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,11 +12,11 @@ from .quant import (Int8Linear, Int8Tensor, SmoothedLinear, W8A8Linear, fast_int
                     w8a8_)
 from .prefix_attn import _split_attention, split_attention, split_attention_int8
 from .kv_cache import Int8KVCache
-from .paged_cache import PagedKVCache, PagedStates
+from .paged_cache import PagedKVCache, PagedStates, pack_int4, unpack_int4
 from .wide_attention import wide_attention
 from .lm_head import Int8Table, Q4Table, token_logprob
 
 __all__ = ["Int8Linear", "Int8Tensor", "SmoothedLinear", "W8A8Linear", "fast_int8_kernels_", "gemlite_a8w8_",
            "int8_to_w8a8_", "kv_mode", "materialize", "maybe_quantize", "quantize_int8_", "smooth_a8w8_",
            "smooth_scales", "w8a8_", "_split_attention", "split_attention", "split_attention_int8", "Int8KVCache", "wide_attention",
-           "Int8Table", "Q4Table", "token_logprob", "PagedKVCache", "PagedStates"]
+           "Int8Table", "Q4Table", "token_logprob", "PagedKVCache", "PagedStates", "pack_int4", "unpack_int4"]

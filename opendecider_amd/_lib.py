@@ -100,6 +100,17 @@ SIGNATURES = {
     "od_paged_attn": [_c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64,
                       _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _i64, _i64, _i64,
                       _i64, _i64, ctypes.c_float, _c_ptr, _i64, _c_ptr],
+    "od_page_append_ex": [_c_ptr, _i64, _i64, _c_ptr, _i64, _i64, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64,
+                          _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _c_ptr],
+    "od_page_read_ex": [ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _i64,
+                        _i64, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
+    "od_paged_attn_ws_ex": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _c_ptr],
+    "od_paged_attn_ex": [_c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                         _i64, _i64, _c_ptr, _i64, _i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr, _i64, _i64, _i64,
+                         _i64, _i64, _i64, _i64, ctypes.c_float, _c_ptr, _i64, _c_ptr],
+    "od_qk_norm_rope_page_append": [_c_ptr, _i64, _c_ptr, _i64, _i64, _i64, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64,
+                                    _c_ptr, ctypes.c_float, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr,
+                                    _i64, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _c_ptr],
     "od_lm_head_logprob_ws": [_i64, _i64, _c_ptr],
     "od_lm_head_logprob": [_c_ptr, _i64, _c_ptr, _i64, ctypes.c_int, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64,
                            _c_ptr, _c_ptr, _i64, _c_ptr],

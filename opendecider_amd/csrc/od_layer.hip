@@ -1,15 +1,14 @@
 // Row kernels of the dense decoder layer around the W8A8 GEMMs and the branched attention (gfx950):
 //   od_rmsnorm_quant   RMSNorm -> (SmoothQuant input scale) -> per-token int8, one pass over HBM
 //   od_qk_norm_rope    per-head RMSNorm of q and k + rotary embedding, in place on the QKV GEMM output
+//   od_qk_norm_rope_page_append  the same with the new tokens' K and V written into a paged cache on the way
 //   od_silu_mul_quant  SwiGLU (silu(gate) * up) -> (SmoothQuant input scale) -> per-token int8
 // All are HBM-bound (a few bytes per element); each fuses what would otherwise be separate bf16 round trips.
 // Rounding follows the bf16 module arithmetic of the decoder they serve (every elementwise product of two bf16
 // tensors is rounded to bf16 once). The two values that a plain fp32 evaluation would leave dependent on the device
 // (the order of a sum, the last bit of exp / rsqrt) are correctly rounded instead: the RMSNorm factor comes from a
 // float64 sum of squares (od_rms_factor) and silu from od_silu_bf16, so the outputs equal the oracle's bit for bit.
-#include <type_traits>
-
-#include "od_common.h"
+#include "od_paged.h"
 
 namespace {
 
@@ -298,6 +297,17 @@ struct KvAppend {
   float* vs;
   int64_t S, cap, n0;
 };
+// What becomes of the key and value heads: kOnly nothing more, kRows the int8 caches of KvAppend, kPages + format the pages of
+// their sequences; then the q and k heads go to `out` (which may be qkv), the rows of K and V as od_page_append writes them.
+// Bound by latency for a decode step, by vector work for chunks: a token of 32 / 8 heads of 128 is 48 lane groups of 16 values a
+// lane, 40 of them with a float64 sum, a root and the rotation.
+// (numbers, not an enum without a name: such a type in a kernel's signature has one name on the host and another on the device)
+constexpr int kOnly = 0, kRows = 1, kPages = 16;
+struct PageAppend {
+  Paged p;
+  uint16_t* out;
+  int64_t ldo;
+};
 
 // H = 4 bf16 values (8 bytes) or H = 8 (16 bytes) of one vector load
 template <int H>
@@ -352,13 +362,56 @@ __device__ __forceinline__ void quant_head(const uint16_t (&oa)[H], const uint16
   if (j == 0) *srow = scale;
 }
 
+// Writes a head's D bf16 values, held as above (H = 8) by the lanes of a rotated head of RD dims, as a row of the pages. The 32
+// values of a 4-bit block are the a or the b halves of 4 lanes where the rotation's halves are whole blocks (SPLIT lanes), else
+// both halves of 2 lanes.
+template <int D, int RD, int P>
+__device__ __forceinline__ void page_head(const Paged& p, bool isv, int64_t row, const uint4& a, const uint4& b, int j, int da,
+                                          int db) {
+  if constexpr (P == kBf16) {
+    uint16_t* dst = static_cast<uint16_t*>(isv ? p.v : p.k) + row * D;
+    *reinterpret_cast<uint4*>(dst + da) = a;
+    *reinterpret_cast<uint4*>(dst + db) = b;
+  } else if constexpr (P == kInt8) {
+    uint16_t ha[8], hb[8];
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ha[2 * k] = (uint16_t)wa[k];
+      ha[2 * k + 1] = (uint16_t)(wa[k] >> 16);
+      hb[2 * k] = (uint16_t)wb[k];
+      hb[2 * k + 1] = (uint16_t)(wb[k] >> 16);
+    }
+    quant_head<D, 8>(ha, hb, j, da, db, static_cast<int8_t*>(isv ? p.v : p.k) + row * D, (isv ? p.vs : p.ks) + row);
+  } else {
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+    uint32_t la = q4_lead(wa, da & 31), lb = q4_lead(wb, db & 31);
+    const bool split = RD >= 64 && j < RD / 16;
+    if (!split) la = lb = max(la, lb);
+    la = max(la, (uint32_t)__shfl_xor((int)la, 1, OD_WAVE));
+    lb = max(lb, (uint32_t)__shfl_xor((int)lb, 1, OD_WAVE));
+    if constexpr (RD >= 64) {
+      const uint32_t ma = (uint32_t)__shfl_xor((int)la, 2, OD_WAVE), mb = (uint32_t)__shfl_xor((int)lb, 2, OD_WAVE);
+      if (split) la = max(la, ma), lb = max(lb, mb);
+    }
+    float ia, ib;
+    const uint32_t sa = q4_scale(la, ia), sb = q4_scale(lb, ib);
+    char* dst = static_cast<char*>(isv ? p.v : p.k) + row * (D / 2);
+    uint16_t* sc = (isv ? p.v4 : p.k4) + row * (D / 32);
+    *reinterpret_cast<uint32_t*>(dst + da / 2) = q4_word(wa, ia);
+    *reinterpret_cast<uint32_t*>(dst + db / 2) = q4_word(wb, ib);
+    if (da % 32 == 0) sc[da / 32] = (uint16_t)sa;
+    if (db % 32 == 0) sc[db / 32] = (uint16_t)sb;
+  }
+}
+
 // Partial rotary (RD < D, Qwen3.5's 64 of 256): rotate_half acts on the first RD dims only (pairs d, d + RD/2) and the
 // other D - RD pass through the norm unrotated. A group of G = D / (2H) lanes owns a head: lane j < RD / (2H) holds
 // the pairs Hj .. Hj + H - 1 and RD/2 + Hj .., a lane j >= RD / (2H) the 2H dims RD + 2H (j - RD / (2H)) .. +2H - 1, so
 // no lane exchange is needed for the rotation. H = 4: 8-byte loads and stores; H = 8: 16-byte ones (rows and tables
 // 16-byte aligned), half the lanes per head. The tables are [n_pos, RD/2]. ZC: the Qwen3.5 norm, one rounding:
 // n_d = bf16((x_d * r) * (1 + w_d)) (fp32 products), instead of bf16(w_d * bf16(x_d * r)).
-template <int D, int RD, bool ZC, bool APPEND, int H>
+template <int D, int RD, bool ZC, int APPEND, int H>
 __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restrict__ qkv, int64_t ld, int64_t M,
                                                                int n_heads_q, int n_heads_k,
                                                                const uint16_t* __restrict__ qw,
@@ -366,12 +419,21 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
                                                                const uint16_t* __restrict__ cos_t,
                                                                const uint16_t* __restrict__ sin_t, int64_t n_pos,
                                                                const int32_t* __restrict__ pos, float eps,
-                                                               KvAppend kv) {
+                                                               std::conditional_t<(APPEND >= kPages), PageAppend,
+                                                                                  KvAppend> kv) {
   constexpr int G = D / (2 * H), RL = RD / (2 * H), RH = RD / 2;
+  constexpr bool PAGED = APPEND >= kPages;
+  static_assert(!PAGED || H == 8, "rows of pages are written 8 values at a time");
   static_assert(RD % (2 * H) == 0 && RD <= D, "rotary dims");
   using V = VecH<H>;
   const int heads = n_heads_q + n_heads_k * (APPEND ? 2 : 1);
   const int64_t gh = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  int b0 = 0;  // pages: the last sequence that starts at or before the wave's first row, by all its lanes
+  if constexpr (PAGED) {
+    const int64_t first = (int64_t)blockIdx.x * (kThreads / G) + (threadIdx.x >> 6) * (64 / G);
+    const int t0 = __builtin_amdgcn_readfirstlane((int)min(first / heads, M - 1));
+    if (first < M * heads && first - (int64_t)t0 * heads + 64 / G > n_heads_q) b0 = seq_search(kv.p.start, kv.p.B, t0);
+  }
   if (gh >= M * heads) return;  // whole G-lane groups exit together
   const int64_t row = gh / heads;
   const int head = (int)(gh % heads);
@@ -381,11 +443,17 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
   uint16_t* hp = qkv + row * ld + (int64_t)head * D;
   const V ra = *reinterpret_cast<const V*>(hp + da), rb = *reinterpret_cast<const V*>(hp + db);
   int64_t crow = 0;
-  if (APPEND) {
+  if constexpr (PAGED) {
+    crow = head >= n_heads_q ? row_to_write(kv.p, b0, (int)row, (head - n_heads_q) % n_heads_k) : -1;
+    if (head >= n_heads_q + n_heads_k) {
+      if (crow >= 0) page_head<D, RD, APPEND - kPages>(kv.p, true, crow, ra, rb, j, da, db);
+      return;
+    }
+  } else if (APPEND) {
     const int64_t b = row / kv.S, i = row % kv.S;
     crow = (b * n_heads_k + (head - n_heads_q) % n_heads_k) * kv.cap + kv.n0 + i;
   }
-  if (APPEND && head >= n_heads_q + n_heads_k) {  // a value head: quantize only
+  if constexpr (APPEND == kRows) if (head >= n_heads_q + n_heads_k) {  // a value head: quantize only
     const uint32_t* wa = reinterpret_cast<const uint32_t*>(&ra);
     const uint32_t* wb = reinterpret_cast<const uint32_t*>(&rb);
     uint16_t va[H], vb[H];
@@ -445,9 +513,18 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
       ob[e] = od_f32_to_bf16(nb[e]);
     }
   }
-  *reinterpret_cast<V*>(hp + da) = packh<H>(oa);
-  *reinterpret_cast<V*>(hp + db) = packh<H>(ob);
-  if (APPEND && head >= n_heads_q) quant_head<D, H>(oa, ob, j, da, db, kv.kq + crow * D, kv.ks + crow);
+  if constexpr (PAGED) {
+    uint16_t* op = kv.out + row * kv.ldo + (int64_t)head * D;
+    const V pa = packh<H>(oa), pb = packh<H>(ob);
+    *reinterpret_cast<V*>(op + da) = pa;
+    *reinterpret_cast<V*>(op + db) = pb;
+    if (head >= n_heads_q && crow >= 0) page_head<D, RD, APPEND - kPages>(kv.p, false, crow, pa, pb, j, da, db);
+  } else {
+    *reinterpret_cast<V*>(hp + da) = packh<H>(oa);
+    *reinterpret_cast<V*>(hp + db) = packh<H>(ob);
+    if constexpr (APPEND == kRows)
+      if (head >= n_heads_q) quant_head<D, H>(oa, ob, j, da, db, kv.kq + crow * D, kv.ks + crow);
+  }
 }
 
 template <int NV>
@@ -659,7 +736,7 @@ namespace {
 
 bool aligned8(const void* p) { return (((uintptr_t)p) & 7u) == 0; }
 
-template <int D, int RD, bool ZC, bool APPEND>
+template <int D, int RD, bool ZC, int APPEND>
 void launch_rope_vec_t(bool wide, int64_t items, hipStream_t st, uint16_t* qkv, int64_t ld, int64_t M,
                        int64_t n_heads_q, int64_t n_heads_k, const uint16_t* q_w, const uint16_t* k_w,
                        const uint16_t* cos_t, const uint16_t* sin_t, int64_t n_pos, const int32_t* pos, float eps,
@@ -682,7 +759,7 @@ bool rope_shape_ok(int64_t D, int64_t rot_dim) {
   return (D == 64 || D == 128 || D == 256) && (rot_dim == D || rot_dim == D / 4);
 }
 
-template <bool APPEND>
+template <int APPEND>
 int launch_rope_vec(uint16_t* qkv, int64_t ld, int64_t M, int64_t n_heads_q, int64_t n_heads_k, int64_t D,
                     int64_t rot_dim, bool zc, const uint16_t* q_w, const uint16_t* k_w, const uint16_t* cos_t,
                     const uint16_t* sin_t, int64_t n_pos, const int32_t* pos, float eps, const KvAppend& kv,
@@ -730,7 +807,7 @@ extern "C" int od_qk_norm_rope_ex(uint16_t* qkv, int64_t ld, int64_t M, int64_t 
                    aligned8(sin_t);
   hipStream_t st = (hipStream_t)stream;
   if (vec)
-    return launch_rope_vec<false>(qkv, ld, M, n_heads_q, n_heads_k, D, rot_dim, weight_offset != 0, q_w, k_w, cos_t,
+    return launch_rope_vec<kOnly>(qkv, ld, M, n_heads_q, n_heads_k, D, rot_dim, weight_offset != 0, q_w, k_w, cos_t,
                                   sin_t, n_pos, pos, eps, KvAppend{}, st);
   // unaligned rows: the scalar kernel, for the full-rotary Llama-style norm at D = 64 or 128 only
   if (rot_dim != D || weight_offset != 0 || D == 256) return OD_ERR_ALIGN;
@@ -774,7 +851,7 @@ extern "C" int od_qk_norm_rope_kv_append_ex(uint16_t* qkv, int64_t ld, int64_t B
       (((uintptr_t)kq) & 3u) || (((uintptr_t)vq) & 3u))
     return OD_ERR_ALIGN;
   KvAppend kv{kq, ks, vq, vs, S, cap, n0};
-  return launch_rope_vec<true>(qkv, ld, M, n_heads_q, n_heads_k, D, rot_dim, weight_offset != 0, q_w, k_w, cos_t,
+  return launch_rope_vec<kRows>(qkv, ld, M, n_heads_q, n_heads_k, D, rot_dim, weight_offset != 0, q_w, k_w, cos_t,
                                sin_t, n_pos, pos, eps, kv, (hipStream_t)stream);
 }
 
@@ -786,6 +863,52 @@ extern "C" int od_qk_norm_rope_kv_append(uint16_t* qkv, int64_t ld, int64_t B, i
   if (D != 64 && D != 128) return OD_ERR_UNSUPPORTED;
   return od_qk_norm_rope_kv_append_ex(qkv, ld, B, S, n_heads_q, n_heads_k, D, D, 0, q_w, k_w, cos_t, sin_t, n_pos,
                                       pos, eps, kq, ks, vq, vs, cap, n0, stream);
+}
+
+extern "C" int od_qk_norm_rope_page_append(const uint16_t* qkv, int64_t ld, uint16_t* out, int64_t ldo, int64_t n_heads_q,
+                                           int64_t rot_dim, int weight_offset, const uint16_t* q_w, const uint16_t* k_w,
+                                           const uint16_t* cos_t, const uint16_t* sin_t, int64_t n_pos, const int32_t* pos,
+                                           float eps, int format, void* k_pages, void* k_scale, void* v_pages, void* v_scale,
+                                           int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table,
+                                           int64_t cols, const int32_t* start, const int32_t* ctx_len, int64_t B, int64_t N,
+                                           int64_t Hkv, int64_t D, od_stream_t stream) {
+  PageAppend a;
+  if (const int rc = paged_args(a.p, format, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table, cols, start,
+                                ctx_len, B, N, Hkv, D))
+    return rc;
+  if (n_heads_q < 0 || n_heads_q > 65535 || ld < (n_heads_q + 2 * Hkv) * D || ldo < (n_heads_q + Hkv) * D) return OD_ERR_SHAPE;
+  if ((weight_offset != 0 && weight_offset != 1) || !rope_shape_ok(D, rot_dim)) return OD_ERR_UNSUPPORTED;
+  if (N == 0) return OD_OK;
+  if (!qkv || !out || !q_w || !k_w || !cos_t || !sin_t || !pos) return OD_ERR_NULL;
+  if (B > 0 && (!start || !ctx_len || (cols > 0 && !table))) return OD_ERR_NULL;
+  if (ld % 8 || ldo % 8 || !od_aligned16(qkv) || !od_aligned16(out) || !od_aligned16(q_w) || !od_aligned16(k_w) ||
+      !od_aligned16(cos_t) || !od_aligned16(sin_t))
+    return OD_ERR_ALIGN;
+  if (n_pages == 0) a.p.cols = 0;
+  a.out = out;
+  a.ldo = ldo;
+  const int64_t items = N * (n_heads_q + 2 * Hkv), per_block = kThreads / (D / 16), blocks = (items + per_block - 1) / per_block;
+  if (blocks > kMaxGroups) return OD_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks), block(kThreads);
+  by_head_dim(D, [&](auto DC) {
+    by_format(format, [&](auto PC) {
+      constexpr int DD = decltype(DC)::value, A = kPages + decltype(PC)::value;
+      auto go = [&](auto RC, auto ZC) {
+        qk_rope_vec_kernel<DD, decltype(RC)::value, decltype(ZC)::value, A, 8><<<grid, block, 0, (hipStream_t)stream>>>(
+            const_cast<uint16_t*>(qkv), ld, N, (int)n_heads_q, (int)Hkv, q_w, k_w, cos_t, sin_t, n_pos, pos, eps, a);
+      };
+      using Full = std::integral_constant<int, DD>;
+      using Part = std::integral_constant<int, DD / 4>;
+      if (weight_offset) {
+        if (rot_dim == D) go(Full{}, std::true_type{});
+        else go(Part{}, std::true_type{});
+      } else {
+        if (rot_dim == D) go(Full{}, std::false_type{});
+        else go(Part{}, std::false_type{});
+      }
+    });
+  });
+  return od_launch_status();
 }
 
 extern "C" int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int norm_offset, float eps,

@@ -1,17 +1,16 @@
 // A paged K/V cache, for gfx950: new tokens written into pages, sequences read back, attention over pages.
 //
 // Layout. A layer's K and V are two pools of n_pages pages; page p holds `page` (a power of two >= 16) token rows of
-// every KV head, [n_pages, Hkv, page, D], int8 with one fp32 scale per row ([n_pages, Hkv, page]) or bf16. Position j
-// of sequence b is row j % page of page table[b, j / page]. A (page, head) block is contiguous, so that an attention
+// every KV head, [n_pages, Hkv, page, D], int8 with one fp32 scale per row ([n_pages, Hkv, page]), bf16, or 4 bits a value with a
+// bf16 scale per 32 ([n_pages, Hkv, page, D / 2] bytes and [n_pages, Hkv, page, D / 32]). Position j of sequence b is row
+// j % page of page table[b, j / page]. A (page, head) block is contiguous, so that an attention
 // workgroup of one head reads whole runs of `page` rows. Batches are packed and ragged: sequence b's new tokens are the
 // packed rows start[b] .. start[b + 1] - 1, at the positions ctx[b], ctx[b] + 1, ...
 //
 // Nothing on the device is trusted to stay in bounds: a table entry outside [0, n_pages), a position past the table's
 // columns, a negative length and packed rows outside [0, N) are found by the kernels and skipped (no such key is seen,
 // no such row written). The host needs no copy of start, ctx or table.
-#include <type_traits>
-
-#include "od_common.h"
+#include "od_paged.h"
 
 namespace {
 
@@ -20,47 +19,6 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-
-// The pages and the sequences in them, as every kernel here takes them.
-struct Paged {
-  void* k;
-  void* v;
-  float* ks;  // null: bf16 pages
-  float* vs;
-  const int32_t* table;
-  const int32_t* start;  // [B + 1]; not used by page_read
-  const int32_t* ctx;    // [B]
-  int64_t ld_table, n_pages;
-  int cols, shift, B, N, Hkv;  // page = 1 << shift
-};
-
-// First row (over all heads of the pool) of the page that holds position `pos` of sequence b for head h, plus the row
-// in the page: the index of a token row of D values and of its scale. -1: no such page.
-__device__ __forceinline__ int64_t row_of(const Paged& p, int b, int h, int64_t pos) {
-  const int64_t col = pos >> p.shift;
-  if (pos < 0 || col >= p.cols) return -1;
-  const int pg = p.table[b * p.ld_table + col];
-  if (pg < 0 || pg >= p.n_pages) return -1;
-  return (((int64_t)pg * p.Hkv + h) << p.shift) + (pos & ((1 << p.shift) - 1));
-}
-
-// The last sequence that starts at or before packed row t, by all 64 lanes together (a 64-way search: one load per lane
-// and level, one level up to 64 sequences, two up to 4096); 0 if there is none. t is wave-uniform. In bounds for any
-// contents of start.
-__device__ __forceinline__ int seq_search(const int32_t* start, int B, int t) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = B;
-  while (n > 1) {
-    const int step = (n + 63) >> 6, at = lane * step;
-    const bool le = at < n && start[lo + at] <= t;
-    const int cnt = __builtin_popcountll(__builtin_amdgcn_ballot_w64(le));
-    if (cnt == 0) return 0;
-    const int skip = (cnt - 1) * step;
-    lo += skip;
-    n = min(step, n - skip);
-  }
-  return lo;
-}
 
 // ------------------------------------------------------------------------------------------------------- append
 // Rows of D values, 16 per lane (two 16-byte loads), G = D / 16 lanes per row. A wave takes 64 / G consecutive items of
@@ -75,7 +33,7 @@ struct AppendArgs {
   int64_t skt, skh, svt, svh;
 };
 
-template <int D, bool Q8>
+template <int D, int P>
 __global__ __launch_bounds__(kThreads) void page_append_kernel(AppendArgs a) {
   constexpr int G = D / 16, RPW = 64 / G;
   const Paged& p = a.p;
@@ -85,24 +43,29 @@ __global__ __launch_bounds__(kThreads) void page_append_kernel(AppendArgs a) {
   const int64_t items = (int64_t)p.N * heads, first = wave * RPW, item = first + lane / G;
   if (first >= items) return;  // wave-uniform
   const int t0 = __builtin_amdgcn_readfirstlane((int)(first >> 31 ? first / heads : (uint32_t)first / (uint32_t)heads));
-  int b = seq_search(p.start, p.B, t0);
+  const int b = seq_search(p.start, p.B, t0);
+  if (item >= items) return;  // whole G-lane groups leave together
   const uint32_t from = (uint32_t)(item - (int64_t)t0 * heads);
   const int t = t0 + (int)(from / (uint32_t)heads), h = (int)(from % (uint32_t)heads);
-  // this lane's row may belong to a later token than the wave's first one
-  while (b < p.B && p.start[b + 1] <= t) ++b;
-  if (item >= items || b >= p.B) return;  // whole G-lane groups leave together
-  const int s0 = p.start[b];
-  if (t < s0 || s0 < 0 || p.start[b + 1] > p.N) return;  // (a range outside the packed rows: no sequence, as seq_of)
   const bool isv = h >= p.Hkv;
   const int kh = isv ? h - p.Hkv : h;
-  const int64_t row = row_of(p, b, kh, (int64_t)max(p.ctx[b], 0) + (t - s0));
+  const int64_t row = row_to_write(p, b, t, kh);  // this lane's row may belong to a later token than the wave's first one
   if (row < 0) return;
   const uint16_t* x = (isv ? a.v + t * a.svt + kh * a.svh : a.k + t * a.skt + kh * a.skh) + 16 * j;
   const uint4 lo = *reinterpret_cast<const uint4*>(x), hi = *reinterpret_cast<const uint4*>(x + 8);
-  if constexpr (!Q8) {
+  if constexpr (P == kBf16) {
     uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(isv ? p.v : p.k) + row * D + 16 * j);
     dst[0] = lo;
     dst[1] = hi;
+  } else if constexpr (P == kInt4) {
+    const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
+    uint32_t lead = max(q4_lead(w0, 16 * (j & 1)), q4_lead(w1, 16 * (j & 1) + 8));
+    lead = max(lead, (uint32_t)__shfl_xor((int)lead, 1, 64));  // two lanes a block
+    float inv;
+    const uint32_t d = q4_scale(lead, inv);
+    *reinterpret_cast<uint2*>(static_cast<char*>(isv ? p.v : p.k) + row * (D / 2) + 8 * j) =
+        make_uint2(q4_word(w0, inv), q4_word(w1, inv));
+    if ((j & 1) == 0) (isv ? p.v4 : p.k4)[row * (D / 32) + j / 2] = (uint16_t)d;
   } else {
     const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     float y[16];
@@ -161,9 +124,10 @@ __device__ __forceinline__ Chunk<BYTES> read_chunk(const void* p) {
   }
   return c;
 }
-template <int D, bool Q8, int OUT>
+template <int D, int P, int OUT>
 __global__ __launch_bounds__(kThreads) void page_read_kernel(ReadArgs a) {
-  constexpr int V = read_values(OUT), G = D / V, BYTES = V * (Q8 ? 1 : 2);
+  constexpr bool Q8 = P == kInt8, Q4 = P == kInt4;
+  constexpr int V = read_values(OUT), G = D / V, BYTES = Q4 ? 4 : V * (Q8 ? 1 : 2);
   const int bh = blockIdx.x / a.tiles, b = bh / a.p.Hkv, h = bh % a.p.Hkv;
   const int pos = (blockIdx.x % a.tiles) * (kThreads / G) + threadIdx.x / G, j = threadIdx.x % G;
   if (pos >= a.T) return;
@@ -171,25 +135,31 @@ __global__ __launch_bounds__(kThreads) void page_read_kernel(ReadArgs a) {
   Chunk<BYTES> x[2] = {};
   float s[2] = {};
   if (row >= 0) {
-    x[0] = read_chunk<BYTES>(static_cast<const char*>(a.p.k) + (row * G + j) * BYTES);
-    x[1] = read_chunk<BYTES>(static_cast<const char*>(a.p.v) + (row * G + j) * BYTES);
+    // 4 bits: the word of 8 values that holds the lane's
+    const int64_t from = Q4 ? row * (D / 2) + 4 * (j * V / 8) : (row * G + j) * BYTES;
+    x[0] = read_chunk<BYTES>(static_cast<const char*>(a.p.k) + from);
+    x[1] = read_chunk<BYTES>(static_cast<const char*>(a.p.v) + from);
     if constexpr (Q8) {
       s[0] = a.p.ks[row];
       s[1] = a.p.vs[row];
+    } else if constexpr (Q4) {
+      s[0] = od_bf16_to_f32(a.p.k4[row * (D / 32) + j * V / 32]);
+      s[1] = od_bf16_to_f32(a.p.v4[row * (D / 32) + j * V / 32]);
     }
   }
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const Chunk<BYTES>& c = x[side];
     v4u o;
-    if constexpr (OUT == kReadI8 || (OUT == kReadBf16 && !Q8)) {
+    if constexpr (OUT == kReadI8 || (OUT == kReadBf16 && P == kBf16)) {
       o = v4u{c.w[0], c.w[1], c.w[2], c.w[3]};
       if (OUT == kReadI8 && j == 0) (side ? a.vs : a.ks)[at] = s[side];
     } else {
       float y[V];
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        y[i] = Q8 ? (float)(int8_t)(c.w[i / 4] >> (8 * (i % 4))) * s[side]
+        y[i] = Q4 ? q4_value(V == 4 ? c.w[0] >> (8 * (j & 1)) : c.w[0], i, s[side])
+             : Q8 ? (float)(int8_t)(c.w[i / 4] >> (8 * (i % 4))) * s[side]
                   : __uint_as_float(i % 2 ? c.w[i / 2] & 0xffff0000u : c.w[i / 2] << 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -855,7 +825,6 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 // The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first
 // in the next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
 constexpr int kBK = 64;
-enum { kBf16 = 0, kInt8 = 1, kImage = 2 };  // what the tile kernels read: bf16 pages, int8 pages, their image
 constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
 
 // K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
@@ -951,6 +920,68 @@ __device__ __forceinline__ void i8x16_scaled(v4u w, float f, v4u& lo, v4u& hi) {
 // s 2^e with 20 significant bits: within 2^-20 of it
 __device__ __forceinline__ float frame_scale(float s, int e) {
   return __uint_as_float(__float_as_uint(__builtin_ldexpf(s, e)) & ~15u);
+}
+
+// A word of 8 four-bit values times their scale, as fp16, in order. A value u at bits 6 to 9 of 16.0's fp16 is 16 + u, so a pair
+// is one shift, one and-or and one fma with 24 s: u - 8 has 3 significant bits and s 8 (f16_scale), so that 24 s and the result
+// are exact (12 instructions a word).
+struct Q4Scale {
+  f16x2 s, c;  // s and -24 s
+};
+__device__ __forceinline__ Q4Scale q4_pair(f16x2 s) {
+  const f16x2 k = {(_Float16)-24.0f, (_Float16)-24.0f};
+  return {s, s * k};
+}
+__device__ __forceinline__ v4u q4x8_f16(uint32_t w, const Q4Scale& q) {
+  const uint32_t at[4] = {w << 6, w << 2, w >> 2, w >> 6};
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 x = __builtin_bit_cast(f16x2, (at[i] & 0x03c003c0u) | 0x4c004c00u);
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, q.s, q.c));
+  }
+  return r;
+}
+// A bf16 scale times 2^e in fp16, NaN where it is not finite (an infinite one would make scores of -inf, which are no keys);
+// exact unless it falls below fp16's normal numbers.
+__device__ __forceinline__ _Float16 f16_scale(uint32_t bits, int e) {
+  const float s = (bits & 0x7f80u) == 0x7f80u ? NAN : __uint_as_float(bits << 16);
+  return (_Float16)__builtin_ldexpf(s, e);
+}
+// The frame of 4-bit values whose largest scale has these bf16 bits: 2^E above it, and values below 8 times it, so that q 2^(7 -
+// (E - 4)) is below 2^14, as for int8.
+__device__ __forceinline__ int q4_frame(uint32_t bits) { return bits ? (int)(bits >> 7) - 126 - 4 : 0; }
+// The largest magnitude of the finite ones of N packed pairs of bf16 scales, as bits.
+template <int N>
+__device__ __forceinline__ uint32_t q4_largest(const uint32_t (&w)[N]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = od_absmax_bf16x2(m, fin_bf16x2(w[i]));
+  return max(m & 0xffffu, m >> 16);
+}
+// The D / 32 scales of a row.
+template <int D>
+__device__ __forceinline__ void q4_row_scales(const uint16_t* scales, int64_t row, uint32_t (&w)[D / 64]) {
+  const uint16_t* at = scales + row * (D / 32);
+  if constexpr (D == 64) {
+    w[0] = *reinterpret_cast<const uint32_t*>(at);
+  } else if constexpr (D == 128) {
+    const uint2 u = *reinterpret_cast<const uint2*>(at);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(at);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  }
+}
+// A block of 32 values (16 bytes, block c of key `key`) into the places of a tile's K or V.
+template <int D>
+__device__ __forceinline__ void q4_put(uint16_t* dst, bool v, int key, int c, const v4u& r, _Float16 s) {
+  const Q4Scale q = q4_pair(f16x2{s, s});
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ch = 4 * c + i, at = v ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch);
+    *reinterpret_cast<uint4*>(dst + at) = __builtin_bit_cast(uint4, q4x8_f16(r[i], q));
+  }
 }
 
 template <int D, int NW>
@@ -1242,11 +1273,12 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
   }
 }
 
-// Waves a SIMD: heads of 64 leave the registers for three, but for the conversion of int8 blocks.
-constexpr int t_waves(int D, int src) { return D == 64 && src != kInt8 ? 3 : 2; }
+// Waves a SIMD: heads of 64 leave the registers for three, but for the conversion of int8 and 4-bit blocks.
+constexpr int t_waves(int D, int src) { return D == 64 && (src == kBf16 || src == kImage) ? 3 : 2; }
 template <int D, int SRC, int NW>
 __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(AttnArgs a) {
-  constexpr bool Q8 = SRC == kInt8, IMG = SRC == kImage, H16 = SRC != kBf16;
+  // REG: blocks that are converted on their way, through registers
+  constexpr bool Q4 = SRC == kInt4, REG = SRC == kInt8 || Q4, IMG = SRC == kImage, H16 = SRC != kBf16;
   constexpr int NT = NW * 64, SPT = 32 * NW, DT = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   TSmem<D, NW>& sm = *reinterpret_cast<TSmem<D, NW>*>(smem_raw);
@@ -1289,9 +1321,11 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       if constexpr (H16) t_q_to_f16<D>(t);
       const int64_t first = ((int64_t)b * a.p.Hkv + g) * a.img_blocks;  // image: the sequence's first block
       if constexpr (IMG) frame = a.img_vexp[b * a.p.Hkv + g] - 7;
-      // int8 blocks pass through registers, NC 16-byte chunks per thread, K's first; bf16 ones go by DMA
-      constexpr int CPK = D / 16, CH = kBK * CPK, NC = 2 * CH / NT;
-      v4u r[Q8 ? NC : 1];
+      // int8 and 4-bit blocks pass through registers, NC 16-byte chunks per thread, K's first; bf16 ones go by DMA
+      constexpr int CPK = D / (Q4 ? 32 : 16), CH = kBK * CPK, NC = 2 * CH / NT;
+      v4u r[REG ? NC : 1];
+      uint32_t rs[Q4 ? NC : 1];         // 4 bits: the scales of the chunks
+      uint32_t ks4 = 0, vs4 = 0;        // 4 bits, lane l: the largest scales of key l of the loaded block
       int pg = -1;             // lane l: the page of key l of the block whose loads come next
       float ks = 0, vs = 0;    // lane l: the scales of key l of the loaded block
       uint64_t there = 0;      // the loaded block's keys that exist
@@ -1317,15 +1351,25 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
         auto row = [&](int key) {
           return (((int64_t)__shfl(page, key, 64) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + key) & in_page);
         };
-        if constexpr (Q8) {
+        if constexpr (REG) {
           const int64_t at = (((int64_t)page * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & in_page);
-          ks = a.p.ks[at];
-          vs = a.p.vs[at];
+          if constexpr (Q4) {
+            uint32_t w[D / 64];
+            q4_row_scales<D>(a.p.k4, at, w);
+            ks4 = q4_largest(w);
+            q4_row_scales<D>(a.p.v4, at, w);
+            vs4 = q4_largest(w);
+          } else {
+            ks = a.p.ks[at];
+            vs = a.p.vs[at];
+          }
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
             const char* pool = static_cast<const char*>(side ? a.p.v : a.p.k);
-            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(pool + row(key) * D + 16 * ch));
+            const int64_t from = row(key);
+            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(pool + from * (16 * CPK) + 16 * ch));
+            if constexpr (Q4) rs[i] = (side ? a.p.v4 : a.p.k4)[from * CPK + ch];
           }
         } else {
           dma_pages<D, NW>(sm.k[buf], wave, false, a.p, g, blk, pg);
@@ -1339,7 +1383,19 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
         seen = there;
         if constexpr (IMG) {
           kexp = kexp_in;
-        } else if constexpr (Q8) {
+        } else if constexpr (Q4) {
+          const bool on = (there >> lane) & 1;
+          kexp = q4_frame(od_wave_umax_dpp(on ? ks4 : 0u));
+          const uint32_t vm = od_wave_umax_dpp(on ? vs4 : 0u);
+          if (vm) vexp = vexp_set ? max(vexp, q4_frame(vm)) : q4_frame(vm);
+          if (vm) vexp_set = true;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            const int cid = i * NT + tid, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
+            const _Float16 sc = f16_scale((there >> key) & 1 ? rs[i] : 0u, 7 - (side ? vexp : kexp));
+            q4_put<D>(side ? sm.v[buf] : sm.k[buf], side, key, ch, r[i], sc);
+          }
+        } else if constexpr (REG) {
           // every wave takes the block's frames from the same 64 scales; keys that are none, and scales that are not
           // finite, leave them alone
           const bool on = (there >> lane) & 1;
@@ -1368,15 +1424,15 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
             if (!((seen >> (c / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[buf][8 * c]) = make_uint4(0, 0, 0, 0);
         }
       };
-      // One step: block blk's products; ahead of them, for int8 the conversion of block blk + 1 (in registers since the
+      // One step: block blk's products; ahead of them, for int8 and 4 bits the conversion of block blk + 1 (in registers since the
       // last step) and the loads of blk + 2, for bf16 the copy of blk + 1.
       pages(b_lo);
       load(b_lo, 0);
       pages(b_lo + 1);
-      if constexpr (!Q8) dma_wait();
+      if constexpr (!REG) dma_wait();
       store(0);
-      if constexpr (Q8) frame = vexp - 7;  // O is 0 still: no rescaling, by what may be no fp32 number
-      if (Q8 && b_lo + 1 < b_hi) {
+      if constexpr (REG) frame = vexp - 7;  // O is 0 still: no rescaling, by what may be no fp32 number
+      if (REG && b_lo + 1 < b_hi) {
         load(b_lo + 1, 1);
         pages(b_lo + 2);
       }
@@ -1384,10 +1440,10 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       for (int blk = b_lo; blk < b_hi; ++blk) {
         const int cur = (blk - b_lo) & 1;
         const float c = H16 ? score_factor(a.scale_log2, t.qe - 14 + kexp - 7) : a.scale_log2;
-        const int f_new = Q8 ? vexp - 7 : 0;
+        const int f_new = REG ? vexp - 7 : 0;
         const uint64_t mask = seen;
         if (blk + 1 < b_hi) {
-          if constexpr (Q8) {
+          if constexpr (REG) {
             store(cur ^ 1);
             if (blk + 2 < b_hi) {
               load(blk + 2, cur);
@@ -1398,7 +1454,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
             pages(blk + 2);
           }
         }
-        if (Q8 && f_new != frame) {  // the values' frame rose: uniform over the workgroup
+        if (REG && f_new != frame) {  // the values' frame rose: uniform over the workgroup
           const float f = __builtin_ldexpf(1.0f, frame - f_new);
 #pragma unroll
           for (auto& o : t.o)
@@ -1421,7 +1477,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
           t_softmax<D, H16>(sc, c, t, pb);
           t_values<D, H16>(sm.v[cur], vb, pb, t);
         }
-        if (!Q8 && blk + 1 < b_hi) {
+        if (!REG && blk + 1 < b_hi) {
           dma_wait();
           store(cur ^ 1);
         }
@@ -1513,7 +1569,8 @@ struct alignas(16) WSmem {
 
 template <int SRC>
 __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
-  constexpr bool Q8 = SRC == kInt8, IMG = SRC == kImage, H16 = SRC != kBf16;
+  // REG: blocks that are converted on their way, through registers
+  constexpr bool Q4 = SRC == kInt4, REG = SRC == kInt8 || Q4, IMG = SRC == kImage, H16 = SRC != kBf16;
   constexpr int D = 256, NW = 8, NT = 512, SPT = 128, DT = 4;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   WSmem& sm = *reinterpret_cast<WSmem*>(smem_raw);
@@ -1635,7 +1692,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       if constexpr (H16) t_q_to_f16<D>(t);
       const int64_t first = ((int64_t)b * a.p.Hkv + g) * a.img_blocks;  // image: the sequence's first block
       if constexpr (IMG) frame = a.img_vexp[b * a.p.Hkv + g] - 7;
-      constexpr int CPK = D / 16, NC = kBK * CPK / NT;  // int8: 16-byte chunks per row; per thread and side
+      constexpr int CPK = D / (Q4 ? 32 : 16), NC = kBK * CPK / NT;  // 16-byte chunks per row; per thread and side
       const int in_page = (1 << a.p.shift) - 1;
       // lane l: the page of key l of a block, or -1
       auto pages = [&](int blk) {
@@ -1678,34 +1735,60 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
           *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
         }
       };
-      v4u rk[Q8 ? NC : 1], rv[Q8 ? NC : 1];
+      // 4 bits: a block's K or V (one chunk a thread), the chunk's scale in the high half of sc and in the low one, lane l, the
+      // largest of key l's
+      auto load4 = [&](int blk, int pg, const void* pool, const uint16_t* scales, v4u (&r)[NC], uint32_t& sc) {
+        const int key = tid / CPK, ch = tid % CPK;
+        uint32_t w[D / 64];
+        q4_row_scales<D>(scales, (((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + ((blk * kBK + lane) & in_page), w);
+        const int64_t from = row(blk, pg, key);
+        r[0] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(pool) + from * (D / 2) + 16 * ch));
+        sc = q4_largest(w) | (uint32_t)scales[from * CPK + ch] << 16;
+      };
+      auto largest4 = [&](int pg, uint32_t sc) { return od_wave_umax_dpp(pg >= 0 ? sc & 0xffffu : 0u); };
+      auto put4 = [&](uint16_t* dst, bool v, const v4u (&r)[NC], uint32_t sc, int pg, int e) {
+        const int key = tid / CPK;
+        q4_put<D>(dst, v, key, tid % CPK, r[0], f16_scale(__shfl(pg, key, 64) >= 0 ? sc >> 16 : 0u, 7 - e));
+      };
+      v4u rk[REG ? NC : 1], rv[REG ? NC : 1];
       float ks = 0, vs = 0;
+      uint32_t ks4 = 0, vs4 = 0;
       int ke0 = 0, ke1 = 0;  // the frames of the K blocks in the two buffers
       int vexp = 0;          // the frame of the last V block stored
       bool vexp_set = false;
       auto store_k = [&](int blk, int pg) {
-        if constexpr (Q8) {
-          const int e = exp_above(scale_bits(pg, ks));
-          put8(sm.k[blk & 1], false, rk, pg >= 0 ? frame_scale(ks, 7 - e) : 0.0f);
+        if constexpr (REG) {
+          int e;
+          if constexpr (Q4) {
+            e = q4_frame(largest4(pg, ks4));
+            put4(sm.k[blk & 1], false, rk, ks4, pg, e);
+          } else {
+            e = exp_above(scale_bits(pg, ks));
+            put8(sm.k[blk & 1], false, rk, pg >= 0 ? frame_scale(ks, 7 - e) : 0.0f);
+          }
           if (blk & 1) ke1 = e;
           else ke0 = e;
         }
       };
       auto store_v = [&](int blk, int pg) {
-        if constexpr (Q8) {
-          const uint32_t bits = scale_bits(pg, vs);
-          if (bits) vexp = vexp_set ? max(vexp, exp_above(bits)) : exp_above(bits);
+        if constexpr (REG) {
+          const uint32_t bits = Q4 ? largest4(pg, vs4) : scale_bits(pg, vs);
+          const int e = Q4 ? q4_frame(bits) : exp_above(bits);
+          if (bits) vexp = vexp_set ? max(vexp, e) : e;
           if (bits) vexp_set = true;
-          put8(sm.v[blk & 1], true, rv, pg >= 0 ? frame_scale(vs, 7 - vexp) : 0.0f);
+          if constexpr (Q4) put4(sm.v[blk & 1], true, rv, vs4, pg, vexp);
+          else put8(sm.v[blk & 1], true, rv, pg >= 0 ? frame_scale(vs, 7 - vexp) : 0.0f);
         }
       };
       auto load_k = [&](int blk, int pg) {
-        if constexpr (Q8) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
+        if constexpr (Q4) load4(blk, pg, a.p.k, a.p.k4, rk, ks4);
+        else if constexpr (REG) load8(blk, pg, a.p.k, a.p.ks, rk, ks);
         else if constexpr (IMG) dma_block<D, NW>(sm.k[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D));
         else dma_pages<D, NW>(sm.k[blk & 1], wave, false, a.p, g, blk, pg);
       };
       auto load_v = [&](int blk, int pg) {
-        if constexpr (Q8) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
+        if constexpr (Q4) load4(blk, pg, a.p.v, a.p.v4, rv, vs4);
+        else if constexpr (REG) load8(blk, pg, a.p.v, a.p.vs, rv, vs);
         else if constexpr (IMG) dma_block<D, NW>(sm.v[blk & 1], wave, a.img + (first + blk) * (2 * kBK * D) + kBK * D);
         else dma_pages<D, NW>(sm.v[blk & 1], wave, true, a.p, g, blk, pg);
       };
@@ -1713,15 +1796,18 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       int p0 = pages(b_lo), p1 = pages(b_lo + 1), p2 = pages(b_lo + 2), p3 = pages(b_lo + 3);
       load_k(b_lo, p0);
       load_v(b_lo, p0);
-      if constexpr (Q8) {
+      if constexpr (REG) {
         v4u rn[NC];
-        float sn;
-        load8(b_lo + 1, p1, a.p.k, a.p.ks, rn, sn);
+        float sn = 0;
+        uint32_t sn4 = 0;
+        if constexpr (Q4) load4(b_lo + 1, p1, a.p.k, a.p.k4, rn, sn4);
+        else load8(b_lo + 1, p1, a.p.k, a.p.ks, rn, sn);
         store_k(b_lo, p0);
         store_v(b_lo, p0);
 #pragma unroll
         for (int i = 0; i < NC; ++i) rk[i] = rn[i];
         ks = sn;
+        ks4 = sn4;
         store_k(b_lo + 1, p1);
         load_k(b_lo + 2, p2);
         load_v(b_lo + 1, p1);
@@ -1730,7 +1816,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         dma_wait();
       }
       int f_cur = vexp - 7;
-      if constexpr (Q8) frame = f_cur;  // O is 0 still: no rescaling, by what may be no fp32 number
+      if constexpr (REG) frame = f_cur;  // O is 0 still: no rescaling, by what may be no fp32 number
       __syncthreads();
       ImageBlock head = {};
       if constexpr (IMG) head = a.img_heads[first + b_lo];
@@ -1751,7 +1837,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
           }
           mine = put_max(x, c);
         }
-        if constexpr (!Q8) dma_wait();  // this wave's part of V(blk) and K(blk + 1)
+        if constexpr (!REG) dma_wait();  // this wave's part of V(blk) and K(blk + 1)
         __syncthreads();
         if (!H16 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
           for (int i = tid; i < kBK * (D / 8); i += NT)
@@ -1759,7 +1845,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
               *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
         }
         const int f_now = f_cur;
-        if constexpr (Q8) {
+        if constexpr (REG) {
           if (blk + 2 < b_hi) store_k(blk + 2, p2);
           if (blk + 1 < b_hi) store_v(blk + 1, p1);
           f_cur = vexp - 7;
@@ -1775,7 +1861,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         p3 = pages(blk + 4);
         v4u pb[4];
         if (live) {
-          if constexpr (Q8) rescale(f_now);
+          if constexpr (REG) rescale(f_now);
           softmax(HT{}, x, c, mine);
         }
         __syncthreads();
@@ -1858,20 +1944,30 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 // img_blocks (the caller's bound was too low) have none; sequences without new tokens need none. A wave takes the frame
 // of one block's V (5 us; of all of them in a workgroup per (sequence, KV head), 32768 tokens took 20). The
 // image of 32768 tokens, 8 heads of 128, takes 35 to 47 us, 4.3 to 5.6 TB/s.
+template <int D, int P>
 __global__ __launch_bounds__(kThreads) void page_frame_kernel(AttnArgs a) {
   const int blk = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), g = blockIdx.y, b = blockIdx.z;
   const Seq s = seq_of(a, b);
   const int blocks = (s.ctx + kBK - 1) / kBK, pos = blk * kBK + (threadIdx.x & 63);
   if (s.n == 0 || blk >= blocks || blocks > a.img_blocks) return;
   const int64_t row = pos < s.ctx ? row_of(a.p, b, g, pos) : -1;
-  const float vs = row >= 0 ? a.p.vs[row] : 0.0f;
-  const uint32_t m = od_wave_umax_dpp(vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u);
+  uint32_t bits = 0;
+  if constexpr (P == kInt4) {
+    uint32_t w[D / 64] = {};
+    if (row >= 0) q4_row_scales<D>(a.p.v4, row, w);
+    bits = q4_largest(w) << 16;
+  } else {
+    const float vs = row >= 0 ? a.p.vs[row] : 0.0f;
+    bits = vs < INFINITY && vs > 0 ? __float_as_uint(vs) : 0u;
+  }
+  const uint32_t m = od_wave_umax_dpp(bits);
   if ((threadIdx.x & 63) == 0)
     a.img_heads[((int64_t)b * a.p.Hkv + g) * a.img_blocks + blk].v_bits = m;
 }
-template <int D>
+template <int D, int P>
 __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
-  constexpr int CPK = D / 16, CH = kBK * CPK, NC = 2 * CH / kThreads;
+  constexpr bool Q4 = P == kInt4;
+  constexpr int CPK = D / (Q4 ? 32 : 16), CH = kBK * CPK, NC = 2 * CH / kThreads;
   const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
   const Seq s = seq_of(a, b);
   const int blocks = (s.ctx + kBK - 1) / kBK;
@@ -1880,14 +1976,25 @@ __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
   const int pos = blk * kBK + lane;
   const int64_t mine = pos < s.ctx ? row_of(a.p, b, g, pos) : -1, row = max(mine, (int64_t)0);
   const bool on = mine >= 0;  // a key that is not there: the pool's first row, times 0
-  const float ks = a.p.ks[row], vs = a.p.vs[row];
+  float ks = 0, vs = 0;       // int8
+  uint32_t k_bits;
+  if constexpr (Q4) {
+    uint32_t w[D / 64];
+    q4_row_scales<D>(a.p.k4, row, w);
+    k_bits = q4_largest(w);
+  } else {
+    ks = a.p.ks[row], vs = a.p.vs[row];
+    k_bits = ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u;
+  }
   const uint64_t seen = __builtin_amdgcn_ballot_w64(on);
-  const int kexp = exp_above(od_wave_umax_dpp(on && ks < INFINITY && ks > 0 ? __float_as_uint(ks) : 0u));
+  const uint32_t km = od_wave_umax_dpp(on ? k_bits : 0u);
+  const int kexp = Q4 ? q4_frame(km) : exp_above(km);
   // the largest of all blocks, by every wave
   uint32_t vm = 0;
 #pragma unroll 4
   for (int i = lane; i < blocks; i += 64) vm = max(vm, a.img_heads[at - blk + i].v_bits);
-  const int vexp = exp_above(od_wave_umax_dpp(vm));
+  vm = od_wave_umax_dpp(vm);
+  const int vexp = Q4 ? q4_frame(vm >> 16) : exp_above(vm);
   const float kf = on ? frame_scale(ks, 7 - kexp) : 0.0f, vf = on ? frame_scale(vs, 7 - vexp) : 0.0f;
   if (threadIdx.x == 0) {
     a.img_heads[at].seen = seen;
@@ -1895,28 +2002,31 @@ __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
     if (blk == 0) a.img_vexp[b * a.p.Hkv + g] = vexp;
   }
   v4u r[NC];
+  uint32_t rs[NC];  // 4 bits: the chunks' scales
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int cid = i * kThreads + threadIdx.x, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
     const int64_t from = ((int64_t)__shfl((int)(row >> 32), key, 64) << 32) | (uint32_t)__shfl((int)row, key, 64);
     r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(static_cast<const char*>(side ? a.p.v : a.p.k) +
-                                                                  from * D + 16 * ch));
+                                                                  from * (16 * CPK) + 16 * ch));
+    if constexpr (Q4) rs[i] = (side ? a.p.v4 : a.p.k4)[from * CPK + ch];
   }
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int cid = i * kThreads + threadIdx.x, side = cid / CH, key = cid % CH / CPK, ch = cid % CPK;
     uint16_t* dst = a.img + at * (2 * kBK * D) + side * (kBK * D);
-    v4u lo, hi;
-    i8x16_scaled(r[i], __shfl(side ? vf : kf, key, 64), lo, hi);
-    const int o0 = side ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
-    const int o1 = side ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
-    *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
-    *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
+    if constexpr (Q4) {
+      q4_put<D>(dst, side, key, ch, r[i], f16_scale((seen >> key) & 1 ? rs[i] : 0u, 7 - (side ? vexp : kexp)));
+    } else {
+      v4u lo, hi;
+      i8x16_scaled(r[i], __shfl(side ? vf : kf, key, 64), lo, hi);
+      const int o0 = side ? key * D + (tv_chunk<D>(key, 2 * ch) << 3) : tk_off<D>(key, 2 * ch);
+      const int o1 = side ? key * D + (tv_chunk<D>(key, 2 * ch + 1) << 3) : tk_off<D>(key, 2 * ch + 1);
+      *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
+      *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
+    }
   }
 }
-
-// A launch has fewer than 2^32 threads: workgroups of 256.
-constexpr int64_t kMaxGroups = (1 << 24) - 1;
 
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
@@ -1928,7 +2038,8 @@ struct Plan {
   int64_t part, vexp, heads, img;
   int64_t floats() const { return part + vexp + heads + img; }
 };
-Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx, bool q8) {
+Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_ctx, int format) {
+  const bool q8 = format == OD_PAGE_INT8, q4 = format == OD_PAGE_INT4;
   Plan p;
   // hints past any call's own size say nothing; below 2^30 no split begins past the positions an int holds
   max_new = max_new < N ? max_new : N;
@@ -1946,6 +2057,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   const int64_t few = B * Hkv * ((slots + 31) / 32);
   const int64_t always = q8 && D <= 128 && Hkv < (1 << 15) ? 64 : 32;  // (a grid has 65535 rows)
   p.stream = slots <= always || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
+  if (q4) p.stream = false;
   p.ct = slots <= 16 ? 1 : 2;
   // workgroups without splits for tiles of spt slots: every sequence's, but no more than the tokens make
   auto wgs_of = [&](int64_t spt) {
@@ -2015,7 +2127,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // 256-wide heads, 4 ragged 900 over 6000 402, 284; 1 x 256 over 6000 (3000 blocks in all) 82, 76; 8 x 64 (2 tiles)
   // 115, 121; heads of 128, 8 x 256 over 6000 (4 tiles) 217, 183, 8 x 128 (2 tiles) 150, 139, 4 x 1024 over 1000 (8000
   // blocks) 85, 87, 4 x 256 over 6000 (12000) 152, 115.
-  p.img_blocks = !p.stream && q8 && tiles >= 4 && wgs * keys * D / spt > 5 << 10 ? keys : 0;
+  p.img_blocks = !p.stream && (q8 || q4) && tiles >= 4 && wgs * keys * D / spt > 5 << 10 ? keys : 0;
   if (p.img_blocks * B * Hkv > (1ll << 28) / (kBK * D)) p.img_blocks = 0;
   p.vexp = p.img_blocks ? (B * Hkv + 3) / 4 * 4 : 0;
   p.heads = p.img_blocks * B * Hkv * 4;
@@ -2025,26 +2137,6 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
 
 // slots of a KV head, so that an int holds them and a stride of tiles past them
 constexpr int64_t kMaxSlots = 0x3fff0000;
-
-bool aligned4(const void* p) { return (((uintptr_t)p) & 3u) == 0; }
-
-// Checks of the pages that every entry point makes; fills P.
-int paged_args(Paged& P, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
-               int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
-               const int32_t* start, const int32_t* ctx, int64_t B, int64_t N, int64_t Hkv, int64_t D) {
-  if (B < 0 || N < 0 || Hkv < 1 || n_pages < 0 || cols < 0 || ld_table < cols) return OD_ERR_SHAPE;
-  if (D != 64 && D != 128 && D != 256) return OD_ERR_UNSUPPORTED;
-  if (page < 16 || page > (1 << 20) || (page & (page - 1))) return OD_ERR_UNSUPPORTED;
-  if (B > (1 << 24) || N > 0x3fffffff || cols > 0x3fffffff || Hkv > 65535 || n_pages > 0x7fffffff) return OD_ERR_SHAPE;
-  if (cols * page > 0x7fffff00ll) return OD_ERR_SHAPE;
-  if (!k_scale != !v_scale) return OD_ERR_NULL;
-  if (n_pages > 0 && (!k_pages || !v_pages)) return OD_ERR_NULL;
-  if (!od_aligned16(k_pages) || !od_aligned16(v_pages) || !aligned4(k_scale) || !aligned4(v_scale)) return OD_ERR_ALIGN;
-  P = Paged{const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<float*>(k_scale),
-            const_cast<float*>(v_scale), table, start, ctx, ld_table, n_pages, (int)cols, __builtin_ctzll(page), (int)B,
-            (int)N, (int)Hkv};
-  return OD_OK;
-}
 
 // A launch with more than 64 KB of LDS, which a kernel has to be allowed once per device.
 template <auto* Kernel>
@@ -2066,22 +2158,15 @@ int launch_tiles(const AttnArgs& a, unsigned groups, hipStream_t st) {
   return launch_big<&paged_tile_kernel<D, SRC, NW>>(a, groups, NW * 64, (int)sizeof(TSmem<D, NW>), st);
 }
 
-template <class F>
-void by_head_dim(int64_t D, F&& f) {
-  if (D == 64) f(std::integral_constant<int, 64>{});
-  else if (D == 128) f(std::integral_constant<int, 128>{});
-  else f(std::integral_constant<int, 256>{});
-}
-
 }  // namespace
 
-extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh,
-                              void* k_pages, float* k_scale, void* v_pages, float* v_scale, int64_t n_pages,
-                              int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
-                              const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D,
-                              od_stream_t stream) {
+extern "C" int od_page_append_ex(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh,
+                                 int format, void* k_pages, void* k_scale, void* v_pages, void* v_scale, int64_t n_pages,
+                                 int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                                 const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D,
+                                 od_stream_t stream) {
   AppendArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+  if (const int rc = paged_args(a.p, format, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
                                 cols, start, ctx_len, B, N, Hkv, D))
     return rc;
   if (B == 0 || N == 0 || cols == 0 || n_pages == 0) return OD_OK;
@@ -2102,23 +2187,33 @@ extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const
   by_head_dim(D, [&](auto DC) {
     constexpr int DD = decltype(DC)::value;
     const dim3 grid((unsigned)blocks);
-    if (k_scale) page_append_kernel<DD, true><<<grid, dim3(kThreads), 0, (hipStream_t)stream>>>(a);
-    else page_append_kernel<DD, false><<<grid, dim3(kThreads), 0, (hipStream_t)stream>>>(a);
+    by_format(format, [&](auto PC) {
+      page_append_kernel<DD, decltype(PC)::value><<<grid, dim3(kThreads), 0, (hipStream_t)stream>>>(a);
+    });
   });
   return od_launch_status();
 }
 
-extern "C" int od_page_read(const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
-                            int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
-                            const int32_t* length, int64_t B, int64_t T, int64_t Hkv, int64_t D, int form, void* k_out,
-                            float* ks_out, void* v_out, float* vs_out, od_stream_t stream) {
+extern "C" int od_page_append(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v, int64_t svt, int64_t svh,
+                              void* k_pages, float* k_scale, void* v_pages, float* v_scale, int64_t n_pages,
+                              int64_t page, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                              const int32_t* ctx_len, int64_t B, int64_t N, int64_t Hkv, int64_t D,
+                              od_stream_t stream) {
+  return od_page_append_ex(k, skt, skh, v, svt, svh, k_scale || v_scale ? OD_PAGE_INT8 : OD_PAGE_BF16, k_pages, k_scale,
+                           v_pages, v_scale, n_pages, page, table, ld_table, cols, start, ctx_len, B, N, Hkv, D, stream);
+}
+
+extern "C" int od_page_read_ex(int format, const void* k_pages, const void* k_scale, const void* v_pages, const void* v_scale,
+                               int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
+                               const int32_t* length, int64_t B, int64_t T, int64_t Hkv, int64_t D, int form, void* k_out,
+                               float* ks_out, void* v_out, float* vs_out, od_stream_t stream) {
   ReadArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+  if (const int rc = paged_args(a.p, format, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
                                 cols, nullptr, length, B, 0, Hkv, D))
     return rc;
   if (T < 0 || T > 0x3fffffff) return OD_ERR_SHAPE;
   if (form != OD_READ_BF16 && form != OD_READ_FP32 && form != OD_READ_INT8) return OD_ERR_UNSUPPORTED;
-  if (form == OD_READ_INT8 && !k_scale) return OD_ERR_UNSUPPORTED;
+  if (form == OD_READ_INT8 && format != OD_PAGE_INT8) return OD_ERR_UNSUPPORTED;
   if (B == 0 || T == 0) return OD_OK;
   if (!length || !k_out || !v_out || (cols > 0 && !table)) return OD_ERR_NULL;
   if (form == OD_READ_INT8 && (!ks_out || !vs_out)) return OD_ERR_NULL;
@@ -2135,26 +2230,38 @@ extern "C" int od_page_read(const void* k_pages, const float* k_scale, const voi
     constexpr int DD = decltype(DC)::value;
     const dim3 grid((unsigned)(B * Hkv * tiles)), block(kThreads);
     hipStream_t st = (hipStream_t)stream;
-    if (k_scale) {
-      if (form == OD_READ_BF16) page_read_kernel<DD, true, kReadBf16><<<grid, block, 0, st>>>(a);
-      else if (form == OD_READ_FP32) page_read_kernel<DD, true, kReadF32><<<grid, block, 0, st>>>(a);
-      else page_read_kernel<DD, true, kReadI8><<<grid, block, 0, st>>>(a);
-    } else {
-      if (form == OD_READ_BF16) page_read_kernel<DD, false, kReadBf16><<<grid, block, 0, st>>>(a);
-      else page_read_kernel<DD, false, kReadF32><<<grid, block, 0, st>>>(a);
-    }
+    by_format(format, [&](auto PC) {
+      constexpr int P = decltype(PC)::value;
+      if (form == OD_READ_BF16) page_read_kernel<DD, P, kReadBf16><<<grid, block, 0, st>>>(a);
+      else if (form == OD_READ_FP32) page_read_kernel<DD, P, kReadF32><<<grid, block, 0, st>>>(a);
+      else if constexpr (P == kInt8) page_read_kernel<DD, P, kReadI8><<<grid, block, 0, st>>>(a);
+    });
   });
   return od_launch_status();
 }
 
-extern "C" int od_paged_attn_ws_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
-                                   int64_t max_ctx, int int8_pages, int64_t* ws_floats) {
+extern "C" int od_page_read(const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
+                            int64_t n_pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t cols,
+                            const int32_t* length, int64_t B, int64_t T, int64_t Hkv, int64_t D, int form, void* k_out,
+                            float* ks_out, void* v_out, float* vs_out, od_stream_t stream) {
+  return od_page_read_ex(k_scale || v_scale ? OD_PAGE_INT8 : OD_PAGE_BF16, k_pages, k_scale, v_pages, v_scale, n_pages, page,
+                         table, ld_table, cols, length, B, T, Hkv, D, form, k_out, ks_out, v_out, vs_out, stream);
+}
+
+extern "C" int od_paged_attn_ws_ex(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                                   int64_t max_ctx, int format, int64_t* ws_floats) {
   if (!ws_floats) return OD_ERR_NULL;
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
   if (Hq % Hkv || (D != 64 && D != 128 && D != 256)) return OD_ERR_UNSUPPORTED;
+  if (format != OD_PAGE_BF16 && format != OD_PAGE_INT8 && format != OD_PAGE_INT4) return OD_ERR_UNSUPPORTED;
   if (B > 65535 || Hq > 65535 || N > kMaxSlots / (Hq / Hkv)) return OD_ERR_SHAPE;
-  *ws_floats = B == 0 || N == 0 ? 0 : plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, int8_pages != 0).floats();
+  *ws_floats = B == 0 || N == 0 ? 0 : plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, format).floats();
   return OD_OK;
+}
+
+extern "C" int od_paged_attn_ws_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                                   int64_t max_ctx, int int8_pages, int64_t* ws_floats) {
+  return od_paged_attn_ws_ex(B, N, Hq, Hkv, D, max_new, max_ctx, int8_pages ? OD_PAGE_INT8 : OD_PAGE_BF16, ws_floats);
 }
 
 extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
@@ -2166,15 +2273,15 @@ extern "C" int od_paged_attn_ws(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, i
   return OD_OK;
 }
 
-extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
-                             const uint16_t* v, int64_t svt, int64_t svh, const void* k_pages, const float* k_scale,
-                             const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page,
-                             const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
-                             const int32_t* ctx_len, const int32_t* row_begin, uint16_t* out, int64_t sot, int64_t soh,
-                             float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
-                             int64_t max_ctx, float scale, float* ws, int64_t ws_floats, od_stream_t stream) {
+extern "C" int od_paged_attn_ex(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
+                                const uint16_t* v, int64_t svt, int64_t svh, int format, const void* k_pages,
+                                const void* k_scale, const void* v_pages, const void* v_scale, int64_t n_pages, int64_t page,
+                                const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                                const int32_t* ctx_len, const int32_t* row_begin, uint16_t* out, int64_t sot, int64_t soh,
+                                float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                                int64_t max_ctx, float scale, float* ws, int64_t ws_floats, od_stream_t stream) {
   AttnArgs a;
-  if (const int rc = paged_args(a.p, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
+  if (const int rc = paged_args(a.p, format, k_pages, k_scale, v_pages, v_scale, n_pages, page, table, ld_table,
                                 cols, start, ctx_len, B, N, Hkv, D))
     return rc;
   if (Hq < 1 || Hq > 65535 || B > 65535 || max_new < 0 || max_ctx < 0) return OD_ERR_SHAPE;
@@ -2204,7 +2311,7 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
   a.Hq = (int)Hq;
   a.rep = (int)(Hq / Hkv);
   a.scale_log2 = scale * kLog2e;
-  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, k_scale != nullptr);
+  const Plan p = plan_of(B, N, Hq, Hkv, D, max_new, max_ctx, format);
   if (p.floats()) {
     if (!ws) return OD_ERR_NULL;
     if (ws_floats < p.floats()) return OD_ERR_SHAPE;
@@ -2243,21 +2350,25 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
       else paged_stream_kernel<DD, Q8, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
     };
     if (p.stream) {
-      if (k_scale) stream(std::true_type{});
+      if (format == OD_PAGE_INT8) stream(std::true_type{});
       else stream(std::false_type{});
-    } else if (!k_scale) {
+    } else if (format == OD_PAGE_BF16) {
       tiles(std::integral_constant<int, kBf16>{});
     } else {
-      if (p.img_blocks) {
-        const dim3 grid((unsigned)p.img_blocks, (unsigned)Hkv, (unsigned)B);
-        page_frame_kernel<<<dim3((unsigned)((p.img_blocks + 3) / 4), grid.y, grid.z), dim3(kThreads), 0, st>>>(a);
-        page_image_kernel<DD><<<grid, dim3(kThreads), 0, st>>>(a);
-        tiles(std::integral_constant<int, kImage>{});
-        a.rest = true;
-      }
-      // the sequences without an image, if the table can hold any
-      if (rc == OD_OK && p.img_blocks * kBK < ((int64_t)a.p.cols << a.p.shift)) tiles(std::integral_constant<int,
-          kInt8>{});
+      by_format(format, [&](auto PC) {
+        constexpr int P = decltype(PC)::value;
+        if constexpr (P != kBf16) {
+          if (p.img_blocks) {
+            const dim3 grid((unsigned)p.img_blocks, (unsigned)Hkv, (unsigned)B);
+            page_frame_kernel<DD, P><<<dim3((unsigned)((p.img_blocks + 3) / 4), grid.y, grid.z), dim3(kThreads), 0, st>>>(a);
+            page_image_kernel<DD, P><<<grid, dim3(kThreads), 0, st>>>(a);
+            tiles(std::integral_constant<int, kImage>{});
+            a.rest = true;
+          }
+          // the sequences without an image, if there can be any
+          if (rc == OD_OK && (p.img_blocks == 0 || p.img_blocks * kBK < ((int64_t)a.p.cols << a.p.shift))) tiles(PC);
+        }
+      });
     }
     if (rc == OD_OK && p.nsplit > 1) {
       // groups when a workgroup has one slot; slots when a slot has one group
@@ -2268,4 +2379,16 @@ extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const 
     }
   });
   return rc == OD_OK ? od_launch_status() : rc;
+}
+
+extern "C" int od_paged_attn(const uint16_t* q, int64_t sqt, int64_t sqh, const uint16_t* k, int64_t skt, int64_t skh,
+                             const uint16_t* v, int64_t svt, int64_t svh, const void* k_pages, const float* k_scale,
+                             const void* v_pages, const float* v_scale, int64_t n_pages, int64_t page,
+                             const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* start,
+                             const int32_t* ctx_len, const int32_t* row_begin, uint16_t* out, int64_t sot, int64_t soh,
+                             float* lse, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                             int64_t max_ctx, float scale, float* ws, int64_t ws_floats, od_stream_t stream) {
+  return od_paged_attn_ex(q, sqt, sqh, k, skt, skh, v, svt, svh, k_scale || v_scale ? OD_PAGE_INT8 : OD_PAGE_BF16, k_pages,
+                          k_scale, v_pages, v_scale, n_pages, page, table, ld_table, cols, start, ctx_len, row_begin, out, sot,
+                          soh, lse, B, N, Hq, Hkv, D, max_new, max_ctx, scale, ws, ws_floats, stream);
 }

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib, kernels
 from .kv_cache import GDNState, HybridState, Int8KVCache, StateKV
-from .paged_cache import PagedStates
+from .paged_cache import PagedKVCache, PagedStates
 
 
 @dataclass
@@ -297,7 +297,8 @@ class DenseDecoder:
     # ---------------------------------------------------------------- forward
     def _attn_in(self, li: int, h: torch.Tensor, ws: dict, pos: torch.Tensor, append=None) -> torch.Tensor:
         """RMSNorm + quantize, W8A8 QKV GEMM, q/k norm + RoPE (in place): the layer's qkv (M, qkv_out) bf16.
-        append = (B, S, K cache, V cache): the same pass also appends the tokens' int8 K/V to the caches."""
+        append = (B, S, K cache, V cache): the same pass also appends the tokens' int8 K/V to the caches; append = (PagedKVCache,
+        table, start, ctx): to its pages."""
         cfg, L = self.cfg, self.layers[li]
         kernels.rmsnorm_quant(h, L["ln1"], cfg.eps, L["qkv"].inv_s, ws["xq"][:, :cfg.hidden], ws["sx"],
                               offset=cfg.norm_offset)
@@ -305,6 +306,9 @@ class DenseDecoder:
         if append is None:
             kernels.qk_norm_rope(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, L["q_norm"], L["k_norm"], self.cos,
                                  self.sin, pos, cfg.eps, cfg.rotary_dims, cfg.norm_offset)
+        elif isinstance(append[0], PagedKVCache):
+            kernels.qk_norm_rope_page_append(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, L["q_norm"], L["k_norm"], self.cos,
+                                             self.sin, pos, cfg.eps, *append, rot_dim=cfg.rotary_dims, offset=cfg.norm_offset)
         else:
             B, S, cache_k, cache_v = append
             kernels.qk_norm_rope_kv_append(qkv, B, S, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, L["q_norm"],
@@ -480,9 +484,10 @@ class DenseDecoder:
 
     # ---------------------------------------------------------------- paged states
     def new_paged_states(self, batch: int, n_pages: int, max_tokens: int, page: int = 64,
-                         quantized: bool = True) -> PagedStates:
+                         quantized: bool | str = True) -> PagedStates:
         """`batch` empty states in pages (n_pages pages of `page` tokens per layer, at most max_tokens tokens a state): each
-        has its own length, takes pages as it grows (extend) and gives them back (PagedStates.release)."""
+        has its own length, takes pages as it grows (extend) and gives them back (PagedStates.release). quantized: int8 pages
+        (True), bf16 ones (False) or 4 bits a value ("int4")."""
         if self.hybrid:
             raise ValueError("paged states hold attention layers only (a Gated DeltaNet layer's state has no tokens)")
         cfg = self.cfg
@@ -504,12 +509,11 @@ class DenseDecoder:
         self._embed(ids, h)
         max_ctx = max(states.lengths)
         for li in range(len(self.layers)):
-            qkv = self._attn_in(li, h, ws, pos)
+            # what is written lies behind the ctx tokens that the attention reads
+            qkv = self._attn_in(li, h, ws, pos, append=(states[li], states.table, start, states.ctx) if write else None)
             q, k, v = (qkv[:, a * D:b * D].view(N, b - a, D) for a, b in ((0, Hq), (Hq, Hq + Hk), (Hq + Hk, Hq + 2 * Hk)))
             kernels.paged_attn(q, k, v, states[li], states.table, start, states.ctx, D ** -0.5, row_begin=row_begin,
                                max_new=max_new, max_ctx=max_ctx, out=ws["attn"].view(N, Hq, D))
-            if write:
-                kernels.page_append(k, v, states[li], states.table, start, states.ctx)
             self._attn_out_mlp(li, h, mid, ws)
         return h
 

@@ -1032,7 +1032,7 @@ def gdn_norm_quant(o: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
 
 # ------------------------------------------------------------------------------------------------ paged K/V cache
 def _paged(cache, table, start, ctx_len, name):
-    """The arguments of a paged batch that every entry point takes, checked: the sequence count, (pages, table) and the table
+    """The arguments of a paged batch that every entry point takes, checked: the sequence count, (format, pages, table) and the table
     that they point to (a copy of rows that share memory: hold it until the call is made)."""
     k, i32 = cache.k, torch.int32
     B = ctx_len.numel()
@@ -1045,7 +1045,7 @@ def _paged(cache, table, start, ctx_len, name):
     cols = table.shape[1]
     if B > 1 and table.stride(0) < cols:
         table = table.contiguous()
-    return B, (k.data_ptr(), ptr(cache.k_scale), cache.v.data_ptr(), ptr(cache.v_scale), k.shape[0], k.shape[2],
+    return B, (cache.format, k.data_ptr(), ptr(cache.k_scale), cache.v.data_ptr(), ptr(cache.v_scale), k.shape[0], k.shape[2],
                table.data_ptr(), table.stride(0) if B > 1 else cols, cols), table
 
 
@@ -1095,24 +1095,82 @@ class _OnDevice:
 
 def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, start: torch.Tensor,
                 ctx_len: torch.Tensor) -> None:
-    """od_page_append: the new tokens' k and v (N, Hkv, D) bf16 into the pages of a PagedKVCache, quantized per (token,
-    head) where the pages are int8 (the bytes of kv_quant_append). table int32 (B, pages per sequence); start int32
+    """od_page_append_ex: the new tokens' k and v (N, Hkv, D) bf16 into the pages of a PagedKVCache, quantized per (token,
+    head) where the pages are int8 (the bytes of kv_quant_append), per 32 values of one where they hold 4 bits. table int32 (B, pages per sequence); start int32
     (B + 1,): sequence b's tokens are the rows start[b] .. start[b + 1] - 1; ctx_len int32 (B,): the tokens it holds
     before, which is where they go. Tokens without a page are not written. The lengths stay: advance them once every layer
     has its tokens."""
     _one_device("page_append", k, v, cache.k, cache.v, table, start, ctx_len)
     B, pages, table = _paged(cache, table, start, ctx_len, "page_append")
-    _, H, _, D = cache.k.shape
+    H, D = cache.k.shape[1], cache.head_dim
     N = k.shape[0]
     k, ka = _new_rows(k, N, H, D, "page_append: k")
     v, va = _new_rows(v, N, H, D, "page_append: v")
     with _OnDevice(k):
-        check(lib().od_page_append(*ka, *va, *pages,
-                                   start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
+        check(lib().od_page_append_ex(*ka, *va, *pages,
+                                      start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
+
+
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor at a multiple of 16 bytes, as the kernels' vector loads need it (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def qk_norm_rope_page_append(qkv: torch.Tensor, n_heads_q: int, n_heads_k: int, D: int, q_w, k_w, cos_t, sin_t, pos,
+                             eps: float, cache, table: torch.Tensor, start: torch.Tensor, ctx_len: torch.Tensor,
+                             rot_dim: int | None = None, offset: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """od_qk_norm_rope_page_append: qk_norm_rope on qkv (N, >= (Hq + 2 Hk) D) and page_append of the rotated keys and the values
+    in one pass (the results of the two calls). The rotated q and k heads go to out (N, (Hq + Hk) D) bf16, or with out None back
+    into qkv (every row, also those of no sequence); cache, table, start and ctx_len as page_append. Returns out, or qkv."""
+    _one_device("qk_norm_rope_page_append", qkv, q_w, k_w, cos_t, sin_t, pos, cache.k, cache.v, table, start, ctx_len, out)
+    _lib.bf16_bits(qkv)
+    B, pages, table = _paged(cache, table, start, ctx_len, "qk_norm_rope_page_append")
+    rot_dim = D if rot_dim is None else rot_dim
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads_q + 2 * n_heads_k) * D or \
+            (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+        raise ValueError(f"qk_norm_rope_page_append: qkv must be (N, >= {(n_heads_q + 2 * n_heads_k) * D}) with contiguous rows")
+    if cache.k.shape[1] != n_heads_k or cache.head_dim != D:
+        raise ValueError(f"qk_norm_rope_page_append: {n_heads_k} heads of {D} into pages of {cache.k.shape[1]} heads of "
+                         f"{cache.head_dim}")
+    N, width = qkv.shape[0], (n_heads_q + n_heads_k) * D
+    q_w, k_w = (_aligned16(_vec(w, D, name)) for w, name in ((q_w, "q_w"), (k_w, "k_w")))
+    _lib.bf16_bits(cos_t)
+    _lib.bf16_bits(sin_t)
+    _rope_tables_ok(cos_t, sin_t, D, rot_dim, "qk_norm_rope_page_append")
+    cos_t, sin_t = _aligned16(cos_t), _aligned16(sin_t)
+    if pos.dtype != torch.int32 or pos.numel() != N:
+        raise ValueError("qk_norm_rope_page_append: pos must be int32 (N,)")
+    pos = pos.contiguous()
+    ok = qkv.data_ptr() % 16 == 0 and (N < 2 or qkv.stride(0) % 8 == 0)
+    x = qkv if ok else qkv.clone(memory_format=torch.contiguous_format)
+    if not ok and x.stride(0) % 8:  # an odd number of columns: rows of their own width
+        x = torch.empty(N, -(-qkv.shape[1] // 8) * 8, dtype=qkv.dtype, device=qkv.device)
+        x[:, :qkv.shape[1]] = qkv
+    if out is None:
+        dst = x
+    else:
+        _check_out(out, (N, width), qkv.device, "qk_norm_rope_page_append")
+        fits = out.data_ptr() % 16 == 0 and (N < 2 or (out.stride(0) % 8 == 0 and out.stride(0) >= width))
+        dst = out if fits else torch.empty(N, width, dtype=out.dtype, device=out.device)
+    ld, ldo = (t.stride(0) if N > 1 else t.shape[1] for t in (x, dst))
+    with _OnDevice(qkv):
+        check(lib().od_qk_norm_rope_page_append(x.data_ptr(), -(-ld // 8) * 8, dst.data_ptr(), -(-ldo // 8) * 8, n_heads_q,
+                                                rot_dim, int(bool(offset)), ptr(q_w), ptr(k_w), ptr(cos_t), ptr(sin_t),
+                                                cos_t.shape[0], ptr(pos), float(eps), *pages, start.data_ptr(),
+                                                ctx_len.data_ptr(), B, N, n_heads_k, D, stream_of(qkv)),
+              "od_qk_norm_rope_page_append")
+    if out is None:
+        if x is not qkv:
+            qkv[:, :width].copy_(x[:, :width])
+        return qkv
+    if dst is not out:
+        out.copy_(dst)
+    return out
 
 
 def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: torch.dtype = torch.bfloat16):
-    """od_page_read: the first length[b] (at most T) tokens of every sequence as dense (B, Hkv, T, D) K and V, zeros behind
+    """od_page_read_ex: the first length[b] (at most T) tokens of every sequence as dense (B, Hkv, T, D) K and V, zeros behind
     them. dtype bfloat16 or float32: the values q * s, one fp32 product (Int8Tensor.dequantize rounds the scale to bf16
     first). int8 (int8 pages only): two Int8Tensors, the stored bytes and scales (scales (B, Hkv, T, 1))."""
     _one_device("page_read", cache.k, cache.v, table, length)
@@ -1120,17 +1178,17 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
     if T < 0:
         raise ValueError(f"page_read: T must not be negative, got {T}")
     forms = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
-    if dtype not in forms or (dtype == torch.int8 and cache.k_scale is None):
+    if dtype not in forms or (dtype == torch.int8 and cache.k.dtype != torch.int8):
         raise TypeError(f"page_read: cannot read {cache.k.dtype} pages as {dtype}")
-    _, H, _, D = cache.k.shape
+    H, D = cache.k.shape[1], cache.head_dim
     dev = cache.k.device
     k, v = (torch.empty(B, H, T, D, dtype=dtype, device=dev) for _ in range(2))
     ks = vs = None
     if dtype == torch.int8:
         ks, vs = (torch.empty(B, H, T, dtype=torch.float32, device=dev) for _ in range(2))
     with _OnDevice(k):
-        check(lib().od_page_read(*pages, length.data_ptr(), B, T, H, D, forms[dtype], k.data_ptr(), ptr(ks), v.data_ptr(),
-                                 ptr(vs), stream_of(k)), "od_page_read")
+        check(lib().od_page_read_ex(*pages, length.data_ptr(), B, T, H, D, forms[dtype], k.data_ptr(), ptr(ks), v.data_ptr(),
+                                    ptr(vs), stream_of(k)), "od_page_read")
     if ks is None:
         return k, v
     from .quant import Int8Tensor
@@ -1138,11 +1196,14 @@ def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: t
 
 
 _PAGED_WS: dict = {}
+# PagedKVCache's `quantized` -> OD_PAGE_* (include/od_mi355x.h)
+PAGE_FORMATS = {False: 0, True: 1, "int8": 1, "int4": 2}
+_FORMAT_NAMES = (False, True, "int4")
 
 
 def paged_attn_workspace_floats(B: int, N: int, Hq: int, Hkv: int, D: int, max_new: int, max_ctx: int, device,
-                                quantized: bool = True) -> int:
-    """Floats of od_paged_attn's workspace for these sizes and pages on the device (0: none)."""
+                                quantized: bool | str = True) -> int:
+    """Floats of od_paged_attn_ex's workspace for these sizes and pages (PagedKVCache's `quantized`) on the device (0: none)."""
     key = (device.index, B, N, Hq, Hkv, D, max_new, max_ctx, quantized)
     n = _PAGED_WS.get(key)
     if n is None:
@@ -1150,15 +1211,15 @@ def paged_attn_workspace_floats(B: int, N: int, Hq: int, Hkv: int, D: int, max_n
             _PAGED_WS.clear()
         w = ctypes.c_int64(0)
         with torch.cuda.device(device):
-            check(lib().od_paged_attn_ws_of(B, N, Hq, Hkv, D, max_new, max_ctx, int(quantized), ctypes.byref(w)),
-                  "od_paged_attn_ws_of")
+            check(lib().od_paged_attn_ws_ex(B, N, Hq, Hkv, D, max_new, max_ctx, PAGE_FORMATS[quantized], ctypes.byref(w)),
+                  "od_paged_attn_ws_ex")
         n = _PAGED_WS[key] = w.value
     return n
 
 
 def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.Tensor, ctx_len: torch.Tensor, scale: float,
                row_begin=None, max_new: int | None = None, max_ctx: int | None = None, out=None, return_lse: bool = False):
-    """od_paged_attn: the new tokens' queries q (N, Hq, D) bf16 attend the ctx_len[b] cached tokens of their sequence and
+    """od_paged_attn_ex: the new tokens' queries q (N, Hq, D) bf16 attend the ctx_len[b] cached tokens of their sequence and
     its new tokens k, v (N, Hkv, D) bf16 causally (both None: the cached ones only). table, start and ctx_len as
     page_append. row_begin int32 (N,): the first new token that a token sees, counted from its sequence's first (option
     rows and packed documents see their own tokens only); None: 0. max_new, max_ctx: bounds on a sequence's new and cached
@@ -1168,7 +1229,7 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
     gets 0 and -inf, rows of no sequence are left as they were."""
     dev = _one_device("paged_attn", q, k, v, cache.k, cache.v, table, start, ctx_len, row_begin, out)
     B, pages, table = _paged(cache, table, start, ctx_len, "paged_attn")
-    n_pages, H, page, D = cache.k.shape
+    H, page, D = cache.k.shape[1], cache.k.shape[2], cache.head_dim
     N, Hq = q.shape[0], q.shape[1]
     q, qa = _new_rows(q, N, Hq, D, "paged_attn: q")
     if (k is None) != (v is None):
@@ -1196,15 +1257,15 @@ def paged_attn(q: torch.Tensor, k, v, cache, table: torch.Tensor, start: torch.T
         dst = out if aligned else out.clone(memory_format=torch.contiguous_format)
         oa = (dst.data_ptr(), dst.stride(0), dst.stride(1))
     lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device) if return_lse else None
-    n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device, cache.k_scale is not None)
+    n = paged_attn_workspace_floats(B, N, Hq, H, D, max_new, max_ctx, q.device, _FORMAT_NAMES[cache.format])
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     args = (*qa, *ka, *va, *pages, start.data_ptr(), ctx_len.data_ptr(), ptr(row_begin), *oa, ptr(lse), B, N, Hq, H, D, max_new,
             max_ctx, float(scale), ptr(ws), n, torch._C._cuda_getCurrentRawStream(dev))
     if dev == torch._C._cuda_getDevice():  # as _OnDevice, without its calls: the host bounds a token over a short state
-        check(lib().od_paged_attn(*args), "od_paged_attn")
+        check(lib().od_paged_attn_ex(*args), "od_paged_attn")
     else:
         with torch.cuda.device(dev):
-            check(lib().od_paged_attn(*args), "od_paged_attn")
+            check(lib().od_paged_attn_ex(*args), "od_paged_attn")
     if dst is not out:
         out.copy_(dst)
     return (out, lse) if return_lse else out

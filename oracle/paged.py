@@ -9,6 +9,46 @@ import torch
 from .quant import quantize_rows
 
 
+def pack4(x):
+    """bf16 rows (..., D) as 4-bit pages hold them: bytes (..., D / 2) and bf16 scales (..., D / 32). Value by value: per 32, m the
+    first of the largest magnitude, d = m / -8, u = floor(x / d + 8.5) within 0..15, in float64 (where x / d + 8.5 of bf16 numbers is
+    never on the wrong side of an integer); value 2 i of 8 at bit 4 i of a little-endian word, value 2 i + 1 at bit 16 + 4 i."""
+    rows = x.double().reshape(-1, x.shape[-1])
+    q = torch.zeros(rows.shape[0], x.shape[-1] // 2, dtype=torch.uint8)
+    s = torch.zeros(rows.shape[0], x.shape[-1] // 32, dtype=torch.float64)
+    for r, row in enumerate(rows.tolist()):
+        for a in range(0, len(row), 32):
+            block = row[a:a + 32]
+            if all(math.isfinite(v) for v in block):
+                m = max(block, key=abs)
+                d = 0.0 if abs(m) < 2.0 ** -100 else m / -8.0
+                u = [8 if d == 0 else min(15, max(0, math.floor(v / d + 8.5))) for v in block]
+            else:
+                d, u = math.nan, [8 if math.isfinite(v) else 0 for v in block]
+            s[r, a // 32] = d
+            for w in range(4):
+                word = sum(u[8 * w + i] << (16 * (i % 2) + 4 * (i // 2)) for i in range(8))
+                q[r, a // 2 + 4 * w:a // 2 + 4 * w + 4] = torch.tensor(list(word.to_bytes(4, "little")), dtype=torch.uint8)
+    return q.view(*x.shape[:-1], -1), s.to(torch.bfloat16).view(*x.shape[:-1], -1)
+
+
+def values4(q, s):
+    """The float64 values (..., D) of 4-bit rows: (u - 8) d, NaN where d is not finite."""
+    y = torch.empty(*q.shape[:-1], 2 * q.shape[-1], dtype=torch.float64)
+    for i in range(8):  # value i of every word: byte 2 (i % 2) + i / 4, its half i / 2 % 2
+        byte = q[..., 2 * (i % 2) + i // 4::4].long()
+        y[..., i::8] = ((byte >> 4 * (i // 2 % 2)) & 15).double() - 8
+    d = s.double()
+    return y * d.masked_fill(~d.isfinite(), math.nan).repeat_interleave(32, -1)
+
+
+def values(rows, scales):
+    """The float64 values of rows (..., D) of any pages."""
+    if rows.dtype == torch.uint8:
+        return values4(rows, scales)
+    return rows.double() if scales is None else rows.double() * scales.double()[..., None]
+
+
 def place(table, n_pages: int, page: int, b: int, pos: int):
     """(page, row) of position pos of sequence b, or None where there is no page."""
     col = pos // page
@@ -25,8 +65,8 @@ def sequences(start, N: int):
 
 
 def append(pages, scales, x, table, start, ctx):
-    """pages (n_pages, H, page, D) (and fp32 scales (n_pages, H, page) or None) after the rows x (N, H, D) are written:
-    new tensors."""
+    """pages (n_pages, H, page, D) (and fp32 scales (n_pages, H, page) or None; or 4 bits, as pack4 gives them) after the rows
+    x (N, H, D) are written: new tensors."""
     pages, scales = pages.clone(), None if scales is None else scales.clone()
     n_pages, _, page, _ = pages.shape
     for b, a, e in sequences(start, x.shape[0]):
@@ -36,6 +76,8 @@ def append(pages, scales, x, table, start, ctx):
                 continue
             if scales is None:
                 pages[at[0], :, at[1]] = x[a + i]
+            elif pages.dtype == torch.uint8:
+                pages[at[0], :, at[1]], scales[at[0], :, at[1]] = pack4(x[a + i])
             else:
                 q, s = quantize_rows(x[a + i])
                 pages[at[0], :, at[1]], scales[at[0], :, at[1]] = q, s[..., 0]
@@ -43,11 +85,12 @@ def append(pages, scales, x, table, start, ctx):
 
 
 def read(pages, scales, table, length, T: int):
-    """(rows (B, H, T, D), scales (B, H, T) or None, valid (B, T)): the stored rows of every sequence, zeros where none is."""
+    """(rows (B, H, T, D), scales (B, H, T) or None, valid (B, T)): the stored rows of every sequence, zeros where none is (4-bit
+    rows keep their own widths)."""
     n_pages, H, page, D = pages.shape
     B = len(length)
     rows = torch.zeros(B, H, T, D, dtype=pages.dtype)
-    sc = None if scales is None else torch.zeros(B, H, T)
+    sc = None if scales is None else torch.zeros(B, H, T, *scales.shape[3:], dtype=scales.dtype)
     valid = torch.zeros(B, T, dtype=torch.bool)
     for b in range(B):
         for j in range(min(T, max(int(length[b]), 0))):
@@ -75,9 +118,7 @@ def attention(q, k, v, pages, table, start, ctx, scale: float, row_begin=None):
         t = min(max(int(ctx[b]), 0), table.shape[1] * pages[0].shape[2])
         kr, ks, valid = read(pages[0], pages[2], table[b:b + 1], [t], t)
         vr, vs, _ = read(pages[1], pages[3], table[b:b + 1], [t], t)
-        kc, vc = kr[0].double(), vr[0].double()
-        if ks is not None:
-            kc, vc = kc * ks[0].double()[..., None], vc * vs[0].double()[..., None]
+        kc, vc = (values(r[0], None if x is None else x[0]) for r, x in ((kr, ks), (vr, vs)))
         seen = valid.expand(n, t)
         if k is not None:
             i = torch.arange(n)
