@@ -111,6 +111,9 @@ SIGNATURES = {
     "od_qk_norm_rope_page_append": [_c_ptr, _i64, _c_ptr, _i64, _i64, _i64, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64,
                                     _c_ptr, ctypes.c_float, ctypes.c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _i64, _i64, _c_ptr,
                                     _i64, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64, _i64, _c_ptr],
+    "od_q4_linear_ws": [_i64, _i64, _i64, _c_ptr],
+    "od_q4_linear": [_c_ptr, _i64, _c_ptr, _i64, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _c_ptr, _i64, _i64, _i64, _i64, _c_ptr, _i64,
+                     _c_ptr],
     "od_lm_head_logprob_ws": [_i64, _i64, _c_ptr],
     "od_lm_head_logprob": [_c_ptr, _i64, _c_ptr, _i64, ctypes.c_int, _c_ptr, _i64, _c_ptr, _c_ptr, _i64, _i64, _i64,
                            _c_ptr, _c_ptr, _i64, _c_ptr],

@@ -1030,6 +1030,81 @@ def gdn_norm_quant(o: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
     return xq, sx
 
 
+# ------------------------------------------------------------------------------------------------ 4-bit weights
+_Q4_WS: dict = {}
+
+
+def q4_linear_workspace_floats(M: int, N: int, K: int, device) -> int:
+    """Floats of od_q4_linear's workspace for these sizes on the device (0: none)."""
+    key = (device.index, M, N, K)
+    n = _Q4_WS.get(key)
+    if n is None:
+        if len(_Q4_WS) >= 65536:  # the sizes are cheap to ask for again
+            _Q4_WS.clear()
+        w = ctypes.c_int64(0)
+        with torch.cuda.device(device):
+            check(lib().od_q4_linear_ws(M, N, K, ctypes.byref(w)), "od_q4_linear_ws")
+        n = _Q4_WS[key] = w.value
+    return n
+
+
+def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Tensor | None = None,
+              residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """od_q4_linear: x (..., K) bf16 times 4-bit weights in Q4Table's layout, qs uint8 (N, K / 2) and d fp16 (N, K / 32), plus
+    bias (N,) and residual (..., N) bf16: (..., N) bf16, rounded once. K a multiple of 32. Up to 32 rows of x no weight is rounded;
+    for more each is once, to fp16. A row of x that holds an infinity or NaN comes out NaN. out (..., N) bf16 may be the
+    residual."""
+    dev = _one_device("q4_linear", x, qs, d, bias, residual, out)
+    _lib.bf16_bits(x)
+    if qs.dtype != torch.uint8 or d.dtype != torch.float16:
+        raise TypeError(f"q4_linear: expected uint8 weights and float16 scales, got {qs.dtype} and {d.dtype}")
+    if qs.dim() != 2 or d.dim() != 2 or x.dim() < 1:
+        raise ValueError("q4_linear: qs must be (N, K / 2) and d (N, K / 32)")
+    N, K = qs.shape[0], 2 * qs.shape[1]
+    if K % 32 or d.shape != (N, K // 32) or x.shape[-1] != K or N < 1 or K < 32:
+        raise ValueError(f"q4_linear: x {tuple(x.shape)}, qs {tuple(qs.shape)} and d {tuple(d.shape)} do not match (K a multiple of 32)")
+    shape = (*x.shape[:-1], N)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    M = x2.shape[0]
+    if x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (x2.stride(0) % 8 or x2.stride(0) < K)):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if qs.stride(1) != 1 or qs.data_ptr() % 16 or (N > 1 and (qs.stride(0) % 16 or qs.stride(0) < K // 2)):
+        qs = qs.clone(memory_format=torch.contiguous_format)
+    if d.stride(1) != 1 or (N > 1 and d.stride(0) < K // 32):
+        d = d.contiguous()
+    bias = _vec(bias, N, "bias")
+    ldr = N
+    if residual is not None:
+        _lib.bf16_bits(residual)
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"q4_linear: residual must be {shape}, got {tuple(residual.shape)}")
+        residual = residual if residual.dim() == 2 else residual.reshape(-1, N)
+        if residual.stride(1) != 1 or (M > 1 and residual.stride(0) < N):
+            residual = residual.contiguous()
+        ldr = residual.stride(0) if M > 1 else N
+    if out is None:
+        dst = res = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+        ldo = N
+    else:
+        res = _check_out(out, shape, x.device, "q4_linear")
+        flat = out if out.dim() == 2 else (out.view(-1, N) if out.is_contiguous() else None)
+        dst = flat if flat is not None and (M < 2 or flat.stride(0) >= N) else torch.empty(M, N, dtype=out.dtype, device=out.device)
+        ldo = dst.stride(0) if M > 1 else N
+    n = q4_linear_workspace_floats(M, N, K, x.device)
+    ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
+    args = (x2.data_ptr(), x2.stride(0) if M > 1 else K, qs.data_ptr(), qs.stride(0) if N > 1 else K // 2, d.data_ptr(),
+            d.stride(0) if N > 1 else K // 32, ptr(bias), ptr(residual), ldr, dst.data_ptr(), ldo, M, N, K, ptr(ws), n,
+            torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        check(lib().od_q4_linear(*args), "od_q4_linear")
+    else:
+        with torch.cuda.device(dev):
+            check(lib().od_q4_linear(*args), "od_q4_linear")
+    if out is not None and dst.data_ptr() != out.data_ptr():
+        out.copy_(dst.view(shape))
+    return res
+
+
 # ------------------------------------------------------------------------------------------------ paged K/V cache
 def _paged(cache, table, start, ctx_len, name):
     """The arguments of a paged batch that every entry point takes, checked: the sequence count, (format, pages, table) and the table

@@ -49,6 +49,22 @@ class Int8Table(nn.Module):
         return self.qweight[ids].to(self.scale.dtype) * self.scale[ids]
 
 
+def q4_rows(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Q4_0 of float rows (N, K), K a multiple of 32: packed values uint8 (N, K / 2) and fp16 scales (N, K / 32), with the
+    reference's round-to-nearest formula (quant.py:206-246)."""
+    K = w.shape[1]
+    qs_parts, d_parts = [], []
+    for a in range(0, w.shape[0], 16384):  # bounded float32 temporaries
+        b = w[a:a + 16384].float().view(-1, K // 32, 32)
+        idx = b.abs().argmax(-1, keepdim=True)
+        dd = b.gather(-1, idx) / -8
+        inv = torch.where(dd != 0, 1 / dd, torch.zeros_like(dd))
+        q = torch.clamp(torch.floor(b * inv + 8.5), 0, 15).to(torch.uint8)
+        qs_parts.append((q[..., :16] | (q[..., 16:] << 4)).view(b.shape[0], K // 2))
+        d_parts.append(dd.squeeze(-1).to(torch.float16))
+    return torch.cat(qs_parts), torch.cat(d_parts)
+
+
 class Q4Table(nn.Module):
     """A frozen Q4_0 table (quant.py:206-246): blocks of 32 values along a row, one fp16 scale d per block,
     w = (q - 8) d with q in 0..15 (a block's positions 0-15 in the low nibbles of its 16 bytes, 16-31 in the high
@@ -58,19 +74,9 @@ class Q4Table(nn.Module):
     def __init__(self, w: torch.Tensor | None = None, *, qs=None, d=None):
         super().__init__()
         if w is not None:
-            N, K = w.shape
-            if K % 32:
+            if w.shape[1] % 32:
                 raise ValueError("Q4Table needs rows whose length is a multiple of 32")
-            qs_parts, d_parts = [], []
-            for a in range(0, N, 16384):  # bounded float32 temporaries
-                b = w[a:a + 16384].float().view(-1, K // 32, 32)
-                idx = b.abs().argmax(-1, keepdim=True)
-                dd = b.gather(-1, idx) / -8
-                inv = torch.where(dd != 0, 1 / dd, torch.zeros_like(dd))
-                q = torch.clamp(torch.floor(b * inv + 8.5), 0, 15).to(torch.uint8)
-                qs_parts.append((q[..., :16] | (q[..., 16:] << 4)).view(b.shape[0], K // 2))
-                d_parts.append(dd.squeeze(-1).to(torch.float16))
-            qs, d = torch.cat(qs_parts), torch.cat(d_parts)
+            qs, d = q4_rows(w)
         if qs is None or d is None:
             raise ValueError("Q4Table needs float rows or (qs, d)")
         self.register_buffer("qs", qs)

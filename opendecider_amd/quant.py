@@ -19,6 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import kernels
+from .lm_head import Q4Table, q4_rows
 
 
 # ---------------------------------------------------------------- int8 tensors (caches)
@@ -227,6 +228,68 @@ def gemlite_a8w8_(module: nn.Module) -> nn.Module:
 
 
 w8a8_ = gemlite_a8w8_
+
+
+# ---------------------------------------------------------------- 4-bit weights
+class Q4Linear(nn.Module):
+    """A frozen linear with 4-bit weights on the MI355X (od_q4_linear): blocks of 32 values along a row, one fp16 scale each (the
+    layout and rounding of Q4Table, quant.py:206-246), activations in bf16. Single tokens and small batches read 4.5 bits a
+    weight; long ones run on the matrix cores.
+
+    Buffers: qs uint8 (out, in / 2) and d fp16 (out, in / 32), in padded to a multiple of 32 with zero columns; bias (bf16 or None)."""
+
+    def __init__(self, qs: torch.Tensor, d: torch.Tensor, bias: torch.Tensor | None = None, in_features: int | None = None):
+        super().__init__()
+        if qs.dtype != torch.uint8 or d.dtype != torch.float16 or qs.dim() != 2 or qs.shape[1] % 16 or \
+                d.shape != (qs.shape[0], qs.shape[1] // 16):
+            raise ValueError("Q4Linear needs uint8 qs (out, in / 2) and fp16 d (out, in / 32)")
+        self.out_features, padded = qs.shape[0], 2 * qs.shape[1]
+        self.in_features = padded if in_features is None else in_features
+        if not padded - 32 < self.in_features <= padded:
+            raise ValueError(f"Q4Linear: {self.in_features} input features in rows of {padded}")
+        self.register_buffer("qs", qs.contiguous())
+        self.register_buffer("d", d.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.to(torch.bfloat16).contiguous())
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear) -> "Q4Linear":
+        w = lin.weight.data
+        qs, d = q4_rows(F.pad(w, (0, -w.shape[1] % 32)))
+        return cls(qs, d, None if lin.bias is None else lin.bias.data, lin.in_features)
+
+    @classmethod
+    def from_table(cls, t: Q4Table) -> "Q4Linear":
+        """The same 4-bit rows as a Q4Table's (a head's logits)."""
+        return cls(t.qs, t.d)
+
+    @property
+    def weight(self) -> torch.Tensor:
+        return Q4Table(qs=self.qs, d=self.d).weight[:, : self.in_features]
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if not x.is_cuda:
+            raise RuntimeError("Q4Linear runs on the MI355X only (no CPU path)")
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Q4Linear: {x.shape[-1]} input features, expected {self.in_features}")
+        xb = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
+        pad = 2 * self.qs.shape[1] - self.in_features
+        y = kernels.q4_linear(F.pad(xb, (0, pad)) if pad else xb, self.qs, self.d, self.bias, residual)
+        return y if x.dtype == torch.bfloat16 else y.to(x.dtype)
+
+    def extra_repr(self) -> str:
+        return f"in={self.in_features}, out={self.out_features}, 4-bit weights"
+
+
+def quantize_q4_(module: nn.Module, skip: tuple[str, ...] = ()) -> nn.Module:
+    """Replace every nn.Linear under `module` in place with Q4Linear (as quantize_int8_ does with Int8Linear)."""
+    for name, child in list(module.named_children()):
+        if name in skip:
+            continue
+        if isinstance(child, nn.Linear):
+            setattr(module, name, Q4Linear.from_linear(child))
+        else:
+            quantize_q4_(child, skip)
+    return module
 
 
 class SmoothedLinear(nn.Module):

@@ -144,3 +144,18 @@ def test_abi_refusals():
     assert rope(ld=760) == SHAPE and rope(ldo=500) == SHAPE and rope(hq=-1) == SHAPE and rope(rot=64) == UNSUP and rope(zc=2) == UNSUP
     assert rope(fmt=4) == UNSUP and rope(D=96) == UNSUP and rope(out=None) == NULL and rope(qw=None) == NULL and rope(start=None) == NULL
     assert rope(ld=772) == ALIGN and rope(qkv=odd) == ALIGN and rope(out=odd) == ALIGN and rope(qw=odd) == ALIGN
+
+    def linear(M=4, N=64, K=128, ldx=128, ldq=64, ldd=4, ldo=64, x=P, qs=P, d=P, out=P, ws=None, nws=0, res=None, ldr=64):
+        return L.od_q4_linear(x, ldx, qs, ldq, d, ldd, None, res, ldr, out, ldo, M, N, K, ws, nws, None)
+
+    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(K=100), dict(ldx=120), dict(ldq=48), dict(ldd=3), dict(ldo=60), dict(res=P, ldr=60),
+                dict(M=1 << 23), dict(ldx=1 << 22), dict(M=40, ws=P, nws=3)):
+        assert linear(**bad) == SHAPE, bad
+    for bad in (dict(x=None), dict(qs=None), dict(d=None), dict(out=None), dict(M=40)):
+        assert linear(**bad) == NULL, bad
+    for bad in (dict(x=odd), dict(qs=odd), dict(ldx=132), dict(ldq=72), dict(d=ctypes.c_void_p(65)), dict(M=40, ws=odd, nws=1 << 30)):
+        assert linear(**bad) == ALIGN, bad
+    assert linear(M=0, x=None) == 0
+    assert L.od_q4_linear_ws(4, 64, 100, ctypes.byref(n)) == SHAPE and L.od_q4_linear_ws(4, 64, 128, None) == NULL
+    assert L.od_q4_linear_ws(32, 64, 128, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.od_q4_linear_ws(33, 64, 128, ctypes.byref(n)) == 0 and n.value >= 33 * 128 // 2
