@@ -264,6 +264,46 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
   hi = __builtin_amdgcn_perm(f3, f2, 0x07060302u);
 }
 
+// exponent e with x < 2^e for the bits of a finite x > 0; 0 for 0
+__device__ __forceinline__ int exp_above(uint32_t bits) { return bits ? (int)(bits >> 23) - 126 : 0; }
+
+constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
+
+// The factor scale 2^e of a block's fp16 scores (of 2^36 at most), a number above 0 whatever the exponents: the scores of
+// masked keys are -inf ahead of it, and 2^-126 makes any score as good as 0.
+__device__ __forceinline__ float score_factor(float scale_log2, int e) {
+  return __builtin_amdgcn_fmed3f(__builtin_ldexpf(scale_log2, e), 0x1p-126f, 0x1.fffffep127f);
+}
+
+// A word of 8 four-bit values times their scale, as fp16, in order. A value u at bits 6 to 9 of 16.0's fp16 is 16 + u, so a pair
+// is one shift, one and-or and one fma with 24 s: u - 8 has 3 significant bits and s 8 (f16_scale), so that 24 s and the result
+// are exact (12 instructions a word).
+struct Q4Scale {
+  f16x2 s, c;  // s and -24 s
+};
+__device__ __forceinline__ Q4Scale q4_pair(f16x2 s) {
+  const f16x2 k = {(_Float16)-24.0f, (_Float16)-24.0f};
+  return {s, s * k};
+}
+__device__ __forceinline__ v4u q4x8_f16(uint32_t w, const Q4Scale& q) {
+  const uint32_t at[4] = {w << 6, w << 2, w >> 2, w >> 6};
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 x = __builtin_bit_cast(f16x2, (at[i] & 0x03c003c0u) | 0x4c004c00u);
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, q.s, q.c));
+  }
+  return r;
+}
+// A bf16 scale times 2^e in fp16, NaN where it is not finite (an infinite one would make scores of -inf, which are no keys);
+// exact unless it falls below fp16's normal numbers.
+__device__ __forceinline__ _Float16 f16_scale(uint32_t bits, int e) {
+  const float s = (bits & 0x7f80u) == 0x7f80u ? NAN : __uint_as_float(bits << 16);
+  return (_Float16)__builtin_ldexpf(s, e);
+}
+// The frame of 4-bit values whose largest scale has these bf16 bits: 2^E above it, and values below 8 times it, so that q 2^(7 -
+// (E - 4)) is below 2^14, as for int8.
+__device__ __forceinline__ int q4_frame(uint32_t bits) { return bits ? (int)(bits >> 7) - 126 - 4 : 0; }
 // ------------------------------------------------------------------------------------------ few slots: streaming
 // Up to 16 or 32 slots of a (sequence, KV head) in a workgroup: decode steps. 4 rep D FLOP per key against 2 D (+ 8)
 // bytes of int8 K and V: bound by reading the pages (64 x 4096 tokens of 8 heads of 128 in 70 us, 5.4 TB/s). A wave holds
@@ -284,21 +324,39 @@ __device__ __forceinline__ void i8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t&
 // the products of the tile ahead of it, unconditionally (past a wave's last tile with descriptors of no length, so that
 // the waits are counted but nothing is read). Rows of 256 go in tiles of one half (R = 1): two sets of whole ones do
 // not fit the registers (16 x 8000 tokens 62 us, 49 with halves); bf16 ones then still take a SIMD alone.
-constexpr int s_halves(int D) { return D == 256 ? 1 : 2; }
-template <int D, bool Q8>
+//
+// 4-bit pages: all of it in fp16, since a value is exact there as (u - 8) d in a power-of-two frame (3 significant bits by 8): the
+// slot's queries as fp16 in its frame (in LDS), a tile's K in the frame of its largest scale, V in that of the largest so far, by
+// which O moves along, probabilities kept 2^7 above their value as in the tile kernels. One product takes P then, no low part.
+// Four lanes of a key read all of it (D / 2 bytes), so a lane's K has one scale (two of heads of 256), loaded with it; V's scales
+// come one or two a lane and go to the lanes that need them through the LDS crossbar. The new tokens come last, in bf16, where O
+// leaves its frame.
+constexpr int s_halves(int D, int P) { return D == 256 && P != kInt4 ? 1 : 2; }
+template <int D, int P>
 struct STile {
-  static constexpr int R = s_halves(D), KW = D / 4 * (Q8 ? 1 : 2) / 16;  // KW: 16-byte loads of a key's D / 4 values
+  static constexpr bool Q8 = P == kInt8;
+  static constexpr int R = s_halves(D, P), KW = D / 4 * (Q8 ? 1 : 2) / 16;  // KW: 16-byte loads of a key's D / 4 values
   static constexpr int VB = D / 16 * (Q8 ? 1 : 2);                           // bytes of a key's D / 16 values: 4 to 32
   v4u k[R][KW];
   uint32_t v[4 * R][VB / 4];
   float ks, vs;  // lane l: the scales of key l % 32
   int len[R];    // keys of the half tiles (wave-uniform)
 };
+template <int D>
+struct STile<D, kInt4> {
+  static constexpr int R = 2, KC = D == 256 ? 2 : 1, KW = D / 32 / KC, VB = D == 256 ? 8 : 4;
+  uint32_t k[R][KC][KW];  // chunk c: bytes (64 c +) D / 8 / KC g .. of key j, its words
+  uint32_t v[4 * R][VB / 4];
+  uint32_t ks[R][KC];  // the scales of those chunks
+  uint32_t vs[R];      // lane l: scale l of the half tile's 16 D / 32 (heads of 64: l % 32; of 256: 2 l and 2 l + 1)
+  int len[R];
+};
 
 // first of the 8 dims that lanes of group g hold in k-step ks
-template <bool Q8>
+template <int D, int P>
 __device__ __forceinline__ int s_dim(int g, int ks) {
-  return Q8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
+  if constexpr (P == kInt4) return D == 256 ? 128 * (ks / 4) + 32 * g + 8 * (ks % 4) : D / 4 * g + 8 * ks;
+  return P == kInt8 ? 64 * (ks / 2) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
 }
 
 constexpr int kOnce = 2;  // non-temporal: each byte is read once
@@ -317,10 +375,11 @@ __device__ __forceinline__ int s_pages(const Paged& p, int b, int pos, int step)
 }
 // A tile's loads, its pages in place `nth` of `pages`. Lane l takes the scales of key l % 32, each 16 lanes their half
 // tile's.
-template <int D, bool Q8>
-__device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth,
-                                       STile<D, Q8>& x) {
-  using T = STile<D, Q8>;
+template <int D, int P>
+__device__ __forceinline__ void s_load_rows(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth,
+                                       STile<D, P>& x) {
+  using T = STile<D, P>;
+  constexpr bool Q8 = T::Q8;
   constexpr int E = Q8 ? 1 : 2;
   const int lane = threadIdx.x & 63, j = lane & 15, gl = lane >> 4;
   int64_t row[T::R];
@@ -365,10 +424,56 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
     x.vs = in ? v1 : 0.0f;
   }
 }
-
+template <int D, int P>
+__device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, int kb, int pages, int nth, STile<D, P>& x) {
+  if constexpr (P == kInt4) {
+    using T = STile<D, P>;
+    const int lane = threadIdx.x & 63, j = lane & 15, gl = lane >> 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int pos = kb + 16 * r, pg = __builtin_amdgcn_readlane(pages, nth * 2 + r);
+      x.len[r] = pg < 0 || pos >= s.ctx ? 0 : min(16, s.ctx - pos);
+      const int64_t row = (((int64_t)max(pg, 0) * a.p.Hkv + g) << a.p.shift) + (pos & ((1 << a.p.shift) - 1));
+      const auto dk = rsrc(static_cast<const char*>(a.p.k) + row * (D / 2), x.len[r] * (D / 2));
+      const auto dv = rsrc(static_cast<const char*>(a.p.v) + row * (D / 2), x.len[r] * (D / 2));
+      const auto sk = rsrc(a.p.k4 + row * (D / 32), x.len[r] * (D / 16)), sv = rsrc(a.p.v4 + row * (D / 32), x.len[r] * (D / 16));
+#pragma unroll
+      for (int c = 0; c < T::KC; ++c) {
+        const int at = j * (D / 2) + 64 * c + 4 * T::KW * gl;
+        if constexpr (T::KW == 4) {
+          const v4u u = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(dk, at, 0, kOnce));
+#pragma unroll
+          for (int w = 0; w < 4; ++w) x.k[r][c][w] = u[w];
+        } else {
+          const auto u = __builtin_amdgcn_raw_buffer_load_b64(dk, at, 0, kOnce);
+          x.k[r][c][0] = u[0], x.k[r][c][1] = u[1];
+        }
+        x.ks[r][c] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sk, 2 * (j * (D / 32) + 4 * c + (D == 64 ? gl / 2 : gl)), 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // heads of 64: two lanes share a word
+        const int at = (4 * gl + i) * (D / 2) + (D == 64 ? 4 * (j / 2) : T::VB * j);
+        if constexpr (T::VB == 4) {
+          x.v[4 * r + i][0] = __builtin_amdgcn_raw_buffer_load_b32(dv, at, 0, kOnce);
+        } else {
+          const auto u = __builtin_amdgcn_raw_buffer_load_b64(dv, at, 0, kOnce);
+          x.v[4 * r + i][0] = u[0], x.v[4 * r + i][1] = u[1];
+        }
+      }
+      if constexpr (D == 256) x.vs[r] = __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * lane, 0, 0);
+      else x.vs[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sv, 2 * (D == 64 ? lane & 31 : lane), 0, 0);
+    }
+  } else {
+    s_load_rows<D, P>(a, s, g, kb, pages, nth, x);
+  }
+}
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                  0, 0);
+}
+
+__device__ __forceinline__ v4f mfma16h(v4u a, v4u b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // The slot state of a lane: column j's running max and its share of the sum, output rows 4 g + i of every d tile.
@@ -378,10 +483,9 @@ struct SAcc {
   v4f o[D / 16];
 };
 
-// One tile's online softmax into bf16 hi and lo parts: y the lane's 8 scores (log2 units, -inf masked), f a factor on p
-// for the P.V product only (the V scales).
-template <int D, bool F>
-__device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
+// One tile's online softmax: y the lane's 8 scores (log2 units, -inf masked); p out, 2^LIFT above its value.
+template <int D, int LIFT>
+__device__ __forceinline__ void s_probabilities(float (&y)[8], SAcc<D>& x, float (&p)[8]) {
   float mx = y[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) mx = fmaxf(mx, y[i]);
@@ -397,13 +501,18 @@ __device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SA
     x.l *= c;
     if (move) x.m = mx;
   }
-  const float ms = x.m == -INFINITY ? 0.0f : x.m;
-  float p[8];
+  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - (float)LIFT;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     p[i] = __builtin_amdgcn_exp2f(y[i] - ms);
     x.l += p[i];
   }
+}
+// The same into bf16 hi and lo parts: f a factor on p for the P.V product only (the V scales).
+template <int D, bool F, int LIFT>
+__device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
+  float p[8];
+  s_probabilities<D, LIFT>(y, x, p);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float u = F ? p[2 * e] * f[2 * e] : p[2 * e], w = F ? p[2 * e + 1] * f[2 * e + 1] : p[2 * e + 1];
@@ -413,8 +522,9 @@ __device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SA
 }
 
 // value dt of each of the lane's 8 keys, as the bf16 A operand
-template <int D, bool Q8, int NK>
-__device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, Q8>::VB / 4], int dt) {
+template <int D, int P, int NK>
+__device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, P>::VB / 4], int dt) {
+  constexpr bool Q8 = P == kInt8;
   v4u r = v4u{0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < NK / 2; ++e) {
@@ -430,21 +540,43 @@ __device__ __forceinline__ v4u s_vfrag(const uint32_t (&v)[NK][STile<D, Q8>::VB 
   return r;
 }
 
+// The maxima of both halves of a word over the wave.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t s_max2_step(uint32_t x) {
+  return od_absmax_bf16x2(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, ROW_MASK, 0xf, false));
+}
+__device__ __forceinline__ uint32_t s_wave_max2(uint32_t x) {
+  x = s_max2_step<0xB1, 0xf>(x);   // quad_perm [1,0,3,2]
+  x = s_max2_step<0x4E, 0xf>(x);   // quad_perm [2,3,0,1]
+  x = s_max2_step<0x124, 0xf>(x);  // row_ror:4
+  x = s_max2_step<0x128, 0xf>(x);  // row_ror:8
+  x = s_max2_step<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x = s_max2_step<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
 constexpr int kStreamWaves = 4;
 // whether a wave has a SIMD's registers to itself
-constexpr bool s_alone(int D, bool q8, int columns) { return D * columns >= (q8 ? 512 : 256); }
+constexpr bool s_alone(int D, int P, int columns) { return D * columns >= (P == kBf16 ? 256 : 512); }
 
-template <int D, bool Q8, int CT>
-__global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+template <int D, int P, int CT>
+__global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+  constexpr bool Q8 = P == kInt8, Q4 = P == kInt4;
+  constexpr int LIFT = Q4 ? (int)kLift : 0;
+  using Tile = STile<D, P>;
   // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
-  constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D), QR = D + 8;
+  constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D, P), QR = D + 8;
   __shared__ __attribute__((aligned(16))) union {
-    uint16_t q[16 * CT * QR];
+    struct {
+      uint16_t q[16 * CT * QR];
+      uint16_t q16[Q4 ? 16 * CT * QR : 8];  // 4-bit pages: the queries as fp16 in their frames, whose exponents are qe
+    };
     float o[NW][16][D + 4];
   } sm;
+  __shared__ int qe[Q4 ? 16 * CT : 1], frames[NW];
   __shared__ float sml[NW][2][16];
   // a tile's per-key factors, from lane order to score order (one wave writes and reads)
-  __shared__ float4 skf[NW][2][8];
+  __shared__ float4 skf[Q8 ? NW : 1][2][8];
   const int sp = blockIdx.x, g = blockIdx.y % a.p.Hkv, b = blockIdx.z;
   constexpr int W = 16 * R, PT = 64 / R, SETS = 2;  // PT: tiles whose pages one load brings
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -470,9 +602,9 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
     }
     int tt = t_lo + wave, pages = pages0, nth = -1;
     // the wave's next tile into x (past the last one: an empty one, without traffic)
-    STile<D, Q8> tl[SETS];
+    Tile tl[SETS];
     int asked = tt - NW;  // the tile last asked for
-    auto next = [&](STile<D, Q8>& x) {
+    auto next = [&](Tile& x) {
       const bool more = asked + NW < t_hi;
       if (more) {
         asked += NW;
@@ -481,7 +613,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
           pages = s_pages<R>(a.p, b, asked * W, NW * W);
         }
       }
-      s_load<D, Q8>(a, s, g, more ? asked * W : s.ctx, pages, nth, x);
+      s_load<D, P>(a, s, g, more ? asked * W : s.ctx, pages, nth, x);
       __builtin_amdgcn_sched_barrier(0);
     };
     if (tt < t_hi) {
@@ -493,11 +625,31 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
     for (int k = 0; k < QC; ++k) {
       const int i = k * NW * 64 + threadIdx.x;
       if (i < QN) *reinterpret_cast<uint4*>(sm.q + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = qw[k];
+      if constexpr (Q4) {  // (D / 8 lanes a slot)
+        uint32_t am = od_absmax_bf16x2(od_absmax_bf16x2(od_absmax_bf16x2(od_absmax_bf16x2(0, qw[k].x), qw[k].y), qw[k].z), qw[k].w);
+        am = max(am & 0xffffu, am >> 16);
+#pragma unroll
+        for (int o = D / 16; o > 0; o >>= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
+        const int e = am < 0x7f80u ? exp_above(am << 16) : 0;
+        const uint32_t w[4] = {qw[k].x, qw[k].y, qw[k].z, qw[k].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int c2 = 0; c2 < 4; ++c2) {
+          const f16x2 r = {(_Float16)__builtin_ldexpf(__uint_as_float(w[c2] << 16), 14 - e),
+                           (_Float16)__builtin_ldexpf(__uint_as_float(w[c2] & 0xffff0000u), 14 - e)};
+          h[c2] = __builtin_bit_cast(uint32_t, r);
+        }
+        if (i < QN) {
+          *reinterpret_cast<uint4*>(sm.q16 + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+          if (i % (D / 8) == 0) qe[i / (D / 8)] = e;
+        }
+      }
     }
     __syncthreads();
     auto qfrag = [&](int ct, int ks) {
-      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + (16 * ct + j) * QR + s_dim<Q8>(qd, ks)));
+      return __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q + (16 * ct + j) * QR + s_dim<D, P>(qd, ks)));
     };
+    int frame = 0;  // 4-bit pages: O is in units of 2^frame
     SAcc<D> acc[CT];
 #pragma unroll
     for (auto& x : acc) {
@@ -512,6 +664,16 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
     // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
+      if (Q4 && frame != 0) {
+        const float f = __builtin_ldexpf(1.0f, frame);
+#pragma unroll
+        for (auto& x : acc)
+#pragma unroll
+          for (auto& o : x.o)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] *= f;
+        frame = 0;
+      }
       const int t_end = min((z0 + 16 * CT - 1) / a.rep, s.n - 1);  // last token of these slots
       int k_lo = 0;                                                // the first one that any of them sees
       if (a.row_begin) {
@@ -527,7 +689,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
         v4u kr[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          kr[ks] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + s_dim<Q8>(qd, ks)));
+          kr[ks] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(kp + s_dim<D, P>(qd, ks)));
         uint32_t v[4][D / 32];
         bool odd = false;
 #pragma unroll
@@ -567,7 +729,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
             f[i] = 1.0f;
           }
           v4u hi, lo;
-          s_softmax<D, false>(y, f, x, hi, lo);
+          s_softmax<D, false, LIFT>(y, f, x, hi, lo);
           if (__builtin_amdgcn_ballot_w64(odd) != 0) {
 #pragma unroll 1
             for (int key = k0; key < k0 + left; ++key) {
@@ -581,17 +743,156 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
           }
 #pragma unroll
           for (int dt = 0; dt < D / 16; ++dt) {
-            const v4u v8 = s_vfrag<D, false, 4>(v, dt);
+            const v4u v8 = s_vfrag<D, kBf16, 4>(v, dt);
             x.o[dt] = mfma16(v8, hi, x.o[dt]);
             x.o[dt] = mfma16(v8, lo, x.o[dt]);
           }
         }
       }
     };
-    if constexpr (D < 256) new_tokens();
+    constexpr bool first = D < 256 && !Q4;
+    if constexpr (first) new_tokens();
 
     // one tile's scores, softmax and products
-    auto products = [&](STile<D, Q8>& tl) {
+    bool framed = false;  // 4-bit pages: whether O has a frame
+    int qexp[CT];
+    if constexpr (Q4) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) qexp[ct] = qe[16 * ct + j];
+    }
+    auto products4 = [&](auto& tl) {
+      using T = std::decay_t<decltype(tl)>;
+      // the largest scales: K's in the low halves, V's in the high ones
+      uint32_t big = 0;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t w = tl.ks[r][0];
+        if constexpr (D == 256) {
+          big = od_absmax_bf16x2(big, tl.ks[r][1] | tl.vs[r] << 16);
+          w |= tl.vs[r] & 0xffff0000u;
+        } else {
+          w |= tl.vs[r] << 16;
+        }
+        big = od_absmax_bf16x2(big, w);
+      }
+      uint32_t all = s_wave_max2(big);
+      if ((all & 0xffffu) >= 0x7f80u || (all >> 16) >= 0x7f80u) {  // some are not finite: those that are
+        big = 0;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          big = od_absmax_bf16x2(big, fin_bf16x2(tl.ks[r][0] | tl.vs[r] << 16));
+          if constexpr (D == 256) big = od_absmax_bf16x2(big, fin_bf16x2(tl.ks[r][1] | (tl.vs[r] & 0xffff0000u)));
+        }
+        all = s_wave_max2(big);
+      }
+      const int kexp = q4_frame(all & 0xffffu), vexp = q4_frame(all >> 16);
+      if (all >> 16 && (!framed || vexp - 7 > frame)) {  // wave-uniform
+        if (framed) {
+          const float f = __builtin_ldexpf(1.0f, frame - (vexp - 7));
+#pragma unroll
+          for (auto& x : acc)
+#pragma unroll
+            for (auto& o : x.o)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[i] *= f;
+        }
+        frame = vexp - 7;
+        framed = true;
+      }
+      v4f sc[CT][2];
+#pragma unroll
+      for (auto& c2 : sc) c2[0] = c2[1] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int c4 = 0; c4 < T::KC; ++c4) {
+        Q4Scale q[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const _Float16 h = (_Float16)__builtin_ldexpf(__uint_as_float(tl.ks[r][c4] << 16), 7 - kexp);
+          q[r] = q4_pair(f16x2{h, h});  // (an infinite scale makes NaN: inf - inf)
+        }
+#pragma unroll
+        for (int w = 0; w < T::KW; ++w) {
+          v4u qf[CT];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            qf[ct] = __builtin_bit_cast(v4u, *reinterpret_cast<const uint4*>(sm.q16 + (16 * ct + j) * QR +
+                                                                            s_dim<D, P>(qd, 4 * c4 + w)));
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const v4u k8 = q4x8_f16(tl.k[r][c4][w], q[r]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) sc[ct][r] = mfma16h(k8, qf[ct], sc[ct][r]);
+          }
+        }
+      }
+      v4u pb[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float c2 = score_factor(a.scale_log2, qexp[ct] - 14 + kexp - 7);
+        float y[8], p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = sc[ct][i >> 2][i & 3] * c2;
+        if (tl.len[0] + tl.len[1] != 32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
+        }
+        s_probabilities<D, LIFT>(y, acc[ct], p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f16x2 w = {(_Float16)p[2 * e], (_Float16)p[2 * e + 1]};
+          pb[ct][e] = __builtin_bit_cast(uint32_t, w);
+        }
+      }
+      // V's scales of the lane's columns and of its 8 keys, in pairs of keys
+      Q4Scale vq[4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const _Float16 h0 = (_Float16)__builtin_ldexpf(__uint_as_float(tl.vs[r] << 16), -frame);
+        uint32_t mine = __builtin_bit_cast(uint16_t, h0);
+        if constexpr (D == 256) {
+          const _Float16 h1 = (_Float16)__builtin_ldexpf(__uint_as_float(tl.vs[r] & 0xffff0000u), -frame);
+          mine |= (uint32_t)__builtin_bit_cast(uint16_t, h1) << 16;
+        }
+        uint32_t of[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int from = D == 64 ? 8 * qd + 2 * i + (j >> 3) : 16 * qd + 4 * i + (j >> 2);
+          of[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)mine);
+        }
+        const uint32_t sel = D == 256 && (j & 2) ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          vq[2 * r + i] = q4_pair(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(of[2 * i + 1], of[2 * i], sel)));
+      }
+      // columns dt: value dt of the lane's D / 16, from the words of two keys the even values and the odd ones side by side
+      constexpr int WORDS = D == 256 ? 2 : 1, PER = D == 64 ? 2 : 4;  // value pairs of a word
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        uint32_t even[4], odd[4];
+#pragma unroll
+        for (int k2 = 0; k2 < 4; ++k2) {
+          uint32_t x0 = tl.v[2 * k2][w], x1 = tl.v[2 * k2 + 1][w];
+          if constexpr (D == 64) x0 >>= 8 * (j & 1), x1 >>= 8 * (j & 1);
+          even[k2] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+          odd[k2] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+        }
+#pragma unroll
+        for (int dt = 0; dt < 2 * PER; ++dt) {
+          v4u v8;
+#pragma unroll
+          for (int k2 = 0; k2 < 4; ++k2) {
+            const uint32_t x = dt & 1 ? odd[k2] : even[k2];
+            const uint32_t at = dt / 2 == 0 ? x << 6 : dt / 2 == 1 ? x << 2 : dt / 2 == 2 ? x >> 2 : x >> 6;
+            const f16x2 u = __builtin_bit_cast(f16x2, (at & 0x03c003c0u) | 0x4c004c00u);
+            v8[k2] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, vq[k2].s, vq[k2].c));
+          }
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct].o[8 * w + dt] = mfma16h(v8, pb[ct], acc[ct].o[8 * w + dt]);
+        }
+      }
+    };
+    auto products = [&](auto& tl) {
       if constexpr (Q8) {  // in-order LDS access within the wave; lanes c and c + 32 write the same value
         // (an infinite scale as NaN: a score of -inf would be no key)
         reinterpret_cast<float*>(skf[wave][0])[c] = tl.ks < INFINITY ? tl.ks * a.scale_log2 : NAN;
@@ -643,7 +944,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
           for (int i = 0; i < 4 * R; ++i)
             if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
-        s_softmax<D, Q8>(y, f, acc[ct], hi[ct], lo[ct]);
+        s_softmax<D, Q8, LIFT>(y, f, acc[ct], hi[ct], lo[ct]);
       }
       if constexpr (!Q8) {
         // The low part of a probability may be 0 or negative: infinities and NaN among the values are taken by the high
@@ -656,7 +957,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
         if (__builtin_amdgcn_ballot_w64((m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u) != 0) {
 #pragma unroll
           for (int dt = 0; dt < D / 16; ++dt) {
-            const v4u v8 = s_vfrag<D, Q8, 4 * R>(tl.v, dt), fin = fin_bf16x8(v8);
+            const v4u v8 = s_vfrag<D, P, 4 * R>(tl.v, dt), fin = fin_bf16x8(v8);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) acc[ct].o[dt] = mfma16(v8 ^ fin, hi[ct], acc[ct].o[dt]);
           }
@@ -668,7 +969,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
       }
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
-        const v4u v8 = s_vfrag<D, Q8, 4 * R>(tl.v, dt);
+        const v4u v8 = s_vfrag<D, P, 4 * R>(tl.v, dt);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
           acc[ct].o[dt] = mfma16(v8, hi[ct], acc[ct].o[dt]);
@@ -681,14 +982,15 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
 #pragma unroll
         for (int i = 0; i < SETS; ++i) {
           next(tl[(i + SETS - 1) % SETS]);
-          products(tl[i]);
+          if constexpr (Q4) products4(tl[i]);
+          else products(tl[i]);
           tt += NW;
           if (!(more = tt < t_hi)) break;
         }
       }
     }
 
-    if constexpr (D == 256) new_tokens();
+    if constexpr (!first) new_tokens();
 
     // merge the waves, then the output or this split's normalized partial
 #pragma unroll
@@ -707,6 +1009,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
         sml[wave][0][j] = x.m;
         sml[wave][1][j] = l;
       }
+      if (Q4 && lane == 0) frames[wave] = frame;
       __syncthreads();
       for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
         const int zz = i / (D / 4), d0 = (i % (D / 4)) * 4, z = z0 + 16 * ct + zz;
@@ -716,21 +1019,33 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, Q8, CT) ? 1 : 2) void
         for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][0][zz]);
         float L = 0.0f;
         float4 sum = make_float4(0, 0, 0, 0);
+        int top = -(1 << 20);  // 4-bit pages: the highest frame of a wave that has seen a key
+        if constexpr (Q4) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w)
+            if (sml[w][0][zz] != -INFINITY) top = max(top, frames[w]);
+        }
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           const float mw = sml[w][0][zz];
-          const float e = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+          float e = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
           const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][zz][d0]);
           L += e * sml[w][1][zz];
+          if constexpr (Q4) e = mw == -INFINITY ? 0.0f : __builtin_ldexpf(e, frames[w] - top);
           sum.x += e * v.x;
           sum.y += e * v.y;
           sum.z += e * v.z;
           sum.w += e * v.w;
         }
         // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L);
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L) - (float)LIFT;
         const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
         sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        if constexpr (Q4) {
+          if (top > -(1 << 20))
+            sum = make_float4(__builtin_ldexpf(sum.x, top), __builtin_ldexpf(sum.y, top), __builtin_ldexpf(sum.z, top),
+                              __builtin_ldexpf(sum.w, top));
+        }
         if (nv == 1) {
           *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(sum.x, sum.y),
               od_pack_bf16x2(sum.z, sum.w));
@@ -825,7 +1140,6 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
 // The next block's loads are in flight during a block's products; its conversion into the other LDS buffer comes first
 // in the next step. Cached keys behind the last one, and pages that are none, enter as zeros with masked scores.
 constexpr int kBK = 64;
-constexpr float kLift = 7.0f;  // probabilities are kept 2^kLift above their value
 
 // K rows in LDS: 16-byte chunks XORed so that 16 rows hit 16 bank groups
 template <int D>
@@ -897,9 +1211,6 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
 }
 __device__ __forceinline__ v16f zero16() { return v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
 
-// exponent e with x < 2^e for the bits of a finite x > 0; 0 for 0
-__device__ __forceinline__ int exp_above(uint32_t bits) { return bits ? (int)(bits >> 23) - 126 : 0; }
-
 // 16 int8 times f, each product rounded once to fp16: byte u = q + 128 becomes the fp16 1024 + u by its bits, and (1024
 // + u) f - 1152 f is one fp32 fma per value (v_fma_mix). f has its last 4 bits clear (frame_scale), so that 1152 f is
 // exact and the result is q f rounded once, 0 for q = 0.
@@ -922,35 +1233,6 @@ __device__ __forceinline__ float frame_scale(float s, int e) {
   return __uint_as_float(__float_as_uint(__builtin_ldexpf(s, e)) & ~15u);
 }
 
-// A word of 8 four-bit values times their scale, as fp16, in order. A value u at bits 6 to 9 of 16.0's fp16 is 16 + u, so a pair
-// is one shift, one and-or and one fma with 24 s: u - 8 has 3 significant bits and s 8 (f16_scale), so that 24 s and the result
-// are exact (12 instructions a word).
-struct Q4Scale {
-  f16x2 s, c;  // s and -24 s
-};
-__device__ __forceinline__ Q4Scale q4_pair(f16x2 s) {
-  const f16x2 k = {(_Float16)-24.0f, (_Float16)-24.0f};
-  return {s, s * k};
-}
-__device__ __forceinline__ v4u q4x8_f16(uint32_t w, const Q4Scale& q) {
-  const uint32_t at[4] = {w << 6, w << 2, w >> 2, w >> 6};
-  v4u r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f16x2 x = __builtin_bit_cast(f16x2, (at[i] & 0x03c003c0u) | 0x4c004c00u);
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, q.s, q.c));
-  }
-  return r;
-}
-// A bf16 scale times 2^e in fp16, NaN where it is not finite (an infinite one would make scores of -inf, which are no keys);
-// exact unless it falls below fp16's normal numbers.
-__device__ __forceinline__ _Float16 f16_scale(uint32_t bits, int e) {
-  const float s = (bits & 0x7f80u) == 0x7f80u ? NAN : __uint_as_float(bits << 16);
-  return (_Float16)__builtin_ldexpf(s, e);
-}
-// The frame of 4-bit values whose largest scale has these bf16 bits: 2^E above it, and values below 8 times it, so that q 2^(7 -
-// (E - 4)) is below 2^14, as for int8.
-__device__ __forceinline__ int q4_frame(uint32_t bits) { return bits ? (int)(bits >> 7) - 126 - 4 : 0; }
 // The largest magnitude of the finite ones of N packed pairs of bf16 scales, as bits.
 template <int N>
 __device__ __forceinline__ uint32_t q4_largest(const uint32_t (&w)[N]) {
@@ -1031,12 +1313,6 @@ __device__ __forceinline__ void t_q_to_f16(TSlot<D>& t) {
                        (_Float16)__builtin_ldexpf(__uint_as_float(w & 0xffff0000u), 14 - t.qe)};
       t.q[ks][i] = __builtin_bit_cast(uint32_t, r);
     }
-}
-
-// The factor scale 2^e of a block's fp16 scores (of 2^36 at most), a number above 0 whatever the exponents: the scores of
-// masked keys are -inf ahead of it, and 2^-126 makes any score as good as 0.
-__device__ __forceinline__ float score_factor(float scale_log2, int e) {
-  return __builtin_amdgcn_fmed3f(__builtin_ldexpf(scale_log2, e), 0x1p-126f, 0x1.fffffep127f);
 }
 
 // S^T of one block.
@@ -2055,9 +2331,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // 100 15 and 24; 32 over 2 x 4000 21 and 32; above it 32 over 1 x 32000 62 and 50, bf16 80 and 42, 120 of one head
   // over 1 x 8000 bf16 tokens 37 and 34.
   const int64_t few = B * Hkv * ((slots + 31) / 32);
-  const int64_t always = q8 && D <= 128 && Hkv < (1 << 15) ? 64 : 32;  // (a grid has 65535 rows)
+  const int64_t always = (q8 || q4) && D <= 128 && Hkv < (1 << 15) ? 64 : 32;  // (a grid has 65535 rows)
   p.stream = slots <= always || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
-  if (q4) p.stream = false;
   p.ct = slots <= 16 ? 1 : 2;
   // workgroups without splits for tiles of spt slots: every sequence's, but no more than the tokens make
   auto wgs_of = [&](int64_t spt) {
@@ -2071,12 +2346,12 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // (bf16 chunks of 2048 over 16000 234 and 202).
   const bool wide8 = D == 128 && slots > 128 && (B == 1 || wgs_of(256) >= cus);
   p.nw = p.stream ? kStreamWaves : D == 256 || wide8 ? 8 : 4;
-  p.width = p.stream ? 16 * s_halves((int)D) : kBK;
+  p.width = p.stream ? 16 * s_halves((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16) : kBK;
   const int64_t spt = p.stream ? 16 * p.ct : D == 256 ? 128 : 32 * p.nw;
   const int64_t tiles = (slots + spt - 1) / spt, wgs = wgs_of(spt), keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
   // how many run at once: two a CU, one where a wave or the shared memory needs it whole
-  const bool one = p.stream ? s_alone((int)D, q8, p.ct) : p.nw == 8;
+  const bool one = p.stream ? s_alone((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16, p.ct) : p.nw == 8;
   const int64_t fit = one ? cus : 2 * cus;
   // key tiles that are worth a workgroup of their own (128 tokens over 1 x 1000: 37 us with 8 blocks at least, 35 with
   // 2)
@@ -2343,15 +2618,14 @@ extern "C" int od_paged_attn_ex(const uint16_t* q, int64_t sqt, int64_t sqh, con
       else if (p.nw == 8) rc = launch_tiles<DD, SRC, 8>(a, (unsigned)groups, st);
       else rc = launch_tiles<DD, SRC, 4>(a, (unsigned)groups, st);
     };
-    auto stream = [&](auto QC) {
-      constexpr bool Q8 = decltype(QC)::value;
+    auto stream = [&](auto PC) {
+      constexpr int P = decltype(PC)::value;
       const dim3 grid((unsigned)p.nsplit, (unsigned)(Hkv * p.tiles), (unsigned)B);
-      if (p.ct == 1) paged_stream_kernel<DD, Q8, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
-      else paged_stream_kernel<DD, Q8, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+      if (p.ct == 1) paged_stream_kernel<DD, P, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+      else paged_stream_kernel<DD, P, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
     };
     if (p.stream) {
-      if (format == OD_PAGE_INT8) stream(std::true_type{});
-      else stream(std::false_type{});
+      by_format(format, stream);
     } else if (format == OD_PAGE_BF16) {
       tiles(std::integral_constant<int, kBf16>{});
     } else {
