@@ -285,15 +285,21 @@ __device__ __forceinline__ Q4Scale q4_pair(f16x2 s) {
   const f16x2 k = {(_Float16)-24.0f, (_Float16)-24.0f};
   return {s, s * k};
 }
-__device__ __forceinline__ v4u q4x8_f16(uint32_t w, const Q4Scale& q) {
-  const uint32_t at[4] = {w << 6, w << 2, w >> 2, w >> 6};
-  v4u r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f16x2 x = __builtin_bit_cast(f16x2, (at[i] & 0x03c003c0u) | 0x4c004c00u);
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, q.s, q.c));
-  }
-  return r;
+// 16 in both halves, from a vector register: the and-or takes one scalar operand, which is the mask.
+__device__ __forceinline__ uint32_t q4_sixteen() {
+  uint32_t b = 0x4c004c00u;
+  asm("" : "+v"(b));
+  return b;
+}
+// Pair i of a word's (bits 4 i of both halves), times its scale.
+__device__ __forceinline__ uint32_t q4_pair_f16(uint32_t w, int i, const Q4Scale& q, uint32_t sixteen) {
+  const uint32_t at = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
+  const f16x2 x = __builtin_bit_cast(f16x2, (at & 0x03c003c0u) | sixteen);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, q.s, q.c));
+}
+__device__ __forceinline__ v4u q4x8_f16(uint32_t w, const Q4Scale& q, uint32_t sixteen) {
+  return v4u{q4_pair_f16(w, 0, q, sixteen), q4_pair_f16(w, 1, q, sixteen), q4_pair_f16(w, 2, q, sixteen),
+             q4_pair_f16(w, 3, q, sixteen)};
 }
 // A bf16 scale times 2^e in fp16, NaN where it is not finite (an infinite one would make scores of -inf, which are no keys);
 // exact unless it falls below fp16's normal numbers.
@@ -342,6 +348,9 @@ struct STile {
   float ks, vs;  // lane l: the scales of key l % 32
   int len[R];    // keys of the half tiles (wave-uniform)
 };
+// The key of a half tile that is row r of the products: those of the four lane groups lie side by side, so that a load of V takes
+// whole lines (a row of heads of 128 has half a line).
+__device__ __forceinline__ constexpr int s_key4(int r) { return 4 * (r & 3) + (r >> 2); }
 template <int D>
 struct STile<D, kInt4> {
   static constexpr int R = 2, KC = D == 256 ? 2 : 1, KW = D / 32 / KC, VB = D == 256 ? 8 : 4;
@@ -439,7 +448,7 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
       const auto sk = rsrc(a.p.k4 + row * (D / 32), x.len[r] * (D / 16)), sv = rsrc(a.p.v4 + row * (D / 32), x.len[r] * (D / 16));
 #pragma unroll
       for (int c = 0; c < T::KC; ++c) {
-        const int at = j * (D / 2) + 64 * c + 4 * T::KW * gl;
+        const int at = s_key4(j) * (D / 2) + 64 * c + 4 * T::KW * gl;
         if constexpr (T::KW == 4) {
           const v4u u = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(dk, at, 0, kOnce));
 #pragma unroll
@@ -448,11 +457,11 @@ __device__ __forceinline__ void s_load(const AttnArgs& a, const Seq& s, int g, i
           const auto u = __builtin_amdgcn_raw_buffer_load_b64(dk, at, 0, kOnce);
           x.k[r][c][0] = u[0], x.k[r][c][1] = u[1];
         }
-        x.ks[r][c] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sk, 2 * (j * (D / 32) + 4 * c + (D == 64 ? gl / 2 : gl)), 0, 0);
+        x.ks[r][c] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sk, 2 * (s_key4(j) * (D / 32) + 4 * c + (D == 64 ? gl / 2 : gl)), 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // heads of 64: two lanes share a word
-        const int at = (4 * gl + i) * (D / 2) + (D == 64 ? 4 * (j / 2) : T::VB * j);
+        const int at = s_key4(4 * gl + i) * (D / 2) + (D == 64 ? 4 * (j / 2) : T::VB * j);
         if constexpr (T::VB == 4) {
           x.v[4 * r + i][0] = __builtin_amdgcn_raw_buffer_load_b32(dv, at, 0, kOnce);
         } else {
@@ -483,8 +492,9 @@ struct SAcc {
   v4f o[D / 16];
 };
 
-// One tile's online softmax: y the lane's 8 scores (log2 units, -inf masked); p out, 2^LIFT above its value.
-template <int D, int LIFT>
+// One tile's online softmax: y the lane's 8 scores (log2 units, -inf masked); p out, 2^s_lift above its value.
+constexpr float s_lift(int P) { return P == kInt4 ? kLift : 0.0f; }
+template <int P, int D>
 __device__ __forceinline__ void s_probabilities(float (&y)[8], SAcc<D>& x, float (&p)[8]) {
   float mx = y[0];
 #pragma unroll
@@ -501,18 +511,47 @@ __device__ __forceinline__ void s_probabilities(float (&y)[8], SAcc<D>& x, float
     x.l *= c;
     if (move) x.m = mx;
   }
-  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - (float)LIFT;
+  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - s_lift(P);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     p[i] = __builtin_amdgcn_exp2f(y[i] - ms);
     x.l += p[i];
   }
 }
+// The same from scores in units of 1 / c (c > 0), into fp16.
+template <int D>
+__device__ __forceinline__ v4u s_half(const float (&y)[8], float c, SAcc<D>& x) {
+  float mx = y[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, y[i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = od_xor32_max(mx) * c;
+  const bool move = mx > x.m + kSlack;
+  if (__builtin_amdgcn_ballot_w64(move) != 0) {
+    const float f = move ? __builtin_amdgcn_exp2f(x.m - mx) : 1.0f;  // m = -inf: 0
+#pragma unroll
+    for (auto& o : x.o) o *= f;
+    x.l *= f;
+    if (move) x.m = mx;
+  }
+  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - kLift;
+  v4u r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * e], c, -ms));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * e + 1], c, -ms));
+    x.l += p0;
+    x.l += p1;
+    const f16x2 w = {(_Float16)p0, (_Float16)p1};
+    r[e] = __builtin_bit_cast(uint32_t, w);
+  }
+  return r;
+}
 // The same into bf16 hi and lo parts: f a factor on p for the P.V product only (the V scales).
-template <int D, bool F, int LIFT>
+template <int D, int P, bool F>
 __device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
   float p[8];
-  s_probabilities<D, LIFT>(y, x, p);
+  s_probabilities<P>(y, x, p);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float u = F ? p[2 * e] * f[2 * e] : p[2 * e], w = F ? p[2 * e + 1] * f[2 * e + 1] : p[2 * e + 1];
@@ -556,13 +595,15 @@ __device__ __forceinline__ uint32_t s_wave_max2(uint32_t x) {
 }
 
 constexpr int kStreamWaves = 4;
-// whether a wave has a SIMD's registers to itself
-constexpr bool s_alone(int D, int P, int columns) { return D * columns >= (P == kBf16 ? 256 : 512); }
+// waves a SIMD's registers hold
+constexpr int s_waves(int D, int P, int columns) {
+  if (D * columns >= (P == kBf16 ? 256 : 512)) return 1;
+  return P == kInt4 && D <= 128 && columns == 1 ? 3 : 2;
+}
 
 template <int D, int P, int CT>
-__global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kStreamWaves * 64, s_waves(D, P, CT)) void paged_stream_kernel(AttnArgs a) {
   constexpr bool Q8 = P == kInt8, Q4 = P == kInt4;
-  constexpr int LIFT = Q4 ? (int)kLift : 0;
   using Tile = STile<D, P>;
   // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
   constexpr int NW = kStreamWaves, KS = D / 32, R = s_halves(D, P), QR = D + 8;
@@ -729,7 +770,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
             f[i] = 1.0f;
           }
           v4u hi, lo;
-          s_softmax<D, false, LIFT>(y, f, x, hi, lo);
+          s_softmax<D, P, false>(y, f, x, hi, lo);
           if (__builtin_amdgcn_ballot_w64(odd) != 0) {
 #pragma unroll 1
             for (int key = k0; key < k0 + left; ++key) {
@@ -754,50 +795,47 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
     if constexpr (first) new_tokens();
 
     // one tile's scores, softmax and products
-    bool framed = false;  // 4-bit pages: whether O has a frame
+    // 4-bit pages: the largest scales within the frames, as bits (0 at first: no frame yet), K's frame
+    uint32_t bound = 0;
+    int kexp = 0;
     int qexp[CT];
     if constexpr (Q4) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) qexp[ct] = qe[16 * ct + j];
     }
-    auto products4 = [&](auto& tl) {
+    auto products4 = [&](auto& tl, auto& acc) {
       using T = std::decay_t<decltype(tl)>;
-      // the largest scales: K's in the low halves, V's in the high ones
-      uint32_t big = 0;
+      const uint32_t sixteen = q4_sixteen();
+      // Scales past the frames (K's in the low halves of a word, V's in the high ones): rare, the frames then rise.
+      uint32_t big = bound;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        uint32_t w = tl.ks[r][0];
-        if constexpr (D == 256) {
-          big = od_absmax_bf16x2(big, tl.ks[r][1] | tl.vs[r] << 16);
-          w |= tl.vs[r] & 0xffff0000u;
-        } else {
-          w |= tl.vs[r] << 16;
-        }
-        big = od_absmax_bf16x2(big, w);
+        big = od_absmax_bf16x2(big, tl.ks[r][0] | tl.vs[r] << 16);
+        if constexpr (D == 256) big = od_absmax_bf16x2(big, tl.ks[r][1] | (tl.vs[r] & 0xffff0000u));
       }
-      uint32_t all = s_wave_max2(big);
-      if ((all & 0xffffu) >= 0x7f80u || (all >> 16) >= 0x7f80u) {  // some are not finite: those that are
-        big = 0;
+      if (__builtin_amdgcn_ballot_w64(big != bound) != 0) {
+        big = bound;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < 2; ++r) {  // the finite ones
           big = od_absmax_bf16x2(big, fin_bf16x2(tl.ks[r][0] | tl.vs[r] << 16));
           if constexpr (D == 256) big = od_absmax_bf16x2(big, fin_bf16x2(tl.ks[r][1] | (tl.vs[r] & 0xffff0000u)));
         }
-        all = s_wave_max2(big);
-      }
-      const int kexp = q4_frame(all & 0xffffu), vexp = q4_frame(all >> 16);
-      if (all >> 16 && (!framed || vexp - 7 > frame)) {  // wave-uniform
-        if (framed) {
-          const float f = __builtin_ldexpf(1.0f, frame - (vexp - 7));
+        big = s_wave_max2(big) | 0x007f007fu;
+        if ((big & 0xffffu) > (bound & 0xffffu)) kexp = q4_frame(big & 0xffffu);
+        if (big >> 16 > bound >> 16) {
+          const int to = q4_frame(big >> 16) - 7;
+          if (bound >> 16) {
+            const float f = __builtin_ldexpf(1.0f, frame - to);
 #pragma unroll
-          for (auto& x : acc)
+            for (auto& x : acc)
 #pragma unroll
-            for (auto& o : x.o)
+              for (auto& o : x.o)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] *= f;
+                for (int i = 0; i < 4; ++i) o[i] *= f;
+          }
+          frame = to;
         }
-        frame = vexp - 7;
-        framed = true;
+        bound = big;
       }
       v4f sc[CT][2];
 #pragma unroll
@@ -819,7 +857,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
                                                                             s_dim<D, P>(qd, 4 * c4 + w)));
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const v4u k8 = q4x8_f16(tl.k[r][c4][w], q[r]);
+            const v4u k8 = q4x8_f16(tl.k[r][c4][w], q[r], sixteen);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) sc[ct][r] = mfma16h(k8, qf[ct], sc[ct][r]);
           }
@@ -828,21 +866,16 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
       v4u pb[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const float c2 = score_factor(a.scale_log2, qexp[ct] - 14 + kexp - 7);
-        float y[8], p[8];
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = sc[ct][i >> 2][i & 3] * c2;
-        if (tl.len[0] + tl.len[1] != 32) {
+        for (int i = 0; i < 8; ++i) y[i] = sc[ct][i >> 2][i & 3];
+        if (__builtin_expect(tl.len[0] + tl.len[1] != 32, 0)) {
+          asm volatile("");  // a branch: else the comparisons are made for every tile
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
+            if (s_key4(4 * qd + (i & 3)) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
-        s_probabilities<D, LIFT>(y, acc[ct], p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f16x2 w = {(_Float16)p[2 * e], (_Float16)p[2 * e + 1]};
-          pb[ct][e] = __builtin_bit_cast(uint32_t, w);
-        }
+        pb[ct] = s_half<D>(y, score_factor(a.scale_log2, qexp[ct] - 14 + kexp - 7), acc[ct]);
       }
       // V's scales of the lane's columns and of its 8 keys, in pairs of keys
       Q4Scale vq[4];
@@ -857,7 +890,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
         uint32_t of[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int from = D == 64 ? 8 * qd + 2 * i + (j >> 3) : 16 * qd + 4 * i + (j >> 2);
+          const int from = D == 64 ? 2 * s_key4(4 * qd + i) + (j >> 3) : 4 * s_key4(4 * qd + i) + (j >> 2);
           of[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)mine);
         }
         const uint32_t sel = D == 256 && (j & 2) ? 0x07060302u : 0x05040100u;
@@ -882,10 +915,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
           v4u v8;
 #pragma unroll
           for (int k2 = 0; k2 < 4; ++k2) {
-            const uint32_t x = dt & 1 ? odd[k2] : even[k2];
-            const uint32_t at = dt / 2 == 0 ? x << 6 : dt / 2 == 1 ? x << 2 : dt / 2 == 2 ? x >> 2 : x >> 6;
-            const f16x2 u = __builtin_bit_cast(f16x2, (at & 0x03c003c0u) | 0x4c004c00u);
-            v8[k2] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, vq[k2].s, vq[k2].c));
+            v8[k2] = q4_pair_f16(dt & 1 ? odd[k2] : even[k2], dt / 2, vq[k2], sixteen);
           }
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) acc[ct].o[8 * w + dt] = mfma16h(v8, pb[ct], acc[ct].o[8 * w + dt]);
@@ -944,7 +974,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
           for (int i = 0; i < 4 * R; ++i)
             if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
-        s_softmax<D, Q8, LIFT>(y, f, acc[ct], hi[ct], lo[ct]);
+        s_softmax<D, P, Q8>(y, f, acc[ct], hi[ct], lo[ct]);
       }
       if constexpr (!Q8) {
         // The low part of a probability may be 0 or negative: infinities and NaN among the values are taken by the high
@@ -982,7 +1012,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
 #pragma unroll
         for (int i = 0; i < SETS; ++i) {
           next(tl[(i + SETS - 1) % SETS]);
-          if constexpr (Q4) products4(tl[i]);
+          if constexpr (Q4) products4(tl[i], acc);
           else products(tl[i]);
           tt += NW;
           if (!(more = tt < t_hi)) break;
@@ -1038,7 +1068,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, s_alone(D, P, CT) ? 1 : 2) void 
           sum.w += e * v.w;
         }
         // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L) - (float)LIFT;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L) - s_lift(P);
         const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
         sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
         if constexpr (Q4) {
@@ -1259,10 +1289,11 @@ __device__ __forceinline__ void q4_row_scales(const uint16_t* scales, int64_t ro
 template <int D>
 __device__ __forceinline__ void q4_put(uint16_t* dst, bool v, int key, int c, const v4u& r, _Float16 s) {
   const Q4Scale q = q4_pair(f16x2{s, s});
+  const uint32_t sixteen = q4_sixteen();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int ch = 4 * c + i, at = v ? key * D + (tv_chunk<D>(key, ch) << 3) : tk_off<D>(key, ch);
-    *reinterpret_cast<uint4*>(dst + at) = __builtin_bit_cast(uint4, q4x8_f16(r[i], q));
+    *reinterpret_cast<uint4*>(dst + at) = __builtin_bit_cast(uint4, q4x8_f16(r[i], q, sixteen));
   }
 }
 
@@ -2350,9 +2381,9 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   const int64_t spt = p.stream ? 16 * p.ct : D == 256 ? 128 : 32 * p.nw;
   const int64_t tiles = (slots + spt - 1) / spt, wgs = wgs_of(spt), keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
-  // how many run at once: two a CU, one where a wave or the shared memory needs it whole
-  const bool one = p.stream ? s_alone((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16, p.ct) : p.nw == 8;
-  const int64_t fit = one ? cus : 2 * cus;
+  // how many run at once: two a CU, one where a wave or the shared memory needs it whole, three that stream 4-bit pages (8 ragged
+  // states of up to 32768 tokens 60 us in 12 splits, 66 in 8; 16 x 16000 59 and 61; but 64 x 4096 55 and 53)
+  const int64_t fit = cus * (p.stream ? s_waves((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16, p.ct) : p.nw == 8 ? 1 : 2);
   // key tiles that are worth a workgroup of their own (128 tokens over 1 x 1000: 37 us with 8 blocks at least, 35 with
   // 2)
   const int64_t least = p.stream ? 8 : 2;
