@@ -36,7 +36,8 @@ PROBE_LIB = os.path.join(PKG, "libod_probe.so")
 SOURCE_FLAGS = {"od_gdn_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 "od_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 "od_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                "od_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                "od_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "od_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Xclang", "-target-feature",
          "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-inline-asm"]

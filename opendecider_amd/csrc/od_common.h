@@ -139,6 +139,13 @@ __device__ __forceinline__ void od_dma16(const void* src, uint32_t lds_base) {
                : "memory", "m0");
 }
 
+// od_dma16 at a wave-uniform address plus the lane's offset in bytes. (Five wait states between a vector instruction
+// that writes a scalar register and a load that reads it: the compiler does not see the load.)
+__device__ __forceinline__ void od_dma16_at(const void* src, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(src)
+               : "memory", "m0");
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t od_lds_addr(T* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(p);

@@ -1198,12 +1198,6 @@ __device__ __forceinline__ void dma_rows(const uint16_t* lds, int wave, bool v, 
   }
 }
 
-// od_dma16 at a wave-uniform address plus the lane's offset in bytes. (Five wait states between a vector instruction
-// that writes a scalar register and a load that reads it: the compiler does not see the load.)
-__device__ __forceinline__ void dma16_at(const void* src, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(src)
-               : "memory", "m0");
-}
 // A block's bf16 rows from the pages; lane l has the page of key l. An instruction's 1 KB is 512 / D keys, which never
 // cross a page, so its address is one of the wave.
 template <int D, int NW>
@@ -1219,7 +1213,7 @@ __device__ __forceinline__ void dma_pages(const uint16_t* lds, int wave, bool v,
     const int key = lane / (D / 8), slot = lane % (D / 8);
     const int ch = v ? tv_chunk<D>(first + key, slot)
                      : slot ^ (D == 64 ? (((first + key) >> 1) & 7) : ((first + key) & 15));
-    dma16_at(pool + row * D, 2 * (key * D + 8 * ch), od_lds_addr(lds) + 1024 * (i * NW + wave));
+    od_dma16_at(pool + row * D, 2 * (key * D + 8 * ch), od_lds_addr(lds) + 1024 * (i * NW + wave));
   }
 }
 // The same from a block of the image, which lies in memory as it does in LDS.
@@ -1227,7 +1221,7 @@ template <int D, int NW>
 __device__ __forceinline__ void dma_block(const uint16_t* lds, int wave, const uint16_t* src) {
 #pragma unroll
   for (int i = 0; i < D / (8 * NW); ++i)
-    dma16_at(src + (i * NW + wave) * 512, 16 * (threadIdx.x & 63), od_lds_addr(lds) + 1024 * (i * NW + wave));
+    od_dma16_at(src + (i * NW + wave) * 512, 16 * (threadIdx.x & 63), od_lds_addr(lds) + 1024 * (i * NW + wave));
 }
 
 template <bool H>

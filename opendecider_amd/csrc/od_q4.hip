@@ -27,8 +27,10 @@ struct Q4Args {
   uint16_t* x16;
   int* xexp;
   float* part;
-  int64_t Kp;  // K in whole stages: the row stride of x16
-  int tiles_m, tiles_n, nsplit, stages;
+  int64_t Kp;  // K in whole stages
+  int tiles_m, tiles_n, nsplit, stages, bm;  // bm: the rows of a tile of x
+  // few rows: the turns of steps whose x lies in LDS at a time; 2^20 / (4 rows of x), rounded up
+  int held, per20;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
@@ -36,16 +38,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t by
 }
 
 // ------------------------------------------------------------------------------------------------ few rows of x
-// Bound by reading the weights. A workgroup's NW waves share 16 RT weight rows, each wave every NW-th step of 128 values (4
-// blocks of every row, 64 contiguous bytes), and add up in LDS. V_MFMA_F32_16X16X32_BF16 with the weights as the A operand, 16
-// rows, and up to 16 rows of x as the B operand, 32 values a time, which is one block: the sums of a block, exact in their
-// products, take the fp32 factor d afterwards, so no weight is rounded. Lane (j, g) = (lane % 16, lane / 16):
+// Bound by reading the weights. V_MFMA_F32_16X16X32_BF16 with 16 weight rows as the A operand and up to 16 rows of x as the B
+// operand, 32 values a time, which is one block: the sums of a block, exact in their products, take the fp32 factor d afterwards,
+// so no weight is rounded. A step of a wave is 4 blocks of 16 weight rows (64 contiguous bytes of each). Lane (j, g) = (lane % 16,
+// lane / 16):
 //  * reads block 4 s + g of weight row j, 16 bytes; four lane exchanges (a transposition over g) give it word g of each of the
 //    four blocks: values 4 g .. 4 g + 3 and 16 + 4 g .. + 3 of the block;
 //  * four bits u at the bottom of 128.0's bf16 are 128 + u: one shift and one and-or for two values. The 136 that it is above
-//    u - 8 leaves by the C operand, -136 times the sum of x over the block, itself a product with a constant A (shared by the RT
-//    row tiles). (A row of x that holds an infinity or NaN so becomes NaN.)
+//    u - 8 leaves by the C operand, -136 times the sum of x over the block, itself a product with a constant A. (A row of x that
+//    holds an infinity or NaN so becomes NaN.)
 //  * holds weight rows 4 g + i of column j of the result; d of row 4 g + i and block b is the one that lane 16 g + 4 i + b loaded.
+// A workgroup's WR x WK waves take WR sets of RT row tiles, WK of them every WK-th step of one, and add up in LDS. x lies in LDS in
+// the order of the B operand, as many steps of it as fit at a time, two buffers of it; the weights of the PD next steps are in
+// registers or on their way meanwhile, whatever the workgroup waits for. One row of x: 4096 x 4096 8.9 us (9.4 MB), 24576 x 4096
+// 20.6 us (2.8 TB/s), 151936 x 4096 87 us (4.0 TB/s); 24 rows over 24576 x 4096 31 us, where it is the products and the exchanges.
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
@@ -57,11 +63,12 @@ __device__ __forceinline__ void transpose4(v4u& w) {
   const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   w = v4u{c[0], c[1], e[0], e[1]};
 }
-// 8 values as bf16 128 + u, in the order 0 2 16 18 1 3 17 19 (from 4 g)
-__device__ __forceinline__ v4u raised(uint32_t t) {
+// 8 values as bf16 128 + u, in the order 0 2 16 18 1 3 17 19 (from 4 g); base: 128 in both halves, from a vector register (the
+// and-or takes one scalar operand, which is the mask)
+__device__ __forceinline__ v4u raised(uint32_t t, uint32_t base) {
   v4u r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = ((t >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  for (int i = 0; i < 4; ++i) r[i] = ((t >> (4 * i)) & 0x000f000fu) | base;
   return r;
 }
 // x in that order
@@ -75,11 +82,10 @@ __device__ __forceinline__ float row_lane(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xf, 0xf, true));
 }
 
-template <int RT, int CT>
+template <int RT>
 struct Q4Step {
   v4u w[RT];
   uint32_t d[RT];
-  v2u x[CT][4][2];
 };
 
 __device__ __forceinline__ void q4_store(const Q4Args& a, int64_t m, int64_t n, v4f y) {
@@ -99,35 +105,65 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, int64_t m, int64_t n, 
   }
 }
 
-template <int RT, int CT, int NW>
-__global__ __launch_bounds__(NW * 64) void q4_rows_kernel(Q4Args a) {
-  __shared__ float4 red[NW][RT * CT][64];
+// A buffer of x in LDS holds up to 2048 units of 8 values. A unit's tokens lie 16 bytes apart, its rows (tokens | 1) times that: the
+// four that a token writes, or reads, at once are in other banks.
+constexpr int kXUnits = 2048, kXBytes = 16 * kXUnits / 16 * 17;
+
+template <int RT, int CT, int WK, int WR, int PD>
+__global__ __launch_bounds__(WK * WR * 64) void q4_rows_kernel(Q4Args a) {
+  constexpr int NT = WK * WR * 64;
+  extern __shared__ __attribute__((aligned(16))) char lds_x[];  // x: [step][block][g][token] 16 bytes; at the end the waves' sums
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * RT), m0 = (int64_t)blockIdx.y * (16 * CT);
-  const int rows = (int)min((int64_t)16 * RT, a.N - n0), toks = (int)min((int64_t)16 * CT, a.M - m0), blocks = (int)(a.K / 32);
-  const auto rw = rsrc(a.qs + n0 * a.ldq, (rows - 1) * a.ldq + a.K / 2);
-  const auto rd = rsrc(a.d + n0 * a.ldd, ((rows - 1) * a.ldd + blocks) * 2);
-  const auto rx = rsrc(a.x + m0 * a.ldx, ((toks - 1) * a.ldx + a.K) * 2);
+  const int wr = wave / WK, wk = wave % WK;
+  const int64_t n0 = ((int64_t)blockIdx.x * WR + wr) * (16 * RT);
+  const int rows = (int)max(min((int64_t)16 * RT, a.N - n0), (int64_t)0), toks = (int)a.M;
+  const int blocks = (int)(a.K / 32), steps = (blocks + 3) / 4, turns = (steps + WK - 1) / WK;
   const auto none = rsrc(a.x, 0);
-  const int steps = (blocks + 3) / 4;
-  const int wo = (int)(j * a.ldq) + 16 * g, dofs = 2 * (int)((lane >> 2) * a.ldd + (lane & 3)), xo = 2 * (int)(j * a.ldx + 4 * g);
-  using Step = Q4Step<RT, CT>;
-  auto load = [&](int s, Step& t) {  // past the last step: nothing is read
+  const auto rw = rows ? rsrc(a.qs + n0 * a.ldq, (rows - 1) * a.ldq + a.K / 2) : none;
+  const auto rd = rows ? rsrc(a.d + n0 * a.ldd, ((rows - 1) * a.ldd + blocks) * 2) : none;
+  const int wo = (int)(j * a.ldq) + 16 * g, dofs = 2 * (int)((lane >> 2) * a.ldd + (lane & 3));
+  auto load = [&](int turn, Q4Step<RT>& t) {  // past the last step: nothing is read
+    const int s = turn * WK + wk;
     const bool in = s < steps;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       t.w[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(in ? rw : none, wo + (int)(16 * r * a.ldq), 64 * s, 2));
       t.d[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(in ? rd : none, dofs + (int)(32 * r * a.ldd), 8 * s, 0);
     }
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          t.x[c][b][h] = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(
-              4 * s + b < blocks ? rx : none, xo + (int)(32 * c * a.ldx) + 64 * b + 32 * h, 256 * s, 0));
     __builtin_amdgcn_sched_barrier(0);
+  };
+  Q4Step<RT> t[PD];
+#pragma unroll
+  for (int i = 0; i < PD; ++i) load(i, t[i]);
+
+  // x in chunks of `held` turns, in units of 8 values of a row (block, token, g). The next chunk's units are in registers while one
+  // is multiplied.
+  constexpr int UX = kXUnits / NT;
+  const int held = a.held, units = held * WK * 16 * toks, tp = toks | 1;
+  const auto rx = rsrc(a.x, ((toks - 1) * a.ldx + a.K) * 2);
+  int from[UX], to[UX], at_block[UX];  // a unit's offset in x in bytes, its place in LDS (below 0: none), its block of a chunk
+#pragma unroll
+  for (int i = 0; i < UX; ++i) {
+    const int u = i * NT + threadIdx.x, blk = (int)((uint32_t)u * (uint32_t)a.per20 >> 20);  // u / (4 toks): u < 2^11, toks <= 2^5
+    const int tok = u / 4 - blk * toks, ug = u & 3;
+    from[i] = (int)(tok * a.ldx * 2) + 64 * blk + 8 * ug;
+    to[i] = u < units ? 16 * ((4 * blk + ug) * tp + tok) : -1;
+    at_block[i] = u < units ? blk : 1 << 30;
+  }
+  v2u xa[UX], xb[UX];
+  auto fetch = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < UX; ++i) {
+      const int at = chunk * (held * WK * 4) + at_block[i] < blocks ? from[i] : (int)0x80000000;  // (past the end: zeros)
+      xa[i] = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(rx, at, chunk * (held * WK * 256), 0));
+      xb[i] = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(rx, at + 32, chunk * (held * WK * 256), 0));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto put = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < UX; ++i)
+      if (to[i] >= 0) *reinterpret_cast<v4u*>(lds_x + (chunk & 1) * kXBytes + to[i]) = ordered(xa[i], xb[i]);
   };
   v4f acc[RT][CT];
 #pragma unroll
@@ -135,75 +171,96 @@ __global__ __launch_bounds__(NW * 64) void q4_rows_kernel(Q4Args a) {
 #pragma unroll
     for (auto& c : r) c = v4f{0, 0, 0, 0};
   const v4u down = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};  // -136
-  auto compute = [&](int s, Step& t) {
-    v4u xf[CT][4];
-    v4f off[CT][4];
+  int mine[CT];  // the lane's row of x (a row past the last one: the last, its result is left out)
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        xf[c][b] = ordered(t.x[c][b][0], t.x[c][b][1]);
-        off[c][b] = mfma16(down, xf[c][b], v4f{0, 0, 0, 0});
-      }
+  for (int c = 0; c < CT; ++c) mine[c] = 16 * (g * tp + min(16 * c + j, toks - 1));
+  uint32_t base = 0x43004300u;
+  asm("" : "+v"(base));
+  auto compute = [&](int turn, int buf, int in_lds, Q4Step<RT>& t) {
+    const int s = turn * WK + wk;
+    float d[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       transpose4(t.w[r]);
       // (past the row's last block lies the next row's first one)
-      const float d = 4 * s + (lane & 3) < blocks ? (float)__builtin_bit_cast(_Float16, (uint16_t)t.d[r]) : 0.0f;
-      auto block = [&](auto B) {
-        constexpr int b = decltype(B)::value;
-        const v4u w = raised(t.w[r][b]);
-        const float d0 = row_lane<b>(d), d1 = row_lane<4 + b>(d), d2 = row_lane<8 + b>(d), d3 = row_lane<12 + b>(d);
+      d[r] = 4 * s + (lane & 3) < blocks ? (float)__builtin_bit_cast(_Float16, (uint16_t)t.d[r]) : 0.0f;
+    }
+    const char* xs = lds_x + buf + (in_lds * WK + wk) * (256 * tp);
+    auto block = [&](auto B) {
+      constexpr int b = decltype(B)::value;
+      v4u x[CT];
+      v4f off[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        x[c] = *reinterpret_cast<const v4u*>(xs + b * 64 * tp + mine[c]);
+        off[c] = mfma16(down, x[c], v4f{0, 0, 0, 0});
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const v4u w = raised(t.w[r][b], base);
+        const float d0 = row_lane<b>(d[r]), d1 = row_lane<4 + b>(d[r]), d2 = row_lane<8 + b>(d[r]), d3 = row_lane<12 + b>(d[r]);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          const v4f p = mfma16(w, xf[c][b], off[c][b]);
+          const v4f p = mfma16(w, x[c], off[c]);
           acc[r][c][0] = __builtin_fmaf(d0, p[0], acc[r][c][0]);
           acc[r][c][1] = __builtin_fmaf(d1, p[1], acc[r][c][1]);
           acc[r][c][2] = __builtin_fmaf(d2, p[2], acc[r][c][2]);
           acc[r][c][3] = __builtin_fmaf(d3, p[3], acc[r][c][3]);
         }
-      };
-      block(std::integral_constant<int, 0>{});
-      block(std::integral_constant<int, 1>{});
-      block(std::integral_constant<int, 2>{});
-      block(std::integral_constant<int, 3>{});
-    }
+      }
+    };
+    block(std::integral_constant<int, 0>{});
+    block(std::integral_constant<int, 1>{});
+    block(std::integral_constant<int, 2>{});
+    block(std::integral_constant<int, 3>{});
   };
-  Step t[2];
-  if (wave < steps) {
-    load(wave, t[0]);
-    for (int s = wave; s < steps; s += 2 * NW) {
-      load(s + NW, t[1]);
-      compute(s, t[0]);
-      if (s + NW >= steps) break;
-      load(s + 2 * NW, t[0]);
-      compute(s + NW, t[1]);
+  int in_lds = held, chunk = -1;  // every wave of a workgroup takes the same turns
+  fetch(0);
+  for (int turn = 0; turn < turns; turn += PD) {
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      if (turn + i >= turns) break;
+      if (in_lds == held) {  // (the buffer's readers, of the chunk before the last, are past a barrier)
+        ++chunk;
+        put(chunk);
+        __syncthreads();
+        if (turn + i + held < turns) fetch(chunk + 1);
+        in_lds = 0;
+      }
+      if ((turn + i) * WK + wk < steps) compute(turn + i, (chunk & 1) * kXBytes, in_lds, t[i]);
+      ++in_lds;
+      load(turn + i + PD, t[i]);
     }
   }
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < CT; ++c) red[wave][r * CT + c][lane] = make_float4(acc[r][c][0], acc[r][c][1], acc[r][c][2], acc[r][c][3]);
+  constexpr int T = RT * CT;
   __syncthreads();
-  for (int i = threadIdx.x; i < RT * CT * 64; i += NW * 64) {
-    const int tile = i >> 6, l = i & 63;
+  float4* red = reinterpret_cast<float4*>(lds_x);
+#pragma unroll
+  for (int i = 0; i < T; ++i) {
+    const v4f v = acc[i / CT][i % CT];
+    red[(wave * T + i) * 64 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < WR * T * 64; i += NT) {
+    const int tile = i / (T * 64), c = i / 64 % T, l = i & 63;
     v4f y = v4f{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float4 v = red[w][tile][l];
+    for (int w = 0; w < WK; ++w) {
+      const float4 v = red[((tile * WK + w) * T + c) * 64 + l];
       y += v4f{v.x, v.y, v.z, v.w};
     }
-    const int64_t m = m0 + tile % CT * 16 + (l & 15), n = n0 + tile / CT * 16 + 4 * (l >> 4);
+    const int64_t m = 16 * (c % CT) + (l & 15), n = (((int64_t)blockIdx.x * WR + tile) * RT + c / CT) * 16 + 4 * (l >> 4);
     if (m < a.M && n < a.N) q4_store(a, m, n, y);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ many rows of x
-// Bound by the matrix cores. x goes to fp16 once, each row in a power-of-two frame (2^(14 - e), 2^e above its largest value: exact
-// but for values below 2^-29 of it, which move by 2^-40 of it at most), zero-padded to whole stages, the values of a block in the
-// order in which its weights come out of the conversion. Weights become (u - 8) d in fp16 on their way into LDS: one rounding,
-// 2^-11 at most (so |W| up to 65504, fp16's range). A row of x that holds an infinity or NaN is NaN.
-constexpr int kXThreads = 256;
+// Matrix products of tiles. x goes to fp16 once, each row in a power-of-two frame (2^(14 - e), 2^e above its largest value: exact
+// but for values below 2^-29 of it, which move by 2^-40 of it at most), zero-padded to whole stages, in tiles that lie in memory as
+// they do in LDS, the values of a block in the order in which its weights come out of the conversion. Weights become (u - 8) d in
+// fp16 in the registers that multiply them: one rounding, 2^-11 at most (so |W| up to 65504, fp16's range). A row of x that holds
+// an infinity or NaN is NaN. (The pass over x: 2000 x 12288 in 22 us, 98 MB, at the rate of a copy.)
+constexpr int kXThreads = 256, BK = 64, kStageBytes = 2 * BK;  // values, and bytes of a row of x, in a stage
 __global__ __launch_bounds__(kXThreads) void q4_x_kernel(Q4Args a) {
   __shared__ uint32_t red[kXThreads / 64];
   const int64_t m = blockIdx.x;
@@ -222,6 +279,8 @@ __global__ __launch_bounds__(kXThreads) void q4_x_kernel(Q4Args a) {
   const bool odd = am >= 0x7f80u;
   const int e = am && !odd ? (int)(am >> 7) - 126 : 0;
   if (threadIdx.x == 0) a.xexp[m] = e;
+  const int r = (int)(m % a.bm);
+  char* at16 = reinterpret_cast<char*>(a.x16) + m / a.bm * a.bm * a.Kp * 2 + r * kStageBytes;
   // chunk c of a block: values 4 c, 4 c + 2, 16 + 4 c, 16 + 4 c + 2, 4 c + 1, 4 c + 3, 16 + 4 c + 1, 16 + 4 c + 3
   for (int i = threadIdx.x; i < a.Kp / 8; i += kXThreads) {
     uint4 o = make_uint4(0, 0, 0, 0);
@@ -235,153 +294,174 @@ __global__ __launch_bounds__(kXThreads) void q4_x_kernel(Q4Args a) {
       };
       o = make_uint4(pair(lo.x, lo.y, false), pair(hi.x, hi.y, false), pair(lo.x, lo.y, true), pair(hi.x, hi.y, true));
     }
-    *reinterpret_cast<uint4*>(a.x16 + m * a.Kp + 8 * i) = o;
+    *reinterpret_cast<uint4*>(at16 + (int64_t)(i / 8) * a.bm * kStageBytes + 16 * ((i % 8) ^ (r / 2 & 7))) = o;
   }
 }
 
-constexpr int kThreads = 512;
-constexpr int BN = 256, BK = 64, kRow = 2 * BK;  // weight rows of a tile, values and bytes of a stage
-__device__ __forceinline__ int swz(int row, int chunk) { return row * kRow + ((chunk ^ ((row >> 1) & 7)) << 4); }
-__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+constexpr int kThreads = 256;
 
-// 8 values (u - 8) d in fp16, each rounded once: u - 8 from 1024 + u, or 16 (u - 8) from 1024 + 16 u, times d or d / 16
-__device__ __forceinline__ v4u q4_f16(uint32_t w, f16x2 d) {
+// Word I of 8 values (u - 8) d in fp16, each rounded once: u - 8 from 1024 + u, or 16 (u - 8) from 1024 + 16 u, times d or d / 16
+// (raised: 1024 in both halves, from a vector register).
+__device__ __forceinline__ uint32_t q4_f16(int i, uint32_t w, f16x2 d, uint32_t raised) {
   const f16x2 base = {(_Float16)-1032.0f, (_Float16)-1032.0f}, base16 = {(_Float16)-72.0f, (_Float16)-72.0f},
               sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  v4u r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t s = i < 2 ? w : w >> 8;
-    const f16x2 u = __builtin_bit_cast(f16x2, (s & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
-    const f16x2 n = i & 1 ? __builtin_elementwise_fma(u, sixteenth, base16) : u + base;
-    r[i] = __builtin_bit_cast(uint32_t, n * d);
-  }
-  return r;
+  const uint32_t s = i < 2 ? w : w >> 8;
+  const f16x2 u = __builtin_bit_cast(f16x2, (s & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | raised);
+  const f16x2 n = i & 1 ? __builtin_elementwise_fma(u, sixteenth, base16) : u + base;
+  return __builtin_bit_cast(uint32_t, n * d);
 }
 
-template <int BM>
+// A tile of 32 MT rows of x by 256 weight rows, by 4 waves of 32 MT by 64. x goes through LDS, two stages of 64 values of it, by DMA,
+// its 16-byte chunks swizzled by row / 2. The weights go straight into the registers of the lanes that multiply them: lane (r, h)
+// of V_MFMA_F32_32X32X16_F16 takes block 2 s + h of weight row r, one 16-byte load, whose four words make the A operands of four
+// instructions (word t of two blocks each; chunk t of x's two blocks is their B operand), so they cost no LDS traffic. They are
+// asked for two stages ahead. 2000 rows over 4096 x 12288: 223 us (900 TF/s), 8000 over 24576 x 4096 1.66 ms (970 TF/s). What it
+// waits for is memory, the 32 bytes of a row that a stage takes of a 128-byte line above all (with the loads of the weights
+// and d on one line: 200 and 1.40 ms; with x's as well 178 us), and the products' own rate.
+constexpr int NT = 2, BN = 256;
+template <int MT>
 __global__ __launch_bounds__(kThreads, 1) void q4_tile_kernel(Q4Args p) {
-  constexpr int WM = BM / 64, WN = 8 / WM, TM = 2, TN = BN / WN / 32;  // waves, and their 32 x 32 tiles
-  constexpr int kSlabA = BM * kRow, kStage = kSlabA + BN * kRow, LA = BM * (kRow / 16) / kThreads;
-  extern __shared__ __attribute__((aligned(16))) int8_t smem[];
+  constexpr int BM = 32 * MT, kStage = BM * kStageBytes, LD = MT;  // LD: 1 KB copies of a wave a stage
+  extern __shared__ __attribute__((aligned(16))) char lds[];
   // flat ids are dealt round-robin over the 8 XCDs; id = the XCD's contiguous range; row tiles fastest
   const int ntiles = p.tiles_m * p.tiles_n * p.nsplit;
   const int f = blockIdx.x, xcd = f & 7, local = f >> 3, per = ntiles >> 3, rem = ntiles & 7;
   const int id = xcd < rem ? xcd * (per + 1) + local : rem * (per + 1) + (xcd - rem) * per + local;
   const int tm = id % p.tiles_m, tn = id / p.tiles_m % p.tiles_n, sp = id / p.tiles_m / p.tiles_n;
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN + wave * (32 * NT);
   const int all = (int)(p.Kp / BK), k_lo = sp * p.stages, nk = min(p.stages, all - k_lo);
+  const int col = lane & 31, h = lane >> 5, blocks = (int)(p.K / 32);
 
-  const int64_t rows_a = min((int64_t)BM, p.M - m0), rows_b = min((int64_t)BN, p.N - n0);
-  const auto ra = rsrc(p.x16 + m0 * p.Kp + (int64_t)k_lo * BK, ((rows_a - 1) * p.Kp + (int64_t)nk * BK) * 2);
-  const auto rb = rsrc(p.qs + n0 * p.ldq, (rows_b - 1) * p.ldq + p.K / 2);
-  const auto rd = rsrc(p.d + n0 * p.ldd, ((rows_b - 1) * p.ldd + p.K / 32) * 2);
+  // weights: rows past N read as zeros
+  const int rows = (int)max(min((int64_t)32 * NT, p.N - n0), (int64_t)0);
   const auto none = rsrc(p.x16, 0);
-  const int a_row = tid / 8, a_chunk = tid % 8;
-  const int a_vo = (int)(a_row * p.Kp * 2) + a_chunk * 16, a_step = (int)(p.Kp * 2 * 64), a_lo = swz(a_row, a_chunk);
-  const int b_row = tid / 2, b_c = tid % 2;  // thread t: block t % 2 of the stage's two, weight row t / 2
-  const int b_vo = (int)(b_row * p.ldq) + 16 * b_c, d_vo = 2 * (int)(b_row * p.ldd + b_c);
-  const int blocks = (int)(p.K / 32);
-
-  v4u ga[LA], gb;
-  uint16_t gd = 0;
-  int g_block = 0;
-  auto gload_a = [&](int kt, int i) {
-    ga[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kt < nk ? ra : none, a_vo, kt * kRow + i * a_step, 0));
+  const auto rb = rows ? rsrc(p.qs + n0 * p.ldq, (rows - 1) * p.ldq + p.K / 2) : none;
+  const auto rd = rows ? rsrc(p.d + n0 * p.ldd, ((rows - 1) * p.ldd + blocks) * 2) : none;
+  const int b_vo = (int)(col * p.ldq) + 16 * h, d_vo = 2 * (int)(col * p.ldd + h);
+  struct Raw {
+    v4u w[NT];
+    uint32_t d[NT];
   };
-  auto gload_b = [&](int kt) {
+  auto load_w = [&](int j, int kt, Raw& r) {
     const int k = k_lo + kt;
-    gb = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kt < nk ? rb : none, b_vo, 32 * k, 0));
-    gd = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kt < nk ? rd : none, d_vo, 4 * k, 0);
-    g_block = 2 * k + b_c;
+    r.w[j] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kt < nk ? rb : none, b_vo + (int)(32 * j * p.ldq), 32 * k, 0));
+    r.d[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kt < nk ? rd : none, d_vo + (int)(64 * j * p.ldd), 4 * k, 0);
   };
-  auto swrite_a = [&](int buf, int i) { *reinterpret_cast<v4u*>(smem + buf * kStage + a_lo + i * 64 * kRow) = ga[i]; };
-  auto swrite_b = [&](int buf) {
-    int8_t* lb = smem + buf * kStage + kSlabA;
-    const _Float16 d = __builtin_bit_cast(_Float16, g_block < blocks ? gd : (uint16_t)0);
-    const f16x2 d2 = {d, d};
+  auto load_w_all = [&](int kt, Raw& r) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *reinterpret_cast<v4u*>(lb + swz(b_row, 4 * b_c + q)) = q4_f16(gb[q], d2);
+    for (int j = 0; j < NT; ++j) load_w(j, kt, r);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto frags = [&](int buf, int s, v4u (&fa)[TM], v4u (&fb)[TN]) {
-    const int chunk = s * 2 + (lane >> 5);
-    const int8_t* la = smem + buf * kStage;
-    const int8_t* lb = la + kSlabA;
+  auto wait_w = [&](Raw& r) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const v4u*>(la + swz(wm * 64 + i * 32 + (lane & 31), chunk));
-#pragma unroll
-    for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const v4u*>(lb + swz(wn * (TN * 32) + j * 32 + (lane & 31), chunk));
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(r.w[j]), "+v"(r.d[j]));
   };
-  v16f acc[TN][TM];
+  // x: copy i of a wave is its i-th KB of every four; a stage of a tile lies in memory as it does in LDS
+  const char* x_at = reinterpret_cast<const char*>(p.x16) + (int64_t)tm * BM * p.Kp * 2 + (int64_t)k_lo * kStage;
+  auto copy_x = [&](int i, int kt, int to) {
+    od_dma16_at(x_at + (int64_t)min(kt, nk - 1) * kStage + 1024 * (4 * i + wave), 16 * lane, od_lds_addr(lds) + to + 1024 * (4 * i + wave));
+  };
+  // chunk 4 h + t of row 32 i + col
+  const int x_sw = (col >> 1) & 7;  // (32 i is a multiple of 16)
+  auto frag_x = [&](int at, int t, int i) {
+    return *reinterpret_cast<const v4u*>(lds + at + (col + 32 * i) * kStageBytes + (((4 * h + t) ^ x_sw) << 4));
+  };
+  uint32_t raised = 0x64006400u;
+  asm("" : "+v"(raised));
+  f16x2 d2[NT];
+  auto scales = [&](int kt, const Raw& r) {  // (past the row's last block lies the next row's first one)
+    const bool in = 2 * (k_lo + kt) + h < blocks;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)(in ? r.d[j] : 0u));
+      d2[j] = f16x2{d, d};
+    }
+  };
+  v16f acc[NT][MT];
 #pragma unroll
   for (auto& r : acc)
 #pragma unroll
     for (auto& c : r) c = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  // the weights as the A operand: a lane then holds 4 neighbouring columns of out
-  constexpr int kMf = TM * TN;
-  auto mma = [&](const v4u (&fa)[TM], const v4u (&fb)[TN], auto fill, auto OPS) {
-    constexpr int kOps = decltype(OPS)::value;
+
+  // A stage is four steps of MT NT products; the next step's operands are made between them. Before the last step the next stage's
+  // x has to be there and everyone done reading this one's: the one wait and barrier of a stage. (The compiler does not see the
+  // copies: its own wait for raw weights counts the loads alone, so a stage's copies go before its loads.)
+  Raw raw[3];
+  v4u fx[2][MT], fw[2][NT];
+  constexpr int kSlots = MT * NT, kWords = 4 * NT;
+  auto step = [&](auto T, int at, const Raw& next, auto between) {  // products of step T; operands of step T + 1, x of it at `at`
+    constexpr int t = decltype(T)::value, cur = t & 1, t1 = (t + 1) & 3;
 #pragma unroll
-    for (int x = 0; x < kMf; ++x) {
-      acc[x / TM][x % TM] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fb[x / TM]),
-                                                                  __builtin_bit_cast(f16x8, fa[x % TM]), acc[x / TM][x % TM], 0, 0, 0);
+    for (int s = 0; s < kSlots; ++s) {
+      const int j = s / MT, i = s % MT;
+      acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fw[cur][j]),
+                                                         __builtin_bit_cast(f16x8, fx[cur][i]), acc[j][i], 0, 0, 0);
+      if (s < MT) fx[cur ^ 1][s] = frag_x(at, t1, s);
 #pragma unroll
-      for (int o = 0; o < kOps; ++o)
-        if (o * kMf / (kOps > 0 ? kOps : 1) == x) fill(o);
+      for (int w = s * kWords / kSlots; w < (s + 1) * kWords / kSlots; ++w)
+        fw[cur ^ 1][w / 4][w % 4] = q4_f16(w % 4, next.w[w / 4][t1], d2[w / 4], raised);
+      between(s);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto nofill = [](int) {};
-  using Zero = std::integral_constant<int, 0>;
-  v4u f0a[TM], f0b[TN], f1a[TM], f1b[TN];
-  auto load_all = [&](int kt) {
+  auto nothing = [](int) {};
+  int here = 0, there = kStage;
+  auto stage = [&](int kt, Raw& r, Raw& r1) {
+    step(std::integral_constant<int, 0>{}, here, r, nothing);
+    step(std::integral_constant<int, 1>{}, here, r, nothing);
+    step(std::integral_constant<int, 2>{}, here, r, nothing);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(2 * NT) : "memory");
+    wait_w(r1);
+    scales(kt + 1, r1);
+    step(std::integral_constant<int, 3>{}, there, r1, [&](int s) {
 #pragma unroll
-    for (int i = 0; i < LA; ++i) gload_a(kt, i);
-    gload_b(kt);
+      for (int c = s * (LD + NT) / kSlots; c < (s + 1) * (LD + NT) / kSlots; ++c) {
+        if (c < LD) {
+          copy_x(c, kt + 2, here);
+        } else {
+          load_w(c - LD, kt + 3, r);
+        }
+      }
+    });
+    const int o = here;
+    here = there;
+    there = o;
   };
-  load_all(0);
 #pragma unroll
-  for (int i = 0; i < LA; ++i) swrite_a(0, i);
-  swrite_b(0);
-  load_all(1);
-  barrier_lds();
-  frags(0, 0, f0a, f0b);
-  constexpr int kOps0 = 2 * (LA + 1);
-  for (int kt = 0; kt < nk; ++kt) {
-    const int cur = kt & 1, nxt = cur ^ 1;
-    frags(cur, 1, f1a, f1b);
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int c = 0; c < LD; ++c) copy_x(c, i, i * kStage);
     __builtin_amdgcn_sched_barrier(0);
-    auto fill0 = [&](int o) {
-      if (o < LA) swrite_a(nxt, o);
-      else if (o == LA) swrite_b(nxt);
-      else if (o < 2 * LA + 1) gload_a(kt + 2, o - LA - 1);
-      else gload_b(kt + 2);
-    };
-    mma(f0a, f0b, fill0, std::integral_constant<int, kOps0>{});
-    frags(cur, 2, f0a, f0b);
-    __builtin_amdgcn_sched_barrier(0);
-    mma(f1a, f1b, nofill, Zero{});
-    frags(cur, 3, f1a, f1b);
-    __builtin_amdgcn_sched_barrier(0);
-    mma(f0a, f0b, nofill, Zero{});
-    barrier_lds();
-    frags(nxt, 0, f0a, f0b);
-    __builtin_amdgcn_sched_barrier(0);
-    mma(f1a, f1b, nofill, Zero{});
+    if (i == 0) load_w_all(0, raw[0]), load_w_all(1, raw[1]);
   }
+  load_w_all(2, raw[2]);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(2 * NT) : "memory");
+  wait_w(raw[0]);
+  scales(0, raw[0]);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) fx[0][i] = frag_x(0, 0, i);
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) fw[0][w / 4][w % 4] = q4_f16(w % 4, raw[0].w[w / 4][0], d2[w / 4], raised);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int kt = 0; kt < nk; kt += 3) {
+    stage(kt, raw[0], raw[1]);
+    if (kt + 1 < nk) stage(kt + 1, raw[1], raw[2]);
+    if (kt + 2 < nk) stage(kt + 2, raw[2], raw[0]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (copies of a stage past the last one may be on their way)
   // lane: row lane % 32 of x, weight rows 8 (r / 4) + 4 (lane / 32) + r % 4 of the tile's 32
-  const int col = lane & 31, h = lane >> 5;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + wm * 64 + i * 32 + col;
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + i * 32 + col;
     if (m >= p.M) continue;
-    const float unit = __builtin_ldexpf(1.0f, p.xexp[m] / 2 - 7), unit2 = __builtin_ldexpf(1.0f, p.xexp[m] - p.xexp[m] / 2 - 7);
+    const int e = p.xexp[m];
+    const float unit = __builtin_ldexpf(1.0f, e / 2 - 7), unit2 = __builtin_ldexpf(1.0f, e - e / 2 - 7);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int64_t n = n0 + wn * (TN * 32) + j * 32 + 8 * q + 4 * h;
+        const int64_t n = n0 + j * 32 + 8 * q + 4 * h;
         if (n >= p.N) continue;
         v4f y = v4f{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
         y = y * unit * unit2;
@@ -403,7 +483,9 @@ __global__ __launch_bounds__(256) void q4_sum_kernel(Q4Args p) {
   q4_store(p, m, n, y);
 }
 
-constexpr int kFewRows = 32;
+// Up to 32 rows take the first kernel, above it the tiles: 24576 x 4096, 32 rows 31 against 45 us, 64 rows 46 (by 64 rows of x
+// at a time) against 45; 4096 x 4096, 32 rows 15 against 20, 64 rows 44 against 23.
+constexpr int64_t kFewRows = 32;
 
 struct Q4Plan {
   int bm, nsplit, stages;
@@ -413,19 +495,20 @@ struct Q4Plan {
 Q4Plan q4_plan(int64_t M, int64_t N, int64_t K) {
   Q4Plan q = {};
   if (M <= kFewRows) return q;
-  const int64_t cus = od_cu_count();
   q.Kp = (K + BK - 1) / BK * BK;
-  q.tiles_n = (N + BN - 1) / BN;
-  q.bm = (M + 255) / 256 * q.tiles_n >= cus ? 256 : 128;
+  q.bm = M <= 64 ? 64 : 128;
   q.tiles_m = (M + q.bm - 1) / q.bm;
-  const int64_t all = q.Kp / BK, tiles = q.tiles_m * q.tiles_n;
-  int64_t n = tiles >= cus ? 1 : cus / tiles;
-  if (n > all / 8) n = all / 8;  // 8 stages at least
+  q.tiles_n = (N + BN - 1) / BN;
+  // K is split for two workgroups a CU, of 8 stages at least: 2000 rows over 4096 x 12288 (256 tiles) 245 us in two parts, 266 in
+  // one; 300 rows 74 in five, 125 in two, 228 in one
+  const int64_t all = q.Kp / BK;
+  int64_t n = 2 * od_cu_count() / (q.tiles_m * q.tiles_n);
+  if (n > all / 8) n = all / 8;
   if (n < 1) n = 1;
   q.stages = (int)((all + n - 1) / n);
   q.nsplit = (int)((all + q.stages - 1) / q.stages);
   q.xexp = (M + 3) / 4 * 4;
-  q.x16 = M * q.Kp / 2;
+  q.x16 = q.tiles_m * q.bm * q.Kp / 2;
   q.part = q.nsplit > 1 ? q.nsplit * M * ((N + 3) / 4 * 4) : 0;
   return q;
 }
@@ -434,19 +517,56 @@ bool q4_sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M >= 0 && N >= 1 && K >= 32 && K % 32 == 0 && M <= (1ll << 22) && N <= (1ll << 24) && K <= (1ll << 20);
 }
 
-template <int BM>
-int launch_tile(const Q4Args& a, unsigned groups, hipStream_t st) {
-  static std::atomic<uint64_t> allowed{0};
-  constexpr int bytes = 2 * (BM + BN) * kRow;
+// Dynamic LDS above 64 KB, which a kernel has to be allowed once per device.
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return OD_ERR_LAUNCH;
   if (!((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(q4_tile_kernel<BM>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-        hipSuccess)
-      return OD_ERR_LAUNCH;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return OD_ERR_LAUNCH;
     allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  q4_tile_kernel<BM><<<dim3(groups), dim3(kThreads), bytes, st>>>(a);
+  return OD_OK;
+}
+
+template <int RT, int CT, int WK, int WR, int PD>
+int launch_rows(Q4Args& a, hipStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  static_assert(16 * CT * 16 * WK <= kXUnits, "a turn's x fits a buffer");
+  const int64_t toks = a.M, turn = 256 * (toks | 1) * WK, turns = (a.K / 32 + 4 * WK - 1) / (4 * WK);  // M <= 16 CT
+  int64_t held = kXUnits / (16 * toks * WK);
+  if (held * turn > kXBytes) held = kXBytes / turn;
+  if (held > turns) held = turns;
+  constexpr int64_t sums = (int64_t)WK * WR * RT * CT * 1024;
+  int64_t bytes = held < turns ? 2 * kXBytes : held * turn;
+  if (bytes < sums) bytes = sums;
+  if (bytes > 65536) {
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(q4_rows_kernel<RT, CT, WK, WR, PD>), 160 << 10, allowed)) return rc;
+  }
+  a.held = (int)held;
+  a.per20 = (int)(((1 << 20) + 4 * toks - 1) / (4 * toks));
+  const unsigned groups = (unsigned)((a.N + 16 * RT * WR - 1) / (16 * RT * WR));
+  q4_rows_kernel<RT, CT, WK, WR, PD><<<dim3(groups), dim3(WK * WR * 64), (size_t)bytes, st>>>(a);
+  return od_launch_status();
+}
+
+// The shapes of the first kernel (one row of x; 16 rows; us). Where the row tiles are few, a tile a workgroup: 4096 x 4096 8.9; 9.5
+// (two sets of two tiles 11.9; 15.3). Then two tiles a wave, which share x: 49152 x 4096 28.6; 37.2 (one tile a workgroup 38.8;
+// 60.7, two 32.2; 44.5). With many of them and several rows of x, four sets, whose x is staged half as often: 98304 x 4096, 16 rows
+// 65.9 against 70.4, 32 rows 79.1 against 87.3; at one row 58.9 against 55.2, and 32 rows over 49152 x 4096 51.8 against 47.7.
+int launch_few(Q4Args& a, hipStream_t st) {
+  const int64_t tiles = (a.N + 15) / 16, cus = od_cu_count();
+  if (a.M <= 16) {
+    if (tiles <= 2 * cus) return launch_rows<1, 1, 8, 1, 4>(a, st);
+    return tiles <= 14 * cus || a.M <= 8 ? launch_rows<2, 1, 4, 2, 2>(a, st) : launch_rows<2, 1, 2, 4, 2>(a, st);
+  }
+  if (tiles <= 2 * cus) return launch_rows<1, 2, 4, 2, 4>(a, st);
+  return tiles <= 14 * cus ? launch_rows<2, 2, 4, 2, 2>(a, st) : launch_rows<2, 2, 2, 4, 2>(a, st);
+}
+
+template <int MT>
+int launch_tiles(const Q4Args& a, unsigned groups, hipStream_t st) {
+  static_assert(2 * 32 * MT * kStageBytes <= 65536, "two stages of x");
+  q4_tile_kernel<MT><<<dim3(groups), dim3(kThreads), 2 * 32 * MT * kStageBytes, st>>>(a);
   return od_launch_status();
 }
 
@@ -477,12 +597,7 @@ extern "C" int od_q4_linear(const uint16_t* x, int64_t ldx, const uint8_t* qs, i
   }
   Q4Args a{x, qs, d, bias, residual, out, ldx, ldq, ldd, ldr, ldo, M, N, K};
   hipStream_t st = (hipStream_t)stream;
-  if (M <= kFewRows) {
-    const unsigned gx = (unsigned)((N + 15) / 16), g2 = (unsigned)((N + 31) / 32);
-    if (M <= 16) q4_rows_kernel<1, 1, 8><<<dim3(gx), dim3(512), 0, st>>>(a);
-    else q4_rows_kernel<2, 2, 8><<<dim3(g2), dim3(512), 0, st>>>(a);
-    return od_launch_status();
-  }
+  if (M <= kFewRows) return launch_few(a, st);
   a.xexp = reinterpret_cast<int*>(ws);
   a.x16 = reinterpret_cast<uint16_t*>(ws + q.xexp);
   a.part = ws + q.xexp + q.x16;
@@ -490,11 +605,12 @@ extern "C" int od_q4_linear(const uint16_t* x, int64_t ldx, const uint8_t* qs, i
   a.tiles_m = (int)q.tiles_m;
   a.tiles_n = (int)q.tiles_n;
   a.nsplit = q.nsplit;
+  a.bm = q.bm;
   a.stages = q.stages;
   const int64_t groups = q.tiles_m * q.tiles_n * q.nsplit;
   if (groups > (1 << 23) || M * ((N + 3) / 4) > (1ll << 32) - 256) return OD_ERR_SHAPE;
   q4_x_kernel<<<dim3((unsigned)M), dim3(kXThreads), 0, st>>>(a);
-  const int rc = q.bm == 256 ? launch_tile<256>(a, (unsigned)groups, st) : launch_tile<128>(a, (unsigned)groups, st);
+  const int rc = q.bm == 128 ? launch_tiles<4>(a, (unsigned)groups, st) : launch_tiles<2>(a, (unsigned)groups, st);
   if (rc != OD_OK || q.nsplit == 1) return rc;
   q4_sum_kernel<<<dim3((unsigned)((M * ((N + 3) / 4) + 255) / 256)), dim3(256), 0, st>>>(a);
   return od_launch_status();
