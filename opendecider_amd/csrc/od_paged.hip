@@ -601,8 +601,8 @@ constexpr int s_waves(int D, int P, int columns) {
   return P == kInt4 && D <= 128 && columns == 1 ? 3 : 2;
 }
 
-template <int D, int P, int CT>
-__global__ __launch_bounds__(kStreamWaves * 64, s_waves(D, P, CT)) void paged_stream_kernel(AttnArgs a) {
+template <int D, int P, int CT, int WAVES = s_waves(D, P, CT)>
+__global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(AttnArgs a) {
   constexpr bool Q8 = P == kInt8, Q4 = P == kInt4;
   using Tile = STile<D, P>;
   // QR: 16 slots' rows start in 16 distinct 16-byte bank groups
@@ -2332,7 +2332,7 @@ __global__ __launch_bounds__(kThreads) void page_image_kernel(AttnArgs a) {
 // How a call is split. Sequences' lengths are on the device; the host knows bounds.
 struct Plan {
   bool stream;
-  int ct;  // stream: columns of 16 slots, 1 or 2
+  int ct, waves;  // stream: columns of 16 slots, 1 or 2; waves a SIMD
   int nw, tiles, run, width, chunk, nsplit;
   int64_t img_blocks;  // of every (sequence, KV head); 0: no image
   // the workspace, in floats: partials, then the image's V frames, heads and blocks
@@ -2376,16 +2376,21 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   const int64_t tiles = (slots + spt - 1) / spt, wgs = wgs_of(spt), keys = (max_ctx + p.width - 1) / p.width;
   p.tiles = (int)tiles;
   // how many run at once: two a CU, one where a wave or the shared memory needs it whole, three that stream 4-bit pages (8 ragged
-  // states of up to 32768 tokens 60 us in 12 splits, 66 in 8; 16 x 16000 59 and 61; but 64 x 4096 55 and 53)
-  const int64_t fit = cus * (p.stream ? s_waves((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16, p.ct) : p.nw == 8 ? 1 : 2);
+  // states of up to 32768 tokens 60 us in 12 splits, 66 in 8; 16 x 16000 59 and 61; but 64 x 4096 55 and 53). Heads of 256 over
+  // 4-bit pages: one, whose wave holds all it works on, where all of them are in at once (a token over 4 x 8000 19.8 us, 23.2 with
+  // two; 64 x 700 19.6 and 24.9, 64 x 2000 39.4 and 47; but 128 x 1000 48.6 and 43.4, 256 x 300 49 and 37)
+  p.waves = !p.stream ? 0 : q4 && D == 256 && p.ct == 1 && wgs <= cus ? 1 : s_waves((int)D, q4 ? kInt4 : q8 ? kInt8 : kBf16, p.ct);
+  const int64_t fit = cus * (p.stream ? p.waves : p.nw == 8 ? 1 : 2);
   // key tiles that are worth a workgroup of their own (128 tokens over 1 x 1000: 37 us with 8 blocks at least, 35 with
   // 2)
-  const int64_t least = p.stream ? 8 : 2;
+  // (4-bit pages: 2 where the workgroups are few or the heads wide: a token over 1 x 1500, heads of 256 10.8 us, 14.7 with 8, heads
+  // of 128 9.0 and 11.4, 4 x 3000 13.3 and 14.4; but 16 x 700 13.9 and 11.9)
+  const int64_t least = !p.stream || (q4 && (D == 256 || 8 * wgs <= cus)) ? 2 : 8;
   int64_t most = keys / least < 128 ? keys / least : 128, n = 1;
   if (N > kMaxGroups) most = 1;  // no merge, which has a workgroup a token
   // two streams of that size take as long as one (a token over 500: 9.9 us, 10.1 whole), with a launch more for the
-  // host
-  if (p.stream && most < 3) most = 1;
+  // host, 4 us of it; not so heads of 256 over 4-bit pages (over 700 10.5 us, 17.4 whole; over 400 10.6 and 14.0)
+  if (p.stream && keys / 8 < (q4 && D == 256 ? 2 : 3)) most = 1;
   if (p.stream) {
     n = fit / (wgs < 1 ? 1 : wgs);
     if (n > most) n = most;
@@ -2646,7 +2651,9 @@ extern "C" int od_paged_attn_ex(const uint16_t* q, int64_t sqt, int64_t sqh, con
     auto stream = [&](auto PC) {
       constexpr int P = decltype(PC)::value;
       const dim3 grid((unsigned)p.nsplit, (unsigned)(Hkv * p.tiles), (unsigned)B);
-      if (p.ct == 1) paged_stream_kernel<DD, P, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+      if (p.ct == 1 && p.waves < s_waves(DD, P, 1)) {
+        if constexpr (P == kInt4 && DD == 256) paged_stream_kernel<DD, P, 1, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
+      } else if (p.ct == 1) paged_stream_kernel<DD, P, 1><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
       else paged_stream_kernel<DD, P, 2><<<grid, dim3(kStreamWaves * 64), 0, st>>>(a);
     };
     if (p.stream) {

@@ -1186,10 +1186,16 @@ def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, st
                                       start.data_ptr(), ctx_len.data_ptr(), B, N, H, D, stream_of(k)), "od_page_append")
 
 
-def _aligned16(t: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor at a multiple of 16 bytes, as the kernels' vector loads need it (a copy where it is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _aligned16(t: torch.Tensor, name: str):
+    """A contiguous bf16 tensor at a multiple of 16 bytes, as the kernels' vector loads need it (a copy where it is not), and its
+    address."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
+    at = t.data_ptr()
+    if at % 16 or not t.is_contiguous():
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = t.data_ptr()
+    return t, at
 
 
 def qk_norm_rope_page_append(qkv: torch.Tensor, n_heads_q: int, n_heads_k: int, D: int, q_w, k_w, cos_t, sin_t, pos,
@@ -1198,43 +1204,54 @@ def qk_norm_rope_page_append(qkv: torch.Tensor, n_heads_q: int, n_heads_k: int, 
     """od_qk_norm_rope_page_append: qk_norm_rope on qkv (N, >= (Hq + 2 Hk) D) and page_append of the rotated keys and the values
     in one pass (the results of the two calls). The rotated q and k heads go to out (N, (Hq + Hk) D) bf16, or with out None back
     into qkv (every row, also those of no sequence); cache, table, start and ctx_len as page_append. Returns out, or qkv."""
-    _one_device("qk_norm_rope_page_append", qkv, q_w, k_w, cos_t, sin_t, pos, cache.k, cache.v, table, start, ctx_len, out)
-    _lib.bf16_bits(qkv)
-    B, pages, table = _paged(cache, table, start, ctx_len, "qk_norm_rope_page_append")
+    name = "qk_norm_rope_page_append"
+    dev = _one_device(name, qkv, q_w, k_w, cos_t, sin_t, pos, cache.k, cache.v, table, start, ctx_len, out)
+    B, pages, table = _paged(cache, table, start, ctx_len, name)
     rot_dim = D if rot_dim is None else rot_dim
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads_q + 2 * n_heads_k) * D or \
-            (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
-        raise ValueError(f"qk_norm_rope_page_append: qkv must be (N, >= {(n_heads_q + 2 * n_heads_k) * D}) with contiguous rows")
+    if qkv.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected bfloat16, got {qkv.dtype}")
+    if qkv.dim() != 2:
+        raise ValueError(f"{name}: qkv must be (N, columns)")
+    (N, cols), (ld, sd) = qkv.shape, qkv.stride()
+    if sd != 1 or cols < (n_heads_q + 2 * n_heads_k) * D or (N > 1 and ld < cols):
+        raise ValueError(f"{name}: qkv must be (N, >= {(n_heads_q + 2 * n_heads_k) * D}) with contiguous rows")
     if cache.k.shape[1] != n_heads_k or cache.head_dim != D:
-        raise ValueError(f"qk_norm_rope_page_append: {n_heads_k} heads of {D} into pages of {cache.k.shape[1]} heads of "
-                         f"{cache.head_dim}")
-    N, width = qkv.shape[0], (n_heads_q + n_heads_k) * D
-    q_w, k_w = (_aligned16(_vec(w, D, name)) for w, name in ((q_w, "q_w"), (k_w, "k_w")))
-    _lib.bf16_bits(cos_t)
-    _lib.bf16_bits(sin_t)
-    _rope_tables_ok(cos_t, sin_t, D, rot_dim, "qk_norm_rope_page_append")
-    cos_t, sin_t = _aligned16(cos_t), _aligned16(sin_t)
+        raise ValueError(f"{name}: {n_heads_k} heads of {D} into pages of {cache.k.shape[1]} heads of {cache.head_dim}")
+    width = (n_heads_q + n_heads_k) * D
+    if q_w.numel() != D or k_w.numel() != D:
+        raise ValueError(f"{name}: q_w and k_w must have {D} elements")
+    _rope_tables_ok(cos_t, sin_t, D, rot_dim, name)
+    q_w, qw_at = _aligned16(q_w, name)
+    k_w, kw_at = _aligned16(k_w, name)
+    cos_t, cos_at = _aligned16(cos_t, name)
+    sin_t, sin_at = _aligned16(sin_t, name)
     if pos.dtype != torch.int32 or pos.numel() != N:
-        raise ValueError("qk_norm_rope_page_append: pos must be int32 (N,)")
+        raise ValueError(f"{name}: pos must be int32 (N,)")
     pos = pos.contiguous()
-    ok = qkv.data_ptr() % 16 == 0 and (N < 2 or qkv.stride(0) % 8 == 0)
-    x = qkv if ok else qkv.clone(memory_format=torch.contiguous_format)
-    if not ok and x.stride(0) % 8:  # an odd number of columns: rows of their own width
-        x = torch.empty(N, -(-qkv.shape[1] // 8) * 8, dtype=qkv.dtype, device=qkv.device)
-        x[:, :qkv.shape[1]] = qkv
+    x, x_at = qkv, qkv.data_ptr()
+    if N < 2:
+        ld = -(-cols // 8) * 8
+    if x_at % 16 or ld % 8:  # rows of their own, of a multiple of 8 columns
+        ld = -(-cols // 8) * 8
+        x = torch.empty(N, ld, dtype=qkv.dtype, device=qkv.device)
+        x[:, :cols] = qkv
+        x_at = x.data_ptr()
     if out is None:
-        dst = x
+        dst, dst_at, ldo = x, x_at, ld
     else:
-        _check_out(out, (N, width), qkv.device, "qk_norm_rope_page_append")
-        fits = out.data_ptr() % 16 == 0 and (N < 2 or (out.stride(0) % 8 == 0 and out.stride(0) >= width))
-        dst = out if fits else torch.empty(N, width, dtype=out.dtype, device=out.device)
-    ld, ldo = (t.stride(0) if N > 1 else t.shape[1] for t in (x, dst))
-    with _OnDevice(qkv):
-        check(lib().od_qk_norm_rope_page_append(x.data_ptr(), -(-ld // 8) * 8, dst.data_ptr(), -(-ldo // 8) * 8, n_heads_q,
-                                                rot_dim, int(bool(offset)), ptr(q_w), ptr(k_w), ptr(cos_t), ptr(sin_t),
-                                                cos_t.shape[0], ptr(pos), float(eps), *pages, start.data_ptr(),
-                                                ctx_len.data_ptr(), B, N, n_heads_k, D, stream_of(qkv)),
-              "od_qk_norm_rope_page_append")
+        _check_out(out, (N, width), qkv.device, name)
+        dst, dst_at, ldo = out, out.data_ptr(), out.stride(0) if N > 1 else width
+        if dst_at % 16 or ldo % 8 or ldo < width:
+            dst, ldo = torch.empty(N, width, dtype=out.dtype, device=out.device), width
+            dst_at = dst.data_ptr()
+    args = (x_at, ld, dst_at, ldo, n_heads_q, rot_dim, 1 if offset else 0, qw_at, kw_at, cos_at, sin_at, cos_t.shape[0],
+            pos.data_ptr(), eps, *pages, start.data_ptr(), ctx_len.data_ptr(), B, N, n_heads_k, D,
+            torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        check(lib().od_qk_norm_rope_page_append(*args), "od_qk_norm_rope_page_append")
+    else:
+        with torch.cuda.device(dev):
+            check(lib().od_qk_norm_rope_page_append(*args), "od_qk_norm_rope_page_append")
     if out is None:
         if x is not qkv:
             qkv[:, :width].copy_(x[:, :width])
@@ -1244,26 +1261,34 @@ def qk_norm_rope_page_append(qkv: torch.Tensor, n_heads_q: int, n_heads_k: int, 
     return out
 
 
+_READ_FORMS = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
+
+
 def page_read(cache, table: torch.Tensor, length: torch.Tensor, T: int, dtype: torch.dtype = torch.bfloat16):
     """od_page_read_ex: the first length[b] (at most T) tokens of every sequence as dense (B, Hkv, T, D) K and V, zeros behind
     them. dtype bfloat16 or float32: the values q * s, one fp32 product (Int8Tensor.dequantize rounds the scale to bf16
     first). int8 (int8 pages only): two Int8Tensors, the stored bytes and scales (scales (B, Hkv, T, 1))."""
-    _one_device("page_read", cache.k, cache.v, table, length)
+    dev = _one_device("page_read", cache.k, cache.v, table, length)
     B, pages, table = _paged(cache, table, None, length, "page_read")
     if T < 0:
         raise ValueError(f"page_read: T must not be negative, got {T}")
-    forms = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
-    if dtype not in forms or (dtype == torch.int8 and cache.k.dtype != torch.int8):
+    form = _READ_FORMS.get(dtype)
+    if form is None or (form == 2 and cache.format != 1):
         raise TypeError(f"page_read: cannot read {cache.k.dtype} pages as {dtype}")
     H, D = cache.k.shape[1], cache.head_dim
-    dev = cache.k.device
-    k, v = (torch.empty(B, H, T, D, dtype=dtype, device=dev) for _ in range(2))
+    device = cache.k.device
+    k = torch.empty((B, H, T, D), dtype=dtype, device=device)
+    v = torch.empty((B, H, T, D), dtype=dtype, device=device)
     ks = vs = None
     if dtype == torch.int8:
-        ks, vs = (torch.empty(B, H, T, dtype=torch.float32, device=dev) for _ in range(2))
-    with _OnDevice(k):
-        check(lib().od_page_read_ex(*pages, length.data_ptr(), B, T, H, D, forms[dtype], k.data_ptr(), ptr(ks), v.data_ptr(),
-                                    ptr(vs), stream_of(k)), "od_page_read")
+        ks, vs = (torch.empty(B, H, T, dtype=torch.float32, device=device) for _ in range(2))
+    args = (*pages, length.data_ptr(), B, T, H, D, form, k.data_ptr(), ptr(ks), v.data_ptr(), ptr(vs),
+            torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        check(lib().od_page_read_ex(*args), "od_page_read")
+    else:
+        with torch.cuda.device(dev):
+            check(lib().od_page_read_ex(*args), "od_page_read")
     if ks is None:
         return k, v
     from .quant import Int8Tensor
