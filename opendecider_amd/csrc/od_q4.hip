@@ -317,7 +317,8 @@ __device__ __forceinline__ uint32_t q4_f16(int i, uint32_t w, f16x2 d, uint32_t 
 // instructions (word t of two blocks each; chunk t of x's two blocks is their B operand), so they cost no LDS traffic. They are
 // asked for two stages ahead. 2000 rows over 4096 x 12288: 223 us (900 TF/s), 8000 over 24576 x 4096 1.66 ms (970 TF/s). What it
 // waits for is memory, the 32 bytes of a row that a stage takes of a 128-byte line above all (with the loads of the weights
-// and d on one line: 200 and 1.40 ms; with x's as well 178 us), and the products' own rate.
+// and d on one line: 200 and 1.40 ms; with x's as well 178 us), and the products' own rate. (Asking for two stages' weights at
+// once, so that the second finds its line in the cache, takes as long.)
 constexpr int NT = 2, BN = 256;
 template <int MT>
 __global__ __launch_bounds__(kThreads, 1) void q4_tile_kernel(Q4Args p) {

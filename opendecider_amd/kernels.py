@@ -1060,28 +1060,35 @@ def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Te
         raise TypeError(f"q4_linear: expected uint8 weights and float16 scales, got {qs.dtype} and {d.dtype}")
     if qs.dim() != 2 or d.dim() != 2 or x.dim() < 1:
         raise ValueError("q4_linear: qs must be (N, K / 2) and d (N, K / 32)")
-    N, K = qs.shape[0], 2 * qs.shape[1]
-    if K % 32 or d.shape != (N, K // 32) or x.shape[-1] != K or N < 1 or K < 32:
+    N, K = qs.shape
+    K *= 2
+    lead, blocks = x.shape[:-1], K // 32
+    if K % 32 or K < 32 or N < 1 or d.shape != (N, blocks) or x.shape[-1] != K:
         raise ValueError(f"q4_linear: x {tuple(x.shape)}, qs {tuple(qs.shape)} and d {tuple(d.shape)} do not match (K a multiple of 32)")
-    shape = (*x.shape[:-1], N)
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    shape = (*lead, N)
+    x2 = x if len(lead) == 1 else x.reshape(-1, K)
     M = x2.shape[0]
-    if x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (x2.stride(0) % 8 or x2.stride(0) < K)):
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    if qs.stride(1) != 1 or qs.data_ptr() % 16 or (N > 1 and (qs.stride(0) % 16 or qs.stride(0) < K // 2)):
-        qs = qs.clone(memory_format=torch.contiguous_format)
-    if d.stride(1) != 1 or (N > 1 and d.stride(0) < K // 32):
-        d = d.contiguous()
-    bias = _vec(bias, N, "bias")
+    # rows as they are where their strides and address suit the kernel's loads, else copied
+    ldx, sx = x2.stride()
+    if sx != 1 or x2.data_ptr() % 16 or (M > 1 and (ldx % 8 or ldx < K)):
+        x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
+    ldq, sq = qs.stride()
+    if sq != 1 or qs.data_ptr() % 16 or (N > 1 and (ldq % 16 or ldq < K // 2)):
+        qs, ldq = qs.clone(memory_format=torch.contiguous_format), K // 2
+    ldd, sd = d.stride()
+    if sd != 1 or (N > 1 and ldd < blocks):
+        d, ldd = d.contiguous(), blocks
+    if bias is not None:
+        bias = _vec(bias, N, "bias")
     ldr = N
     if residual is not None:
         _lib.bf16_bits(residual)
-        if tuple(residual.shape) != shape:
+        if residual.shape != shape:
             raise ValueError(f"q4_linear: residual must be {shape}, got {tuple(residual.shape)}")
-        residual = residual if residual.dim() == 2 else residual.reshape(-1, N)
-        if residual.stride(1) != 1 or (M > 1 and residual.stride(0) < N):
-            residual = residual.contiguous()
-        ldr = residual.stride(0) if M > 1 else N
+        residual = residual if len(lead) == 1 else residual.reshape(-1, N)
+        ldr, sr = residual.stride()
+        if sr != 1 or (M > 1 and ldr < N):
+            residual, ldr = residual.contiguous(), N
     if out is None:
         dst = res = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
         ldo = N
@@ -1092,8 +1099,8 @@ def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Te
         ldo = dst.stride(0) if M > 1 else N
     n = q4_linear_workspace_floats(M, N, K, x.device)
     ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-    args = (x2.data_ptr(), x2.stride(0) if M > 1 else K, qs.data_ptr(), qs.stride(0) if N > 1 else K // 2, d.data_ptr(),
-            d.stride(0) if N > 1 else K // 32, ptr(bias), ptr(residual), ldr, dst.data_ptr(), ldo, M, N, K, ptr(ws), n,
+    args = (x2.data_ptr(), ldx if M > 1 else K, qs.data_ptr(), ldq if N > 1 else K // 2, d.data_ptr(), ldd if N > 1 else blocks,
+            ptr(bias), ptr(residual), ldr if M > 1 else N, dst.data_ptr(), ldo, M, N, K, ptr(ws), n,
             torch._C._cuda_getCurrentRawStream(dev))
     if dev == torch._C._cuda_getDevice():
         check(lib().od_q4_linear(*args), "od_q4_linear")
