@@ -51,7 +51,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t by
 // A workgroup's WR x WK waves take WR sets of RT row tiles, WK of them every WK-th step of one, and add up in LDS. x lies in LDS in
 // the order of the B operand, as many steps of it as fit at a time, two buffers of it; the weights of the PD next steps are in
 // registers or on their way meanwhile, whatever the workgroup waits for. One row of x: 4096 x 4096 8.9 us (9.4 MB), 24576 x 4096
-// 20.6 us (2.8 TB/s), 151936 x 4096 87 us (4.0 TB/s); 24 rows over 24576 x 4096 31 us, where it is the products and the exchanges.
+// 20.6 us (2.8 TB/s), 151936 x 4096 87 us (4.0 TB/s); 24 rows over 24576 x 4096 27.5 us, where x, staged by every workgroup, is as much as the weights.
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256) void q4_sum_kernel(Q4Args p) {
   q4_store(p, m, n, y);
 }
 
-// Up to 32 rows take the first kernel, above it the tiles: 24576 x 4096, 32 rows 31 against 45 us, 64 rows 46 (by 64 rows of x
+// Up to 32 rows take the first kernel, above it the tiles: 24576 x 4096, 32 rows 29 against 45 us, 64 rows 46 (by 64 rows of x
 // at a time) against 45; 4096 x 4096, 32 rows 15 against 20, 64 rows 44 against 23.
 constexpr int64_t kFewRows = 32;
 
@@ -554,6 +554,8 @@ int launch_rows(Q4Args& a, hipStream_t st) {
 // (two sets of two tiles 11.9; 15.3). Then two tiles a wave, which share x: 49152 x 4096 28.6; 37.2 (one tile a workgroup 38.8;
 // 60.7, two 32.2; 44.5). With many of them and several rows of x, four sets, whose x is staged half as often: 98304 x 4096, 16 rows
 // 65.9 against 70.4, 32 rows 79.1 against 87.3; at one row 58.9 against 55.2, and 32 rows over 49152 x 4096 51.8 against 47.7.
+// Above 16 rows x is as much to stage as the weights are to read: eight sets of a tile where these are one workgroup for every CU
+// (24 rows over 24576 x 4096 27.5 against 31.6, 32768 x 4096 27.7 and 32.0; but 12288 x 4096 26.7 and 20.7).
 int launch_few(Q4Args& a, hipStream_t st) {
   const int64_t tiles = (a.N + 15) / 16, cus = od_cu_count();
   if (a.M <= 16) {
@@ -561,6 +563,7 @@ int launch_few(Q4Args& a, hipStream_t st) {
     return tiles <= 14 * cus || a.M <= 8 ? launch_rows<2, 1, 4, 2, 2>(a, st) : launch_rows<2, 1, 2, 4, 2>(a, st);
   }
   if (tiles <= 2 * cus) return launch_rows<1, 2, 4, 2, 4>(a, st);
+  if (tiles > 4 * cus && tiles <= 8 * cus) return launch_rows<1, 2, 2, 8, 4>(a, st);
   return tiles <= 14 * cus ? launch_rows<2, 2, 4, 2, 2>(a, st) : launch_rows<2, 2, 2, 4, 2>(a, st);
 }
 

@@ -77,6 +77,20 @@ def test_attention(gpu_lib, shape, d, heads, kv):
     check_attn(c, *run_attn(c))
 
 
+@pytest.mark.parametrize("d,heads,kv", [(64, 4, 4), (128, 8, 2), (256, 8, 4), (256, 4, 1)])
+@pytest.mark.parametrize("seqs", [1, 3, 90])
+def test_tokens_of_many_sequences(gpu_lib, seqs, d, heads, kv):
+    """One token a sequence, from few (the cached tokens in many parts) to more workgroups than CUs."""
+    g = torch.Generator().manual_seed(seqs)
+    ctx = torch.randint(0, 2600 if seqs < 10 else 300, (seqs,), generator=g).tolist()
+    ctx[-1] = 2600 if seqs < 10 else 300
+    c = tp.make(70 + seqs, [1] * seqs, ctx, heads, kv, d, page=32, int8=False)
+    shape = c["pages"][0].shape[:3]  # any bytes are rows of 4 bits
+    c["pages"] = [torch.randint(0, 256, (*shape, d // 2), generator=g, dtype=torch.uint8) for _ in range(2)]
+    c["scales"] = [(torch.randn(*shape, d // 32, generator=g) / 4).to(BF) for _ in range(2)]
+    check_attn(c, *run_attn(c))
+
+
 @pytest.mark.parametrize("d,heads,kv", [(64, 4, 4), (128, 8, 2), (256, 4, 1), (128, 7, 1)])
 @pytest.mark.parametrize("form", FORMS[1:])
 @pytest.mark.parametrize("shape", range(len(MANY)))

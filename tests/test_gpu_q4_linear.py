@@ -69,6 +69,12 @@ def test_linear(gpu_lib, M, N, K):
     check(kernels.q4_linear(x.to(DEV), qs.to(DEV), d.to(DEV)), x, w, d)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 9000, 160), (16, 9001, 2080), (7, 60000, 96), (1, 60001, 1056), (12, 60001, 1056), (20, 9000, 288),
+                                   (32, 9001, 2080), (29, 17000, 2080), (18, 30007, 160), (24, 40000, 544), (30, 60001, 1056), (40, 30000, 224)])
+def test_many_rows_of_weights(gpu_lib, M, N, K):
+    test_linear(gpu_lib, M, N, K)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 50, 96), (20, 100, 544), (70, 131, 1056)])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("residual", [False, True])
