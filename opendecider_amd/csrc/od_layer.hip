@@ -431,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
   int head, b0 = 0;  // pages: b0 the last sequence that starts at or before the wave's first row, by all its lanes
   if constexpr (PAGED) {
     // (M heads is below 2^32; a wave's first item divides, its others follow: 64-bit divisions by every lane cost as much as the
-    // norm: 7200 tokens of 48 heads of 128 into 4-bit pages 33 us with them, 30.5 without)
+    // norm: 5150 tokens of 48 heads of 128 into 4-bit pages 33 us with them, 30.5 without)
     const uint32_t first = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / G) + (threadIdx.x >> 6) * (64 / G));
     if (first >= (uint32_t)(M * heads)) return;
     const int t0 = (int)(first / (uint32_t)heads), h0 = (int)(first - (uint32_t)t0 * (uint32_t)heads);

@@ -1051,9 +1051,9 @@ def q4_linear_workspace_floats(M: int, N: int, K: int, device) -> int:
 def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Tensor | None = None,
               residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """od_q4_linear: x (..., K) bf16 times 4-bit weights in Q4Table's layout, qs uint8 (N, K / 2) and d fp16 (N, K / 32), plus
-    bias (N,) and residual (..., N) bf16: (..., N) bf16, rounded once. K a multiple of 32. Up to 32 rows of x no weight is rounded;
-    for more each is once, to fp16. A row of x that holds an infinity or NaN comes out NaN. out (..., N) bf16 may be the
-    residual."""
+    bias (N,) and residual (..., N) bf16: (..., N) bf16, rounded once. K a multiple of 32. Up to 32 rows of x no weight is rounded
+    (|x| up to 2^115); for more each is once, to fp16. A row of x that holds an infinity or NaN comes out NaN. out (..., N) bf16
+    may be the residual, and overlaps no other input. No gradients."""
     dev = _one_device("q4_linear", x, qs, d, bias, residual, out)
     _lib.bf16_bits(x)
     if qs.dtype != torch.uint8 or d.dtype != torch.float16:
@@ -1178,8 +1178,8 @@ class _OnDevice:
 def page_append(k: torch.Tensor, v: torch.Tensor, cache, table: torch.Tensor, start: torch.Tensor,
                 ctx_len: torch.Tensor) -> None:
     """od_page_append_ex: the new tokens' k and v (N, Hkv, D) bf16 into the pages of a PagedKVCache, quantized per (token,
-    head) where the pages are int8 (the bytes of kv_quant_append), per 32 values of one where they hold 4 bits. table int32 (B, pages per sequence); start int32
-    (B + 1,): sequence b's tokens are the rows start[b] .. start[b + 1] - 1; ctx_len int32 (B,): the tokens it holds
+    head) where the pages are int8 (the bytes of kv_quant_append), per 32 values of one where they hold 4 bits. table int32 (B, pages
+    per sequence); start int32 (B + 1,): sequence b's tokens are the rows start[b] .. start[b + 1] - 1; ctx_len int32 (B,): the tokens it holds
     before, which is where they go. Tokens without a page are not written. The lengths stay: advance them once every layer
     has its tokens."""
     _one_device("page_append", k, v, cache.k, cache.v, table, start, ctx_len)

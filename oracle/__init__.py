@@ -18,8 +18,8 @@ Modules
              gates, the gated delta rule, the gated RMSNorm. Reference: transformers' Qwen3.5 modules, which the
              reference runs (src/opendecider/backbone.py:256-289, skipkv.py:208-231).
 
-  paged      The paged K/V cache: where a packed token lies, writing, reading back, and attention over pages in float64.
-             No counterpart in the reference (its caches are rectangular); written from the layout.
+  paged      The paged K/V cache: where a packed token lies, writing, reading back, and attention over pages in float64,
+             int8, bf16 and 4-bit pages. No counterpart in the reference (its caches are rectangular); written from the layout.
 
 Pinning (how each function is checked, in tests/test_oracle_*.py)
   quant.quantize_rows      brute-force per-element IEEE float32 arithmetic with numpy and round-half-even, hand
