@@ -323,15 +323,6 @@ __device__ __forceinline__ void unpackh(const VecH<H>& u, float (&f)[H]) {
   }
 }
 
-template <int H>
-__device__ __forceinline__ VecH<H> packh(const uint16_t (&h)[H]) {
-  VecH<H> v;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-  for (int k = 0; k < H / 2; ++k) w[k] = (uint32_t)h[2 * k] | ((uint32_t)h[2 * k + 1] << 16);
-  return v;
-}
-
 // Quantizes a head's D bf16 values held 2H per lane (oa: d = da .. da + H - 1, ob: d = db .. db + H - 1) over the G
 // lanes of its group and writes the int8 row and its scale.
 template <int D, int H>
@@ -431,7 +422,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
   int head, b0 = 0;  // pages: b0 the last sequence that starts at or before the wave's first row, by all its lanes
   if constexpr (PAGED) {
     // (M heads is below 2^32; a wave's first item divides, its others follow: 64-bit divisions by every lane cost as much as the
-    // norm: 5150 tokens of 48 heads of 128 into 4-bit pages 33 us with them, 30.5 without)
+    // norm: 5150 tokens of 48 heads of 128 into 4-bit pages 33 us with them, 30.5 without; 28.5 with two values
+    // a rounding below)
     const uint32_t first = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / G) + (threadIdx.x >> 6) * (64 / G));
     if (first >= (uint32_t)(M * heads)) return;
     const int t0 = (int)(first / (uint32_t)heads), h0 = (int)(first - (uint32_t)t0 * (uint32_t)heads);
@@ -489,18 +481,20 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
   for (int e = 0; e < H; ++e) ss = fma((double)b[e], (double)b[e], fma((double)a[e], (double)a[e], ss));
   ss = od_group_sum_f64<G>(ss);
   const float r = od_rms_factor(ss, D, eps);
-  float na[H], nb[H];
+  float na[H], nb[H];  // (two values a rounding)
 #pragma unroll
   for (int e = 0; e < H; ++e) {
     if constexpr (ZC) {
-      na[e] = bfr((a[e] * r) * (1.0f + fa[e]));
-      nb[e] = bfr((b[e] * r) * (1.0f + fb[e]));
+      na[e] = (a[e] * r) * (1.0f + fa[e]);
+      nb[e] = (b[e] * r) * (1.0f + fb[e]);
     } else {
-      na[e] = bfr(fa[e] * bfr(a[e] * r));
-      nb[e] = bfr(fb[e] * bfr(b[e] * r));
+      float ta = a[e] * r, tb = b[e] * r;
+      od_bfr2(ta, tb);
+      na[e] = fa[e] * ta;
+      nb[e] = fb[e] * tb;
     }
+    od_bfr2(na[e], nb[e]);
   }
-  uint16_t oa[H], ob[H];
   if (rot) {
     const int64_t p = pos[row];
     const bool in_table = p >= 0 && p < n_pos;  // a position past the tables yields NaN, never an out-of-bounds read
@@ -514,27 +508,41 @@ __global__ __launch_bounds__(kThreads) void qk_rope_vec_kernel(uint16_t* __restr
     }
 #pragma unroll
     for (int e = 0; e < H; ++e) {
-      oa[e] = od_f32_to_bf16(bfr(na[e] * c[e]) + bfr(-nb[e] * sn[e]));
-      ob[e] = od_f32_to_bf16(bfr(nb[e] * c[e]) + bfr(na[e] * sn[e]));
+      float ac = na[e] * c[e], bs = -nb[e] * sn[e], bc = nb[e] * c[e], as = na[e] * sn[e];
+      od_bfr2(ac, bs);
+      od_bfr2(bc, as);
+      na[e] = ac + bs;
+      nb[e] = bc + as;
     }
-  } else {
+  }
+  V pa, pb;
+  uint32_t* pwa = reinterpret_cast<uint32_t*>(&pa);
+  uint32_t* pwb = reinterpret_cast<uint32_t*>(&pb);
 #pragma unroll
-    for (int e = 0; e < H; ++e) {
-      oa[e] = od_f32_to_bf16(na[e]);
-      ob[e] = od_f32_to_bf16(nb[e]);
-    }
+  for (int k = 0; k < H / 2; ++k) {
+    pwa[k] = od_pack_bf16x2(na[2 * k], na[2 * k + 1]);
+    pwb[k] = od_pack_bf16x2(nb[2 * k], nb[2 * k + 1]);
   }
   if constexpr (PAGED) {
     uint16_t* op = kv.out + row * kv.ldo + (int64_t)head * D;
-    const V pa = packh<H>(oa), pb = packh<H>(ob);
     *reinterpret_cast<V*>(op + da) = pa;
     *reinterpret_cast<V*>(op + db) = pb;
     if (head >= n_heads_q && crow >= 0) page_head<D, RD, APPEND - kPages>(kv.p, false, crow, pa, pb, j, da, db);
   } else {
-    *reinterpret_cast<V*>(hp + da) = packh<H>(oa);
-    *reinterpret_cast<V*>(hp + db) = packh<H>(ob);
+    *reinterpret_cast<V*>(hp + da) = pa;
+    *reinterpret_cast<V*>(hp + db) = pb;
     if constexpr (APPEND == kRows)
-      if (head >= n_heads_q) quant_head<D, H>(oa, ob, j, da, db, kv.kq + crow * D, kv.ks + crow);
+      if (head >= n_heads_q) {
+        uint16_t oa[H], ob[H];
+#pragma unroll
+        for (int k = 0; k < H / 2; ++k) {
+          oa[2 * k] = (uint16_t)pwa[k];
+          oa[2 * k + 1] = (uint16_t)(pwa[k] >> 16);
+          ob[2 * k] = (uint16_t)pwb[k];
+          ob[2 * k + 1] = (uint16_t)(pwb[k] >> 16);
+        }
+        quant_head<D, H>(oa, ob, j, da, db, kv.kq + crow * D, kv.ks + crow);
+      }
   }
 }
 
