@@ -110,6 +110,23 @@ def test_every_value_and_place(gpu_lib, M):
     assert torch.equal(got, want.to(BF).double())
 
 
+@pytest.mark.parametrize("lead", [(), (0,), (2, 0), (3, 1), (2, 20)])
+def test_leading_dims(gpu_lib, lead):
+    """A vector, no rows, several leading dims; an output and a residual of that shape, which may be one tensor."""
+    from opendecider_amd import kernels
+    N, K = 70, 160
+    M = math.prod(lead)
+    qs, d, w = weights(N, K, 12)
+    x, r = rows(M, K, 13), rows(M, N, 14)
+    y = kernels.q4_linear(x.view(*lead, K).to(DEV), qs.to(DEV), d.to(DEV), residual=r.view(*lead, N).to(DEV))
+    assert y.shape == (*lead, N) and y.dtype == BF
+    if M:
+        check(y.view(M, N), x, w, d, residual=r)
+    both = r.view(*lead, N).to(DEV)
+    assert kernels.q4_linear(x.view(*lead, K).to(DEV), qs.to(DEV), d.to(DEV), residual=both, out=both) is both
+    assert torch.equal(both, y)
+
+
 @pytest.mark.parametrize("M", [3, 50])
 def test_strides(gpu_lib, M):
     from opendecider_amd import kernels
