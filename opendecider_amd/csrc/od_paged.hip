@@ -1756,7 +1756,8 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
           }
         }
         if (REG && f_new != frame) {  // the values' frame rose: uniform over the workgroup
-          const float f = __builtin_ldexpf(1.0f, frame - f_new);
+          // (or is the first one, and may lie lower by any amount: O is 0 still, or NaN)
+          const float f = __builtin_ldexpf(1.0f, min(frame - f_new, 0));
 #pragma unroll
           for (auto& o : t.o)
 #pragma unroll
@@ -1977,9 +1978,9 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) pb[k] = sm.p[grp][k][lane];
     };
-    auto rescale = [&](int f_new) {  // uniform over the workgroup
+    auto rescale = [&](int f_new, int by) {  // uniform over the workgroup
       if (f_new == frame) return;
-      const float f = __builtin_ldexpf(1.0f, frame - f_new);
+      const float f = __builtin_ldexpf(1.0f, by);
 #pragma unroll
       for (auto& o : t.o)
 #pragma unroll
@@ -2162,7 +2163,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         p3 = pages(blk + 4);
         v4u pb[4];
         if (live) {
-          if constexpr (REG) rescale(f_now);
+          // the values' frame rose (or is the first one, and may lie lower by any amount: O is 0 still, or NaN)
+          if constexpr (REG) rescale(f_now, min(frame - f_now, 0));
           softmax(HT{}, x, c, mine);
         }
         __syncthreads();
@@ -2177,7 +2179,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     if (sp == 0 && a.k) {
       if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
-        rescale(0);
+        rescale(0, frame);
       }
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load_k = [&](int blk) {
