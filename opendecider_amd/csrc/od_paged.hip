@@ -492,10 +492,10 @@ struct SAcc {
   v4f o[D / 16];
 };
 
-// One tile's online softmax: y the lane's 8 scores (log2 units, -inf masked); p out, 2^lift above its value.
+// One tile's online softmax: y the lane's 8 scores (log2 units, -inf masked); p out, 2^s_lift above its value.
 constexpr float s_lift(int P) { return P == kInt4 ? kLift : 0.0f; }
-template <int D>
-__device__ __forceinline__ void s_probabilities(float (&y)[8], float lift, SAcc<D>& x, float (&p)[8]) {
+template <int P, int D>
+__device__ __forceinline__ void s_probabilities(float (&y)[8], SAcc<D>& x, float (&p)[8]) {
   float mx = y[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) mx = fmaxf(mx, y[i]);
@@ -511,7 +511,7 @@ __device__ __forceinline__ void s_probabilities(float (&y)[8], float lift, SAcc<
     x.l *= c;
     if (move) x.m = mx;
   }
-  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - lift;
+  const float ms = (x.m == -INFINITY ? 0.0f : x.m) - s_lift(P);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     p[i] = __builtin_amdgcn_exp2f(y[i] - ms);
@@ -548,10 +548,10 @@ __device__ __forceinline__ v4u s_half(const float (&y)[8], float c, SAcc<D>& x) 
   return r;
 }
 // The same into bf16 hi and lo parts: f a factor on p for the P.V product only (the V scales).
-template <int D, bool F>
-__device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], float lift, SAcc<D>& x, v4u& hi, v4u& lo) {
+template <int D, int P, bool F>
+__device__ __forceinline__ void s_softmax(float (&y)[8], const float (&f)[8], SAcc<D>& x, v4u& hi, v4u& lo) {
   float p[8];
-  s_probabilities(y, lift, x, p);
+  s_probabilities<P>(y, x, p);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float u = F ? p[2 * e] * f[2 * e] : p[2 * e], w = F ? p[2 * e + 1] * f[2 * e + 1] : p[2 * e + 1];
@@ -594,12 +594,6 @@ __device__ __forceinline__ uint32_t s_wave_max2(uint32_t x) {
   return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// In the frames of fp16, values are below 2^14 and no sum of them passes fp32. The new tokens' bf16 values are as they are, and
-// probabilities of up to 2^(kLift + kSlack) beside values of 2^113 do pass it, though O / l is finite. Work whose O is not, once they
-// were added, is done again with their probabilities lowered by 2^64: no sum of finite values passes fp32 then, and what a probability
-// loses is 2^-69 of the largest. Rare: it costs a look at O.
-constexpr int kLower = 64;
-
 constexpr int kStreamWaves = 4;
 // waves a SIMD's registers hold
 constexpr int s_waves(int D, int P, int columns) {
@@ -620,7 +614,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
     };
     float o[NW][16][D + 4];
   } sm;
-  __shared__ int qe[Q4 ? 16 * CT : 1], frames[NW], over;  // over: some O is not finite
+  __shared__ int qe[Q4 ? 16 * CT : 1], frames[NW];
   __shared__ float sml[NW][2][16];
   // a tile's per-key factors, from lane order to score order (one wave writes and reads)
   __shared__ float4 skf[Q8 ? NW : 1][2][8];
@@ -636,9 +630,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
   if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
   const int t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
   // one round unless max_new was too small
-  int lower = 0;  // the power of two that the new tokens' probabilities are lowered by
-  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep;) {
-    const float lift = s_lift(P) - lower;
+  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep; z0 += a.tiles * 16 * CT) {
     constexpr int QN = 16 * CT * (D / 8), QC = QN / (NW * 64) ? QN / (NW * 64) : 1;
     uint4 qw[QC];
 #pragma unroll
@@ -670,7 +662,6 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
       for (int i = 0; i < SETS - 1; ++i) next(tl[i]);
     }
     __syncthreads();  // an earlier round's readers are done
-    if (Q4 && threadIdx.x == 0) over = 0;
 #pragma unroll
     for (int k = 0; k < QC; ++k) {
       const int i = k * NW * 64 + threadIdx.x;
@@ -714,19 +705,15 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
     // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
-      if (Q4 && frame != lower) {
-        const float f = __builtin_ldexpf(1.0f, frame - lower);
+      if (Q4 && frame != 0) {
+        const float f = __builtin_ldexpf(1.0f, frame);
 #pragma unroll
         for (auto& x : acc)
 #pragma unroll
           for (auto& o : x.o)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] *= f;
-      }
-      if constexpr (Q4) {
         frame = 0;
-#pragma unroll
-        for (auto& x : acc) x.l *= __builtin_ldexpf(1.0f, -lower);
       }
       const int t_end = min((z0 + 16 * CT - 1) / a.rep, s.n - 1);  // last token of these slots
       int k_lo = 0;                                                // the first one that any of them sees
@@ -783,7 +770,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
             f[i] = 1.0f;
           }
           v4u hi, lo;
-          s_softmax<D, false>(y, f, lift, x, hi, lo);
+          s_softmax<D, P, false>(y, f, x, hi, lo);
           if (__builtin_amdgcn_ballot_w64(odd) != 0) {
 #pragma unroll 1
             for (int key = k0; key < k0 + left; ++key) {
@@ -987,7 +974,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
           for (int i = 0; i < 4 * R; ++i)
             if (4 * qd + (i & 3) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
-        s_softmax<D, Q8>(y, f, s_lift(P), acc[ct], hi[ct], lo[ct]);
+        s_softmax<D, P, Q8>(y, f, acc[ct], hi[ct], lo[ct]);
       }
       if constexpr (!Q8) {
         // The low part of a probability may be 0 or negative: infinities and NaN among the values are taken by the high
@@ -1035,28 +1022,13 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
 
     if constexpr (!first) new_tokens();
 
-    if (Q4 && sp == 0 && a.k && lower == 0) {
-      float sum = 0.0f;  // NaN where an O is past 2^124: the waves' sum is finite then
-#pragma unroll
-      for (auto& x : acc)
-#pragma unroll
-        for (auto& o : x.o)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(o[i] * 16.0f, 0.0f, sum);
-      if (sum != 0.0f) over = 1;
-    }
     // merge the waves, then the output or this split's normalized partial
-    bool again = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const SAcc<D>& x = acc[ct];
       float l = x.l + __shfl_xor(x.l, 16, 64);
       l = od_xor32_sum(l);
       __syncthreads();  // every wave is done with the queries, or the columns before
-      if (Q4 && ct == 0 && lower == 0 && __builtin_amdgcn_readfirstlane(over)) {
-        again = true;
-        break;
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1096,7 +1068,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
           sum.w += e * v.w;
         }
         // a sum of 0: no key seen (o is 0 then); a wave with NaN scores has a NaN sum, which reaches L
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L) - lift;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L, ls = M + __log2f(L) - s_lift(P);
         const int64_t n = s.s0 + z / a.rep, head = g * a.rep + z % a.rep;
         sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
         if constexpr (Q4) {
@@ -1115,8 +1087,6 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
         }
       }
     }
-    lower = again ? kLower : 0;
-    if (!again) z0 += a.tiles * 16 * CT;
   }
 }
 
@@ -1148,8 +1118,6 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
   if (n < s.s0 || n >= s.s0 + s.n || nv == 1) return;  // uniform over the workgroup
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0, 0, 0, 0);
-  // (parts in units of 2^8: the sum of as many as a call is split into, 128, is finite)
-  auto part = [](float4 u) { return make_float4(u.x * 0x1p-8f, u.y * 0x1p-8f, u.z * 0x1p-8f, u.w * 0x1p-8f); };
   auto add = [&](float l, float w, float4 u) {  // w: the weight that comes with l
     const float m2 = fmaxf(M, l), ms = m2 == -INFINITY ? 0.0f : m2;  // a NaN l leaves M and makes the sums NaN
     const float r = __builtin_amdgcn_exp2f(M - ms), f = __builtin_amdgcn_exp2f(l - ms);
@@ -1159,10 +1127,10 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
-    if (grp + i * S < nv) add(l4[i], 1.0f, part(u4[i]));
+    if (grp + i * S < nv) add(l4[i], 1.0f, u4[i]);
 #pragma unroll 4
   for (int sp = grp + AHEAD * S; sp < nv; sp += S)
-    add(ls[sp * step + slot], 1.0f, part(*reinterpret_cast<const float4*>(po + sp * step * D)));
+    add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
   if constexpr (S > 1) {
     so[sl][grp][c] = acc;
     if (c == 0) {
@@ -1175,7 +1143,7 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
       if (grp == 0) add(sml[sl][k][0], sml[sl][k][1], so[sl][k][c]);
   }
   if (grp != 0 || my >= a.Hq) return;
-  const float inv = L == 0.0f ? 0.0f : 0x1p8f / L;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + 4 * c) =
       make_uint2(od_pack_bf16x2(acc.x * inv, acc.y * inv), od_pack_bf16x2(acc.z * inv, acc.w * inv));
   if (a.lse && c == 0) a.lse[slot] = (M + __log2f(L)) * kLn2;
@@ -1328,7 +1296,6 @@ struct alignas(16) TSmem {
   uint16_t k[2][kBK * D];
   uint16_t v[2][kBK * D];
   int lo[NW], hi[NW];
-  int over;  // a slot's O is not finite
   int odd;  // infinities or NaN among the new values of a block that some slot sees only a part of
 };
 
@@ -1402,9 +1369,9 @@ __device__ __forceinline__ void t_scores(const uint16_t* kb, const TSlot<D>& t, 
   }
 }
 
-// The block's online softmax into P, 2^lift above its value; c > 0: the scores' factor (log2 units), masked scores -inf.
+// The block's online softmax into P; c > 0: the scores' factor (log2 units), masked scores -inf.
 template <int D, bool H>
-__device__ __forceinline__ void t_softmax(v16f (&s)[2], float c, float lift, TSlot<D>& t, v4u (&pb)[4]) {
+__device__ __forceinline__ void t_softmax(v16f (&s)[2], float c, TSlot<D>& t, v4u (&pb)[4]) {
   float mx = -INFINITY;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
@@ -1421,7 +1388,7 @@ __device__ __forceinline__ void t_softmax(v16f (&s)[2], float c, float lift, TSl
     t.l *= f;
     if (move) t.m = mx;
   }
-  const float ms = (t.m == -INFINITY ? 0.0f : t.m) - lift;
+  const float ms = (t.m == -INFINITY ? 0.0f : t.m) - kLift;
   float sum = 0.0f;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt)
@@ -1581,12 +1548,12 @@ __device__ __forceinline__ void add_odd(const AttnArgs& a, const Seq& s, int g, 
 }
 // out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
 template <int D>
-__device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, float lift, int frame,
-    int sp, int nv, int half) {
+__device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, int frame, int sp,
+    int nv, int half) {
   if (!t.ok) return;
   const int h = (threadIdx.x & 63) >> 5;
   // 2^frame may be subnormal, so it comes last
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = __builtin_ldexpf(1.0f, frame), ls = t.m + __log2f(l) - lift;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = __builtin_ldexpf(1.0f, frame), ls = t.m + __log2f(l) - kLift;
   const int64_t n = s.s0 + t.tok;
 #pragma unroll
   for (int dt = 0; dt < t_cols(D); ++dt)
@@ -1605,17 +1572,6 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
     if (nv > 1) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + ((int64_t)sp * a.p.N + n) * a.Hq + t.head] = ls;
     else if (a.lse) a.lse[n * a.Hq + t.head] = ls * kLn2;
   }
-}
-
-// Whether an O is infinite or NaN, after bf16 values (kLower).
-template <int D>
-__device__ __forceinline__ bool t_over(const TSlot<D>& t) {
-  float x = 0.0f;
-#pragma unroll
-  for (int dt = 0; dt < t_cols(D); ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x = __builtin_fmaf(t.o[dt][i], 0.0f, x);
-  return t.ok && x != 0.0f;
 }
 
 // Waves a SIMD: heads of 64 leave the registers for three, but for the conversion of int8 and 4-bit blocks.
@@ -1644,11 +1600,8 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
-  int lower = 0;  // the power of two that bf16 probabilities are lowered by
-  for (int tile = at.tile; tile * SPT < nslots;) {
+  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
     __syncthreads();  // an earlier tile's readers are done
-    if (tid == 0) sm.over = 0;
-    const float lift = kLift - lower;
     TSlot<D> t;
     const int zw = tile * SPT + wave * 32, z = zw + col;
     const bool live = zw < nslots;  // the wave has slots
@@ -1823,7 +1776,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
               for (int i = 0; i < 16; ++i)
                 if (!((m4 >> (kt * 32 + 8 * (i >> 2) + (i & 3))) & 1)) sc[kt][i] = -INFINITY;
           }
-          t_softmax<D, H16>(sc, c, H16 ? kLift : lift, t, pb);
+          t_softmax<D, H16>(sc, c, t, pb);
           t_values<D, H16>(sm.v[cur], vb, pb, t);
         }
         if (!REG && blk + 1 < b_hi) {
@@ -1838,15 +1791,14 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
     if (sp == 0 && a.k) {
       if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
-        if (frame != lower) {
-          const float f = __builtin_ldexpf(1.0f, frame - lower);
+        if (frame != 0) {
+          const float f = __builtin_ldexpf(1.0f, frame);
 #pragma unroll
           for (auto& o : t.o)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= f;
+          frame = 0;
         }
-        frame = 0;
-        t.l *= __builtin_ldexpf(1.0f, -lower);
       }
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load = [&](int blk, int buf) {
@@ -1881,7 +1833,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
                   if (key > t.tok || key < t.begin) sc[kt][i] = -INFINITY;
                 }
             }
-            t_softmax<D, false>(sc, a.scale_log2, lift, t, pb);
+            t_softmax<D, false>(sc, a.scale_log2, t, pb);
             t_values<D, false>(sm.v[cur], vb, pb, t);
           }
           if (blk + 1 < n.hi) {
@@ -1894,17 +1846,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       }
     }
 
-    if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
-      if (t_over<D>(t)) sm.over = 1;
-      __syncthreads();
-      if (__builtin_amdgcn_readfirstlane(sm.over)) {
-        lower = kLower;
-        continue;
-      }
-    }
-    t_out<D>(a, s, t, od_xor32_sum(t.l), lift, frame, sp, nv, 0);
-    lower = 0;
-    tile += a.tiles;
+    t_out<D>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, 0);
   }
 }
 
@@ -1924,7 +1866,7 @@ struct alignas(16) WSmem {
   v4u p[4][4][64];     // [slot group][k-step][lane]
   float mx[2][4][32];  // [half][slot group][slot]
   int lo[8], hi[8];
-  int over, odd;
+  int odd;
 };
 
 template <int SRC>
@@ -1950,11 +1892,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
-  int lower = 0;  // the power of two that bf16 probabilities are lowered by
-  for (int tile = at.tile; tile * SPT < nslots;) {
+  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
     __syncthreads();  // an earlier tile's readers are done
-    if (tid == 0) sm.over = 0;
-    const float lift = kLift - lower;
     TSlot<D> t;
     const int zw = tile * SPT + grp * 32, z = zw + col;
     const bool live = zw < nslots;  // the wave has slots
@@ -2015,7 +1954,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         t.l *= f;
         if (move) t.m = mx;
       }
-      const float ms = (t.m == -INFINITY ? 0.0f : t.m) - (decltype(H)::value ? kLift : lift);
+      const float ms = (t.m == -INFINITY ? 0.0f : t.m) - kLift;
       float sum = 0.0f;
       v4u mp[2];
 #pragma unroll
@@ -2240,9 +2179,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     if (sp == 0 && a.k) {
       if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
-        rescale(lower, frame - lower);
-        frame = 0;
-        t.l *= __builtin_ldexpf(1.0f, -lower);
+        rescale(0, frame);
       }
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load_k = [&](int blk) {
@@ -2293,23 +2230,13 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       }
     }
 
-    if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
-      if (t_over<D>(t)) sm.over = 1;
-      __syncthreads();
-      if (__builtin_amdgcn_readfirstlane(sm.over)) {
-        lower = kLower;
-        continue;
-      }
-    }
     // ---- the sum of both halves, then as above
     float l = od_xor32_sum(t.l);
     __syncthreads();  // the last block's maxima are read
     if (h == 0) sm.mx[half][grp][col] = l;
     __syncthreads();
     l += sm.mx[half ^ 1][grp][col];
-    t_out<D>(a, s, t, l, lift, frame, sp, nv, half);
-    lower = 0;
-    tile += a.tiles;
+    t_out<D>(a, s, t, l, frame, sp, nv, half);
   }
 }
 
