@@ -598,7 +598,8 @@ int od_readout(const uint16_t* h, int64_t ldh, const uint16_t* final_norm, int n
  *   nothing gets 0 and -inf. The pages are read, not written: append before or after. scale > 0 and finite. max_new and
  *   max_ctx are the caller's bounds on a sequence's new and cached tokens; they size the grid, the key splits and the
  *   workspace (od_paged_attn_ws floats, 16-byte aligned, NULL where that is 0; one call's at a time), not the result. out
- *   must not overlap the inputs. B <= 65535, N Hq / Hkv < 2^30.
+ *   must not overlap the inputs. Finite scores and values give finite outputs (a few new tokens over int8 or bf16 pages: where 2^8
+ *   |v| times the keys stays below 2^128). B <= 65535, N Hq / Hkv < 2^30.
  */
 #define OD_READ_BF16 0
 #define OD_READ_FP32 1

@@ -594,6 +594,21 @@ __device__ __forceinline__ uint32_t s_wave_max2(uint32_t x) {
   return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
+// In the frames of fp16, values are below 2^14 and no sum of them passes fp32. The new tokens' bf16 values are as they are, and
+// probabilities of up to 2^(kLift + kSlack) beside values of 2^113 do pass it, though O / l is finite. Work whose O is not, once they
+// were added, is done again with one factor of the products times 2^-64 (0 below 2^-63) and O in units of 2^64: no sum of finite values
+// passes fp32 then, and the other outputs keep their bits. Rare: it costs a look at O.
+constexpr int kLower = 64;
+__device__ __forceinline__ uint32_t lower_bf16x2(uint32_t w) {  // infinities and NaN as they are
+  uint32_t r = w & 0x80008000u;
+#pragma unroll
+  for (int i = 0; i < 32; i += 16) {
+    const int m = (int)(w >> i & 0x7fffu);
+    r |= (uint32_t)(m >= 0x7f80 ? m : max(m - (kLower << 7), 0)) << i;
+  }
+  return r;
+}
+
 constexpr int kStreamWaves = 4;
 // waves a SIMD's registers hold
 constexpr int s_waves(int D, int P, int columns) {
@@ -614,7 +629,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
     };
     float o[NW][16][D + 4];
   } sm;
-  __shared__ int qe[Q4 ? 16 * CT : 1], frames[NW];
+  __shared__ int qe[Q4 ? 16 * CT : 1], frames[NW], over;  // over: some O is not finite
   __shared__ float sml[NW][2][16];
   // a tile's per-key factors, from lane order to score order (one wave writes and reads)
   __shared__ float4 skf[Q8 ? NW : 1][2][8];
@@ -630,7 +645,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
   if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
   const int t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
   // one round unless max_new was too small
-  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep; z0 += a.tiles * 16 * CT) {
+  int lower = 0;  // the power of two that the new tokens' probabilities are lowered by
+  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep;) {
     constexpr int QN = 16 * CT * (D / 8), QC = QN / (NW * 64) ? QN / (NW * 64) : 1;
     uint4 qw[QC];
 #pragma unroll
@@ -662,6 +678,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
       for (int i = 0; i < SETS - 1; ++i) next(tl[i]);
     }
     __syncthreads();  // an earlier round's readers are done
+    if (Q4 && threadIdx.x == 0) over = 0;
 #pragma unroll
     for (int k = 0; k < QC; ++k) {
       const int i = k * NW * 64 + threadIdx.x;
@@ -705,16 +722,16 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
     // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
-      if (Q4 && frame != 0) {
-        const float f = __builtin_ldexpf(1.0f, frame);
+      if (Q4 && frame != lower) {
+        const float f = __builtin_ldexpf(1.0f, frame - lower);
 #pragma unroll
         for (auto& x : acc)
 #pragma unroll
           for (auto& o : x.o)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] *= f;
-        frame = 0;
       }
+      if constexpr (Q4) frame = lower;
       const int t_end = min((z0 + 16 * CT - 1) / a.rep, s.n - 1);  // last token of these slots
       int k_lo = 0;                                                // the first one that any of them sees
       if (a.row_begin) {
@@ -771,6 +788,10 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
           }
           v4u hi, lo;
           s_softmax<D, P, false>(y, f, x, hi, lo);
+          if (Q4 && lower) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) hi[e] = lower_bf16x2(hi[e]), lo[e] = lower_bf16x2(lo[e]);
+          }
           if (__builtin_amdgcn_ballot_w64(odd) != 0) {
 #pragma unroll 1
             for (int key = k0; key < k0 + left; ++key) {
@@ -1022,13 +1043,28 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
 
     if constexpr (!first) new_tokens();
 
+    if (Q4 && sp == 0 && a.k && lower == 0) {
+      v4f sum = v4f{0, 0, 0, 0};  // NaN where an O is past 2^124: the waves' sum is finite below it
+#pragma unroll
+      for (auto& x : acc)
+#pragma unroll
+        for (auto& o : x.o)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(o[i] * 16.0f, 0.0f, sum[i]);
+      if (sum[0] + sum[1] + sum[2] + sum[3] != 0.0f) over = 1;
+    }
     // merge the waves, then the output or this split's normalized partial
+    bool again = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const SAcc<D>& x = acc[ct];
       float l = x.l + __shfl_xor(x.l, 16, 64);
       l = od_xor32_sum(l);
       __syncthreads();  // every wave is done with the queries, or the columns before
+      if (Q4 && ct == 0 && lower == 0 && __builtin_amdgcn_readfirstlane(over)) {
+        again = true;
+        break;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1087,6 +1123,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
         }
       }
     }
+    lower = again ? kLower : 0;
+    if (!again) z0 += a.tiles * 16 * CT;
   }
 }
 
@@ -1118,6 +1156,8 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
   if (n < s.s0 || n >= s.s0 + s.n || nv == 1) return;  // uniform over the workgroup
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0, 0, 0, 0);
+  // (parts in units of 2^8: the sum of as many as a call is split into, 128, is finite)
+  auto part = [](float4 u) { return make_float4(u.x * 0x1p-8f, u.y * 0x1p-8f, u.z * 0x1p-8f, u.w * 0x1p-8f); };
   auto add = [&](float l, float w, float4 u) {  // w: the weight that comes with l
     const float m2 = fmaxf(M, l), ms = m2 == -INFINITY ? 0.0f : m2;  // a NaN l leaves M and makes the sums NaN
     const float r = __builtin_amdgcn_exp2f(M - ms), f = __builtin_amdgcn_exp2f(l - ms);
@@ -1127,10 +1167,10 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
-    if (grp + i * S < nv) add(l4[i], 1.0f, u4[i]);
+    if (grp + i * S < nv) add(l4[i], 1.0f, part(u4[i]));
 #pragma unroll 4
   for (int sp = grp + AHEAD * S; sp < nv; sp += S)
-    add(ls[sp * step + slot], 1.0f, *reinterpret_cast<const float4*>(po + sp * step * D));
+    add(ls[sp * step + slot], 1.0f, part(*reinterpret_cast<const float4*>(po + sp * step * D)));
   if constexpr (S > 1) {
     so[sl][grp][c] = acc;
     if (c == 0) {
@@ -1143,7 +1183,7 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(AttnArgs a, int
       if (grp == 0) add(sml[sl][k][0], sml[sl][k][1], so[sl][k][c]);
   }
   if (grp != 0 || my >= a.Hq) return;
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const float inv = L == 0.0f ? 0.0f : 0x1p8f / L;
   *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + 4 * c) =
       make_uint2(od_pack_bf16x2(acc.x * inv, acc.y * inv), od_pack_bf16x2(acc.z * inv, acc.w * inv));
   if (a.lse && c == 0) a.lse[slot] = (M + __log2f(L)) * kLn2;
@@ -1296,6 +1336,7 @@ struct alignas(16) TSmem {
   uint16_t k[2][kBK * D];
   uint16_t v[2][kBK * D];
   int lo[NW], hi[NW];
+  int over;  // a slot's O is not finite
   int odd;  // infinities or NaN among the new values of a block that some slot sees only a part of
 };
 
@@ -1574,6 +1615,26 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
   }
 }
 
+// A block's bf16 values times 2^-kLower. (A thread takes the chunks that it does in make_finite.)
+template <int D, int NT>
+__device__ __forceinline__ void t_lower(uint16_t* v) {
+  for (int c = threadIdx.x; c < kBK * (D / 8); c += NT) {
+    uint4* at = reinterpret_cast<uint4*>(&v[8 * c]);
+    const uint4 x = *at;
+    *at = make_uint4(lower_bf16x2(x.x), lower_bf16x2(x.y), lower_bf16x2(x.z), lower_bf16x2(x.w));
+  }
+}
+// Whether an O is infinite or NaN, after bf16 values (kLower).
+template <int D>
+__device__ __forceinline__ bool t_over(const TSlot<D>& t) {
+  v4f x = v4f{0, 0, 0, 0};
+#pragma unroll
+  for (int dt = 0; dt < t_cols(D); ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i & 3] = __builtin_fmaf(t.o[dt][i], 0.0f, x[i & 3]);
+  return t.ok && x[0] + x[1] + x[2] + x[3] != 0.0f;
+}
+
 // Waves a SIMD: heads of 64 leave the registers for three, but for the conversion of int8 and 4-bit blocks.
 constexpr int t_waves(int D, int src) { return D == 64 && (src == kBf16 || src == kImage) ? 3 : 2; }
 template <int D, int SRC, int NW>
@@ -1600,8 +1661,10 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
-  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
+  int lower = 0;  // the power of two that bf16 values are lowered by
+  for (int tile = at.tile; tile * SPT < nslots;) {
     __syncthreads();  // an earlier tile's readers are done
+    if (tid == 0) sm.over = 0;
     TSlot<D> t;
     const int zw = tile * SPT + wave * 32, z = zw + col;
     const bool live = zw < nslots;  // the wave has slots
@@ -1615,7 +1678,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
 #pragma unroll
     for (auto& o : t.o) o = zero16();
     t_load_q<D>(a, s, t);
-    int frame = 0;  // O is in units of 2^frame
+    int frame = H16 ? 0 : lower;  // O is in units of 2^frame
 
     // ---- the cached blocks b_lo .. b_hi - 1
     if (b_lo < b_hi) {
@@ -1718,11 +1781,12 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
             *reinterpret_cast<uint4*>(dst + o0) = __builtin_bit_cast(uint4, lo);
             *reinterpret_cast<uint4*>(dst + o1) = __builtin_bit_cast(uint4, hi);
           }
-        } else if (seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
+        } else if (seen != ~0ull || lower) {  // values of keys that are not there: 0 (their scores are masked)
           dma_wait();
           __syncthreads();
           for (int c = tid; c < kBK * (D / 8); c += NT)
             if (!((seen >> (c / (D / 8))) & 1)) *reinterpret_cast<uint4*>(&sm.v[buf][8 * c]) = make_uint4(0, 0, 0, 0);
+          if (lower) t_lower<D, NT>(sm.v[buf]);
         }
       };
       // One step: block blk's products; ahead of them, for int8 and 4 bits the conversion of block blk + 1 (in registers since the
@@ -1791,15 +1855,15 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
     if (sp == 0 && a.k) {
       if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
-        if (frame != 0) {
-          const float f = __builtin_ldexpf(1.0f, frame);
+        if (frame != lower) {
+          const float f = __builtin_ldexpf(1.0f, frame - lower);
 #pragma unroll
           for (auto& o : t.o)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= f;
-          frame = 0;
         }
       }
+      frame = lower;
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load = [&](int blk, int buf) {
         const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
@@ -1808,9 +1872,10 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
         dma_rows<D, NW>(sm.v[buf], wave, true, [&](int key) { return vp + min(blk * kBK + key, s.n - 1) * a.svt; });
       };
       auto finite = [&](int blk, int buf) {
-        if (!n.partial(blk)) return;
+        if (!n.partial(blk) && !lower) return;
         __syncthreads();  // every wave's part of the copy is there
-        make_finite<D, NT>(sm.v[buf], &sm.odd);
+        if (n.partial(blk)) make_finite<D, NT>(sm.v[buf], &sm.odd);
+        if (lower) t_lower<D, NT>(sm.v[buf]);
       };
       if (n.lo < n.hi) {
         load(n.lo, 0);
@@ -1846,7 +1911,17 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       }
     }
 
+    if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
+      if (t_over<D>(t)) sm.over = 1;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(sm.over)) {
+        lower = kLower;
+        continue;
+      }
+    }
     t_out<D>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, 0);
+    lower = 0;
+    tile += a.tiles;
   }
 }
 
@@ -1866,7 +1941,7 @@ struct alignas(16) WSmem {
   v4u p[4][4][64];     // [slot group][k-step][lane]
   float mx[2][4][32];  // [half][slot group][slot]
   int lo[8], hi[8];
-  int odd;
+  int over, odd;
 };
 
 template <int SRC>
@@ -1892,8 +1967,10 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     vb[dt] = (4 * hh + e) * D + (tv_chunk<D>(e, half * 16 + 4 * dt + 2 * mh + (c >> 1)) << 3) + 4 * (c & 1);
   }
 
-  for (int tile = at.tile; tile * SPT < nslots; tile += a.tiles) {
+  int lower = 0;  // the power of two that bf16 values are lowered by
+  for (int tile = at.tile; tile * SPT < nslots;) {
     __syncthreads();  // an earlier tile's readers are done
+    if (tid == 0) sm.over = 0;
     TSlot<D> t;
     const int zw = tile * SPT + grp * 32, z = zw + col;
     const bool live = zw < nslots;  // the wave has slots
@@ -1907,7 +1984,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
 #pragma unroll
     for (auto& o : t.o) o = zero16();
     t_load_q<D>(a, s, t);
-    int frame = 0;  // O is in units of 2^frame
+    int frame = H16 ? 0 : lower;  // O is in units of 2^frame
 
     // this wave's half of a block's scores: keys 32 half + 8 (i / 4) + 4 h + i % 4
     auto scores = [&](auto H, const uint16_t* kb) {
@@ -2141,10 +2218,11 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         }
         if constexpr (!REG) dma_wait();  // this wave's part of V(blk) and K(blk + 1)
         __syncthreads();
-        if (!H16 && seen != ~0ull) {  // values of keys that are not there: 0 (their scores are masked)
+        if (!H16 && (seen != ~0ull || lower)) {  // values of keys that are not there: 0 (their scores are masked)
           for (int i = tid; i < kBK * (D / 8); i += NT)
             if (!((seen >> (i / (D / 8))) & 1))
               *reinterpret_cast<uint4*>(&sm.v[blk & 1][8 * i]) = make_uint4(0, 0, 0, 0);
+          if (lower) t_lower<D, NT>(sm.v[blk & 1]);
         }
         const int f_now = f_cur;
         if constexpr (REG) {
@@ -2179,8 +2257,9 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     if (sp == 0 && a.k) {
       if (H16 && b_lo < b_hi) {  // back to bf16 queries and values as they are
         t_load_q<D>(a, s, t);
-        rescale(0, frame);
+        rescale(lower, frame - lower);
       }
+      frame = lower;
       const NewSpan n = new_span(a, s, tile, SPT, zw, live, t, sm.lo, sm.hi, &sm.odd, NW, wave);
       auto load_k = [&](int blk) {
         const uint16_t* kp = a.k + (int64_t)s.s0 * a.skt + (int64_t)g * a.skh;
@@ -2216,6 +2295,7 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
           dma_wait();
           __syncthreads();
           if (n.partial(blk)) make_finite<D, NT>(sm.v[blk & 1], &sm.odd);
+          if (lower) t_lower<D, NT>(sm.v[blk & 1]);
           if (blk + 2 < n.hi) load_k(blk + 2);
           if (blk + 1 < n.hi) load_v(blk + 1);
           v4u pb[4];
@@ -2230,6 +2310,14 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       }
     }
 
+    if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
+      if (t_over<D>(t)) sm.over = 1;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(sm.over)) {
+        lower = kLower;
+        continue;
+      }
+    }
     // ---- the sum of both halves, then as above
     float l = od_xor32_sum(t.l);
     __syncthreads();  // the last block's maxima are read
@@ -2237,6 +2325,8 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
     __syncthreads();
     l += sm.mx[half ^ 1][grp][col];
     t_out<D>(a, s, t, l, frame, sp, nv, half);
+    lower = 0;
+    tile += a.tiles;
   }
 }
 

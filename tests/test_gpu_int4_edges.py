@@ -1,15 +1,18 @@
-"""Attention over 4-bit pages at the ends of what values may be, on the GPU against its float64 restatement: first values that are
-zeros and others that are the smallest numbers. Batches and checks are test_gpu_int4_pages.py's; the forms send them through each
-kernel that they can reach."""
+"""Attention over pages at the ends of what values may be, on the GPU against its float64 restatement: 4-bit pages whose first
+values are zeros and whose others are the smallest numbers, and values up to the largest finite ones, in 4-bit pages, in the others
+where they share the kernels, and among the new tokens. Batches, bounds and checks are test_gpu_int4_pages.py's and
+test_gpu_paged.py's; the forms send them through each kernel that they can reach."""
 import pytest
 import torch
 
 import test_gpu_int4_pages as t4
+import test_gpu_paged as tp
 from oracle import paged as op
 
 pytestmark = pytest.mark.gpu
 
 BF, FORMS = t4.BF, t4.FORMS
+MOST = torch.finfo(BF).max
 
 
 def zero_values(c, first):
@@ -43,3 +46,48 @@ def test_no_values_before_the_smallest(gpu_lib, own, exp, d, form):
             2.0 ** -133
         out = out[:n].double().cpu()
         assert ((out - ref).abs() <= bound).all(), ((out - ref).abs() / bound).max()
+
+
+LARGE = [(122, 125), (0, 125), (122, 0), (113, 113)]  # 2^ of the cached values' size over the usual one, and the new ones'
+
+
+def enlarged(c, cached, new):
+    i = 0 if c["scales"][1] is None else 1
+    side = (c["pages"], c["scales"])[i]
+    side[1] = (side[1].double() * 2.0 ** cached).clamp(-MOST, MOST).to(side[1].dtype)
+    c["v"] = (c["v"].double() * 2.0 ** new).clamp(-MOST, MOST).to(BF)
+    return c
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cached,new", LARGE)
+def test_values_up_to_the_largest(gpu_lib, cached, new, d, form):
+    """Averages of finite values are finite, whatever their size."""
+    for n, ctx, rows in (([1, 1], [600, 90], 0), ([40], [300], 0), ([30, 3], [130, 0], 8)):
+        c = enlarged(t4.as_many(t4.make(32, n, ctx, 4, 1, d, rows=rows, **t4.padded(form)), form), cached, new)
+        t4.check_attn(c, *t4.run_attn(c))
+        t4.check_attn(c, *t4.run_attn(c, own=False), own=False)
+
+
+@pytest.mark.parametrize("d,heads,kv", [(64, 8, 8), (128, 8, 1), (256, 4, 1)])
+def test_large_values_of_many_splits(gpu_lib, d, heads, kv):
+    """The merge of as many parts as a call is split into, each of them near the largest number."""
+    c = enlarged(t4.make(33, [1], [9000], heads, kv, d, page=64), 122, 122)
+    g = torch.Generator().manual_seed(5)
+    c["scales"][1] = (2.0 ** 124 * (1 + torch.rand(c["scales"][1].shape, generator=g) * 0.5)).to(BF)
+    c["pages"][1].fill_(0xFF)  # every value 7 times its scale: far past half of the largest number
+    c["q"] = c["q"] * 0.0  # a plain average of them all
+    c["v"] = torch.full(c["v"].shape, 2.0 ** 127).to(BF)
+    t4.check_attn(c, *t4.run_attn(c))
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("form", ["rows", "image"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cached,new", LARGE)
+def test_values_up_to_the_largest_in_other_pages(gpu_lib, cached, new, d, form, int8):
+    """Chunks and option rows over int8 and bf16 pages."""
+    for n, ctx, rows in (([40], [300], 0), ([30, 3], [130, 0], 8)):
+        c = enlarged(t4.as_many(tp.make(34, n, ctx, 4, 1, d, int8=int8, rows=rows, **t4.padded(form)), form), cached, new)
+        tp.check_attn(c, *t4.run_attn(c))
