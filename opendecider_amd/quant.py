@@ -236,7 +236,9 @@ class Q4Linear(nn.Module):
     layout and rounding of Q4Table, quant.py:206-246), activations in bf16. Single tokens and small batches read 4.5 bits a
     weight; long ones run on the matrix cores.
 
-    Buffers: qs uint8 (out, in / 2) and d fp16 (out, in / 32), in padded to a multiple of 32 with zero columns; bias (bf16 or None)."""
+    Buffers: qs uint8 (out, in / 2) and d fp16 (out, in / 32), in padded to a multiple of 32 with zero columns; bias (bf16 or None).
+    They keep their types where a model is cast; inputs and residuals of other types are cast to bf16, the output back to the
+    input's."""
 
     def __init__(self, qs: torch.Tensor, d: torch.Tensor, bias: torch.Tensor | None = None, in_features: int | None = None):
         super().__init__()
@@ -266,6 +268,16 @@ class Q4Linear(nn.Module):
     def weight(self) -> torch.Tensor:
         return Q4Table(qs=self.qs, d=self.d).weight[:, : self.in_features]
 
+    def _apply(self, fn, recurse=True):
+        # what a cast of the model (.to(dtype), .half(), .float()) does to parameters: the scales and the bias are of the format's
+        # types and keep them, bit for bit; moves between devices reach them
+        kept = {name: self._buffers[name] for name in ("d", "bias")}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if t is not None and self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         if not x.is_cuda:
             raise RuntimeError("Q4Linear runs on the MI355X only (no CPU path)")
@@ -273,6 +285,8 @@ class Q4Linear(nn.Module):
             raise ValueError(f"Q4Linear: {x.shape[-1]} input features, expected {self.in_features}")
         xb = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
         pad = 2 * self.qs.shape[1] - self.in_features
+        if residual is not None and residual.dtype != torch.bfloat16:
+            residual = residual.to(torch.bfloat16)
         y = kernels.q4_linear(F.pad(xb, (0, pad)) if pad else xb, self.qs, self.d, self.bias, residual)
         return y if x.dtype == torch.bfloat16 else y.to(x.dtype)
 
