@@ -25,6 +25,8 @@ class PagedKVCache:
         quantized = quantized if isinstance(quantized, str) else bool(quantized)
         if quantized not in kernels.PAGE_FORMATS:
             raise ValueError(f"PagedKVCache: quantized must be True, False, 'int8' or 'int4', got {quantized!r}")
+        if head_dim not in (64, 128, 256):  # (half of an odd one would be the width of another)
+            raise ValueError(f"PagedKVCache: head_dim must be 64, 128 or 256, got {head_dim}")
         dtype, width, scales = {0: (torch.bfloat16, head_dim, None), 1: (torch.int8, head_dim, ((), torch.float32)),
                                 2: (torch.uint8, head_dim // 2, ((head_dim // 32,), torch.bfloat16))}[kernels.PAGE_FORMATS[quantized]]
         k, v = (torch.zeros(n_pages, n_heads, page, width, dtype=dtype, device=device) for _ in range(2))
