@@ -1068,15 +1068,15 @@ def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Te
     shape = (*lead, N)
     x2 = x if len(lead) == 1 else x.reshape(-1, K)
     M = x2.shape[0]
-    # rows as they are where their strides and address suit the kernel's loads, else copied
+    # rows as they are where their strides and address suit the kernel's loads and 32-bit offsets, else copied
     ldx, sx = x2.stride()
-    if sx != 1 or x2.data_ptr() % 16 or (M > 1 and (ldx % 8 or ldx < K)):
+    if sx != 1 or x2.data_ptr() % 16 or (M > 1 and (ldx % 8 or not K <= ldx <= 1 << 21)):
         x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
     ldq, sq = qs.stride()
-    if sq != 1 or qs.data_ptr() % 16 or (N > 1 and (ldq % 16 or ldq < K // 2)):
+    if sq != 1 or qs.data_ptr() % 16 or (N > 1 and (ldq % 16 or not K // 2 <= ldq <= 1 << 22)):
         qs, ldq = qs.clone(memory_format=torch.contiguous_format), K // 2
     ldd, sd = d.stride()
-    if sd != 1 or (N > 1 and ldd < blocks):
+    if sd != 1 or (N > 1 and not blocks <= ldd <= 1 << 21):
         d, ldd = d.contiguous(), blocks
     if bias is not None:
         bias = _vec(bias, N, "bias")
