@@ -717,11 +717,19 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
       for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
     }
 
+    // 4-bit pages: what is not needed in the loop over the tiles is formed from the thread's number where it is, not kept in
+    // registers over it (they spill else, and a kernel with scratch memory costs 64 tokens over 4096 each 57 us, 52 without).
+    auto thread = [&] {
+      int t = threadIdx.x;
+      if constexpr (Q4) asm volatile("" : "+v"(t));
+      return t;
+    };
     // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which
     // have the fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do
     // not hold both).
     auto new_tokens = [&] {
       if (sp != 0 || !a.k) return;
+      const int t0 = thread(), j = t0 & 15, qd = t0 >> 4 & 3, c = t0 & 31;
       if (Q4 && frame != lower) {
         const float f = __builtin_ldexpf(1.0f, frame - lower);
 #pragma unroll
@@ -891,10 +899,11 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = sc[ct][i >> 2][i & 3];
         if (__builtin_expect(tl.len[0] + tl.len[1] != 32, 0)) {
-          asm volatile("");  // a branch: else the comparisons are made for every tile
+          // a branch: else the comparisons are made for every tile, and the keys' places kept over all of them
+          const int q = thread() >> 4 & 3;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (s_key4(4 * qd + (i & 3)) >= tl.len[i >> 2]) y[i] = -INFINITY;
+            if (s_key4(4 * q + (i & 3)) >= tl.len[i >> 2]) y[i] = -INFINITY;
         }
         pb[ct] = s_half<D>(y, score_factor(a.scale_log2, qexp[ct] - 14 + kexp - 7), acc[ct]);
       }
@@ -1054,6 +1063,7 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
       if (sum[0] + sum[1] + sum[2] + sum[3] != 0.0f) over = 1;
     }
     // merge the waves, then the output or this split's normalized partial
+    const int tid = thread(), j = tid & 15, qd = tid >> 4 & 3;
     bool again = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -1075,9 +1085,9 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
         sml[wave][0][j] = x.m;
         sml[wave][1][j] = l;
       }
-      if (Q4 && lane == 0) frames[wave] = frame;
+      if (Q4 && (tid & 63) == 0) frames[wave] = frame;
       __syncthreads();
-      for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+      for (int i = tid; i < 16 * (D / 4); i += NW * 64) {
         const int zz = i / (D / 4), d0 = (i % (D / 4)) * 4, z = z0 + 16 * ct + zz;
         if (z >= s.n * a.rep) continue;
         float M = -INFINITY;
