@@ -675,8 +675,10 @@ int od_qk_norm_rope_page_append(const uint16_t* qkv, int64_t ld, uint16_t* out, 
  * bias[n] (bf16, or NULL) and residual[m, n] (bf16, row stride ldr, or NULL; out itself may be it), rounded once to bf16 from
  * fp32. x bf16 [M, ldx >= K]; W = (u - 8) d: qs uint8 [N, ldq >= K / 2], a block of 32 values in 16 bytes, values 0 - 15 in the
  * low halves, 16 - 31 in the high ones; d fp16 [N, ldd >= K / 32]. K % 32 == 0; x and qs 16-byte aligned, ldx % 8 == 0,
- * ldq % 16 == 0. Up to 32 rows of x: no weight is rounded, |x| up to 2^115. More: weights are rounded once to fp16 (|W| up to
- * 65504), x stays exact but for what is below 2^-29 of its row's largest value. A row of x that holds an infinity or NaN is NaN.
+ * ldq % 16 == 0. Up to 32 rows of x: no weight is rounded, |x| up to 2^115, sums in fp32 that are off by about 2^-17 of |x| d a
+ * value. More: weights are rounded once to fp16 (|W| up to 65504), x stays exact but for what is below 2^-29 of its row's largest
+ * value. (So a row's result depends, within these bounds, on whether it is one of 32 or of 33.) A row of x that holds an infinity or
+ * NaN is NaN.
  * ws: od_q4_linear_ws(M, N, K) floats, 16-byte aligned, NULL where that is 0; one call's at a time. M <= 2^22, N <= 2^24,
  * K <= 2^20, ldx <= 2^21, ldq <= 2^22, ldd <= 2^21.
  */

@@ -332,8 +332,10 @@ __device__ __forceinline__ int q4_frame(uint32_t bits) { return bits ? (int)(bit
 // not fit the registers (16 x 8000 tokens 62 us, 49 with halves); bf16 ones then still take a SIMD alone.
 //
 // 4-bit pages: all of it in fp16, since a value is exact there as (u - 8) d in a power-of-two frame (3 significant bits by 8): the
-// slot's queries as fp16 in its frame (in LDS), a tile's K in the frame of its largest scale, V in that of the largest so far, by
-// which O moves along, probabilities kept 2^7 above their value as in the tile kernels. One product takes P then, no low part.
+// slot's queries as fp16 in its frame (in LDS), K and V each in the frame of the largest scale that the wave has seen so far (O moves
+// along with V's), probabilities kept 2^7 above their value as in the tile kernels. One product takes P then, no low part: fp16 is
+// off by 2^-11 of a probability at most, an eighth of the output's own rounding, and the loop, which the conversions bound beside
+// memory, is spared four packings and eight products a tile; l is summed from the unrounded ones.
 // Four lanes of a key read all of it (D / 2 bytes), so a lane's K has one scale (two of heads of 256), loaded with it; V's scales
 // come one or two a lane and go to the lanes that need them through the LDS crossbar. The new tokens come last, in bf16, where O
 // leaves its frame.
@@ -2457,6 +2459,11 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // more than 128 KB of K a CU to read, from the L2 mostly: 16 tokens over 1 x 4000 16 us, 30 as tiles; 256 over 1 x
   // 100 15 and 24; 32 over 2 x 4000 21 and 32; above it 32 over 1 x 32000 62 and 50, bf16 80 and 42, 120 of one head
   // over 1 x 8000 bf16 tokens 37 and 34.
+  // 4-bit pages take int8's limit of slots and bf16's of bytes. Streaming and as tiles they take: heads of 128, 64 slots, 16 x 16
+  // tokens over 4000 49 us and 59, 32 x 16 over 8000 135 and 191; 80 slots 72 and 61; 96, 8 x 24 over 2000 33 and 35; heads of 64, 64
+  // slots, 16 x 16 over 4000 25 and 35, 80 slots 34 and 37; within the bytes 128 x 1 over 1000 22 and 35, 256 over 100 17 and 25;
+  // past them 1 x 64 over 4000 26 and 35, 1 x 32 over 32000 48 and 43, 2 x 64 over 16000 78 and 67. Both limits are low for heads of
+  // 256: 16 x 16 over 4000 55 and 86, 8 x 32 over 4000 55 and 69, 2 x 64 over 16000 86 and 93.
   const int64_t few = B * Hkv * ((slots + 31) / 32);
   const int64_t always = (q8 || q4) && D <= 128 && Hkv < (1 << 15) ? 64 : 32;  // (a grid has 65535 rows)
   p.stream = slots <= always || (slots <= 1024 && few <= 2 * cus && few * max_ctx * D * (q8 ? 1 : 2) <= (cus << 17));
@@ -2534,6 +2541,10 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // 256-wide heads, 4 ragged 900 over 6000 402, 284; 1 x 256 over 6000 (3000 blocks in all) 82, 76; 8 x 64 (2 tiles)
   // 115, 121; heads of 128, 8 x 256 over 6000 (4 tiles) 217, 183, 8 x 128 (2 tiles) 150, 139, 4 x 1024 over 1000 (8000
   // blocks) 85, 87, 4 x 256 over 6000 (12000) 152, 115.
+  // 4-bit pages take the same rule, without the image and with it: heads of 128, 2048 over 16384 660 us and 565, 4 x 1024 over 1000
+  // 150 and 145, 4 x 256 over 6000 151 and 154; heads of 256, 4 x 900 over 6000 770 and 532, 256 over 6000 86 and 80, 8 x 64 121 and
+  // 165; heads of 64, 2048 over 16000 298 and 192. Several sequences of few tiles of 128-wide heads would do better without: 8 x
+  // 256 over 6000 240 and 279, 8 x 128 151 and 200, 4 x 256 over 2000 68 and 76; option rows, 8 x 512 over 2048, take as long.
   p.img_blocks = !p.stream && (q8 || q4) && tiles >= 4 && wgs * keys * D / spt > 5 << 10 ? keys : 0;
   if (p.img_blocks * B * Hkv > (1ll << 28) / (kBK * D)) p.img_blocks = 0;
   p.vexp = p.img_blocks ? (B * Hkv + 3) / 4 * 4 : 0;

@@ -46,12 +46,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t by
 //    four blocks: values 4 g .. 4 g + 3 and 16 + 4 g .. + 3 of the block;
 //  * four bits u at the bottom of 128.0's bf16 are 128 + u: one shift and one and-or for two values. The 136 that it is above
 //    u - 8 leaves by the C operand, -136 times the sum of x over the block, itself a product with a constant A. (A row of x that
-//    holds an infinity or NaN so becomes NaN.)
+//    holds an infinity or NaN so becomes NaN. The block's fp32 sums are of up to 143 |x| a value for the 8 |x| that are left: their
+//    roundings are some seven bits more than of the plain sums, 2^-17 of |x| d a value, far below the output's 2^-8 unless x is
+//    thousands of times larger where the weights are near 0 than elsewhere.)
 //  * holds weight rows 4 g + i of column j of the result; d of row 4 g + i and block b is the one that lane 16 g + 4 i + b loaded.
 // A workgroup's WR x WK waves take WR sets of RT row tiles, WK of them every WK-th step of one, and add up in LDS. x lies in LDS in
 // the order of the B operand, as many steps of it as fit at a time, two buffers of it; the weights of the PD next steps are in
-// registers or on their way meanwhile, whatever the workgroup waits for. One row of x: 4096 x 4096 8.9 us (9.4 MB), 24576 x 4096
-// 20.6 us (2.8 TB/s), 151936 x 4096 87 us (4.0 TB/s); 24 rows over 24576 x 4096 27.5 us, where x, staged by every workgroup, is as much as the weights.
+// registers or on their way meanwhile, whatever the workgroup waits for. One row of x, in a captured graph: 4096 x
+// 4096 6.3 us (9.4 MB; an eager call takes the host 9.5), 24576 x 4096 19.9 us (2.8 TB/s), 151936 x 4096 88 us (4.0 TB/s); 24 rows over
+// 24576 x 4096 27.4 us, where x, staged by every workgroup, is as much as the weights.
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
@@ -256,10 +259,11 @@ __global__ __launch_bounds__(WK * WR * 64) void q4_rows_kernel(Q4Args a) {
 
 // ------------------------------------------------------------------------------------------------ many rows of x
 // Matrix products of tiles. x goes to fp16 once, each row in a power-of-two frame (2^(14 - e), 2^e above its largest value: exact
-// but for values below 2^-29 of it, which move by 2^-40 of it at most), zero-padded to whole stages, in tiles that lie in memory as
+// but for values below 2^-29 of it, which move by 2^-38 of it at most), zero-padded to whole stages, in tiles that lie in memory as
 // they do in LDS, the values of a block in the order in which its weights come out of the conversion. Weights become (u - 8) d in
 // fp16 in the registers that multiply them: one rounding, 2^-11 at most (so |W| up to 65504, fp16's range). A row of x that holds
-// an infinity or NaN is NaN. (The pass over x: 2000 x 12288 in 22 us, 98 MB, at the rate of a copy.)
+// an infinity or NaN is NaN. (The pass over x reads a row twice, the second time past the L2 as well: 2000 x
+// 12288 in 22 us, 96 MB read and 48 written.)
 constexpr int kXThreads = 256, BK = 64, kStageBytes = 2 * BK;  // values, and bytes of a row of x, in a stage
 __global__ __launch_bounds__(kXThreads) void q4_x_kernel(Q4Args a) {
   __shared__ uint32_t red[kXThreads / 64];
@@ -550,8 +554,8 @@ int launch_rows(Q4Args& a, hipStream_t st) {
   return od_launch_status();
 }
 
-// The shapes of the first kernel (one row of x; 16 rows; us). Where the row tiles are few, a tile a workgroup: 4096 x 4096 8.9; 9.5
-// (two sets of two tiles 11.9; 15.3). Then two tiles a wave, which share x: 49152 x 4096 28.6; 37.2 (one tile a workgroup 38.8;
+// The shapes of the first kernel (one row of x; 16 rows; us). Where the row tiles are few, a tile a workgroup: 4096 x 4096 6.3; 8.6
+// (as eager calls 8.9; 9.5, two sets of two tiles 11.9; 15.3). Then two tiles a wave, which share x: 49152 x 4096 28.6; 37.2 (one tile a workgroup 38.8;
 // 60.7, two 32.2; 44.5). With many of them and several rows of x, four sets, whose x is staged half as often: 98304 x 4096, 16 rows
 // 65.9 against 70.4, 32 rows 79.1 against 87.3; at one row 58.9 against 55.2, and 32 rows over 49152 x 4096 51.8 against 47.7.
 // Above 16 rows x is as much to stage as the weights are to read: eight sets of a tile where these are one workgroup for every CU

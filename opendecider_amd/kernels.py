@@ -1052,8 +1052,8 @@ def q4_linear(x: torch.Tensor, qs: torch.Tensor, d: torch.Tensor, bias: torch.Te
               residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """od_q4_linear: x (..., K) bf16 times 4-bit weights in Q4Table's layout, qs uint8 (N, K / 2) and d fp16 (N, K / 32), plus
     bias (N,) and residual (..., N) bf16: (..., N) bf16, rounded once. K a multiple of 32. Up to 32 rows of x no weight is rounded
-    (|x| up to 2^115); for more each is once, to fp16. A row of x that holds an infinity or NaN comes out NaN. out (..., N) bf16
-    may be the residual, and overlaps no other input. No gradients."""
+    (|x| up to 2^115) and the fp32 sums are off by about 2^-17 of |x| d a value; for more each weight is once, to fp16. A row of x
+    that holds an infinity or NaN comes out NaN. out (..., N) bf16 may be the residual, and overlaps no other input. No gradients."""
     dev = _one_device("q4_linear", x, qs, d, bias, residual, out)
     _lib.bf16_bits(x)
     if qs.dtype != torch.uint8 or d.dtype != torch.float16:
