@@ -599,8 +599,30 @@ __device__ __forceinline__ uint32_t s_wave_max2(uint32_t x) {
 // In the frames of fp16, values are below 2^14 and no sum of them passes fp32. The new tokens' bf16 values are as they are, and
 // probabilities of up to 2^(kLift + kSlack) beside values of 2^113 do pass it, though O / l is finite. Work whose O is not, once they
 // were added, is done again with one factor of the products times 2^-64 (0 below 2^-63) and O in units of 2^64: no sum of finite values
-// passes fp32 then, and the other outputs keep their bits. Rare: it costs a look at O.
+// passes fp32 then. Only the outputs that were not finite are taken from it: what is small beside large or infinite values stays as it
+// was. Rare: it costs a look at O.
 constexpr int kLower = 64;
+// Four outputs, or a split's, at their place; again: only those that are not finite there (the lane's own, written before).
+__device__ __forceinline__ void put4(uint16_t* at, float4 y, bool again) {
+  uint2 w = make_uint2(od_pack_bf16x2(y.x, y.y), od_pack_bf16x2(y.z, y.w));
+  if (again) {
+    const uint2 old = *reinterpret_cast<const uint2*>(at);
+    auto pick = [](uint32_t o, uint32_t n) {
+      const uint32_t keep = ((o & 0x7f80u) != 0x7f80u ? 0xffffu : 0u) | ((o & 0x7f800000u) != 0x7f800000u ? 0xffff0000u : 0u);
+      return (o & keep) | (n & ~keep);
+    };
+    w = make_uint2(pick(old.x, w.x), pick(old.y, w.y));
+  }
+  *reinterpret_cast<uint2*>(at) = w;
+}
+__device__ __forceinline__ void put4(float* at, float4 y, bool again) {
+  if (again) {
+    const float4 old = *reinterpret_cast<const float4*>(at);
+    auto pick = [](float o, float n) { return fabsf(o) < INFINITY ? o : n; };
+    y = make_float4(pick(old.x, y.x), pick(old.y, y.y), pick(old.z, y.z), pick(old.w, y.w));
+  }
+  *reinterpret_cast<float4*>(at) = y;
+}
 __device__ __forceinline__ uint32_t lower_bf16x2(uint32_t w) {  // infinities and NaN as they are
   uint32_t r = w & 0x80008000u;
 #pragma unroll
@@ -646,9 +668,17 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
   const int tiles = (s.ctx + W - 1) / W, nv = splits_of(a, tiles);
   if (s.n == 0 || sp >= nv) return;  // uniform over the workgroup
   const int t_hi = sp == a.nsplit - 1 ? tiles : min(tiles, t_lo + a.chunk);
+  // 4-bit pages: what is not needed in the loop over the tiles is formed from the thread's number where it is, not kept in
+  // registers over it (they spill else, and a kernel with scratch memory costs 64 tokens over 4096 each 57 us, 52 without).
+  auto thread = [&] {
+    int t = threadIdx.x;
+    if constexpr (Q4) asm volatile("" : "+v"(t));
+    return t;
+  };
   // one round unless max_new was too small
   int lower = 0;  // the power of two that the new tokens' probabilities are lowered by
-  for (int z0 = blockIdx.y / a.p.Hkv * 16 * CT; z0 < s.n * a.rep;) {
+  const int z_lo = blockIdx.y / a.p.Hkv * 16 * CT;
+  for (int z0 = z_lo; z0 < s.n * a.rep;) {
     constexpr int QN = 16 * CT * (D / 8), QC = QN / (NW * 64) ? QN / (NW * 64) : 1;
     uint4 qw[QC];
 #pragma unroll
@@ -659,7 +689,8 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
         qw[k] = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.s0 + z / a.rep) * a.sqt +
                                                 (int64_t)(g * a.rep + z % a.rep) * a.sqh + d0);
     }
-    int tt = t_lo + wave, pages = pages0, nth = -1;
+    int tt = t_lo + wave, nth = -1;
+    int pages = !Q4 || (z0 == z_lo && lower == 0) ? pages0 : s_pages<R>(a.p, b, tt * W, NW * W);
     // the wave's next tile into x (past the last one: an empty one, without traffic)
     Tile tl[SETS];
     int asked = tt - NW;  // the tile last asked for
@@ -699,9 +730,10 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
                            (_Float16)__builtin_ldexpf(__uint_as_float(w[c2] & 0xffff0000u), 14 - e)};
           h[c2] = __builtin_bit_cast(uint32_t, r);
         }
-        if (i < QN) {
-          *reinterpret_cast<uint4*>(sm.q16 + (i / (D / 8)) * QR + (i % (D / 8)) * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-          if (i % (D / 8) == 0) qe[i / (D / 8)] = e;
+        const int i4 = k * NW * 64 + thread();
+        if (i4 < QN) {
+          *reinterpret_cast<uint4*>(sm.q16 + (i4 / (D / 8)) * QR + (i4 % (D / 8)) * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+          if (i4 % (D / 8) == 0) qe[i4 / (D / 8)] = e;
         }
       }
     }
@@ -719,13 +751,6 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
       for (int dt = 0; dt < D / 16; ++dt) x.o[dt] = v4f{0, 0, 0, 0};
     }
 
-    // 4-bit pages: what is not needed in the loop over the tiles is formed from the thread's number where it is, not kept in
-    // registers over it (they spill else, and a kernel with scratch memory costs 64 tokens over 4096 each 57 us, 52 without).
-    auto thread = [&] {
-      int t = threadIdx.x;
-      if constexpr (Q4) asm volatile("" : "+v"(t));
-      return t;
-    };
     // The new tokens, tiles of 16 bf16 keys (as many as the slots have tokens), in split 0: by the last waves, which
     // have the fewest tiles of pages, and first, while the pages are on their way (heads of 256: last, the registers do
     // not hold both).
@@ -1066,17 +1091,12 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
     }
     // merge the waves, then the output or this split's normalized partial
     const int tid = thread(), j = tid & 15, qd = tid >> 4 & 3;
-    bool again = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const SAcc<D>& x = acc[ct];
       float l = x.l + __shfl_xor(x.l, 16, 64);
       l = od_xor32_sum(l);
       __syncthreads();  // every wave is done with the queries, or the columns before
-      if (Q4 && ct == 0 && lower == 0 && __builtin_amdgcn_readfirstlane(over)) {
-        again = true;
-        break;
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1125,18 +1145,17 @@ __global__ __launch_bounds__(kStreamWaves * 64, WAVES) void paged_stream_kernel(
                               __builtin_ldexpf(sum.w, top));
         }
         if (nv == 1) {
-          *reinterpret_cast<uint2*>(a.out + n * a.sot + head * a.soh + d0) = make_uint2(od_pack_bf16x2(sum.x, sum.y),
-              od_pack_bf16x2(sum.z, sum.w));
+          put4(a.out + n * a.sot + head * a.soh + d0, sum, lower != 0);
           if (a.lse && d0 == 0) a.lse[n * a.Hq + head] = ls * kLn2;
         } else {
           const int64_t slot = ((int64_t)sp * a.p.N + n) * a.Hq + head;
-          *reinterpret_cast<float4*>(a.part + slot * D + d0) = sum;
+          put4(a.part + slot * D + d0, sum, lower != 0);
           if (d0 == 0) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + slot] = ls;
         }
       }
     }
-    lower = again ? kLower : 0;
-    if (!again) z0 += a.tiles * 16 * CT;
+    lower = Q4 && lower == 0 && __builtin_amdgcn_readfirstlane(over) ? kLower : 0;
+    if (lower == 0) z0 += a.tiles * 16 * CT;
   }
 }
 
@@ -1599,10 +1618,10 @@ __device__ __forceinline__ void add_odd(const AttnArgs& a, const Seq& s, int g, 
       for (int i = 0; i < 16; ++i) t.o[dt][i] += odd_bf16(vp[dt * 32 + 8 * (i >> 2) + (i & 3)]);
   }
 }
-// out = O / l, or the split's normalized partial; lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
+// out = O / l, or the split's normalized partial (again: as put4); lane: slot col, value rows 32 dt + 8 (i / 4) + 4 h + i % 4
 template <int D>
 __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSlot<D>& t, float l, int frame, int sp,
-    int nv, int half) {
+    int nv, int half, bool again) {
   if (!t.ok) return;
   const int h = (threadIdx.x & 63) >> 5;
   // 2^frame may be subnormal, so it comes last
@@ -1616,10 +1635,9 @@ __device__ __forceinline__ void t_out(const AttnArgs& a, const Seq& s, const TSl
       const float4 y = make_float4(t.o[dt][4 * i4] * inv * unit, t.o[dt][4 * i4 + 1] * inv * unit,
           t.o[dt][4 * i4 + 2] * inv * unit, t.o[dt][4 * i4 + 3] * inv * unit);
       if (nv == 1)
-        *reinterpret_cast<uint2*>(a.out + n * a.sot + t.head * a.soh + d0) = make_uint2(od_pack_bf16x2(y.x, y.y),
-            od_pack_bf16x2(y.z, y.w));
+        put4(a.out + n * a.sot + t.head * a.soh + d0, y, again);
       else
-        *reinterpret_cast<float4*>(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0) = y;
+        put4(a.part + (((int64_t)sp * a.p.N + n) * a.Hq + t.head) * D + d0, y, again);
     }
   if (h == 0 && half == 0) {
     if (nv > 1) a.part[(int64_t)a.nsplit * a.p.N * a.Hq * D + ((int64_t)sp * a.p.N + n) * a.Hq + t.head] = ls;
@@ -1706,9 +1724,11 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       float ks = 0, vs = 0;    // lane l: the scales of key l of the loaded block
       uint64_t there = 0;      // the loaded block's keys that exist
       const int in_page = (1 << a.p.shift) - 1;
-      auto pages = [&](int blk) {
+      int first_lane = lane;  // (so that the first blocks' places are not kept in registers from tile to tile)
+      if constexpr (REG) asm volatile("" : "+v"(first_lane));
+      auto pages = [&](int blk, int l) {
         if constexpr (IMG) return;
-        const int pos = blk * kBK + lane;
+        const int pos = blk * kBK + l;
         pg = pos < s.ctx ? a.p.table[b * a.p.ld_table + (pos >> a.p.shift)] : -1;
         if (pg >= a.p.n_pages) pg = -1;
       };
@@ -1803,15 +1823,15 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       };
       // One step: block blk's products; ahead of them, for int8 and 4 bits the conversion of block blk + 1 (in registers since the
       // last step) and the loads of blk + 2, for bf16 the copy of blk + 1.
-      pages(b_lo);
+      pages(b_lo, first_lane);
       load(b_lo, 0);
-      pages(b_lo + 1);
+      pages(b_lo + 1, first_lane);
       if constexpr (!REG) dma_wait();
       store(0);
       if constexpr (REG) frame = vexp - 7;  // O is 0 still: no rescaling, by what may be no fp32 number
       if (REG && b_lo + 1 < b_hi) {
         load(b_lo + 1, 1);
-        pages(b_lo + 2);
+        pages(b_lo + 2, first_lane);
       }
       __syncthreads();
       for (int blk = b_lo; blk < b_hi; ++blk) {
@@ -1824,11 +1844,11 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
             store(cur ^ 1);
             if (blk + 2 < b_hi) {
               load(blk + 2, cur);
-              pages(blk + 3);
+              pages(blk + 3, lane);
             }
           } else {
             load(blk + 1, cur ^ 1);
-            pages(blk + 2);
+            pages(blk + 2, lane);
           }
         }
         if (REG && f_new != frame) {  // the values' frame rose: uniform over the workgroup
@@ -1923,6 +1943,7 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
       }
     }
 
+    t_out<D>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, 0, lower != 0);
     if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
       if (t_over<D>(t)) sm.over = 1;
       __syncthreads();
@@ -1931,7 +1952,6 @@ __global__ __launch_bounds__(NW * 64, t_waves(D, SRC)) void paged_tile_kernel(At
         continue;
       }
     }
-    t_out<D>(a, s, t, od_xor32_sum(t.l), frame, sp, nv, 0);
     lower = 0;
     tile += a.tiles;
   }
@@ -2322,6 +2342,13 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
       }
     }
 
+    // ---- the sum of both halves, then as above
+    float l = od_xor32_sum(t.l);
+    __syncthreads();  // the last block's maxima are read
+    if (h == 0) sm.mx[half][grp][col] = l;
+    __syncthreads();
+    l += sm.mx[half ^ 1][grp][col];
+    t_out<D>(a, s, t, l, frame, sp, nv, half, lower != 0);
     if (lower == 0 && (!H16 || (sp == 0 && a.k))) {
       if (t_over<D>(t)) sm.over = 1;
       __syncthreads();
@@ -2330,13 +2357,6 @@ __global__ __launch_bounds__(512, 2) void paged_wide_kernel(AttnArgs a) {
         continue;
       }
     }
-    // ---- the sum of both halves, then as above
-    float l = od_xor32_sum(t.l);
-    __syncthreads();  // the last block's maxima are read
-    if (h == 0) sm.mx[half][grp][col] = l;
-    __syncthreads();
-    l += sm.mx[half ^ 1][grp][col];
-    t_out<D>(a, s, t, l, frame, sp, nv, half);
     lower = 0;
     tile += a.tiles;
   }

@@ -91,3 +91,36 @@ def test_values_up_to_the_largest_in_other_pages(gpu_lib, cached, new, d, form, 
     for n, ctx, rows in (([40], [300], 0), ([30, 3], [130, 0], 8)):
         c = enlarged(t4.as_many(tp.make(34, n, ctx, 4, 1, d, int8=int8, rows=rows, **t4.padded(form)), form), cached, new)
         tp.check_attn(c, *t4.run_attn(c))
+
+
+def small_and(c, exp):
+    """New values around 2^-100 in every column, those of every third one times 2^exp; the cached ones as they are."""
+    e = torch.full((c["v"].shape[2],), -100.0)
+    e[::3] = exp
+    c["v"] = (c["v"].double() * torch.exp2(e.double())).clamp(-MOST, MOST).to(BF)
+    return c
+
+
+@pytest.mark.parametrize("int8", [None, True, False])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_values_beside_large_and_infinite_ones(gpu_lib, d, form, int8):
+    """A column's large or infinite values change nothing in the others, whatever their size."""
+    if int8 is not None and form in ("few", "table"):
+        pytest.skip("few slots over int8 and bf16 pages sum as they are")
+    for n, ctx, rows in (([1, 1], [600, 0], 0), ([40], [300], 0), ([30, 3], [0, 130], 8)):
+        c = t4.as_many(t4.make(35, n, ctx, 4, 1, d, int8=int8, rows=rows, **t4.padded(form)), form)
+        v, live = c["v"], sum(n)
+        plain = t4.run_attn(small_and(c, -100))
+        for exp in (0, 125, None):
+            c["v"] = v
+            small_and(c, exp or 0)
+            if exp is None:
+                c["v"][:, :, ::3] = float("inf")
+            out, lse = t4.run_attn(c)
+            others = torch.arange(d) % 3 != 0
+            assert torch.equal(out[:live, :, others], plain[0][:live, :, others]) and torch.equal(lse[:live], plain[1][:live]), exp
+            if exp is None:
+                assert (out[:live, :, ::3] == float("inf")).all()
+            else:
+                (t4.check_attn if int8 is None else tp.check_attn)(c, out, lse)
