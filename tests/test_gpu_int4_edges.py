@@ -101,13 +101,11 @@ def small_and(c, exp):
     return c
 
 
-@pytest.mark.parametrize("int8", [None, True, False])
-@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("int8,form", [*((None, f) for f in FORMS), *((q, f) for q in (True, False) for f in ("rows", "image"))])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_small_values_beside_large_and_infinite_ones(gpu_lib, d, form, int8):
-    """A column's large or infinite values change nothing in the others, whatever their size."""
-    if int8 is not None and form in ("few", "table"):
-        pytest.skip("few slots over int8 and bf16 pages sum as they are")
+    """A column's large or infinite values change nothing in the others, whatever their size. (Few slots over int8 and bf16 pages
+    sum as they are.)"""
     for n, ctx, rows in (([1, 1], [600, 0], 0), ([40], [300], 0), ([30, 3], [0, 130], 8)):
         c = t4.as_many(t4.make(35, n, ctx, 4, 1, d, int8=int8, rows=rows, **t4.padded(form)), form)
         v, live = c["v"], sum(n)
