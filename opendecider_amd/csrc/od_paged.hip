@@ -2481,7 +2481,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
   // over 1 x 8000 bf16 tokens 37 and 34.
   // 4-bit pages take int8's limit of slots and bf16's of bytes. Streaming and as tiles they take: heads of 128, 64 slots, 16 x 16
   // tokens over 4000 49 us and 59, 32 x 16 over 8000 135 and 191; 80 slots 72 and 61; 96, 8 x 24 over 2000 33 and 35; heads of 64, 64
-  // slots, 16 x 16 over 4000 25 and 35, 80 slots 34 and 37; within the bytes 128 x 1 over 1000 22 and 35, 256 over 100 17 and 25;
+  // slots, 16 x 16 over 4000 25 and 35, 80 slots 34 and 37; within the bytes 1 x 128 over 1000 22 and 35, 1 x 256 over 100 17 and 25;
   // past them 1 x 64 over 4000 26 and 35, 1 x 32 over 32000 48 and 43, 2 x 64 over 16000 78 and 67. Both limits are low for heads of
   // 256: 16 x 16 over 4000 55 and 86, 8 x 32 over 4000 55 and 69, 2 x 64 over 16000 86 and 93.
   const int64_t few = B * Hkv * ((slots + 31) / 32);
